@@ -23,6 +23,9 @@ EXPORTS = (
     "nf4b200_swiglu_fwd", "nf4b200_swiglu_bwd", "nf4b200_linear_bwd_dx_swiglu",
     "nf4b200_linear_bwd_dx_swiglu_workspace_bytes", "nf4b200_rmsnorm_fwd", "nf4b200_rmsnorm_bwd",
     "nf4b200_add_rmsnorm_bwd",
+    "nf4b200_act8_quantize", "nf4b200_act8_dequantize", "nf4b200_act8_swiglu_fwd", "nf4b200_act8_swiglu_bwd",
+    "nf4b200_act8_lora_grad", "nf4b200_act8_lora_grad_workspace_bytes", "nf4b200_sandwich_norm_fwd",
+    "nf4b200_sandwich_norm_bwd", "nf4b200_sandwich_norm_workspace_bytes",
     "nf4b200_qkv_rotate", "nf4b200_ce_stats", "nf4b200_ce_grad", "nf4b200_selftest_wait", "nf4b200_fp16_linear",
 )
 
@@ -131,9 +134,25 @@ def lib() -> ctypes.CDLL:
     handle.nf4b200_swiglu_fwd.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]
     handle.nf4b200_swiglu_bwd.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                           c_void_p]
+    handle.nf4b200_act8_quantize.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p]
+    handle.nf4b200_act8_dequantize.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]
+    handle.nf4b200_act8_swiglu_fwd.argtypes = [c_void_p] * 7 + [c_int64, c_int64, c_void_p]
+    handle.nf4b200_act8_swiglu_bwd.argtypes = [c_void_p] * 7 + [c_int64, c_int64, c_void_p]
+    handle.nf4b200_act8_lora_grad.argtypes = [c_void_p] * 4 + [c_int64, c_int64, c_void_p, c_size_t, c_void_p]
+    handle.nf4b200_act8_lora_grad_workspace_bytes.argtypes = [c_int64, c_int64]
+    handle.nf4b200_act8_lora_grad_workspace_bytes.restype = c_int64
+    handle.nf4b200_sandwich_norm_fwd.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+                                                 c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_float,
+                                                 c_float, c_void_p]
+    handle.nf4b200_sandwich_norm_bwd.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+                                                 c_void_p, c_void_p, c_void_p, c_int] + [c_void_p] * 5 + [
+                                                     c_int64, c_int64, c_float, c_void_p, c_size_t, c_void_p]
+    handle.nf4b200_sandwich_norm_workspace_bytes.argtypes = [c_int64, c_int64, c_int64]
+    handle.nf4b200_sandwich_norm_workspace_bytes.restype = c_int64
     for name in EXPORTS:
         if name not in ("nf4b200_last_error", "nf4b200_workspace_bytes",
                         "nf4b200_workspace_bytes_group", "nf4b200_scales16_bytes",
+                        "nf4b200_act8_lora_grad_workspace_bytes", "nf4b200_sandwich_norm_workspace_bytes",
                         "nf4b200_gate_up_swiglu_workspace_bytes",
                         "nf4b200_linear_bwd_dx_swiglu_workspace_bytes"):
             getattr(handle, name).restype = c_int

@@ -837,6 +837,189 @@ int nf4b200_swiglu_bwd(const void* d_hidden, const void* gate, const void* up, v
     return NF4B200_OK;
 }
 
+static int act8_check(const char* what, int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 0 || cols > 0x7FFFFFC0)
+        return fail(NF4B200_EINVAL, "%s: bad shape %lld x %lld", what, (long long)rows, (long long)cols);
+    return NF4B200_OK;
+}
+
+// (the kernels' flat grids: a CTA per 4096 values)
+static int act8_size(const char* what, int64_t rows, int64_t cols) {
+    if (rows > 0 && cols > 0 && rows > (int64_t)0x7FFFFFFF * 4096 / cols)
+        return fail(NF4B200_EINVAL, "%s: %lld x %lld values are too many", what, (long long)rows, (long long)cols);
+    return NF4B200_OK;
+}
+
+int nf4b200_act8_quantize(const void* x, int dtype, void* codes, void* steps, int64_t rows, int64_t cols, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = act8_check("act8_quantize", rows, cols);
+    if (rc == NF4B200_OK) rc = act8_size("act8_quantize", rows, cols);
+    if (rc != NF4B200_OK) return rc;
+    if (dtype < NF4B200_F16 || dtype > NF4B200_F32) return fail(NF4B200_EINVAL, "act8_quantize: dtype %d", dtype);
+    if (rows > 0 && cols > 0 && (!x || !codes || !steps)) return fail(NF4B200_EINVAL, "act8_quantize: NULL argument");
+    nf4::Act8Convert a = {const_cast<void*>(x), static_cast<int8_t*>(codes), static_cast<uint8_t*>(steps), rows, cols, dtype, d->sms};
+    cudaError_t e = nf4::launch_act8_quantize(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "act8_quantize: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+int nf4b200_act8_dequantize(const void* codes, const void* steps, void* x, int dtype, int64_t rows, int64_t cols,
+                            void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = act8_check("act8_dequantize", rows, cols);
+    if (rc == NF4B200_OK) rc = act8_size("act8_dequantize", rows, cols);
+    if (rc != NF4B200_OK) return rc;
+    if (dtype < NF4B200_F16 || dtype > NF4B200_F32) return fail(NF4B200_EINVAL, "act8_dequantize: dtype %d", dtype);
+    if (rows > 0 && cols > 0 && (!x || !codes || !steps)) return fail(NF4B200_EINVAL, "act8_dequantize: NULL argument");
+    nf4::Act8Convert a = {x, static_cast<int8_t*>(const_cast<void*>(codes)), static_cast<uint8_t*>(const_cast<void*>(steps)),
+                          rows, cols, dtype, d->sms};
+    cudaError_t e = nf4::launch_act8_dequantize(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "act8_dequantize: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+int nf4b200_act8_swiglu_fwd(const void* gate, const void* up, void* hidden, void* gate_codes, void* gate_steps,
+                            void* up_codes, void* up_steps, int64_t rows, int64_t cols, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = act8_check("act8_swiglu_fwd", rows, cols);
+    if (rc == NF4B200_OK) rc = act8_size("act8_swiglu_fwd", rows, cols);
+    if (rc != NF4B200_OK) return rc;
+    if (rows > 0 && cols > 0 && (!gate || !up || !hidden || !gate_codes || !gate_steps || !up_codes || !up_steps))
+        return fail(NF4B200_EINVAL, "act8_swiglu_fwd: NULL argument");
+    nf4::Act8Swiglu a = {};
+    a.gate = static_cast<const __half*>(gate); a.up = static_cast<const __half*>(up); a.hidden = static_cast<__half*>(hidden);
+    a.gate_codes = static_cast<int8_t*>(gate_codes); a.up_codes = static_cast<int8_t*>(up_codes);
+    a.gate_steps = static_cast<uint8_t*>(gate_steps); a.up_steps = static_cast<uint8_t*>(up_steps);
+    a.rows = rows; a.cols = cols; a.sm_count = d->sms;
+    cudaError_t e = nf4::launch_act8_swiglu(a, false, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "act8_swiglu_fwd: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+int nf4b200_act8_swiglu_bwd(const void* d_hidden, const void* gate_codes, const void* gate_steps, const void* up_codes,
+                            const void* up_steps, void* d_gate, void* d_up, int64_t rows, int64_t cols, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = act8_check("act8_swiglu_bwd", rows, cols);
+    if (rc == NF4B200_OK) rc = act8_size("act8_swiglu_bwd", rows, cols);
+    if (rc != NF4B200_OK) return rc;
+    if (rows > 0 && cols > 0 && (!d_hidden || !gate_codes || !gate_steps || !up_codes || !up_steps || !d_gate || !d_up))
+        return fail(NF4B200_EINVAL, "act8_swiglu_bwd: NULL argument");
+    nf4::Act8Swiglu a = {};
+    a.d_hidden = static_cast<const __half*>(d_hidden);
+    a.d_gate = static_cast<__half*>(d_gate); a.d_up = static_cast<__half*>(d_up);
+    a.gate_codes = static_cast<int8_t*>(const_cast<void*>(gate_codes));
+    a.up_codes = static_cast<int8_t*>(const_cast<void*>(up_codes));
+    a.gate_steps = static_cast<uint8_t*>(const_cast<void*>(gate_steps));
+    a.up_steps = static_cast<uint8_t*>(const_cast<void*>(up_steps));
+    a.rows = rows; a.cols = cols; a.sm_count = d->sms;
+    cudaError_t e = nf4::launch_act8_swiglu(a, true, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "act8_swiglu_bwd: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+int64_t nf4b200_act8_lora_grad_workspace_bytes(int64_t rows, int64_t cols) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = act8_check("act8_lora_grad_workspace_bytes", rows, cols);
+    if (rc != NF4B200_OK) return rc;
+    const int splits = nf4::act8_lora_grad_splits(rows, cols, d->sms);
+    return splits > 1 ? (int64_t)splits * 16 * cols * 4 : 0;
+}
+
+int nf4b200_act8_lora_grad(const void* codes, const void* steps, const void* s, void* out, int64_t rows, int64_t cols,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = act8_check("act8_lora_grad", rows, cols);
+    if (rc != NF4B200_OK) return rc;
+    if (rows <= 0 || cols <= 0) return fail(NF4B200_EINVAL, "act8_lora_grad: bad shape %lld x %lld", (long long)rows, (long long)cols);
+    if (!codes || !steps || !s || !out) return fail(NF4B200_EINVAL, "act8_lora_grad: NULL argument");
+    if (!aligned16(codes)) return fail(NF4B200_EINVAL, "act8_lora_grad: codes are not 16-byte aligned");
+    const int64_t need = nf4b200_act8_lora_grad_workspace_bytes(rows, cols);
+    if (need > 0 && (!workspace || workspace_bytes < (size_t)need || !aligned16(workspace)))
+        return fail(NF4B200_EINVAL, "act8_lora_grad: needs %lld bytes of scratch", (long long)need);
+    nf4::Act8LoraGrad a = {};
+    a.codes = static_cast<const int8_t*>(codes); a.steps = static_cast<const uint8_t*>(steps);
+    a.s = static_cast<const __half*>(s); a.out = static_cast<float*>(out); a.planes = static_cast<float*>(workspace);
+    a.rows = rows; a.cols = cols; a.sm_count = d->sms;
+    cudaError_t e = nf4::launch_act8_lora_grad(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "act8_lora_grad: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+static int sandwich_check(const char* what, int64_t rows, int64_t hidden, int64_t gates, int delta_dtype, int normed_dtype) {
+    if (rows < 0 || rows > 0x7FFFFFFF || hidden <= 0 || hidden > nf4::SANDWICH_MAX_HIDDEN)
+        return fail(NF4B200_EINVAL, "%s: bad shape %lld x %lld (hidden up to %d)", what, (long long)rows, (long long)hidden,
+                    nf4::SANDWICH_MAX_HIDDEN);
+    if (gates < 0 || (gates > 0 && rows % gates != 0))
+        return fail(NF4B200_EINVAL, "%s: %lld gate rows for %lld rows", what, (long long)gates, (long long)rows);
+    if (delta_dtype < NF4B200_F16 || delta_dtype > NF4B200_F32 || (normed_dtype != delta_dtype && normed_dtype != NF4B200_F32))
+        return fail(NF4B200_EINVAL, "%s: dtypes %d, %d", what, delta_dtype, normed_dtype);
+    return NF4B200_OK;
+}
+
+int nf4b200_sandwich_norm_fwd(const void* residual, const void* delta, int delta_dtype, const void* post, const void* pre,
+                              const void* gate, int64_t gates, void* stream_out, void* normed, int normed_dtype, void* rstd,
+                              int64_t rows, int64_t hidden, float scale, float eps, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = sandwich_check("sandwich_norm_fwd", rows, hidden, gates, delta_dtype, normed_dtype);
+    if (rc != NF4B200_OK) return rc;
+    if (rows > 0 && (!residual || !delta || !post || !pre || !stream_out || !normed || (gates > 0) != (gate != nullptr)))
+        return fail(NF4B200_EINVAL, "sandwich_norm_fwd: NULL argument");
+    nf4::SandwichArgs a = {};
+    a.residual = static_cast<const float*>(residual); a.delta = delta;
+    a.post = static_cast<const float*>(post); a.pre = static_cast<const float*>(pre); a.gate = static_cast<const float*>(gate);
+    a.stream = static_cast<float*>(stream_out); a.normed = normed; a.rstd = static_cast<float*>(rstd);
+    a.rows = rows; a.hidden = (int)hidden; a.gates = gates; a.scale = scale; a.eps = eps;
+    a.delta_type = delta_dtype; a.normed_type = normed_dtype; a.sm_count = d->sms;
+    cudaError_t e = nf4::launch_sandwich(a, false, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "sandwich_norm_fwd: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+int64_t nf4b200_sandwich_norm_workspace_bytes(int64_t rows, int64_t hidden, int64_t gates) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = sandwich_check("sandwich_norm_workspace_bytes", rows, hidden, gates, NF4B200_F32, NF4B200_F32);
+    if (rc != NF4B200_OK) return rc;
+    return rows == 0 ? 0 : 4 * nf4::sandwich_workspace_floats(rows, (int)hidden, gates, d->sms);
+}
+
+int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delta_dtype, const void* post, const void* pre,
+                              const void* gate, int64_t gates, const void* rstd, const void* d_stream, const void* d_normed,
+                              int normed_dtype, void* d_residual, void* d_delta, void* d_post, void* d_pre, void* d_gate,
+                              int64_t rows, int64_t hidden, float scale, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = sandwich_check("sandwich_norm_bwd", rows, hidden, gates, delta_dtype, normed_dtype);
+    if (rc != NF4B200_OK) return rc;
+    if (rows > 0 && (!stream_in || !delta || !post || !pre || !rstd || !d_normed || (gates > 0) != (gate != nullptr) ||
+                     (gates == 0 && d_gate)))
+        return fail(NF4B200_EINVAL, "sandwich_norm_bwd: NULL argument, or a gradient of no gate");
+    const int64_t need = rows == 0 ? 0 : 4 * nf4::sandwich_workspace_floats(rows, (int)hidden, gates, d->sms);
+    if (need > 0 && (!workspace || workspace_bytes < (size_t)need || !aligned16(workspace)))
+        return fail(NF4B200_EINVAL, "sandwich_norm_bwd: needs %lld bytes of scratch", (long long)need);
+    nf4::SandwichArgs a = {};
+    a.stream = static_cast<float*>(const_cast<void*>(stream_in)); a.delta = delta;
+    a.post = static_cast<const float*>(post); a.pre = static_cast<const float*>(pre); a.gate = static_cast<const float*>(gate);
+    a.rstd = static_cast<float*>(const_cast<void*>(rstd));
+    a.d_stream = static_cast<const float*>(d_stream); a.d_normed = d_normed;
+    a.d_residual = static_cast<float*>(d_residual); a.d_delta = d_delta;
+    a.d_post = static_cast<float*>(d_post); a.d_pre = static_cast<float*>(d_pre); a.d_gate = static_cast<float*>(d_gate);
+    a.planes_post = static_cast<float*>(workspace);
+    a.rows = rows; a.hidden = (int)hidden; a.gates = gates; a.scale = scale;
+    a.delta_type = delta_dtype; a.normed_type = normed_dtype; a.sm_count = d->sms;
+    cudaError_t e = nf4::launch_sandwich(a, true, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "sandwich_norm_bwd: %s", cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
 int64_t nf4b200_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t m, int backward) {
     DeviceInfo* d = nullptr;
     int rc = require_sm100(&d);

@@ -316,6 +316,109 @@ Tensor rmsnorm_bwd(const Tensor& x2, const Tensor& weight, const Tensor& rstd, c
     return dx;
 }
 
+int type_code(at::ScalarType t) { return t == at::kHalf ? NF4B200_F16 : t == at::kBFloat16 ? NF4B200_BF16 : NF4B200_F32; }
+
+// (codes, steps) of a contiguous [rows, cols] tensor; see hackaton_b200.act8.
+std::tuple<Tensor, Tensor> act8_room(const Tensor& like, int64_t rows, int64_t cols) {
+    const int64_t blocks = (cols + 31) / 32;
+    const auto options = like.options().memory_format(c10::nullopt);
+    return {at::empty({rows, blocks * 32}, options.dtype(at::kChar)), at::empty({rows, blocks}, options.dtype(at::kByte))};
+}
+
+std::tuple<Tensor, Tensor> act8_quantize(const Tensor& x2) {
+    const c10::cuda::CUDAGuard guard(x2.device());
+    auto [codes, steps] = act8_room(x2, x2.size(0), x2.size(1));
+    check(nf4b200_act8_quantize(x2.const_data_ptr(), type_code(x2.scalar_type()), codes.data_ptr(), steps.data_ptr(),
+                                x2.size(0), x2.size(1), stream_of(x2)));
+    return {codes, steps};
+}
+
+Tensor act8_dequantize(const Tensor& codes, const Tensor& steps, const Tensor& out) {
+    const c10::cuda::CUDAGuard guard(codes.device());
+    check(nf4b200_act8_dequantize(codes.const_data_ptr(), steps.const_data_ptr(), out.data_ptr(),
+                                  type_code(out.scalar_type()), out.size(0), out.size(1), stream_of(codes)));
+    return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> act8_swiglu_fwd(const Tensor& gate2, const Tensor& up2) {
+    const c10::cuda::CUDAGuard guard(gate2.device());
+    const int64_t rows = gate2.size(0), cols = gate2.size(1);
+    Tensor hidden = at::empty_like(gate2);
+    auto [gc, gs] = act8_room(gate2, rows, cols);
+    auto [uc, us] = act8_room(up2, rows, cols);
+    check(nf4b200_act8_swiglu_fwd(gate2.const_data_ptr(), up2.const_data_ptr(), hidden.data_ptr(), gc.data_ptr(),
+                                  gs.data_ptr(), uc.data_ptr(), us.data_ptr(), rows, cols, stream_of(gate2)));
+    return {hidden, gc, gs, uc, us};
+}
+
+std::tuple<Tensor, Tensor> act8_swiglu_bwd(const Tensor& d2, const Tensor& gc, const Tensor& gs, const Tensor& uc,
+                                           const Tensor& us) {
+    const c10::cuda::CUDAGuard guard(d2.device());
+    Tensor dg = at::empty_like(d2), du = at::empty_like(d2);
+    check(nf4b200_act8_swiglu_bwd(d2.const_data_ptr(), gc.const_data_ptr(), gs.const_data_ptr(), uc.const_data_ptr(),
+                                  us.const_data_ptr(), dg.data_ptr(), du.data_ptr(), d2.size(0), d2.size(1),
+                                  stream_of(d2)));
+    return {dg, du};
+}
+
+Tensor act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s2, int64_t cols) {
+    const c10::cuda::CUDAGuard guard(codes.device());
+    const int64_t rows = codes.size(0);
+    const auto options = s2.options().dtype(at::kFloat).memory_format(c10::nullopt);
+    if (rows == 0 || cols == 0) return at::zeros({RANK, cols}, options);
+    Tensor out = at::empty({RANK, cols}, options);
+    const int64_t need = nf4b200_act8_lora_grad_workspace_bytes(rows, cols);
+    if (need < 0) check((int)need);
+    const Scratch ws(need, s2);
+    check(nf4b200_act8_lora_grad(codes.const_data_ptr(), steps.const_data_ptr(), s2.const_data_ptr(), out.data_ptr(),
+                                 rows, cols, ws.get(), (size_t)need, stream_of(codes)));
+    return out;
+}
+
+// (stream, normed rows, what the gradient needs or None)
+std::tuple<Tensor, Tensor, Opt> sandwich_fwd(const Tensor& r2, const Tensor& d2, const Tensor& post, const Tensor& pre,
+                                             const Opt& gate2, double scale, double eps, bool f32_out, bool train) {
+    const c10::cuda::CUDAGuard guard(r2.device());
+    const int64_t rows = r2.size(0), hidden = r2.size(1);
+    Tensor out = at::empty_like(r2);
+    Tensor normed = at::empty({rows, hidden}, d2.options().dtype(f32_out ? at::kFloat : d2.scalar_type()));
+    Opt rstd;
+    if (train) rstd = at::empty({rows, 2}, r2.options());
+    check(nf4b200_sandwich_norm_fwd(r2.const_data_ptr(), d2.const_data_ptr(), type_code(d2.scalar_type()),
+                                    post.const_data_ptr(), pre.const_data_ptr(), ptr(gate2),
+                                    gate2.has_value() ? gate2->size(0) : 0, out.data_ptr(), normed.data_ptr(),
+                                    type_code(normed.scalar_type()), train ? rstd->data_ptr() : nullptr, rows, hidden,
+                                    (float)scale, (float)eps, stream_of(r2)));
+    return {out, normed, rstd};
+}
+
+// Gradients of residual, delta, post, pre and gate, as far as they are wanted.
+std::vector<Opt> sandwich_bwd(const Tensor& s2, const Tensor& d2, const Tensor& post, const Tensor& pre, const Opt& gate2,
+                              const Tensor& rstd, const Tensor& d_stream, const Tensor& d_normed, double scale,
+                              const std::vector<bool>& wants) {
+    const c10::cuda::CUDAGuard guard(s2.device());
+    TORCH_CHECK(wants.size() == 5, "sandwich_bwd: five wishes");
+    const int64_t rows = s2.size(0), hidden = s2.size(1), gates = gate2.has_value() ? gate2->size(0) : 0;
+    std::vector<Opt> g(5);
+    const Tensor* like[] = {&s2, &d2, &post, &pre, gate2.has_value() ? &*gate2 : nullptr};
+    void* at_[5];
+    for (int i = 0; i < 5; ++i) {
+        if (wants[i] && like[i] != nullptr)
+            g[i] = rows == 0 ? at::zeros_like(*like[i]) : at::empty_like(*like[i]);
+        at_[i] = g[i].has_value() ? g[i]->data_ptr() : nullptr;
+    }
+    if (rows == 0) return g;
+    const int64_t need = nf4b200_sandwich_norm_workspace_bytes(rows, hidden, gates);
+    if (need < 0) check((int)need);
+    const Scratch ws(need, s2);
+    check(nf4b200_sandwich_norm_bwd(s2.const_data_ptr(), d2.const_data_ptr(), type_code(d2.scalar_type()),
+                                    post.const_data_ptr(), pre.const_data_ptr(), ptr(gate2), gates, rstd.const_data_ptr(),
+                                    d_stream.const_data_ptr(), d_normed.const_data_ptr(), type_code(d_normed.scalar_type()),
+                                    at_[0], at_[1], at_[2], at_[3], at_[4], rows, hidden, (float)scale, ws.get(),
+                                    (size_t)need, stream_of(s2)));
+    return g;
+}
+
 struct Rotation {   // everything about one rotation that is not a tensor
     int64_t tokens, seq, heads, kv_heads, dim, batch_stride;
     bool padded, f32;
@@ -385,6 +488,13 @@ PYBIND11_MODULE(_host, m) {
     m.def("lora_grad_batch", &lora_grad_batch, unlocked());
     m.def("rmsnorm_fwd", &rmsnorm_fwd, unlocked());
     m.def("rmsnorm_bwd", &rmsnorm_bwd, unlocked());
+    m.def("act8_quantize", &act8_quantize, unlocked());
+    m.def("act8_dequantize", &act8_dequantize, unlocked());
+    m.def("act8_swiglu_fwd", &act8_swiglu_fwd, unlocked());
+    m.def("act8_swiglu_bwd", &act8_swiglu_bwd, unlocked());
+    m.def("act8_lora_grad", &act8_lora_grad, unlocked());
+    m.def("sandwich_fwd", &sandwich_fwd, unlocked());
+    m.def("sandwich_bwd", &sandwich_bwd, unlocked());
     m.def("rotate_fwd", &rotate_fwd, unlocked());
     m.def("rotate_bwd", &rotate_bwd, unlocked());
 }

@@ -144,6 +144,46 @@ cudaError_t launch_swiglu_bwd(const __half* d_hidden, const __half* gate, const 
                               __half* d_gate, __half* d_up, long long n, int sm_count,
                               cudaStream_t stream);
 
+// Activations kept in 8 bits (act8.cu; the form: act8.cuh).
+struct Act8Convert {
+    void* x;             // [rows, cols] contiguous, read by quantize, written by dequantize
+    int8_t* codes;       // [rows, whole blocks of 32]
+    uint8_t* steps;
+    long long rows, cols;
+    int dtype;           // 0 fp16, 1 bf16, 2 fp32
+    int sm_count;
+};
+cudaError_t launch_act8_quantize(const Act8Convert& a, cudaStream_t stream);
+cudaError_t launch_act8_dequantize(const Act8Convert& a, cudaStream_t stream);
+struct Act8Swiglu {
+    const __half* gate;      // forward: [rows, cols] contiguous
+    const __half* up;
+    __half* hidden;          // forward: silu(gate) * up
+    const __half* d_hidden;  // backward
+    __half* d_gate;
+    __half* d_up;
+    int8_t* gate_codes;      // written by the forward, read by the backward
+    int8_t* up_codes;
+    uint8_t* gate_steps;
+    uint8_t* up_steps;
+    long long rows, cols;
+    int sm_count;
+};
+cudaError_t launch_act8_swiglu(const Act8Swiglu& a, bool backward, cudaStream_t stream);
+struct Act8LoraGrad {
+    const int8_t* codes;     // of the fp16 input [rows, cols]
+    const uint8_t* steps;
+    const __half* s;         // [rows, 16]
+    float* out;              // [16, cols]
+    float* planes;           // scratch [splits, 16, cols] where there are several row shares
+    long long rows, cols;
+    int sm_count;
+    long long pitch, rows_per_split;   // set by the launcher
+    int splits;
+};
+int act8_lora_grad_splits(long long rows, long long cols, int sm_count);   // (an upper bound)
+cudaError_t launch_act8_lora_grad(const Act8LoraGrad& a, cudaStream_t stream);
+
 // RMSNorm / add + RMSNorm on the fp32 stream (rmsnorm.cu); mode as in the reference kernel:
 // 0 forward, 1 backward, 2 add then forward, 3 backward plus the sum's own gradient.
 struct RmsNormArgs {
@@ -164,6 +204,39 @@ struct RmsNormArgs {
     float eps;
 };
 cudaError_t launch_rmsnorm(const RmsNormArgs& a, cudaStream_t stream);
+
+// Norm behind a block, gate, scaled residual and the norm before the next block (sandwich.cu).
+struct SandwichArgs {
+    const float* residual;   // forward [rows, hidden]
+    const void* delta;       // [rows, hidden] of delta_type
+    const float* post;       // [hidden]
+    const float* pre;        // [hidden]
+    const float* gate;       // [gates, hidden], or null (gates = 0)
+    float* stream;           // [rows, hidden]: written by the forward, read by the backward
+    void* normed;            // forward, of normed_type
+    float* rstd;             // [rows, 2]: of delta and of the stream; forward: may be null
+    const float* d_stream;   // backward: gradient that reaches the stream directly, or null
+    const void* d_normed;    // backward: of normed_type
+    float* d_residual;       // backward: each may be null
+    void* d_delta;
+    float* d_post;
+    float* d_pre;
+    float* d_gate;
+    float* planes_post;      // backward: scratch (sandwich_workspace_floats)
+    long long rows;
+    int hidden;
+    long long gates;         // divides rows
+    float scale, eps;
+    int delta_type, normed_type;   // 0 fp16, 1 bf16, 2 fp32; the second is the first or fp32
+    int sm_count;
+    // set by the launcher
+    float* planes_pre;
+    float* planes_gate;
+    long long groups, group_rows, shares, share_rows, units, grid;
+};
+constexpr int SANDWICH_MAX_HIDDEN = 16384;
+long long sandwich_workspace_floats(long long rows, int hidden, long long gates, int sm_count);
+cudaError_t launch_sandwich(const SandwichArgs& a, bool backward, cudaStream_t stream);
 
 // Rotary embedding + grouped-query expansion of the packed q / k / v projections (rope.cu).
 struct RopeArgs {

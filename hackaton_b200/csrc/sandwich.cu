@@ -1,0 +1,461 @@
+// The norm behind a block, its gate, the scaled residual and the norm before the next block in one pass each
+// way, on the fp32 stream:
+//   n = delta * rd * post              rd = 1 / sqrt(mean(delta^2) + eps)
+//   s = scale * residual + gate * n    gate: none, or [gates, hidden], a row for rows / gates rows in a row
+//   y = s * rs * pre                   rs = 1 / sqrt(mean(s^2) + eps)
+// and, from d_stream (what reaches s directly) and dy, with dh = delta * rd, sh = s * rs, w = dy * pre, g = gate * post:
+//   ds = d_stream + rs * (w - sh * mean(w * sh))
+//   d_residual = scale * ds            d_delta = rd * (g ds - dh * mean(g ds * dh))
+//   d_gate = post * sum ds dh          d_post = sum gate * ds dh        d_pre = sum dy * sh      (over rows)
+// The backward's second mean is linear in ds, so that both means come out of one reduction of three sums:
+//   mean(g ds dh) = mean(g dh (d_stream + rs w)) - rs mean(w sh) mean(g dh sh)
+// Memory bound: 4 + 4 bytes per value of the stream and 2 + 2 of 16-bit delta and y forward (12), 18 backward. A CTA
+// keeps a thread's columns of the weights in registers over all its rows, asks for the next row before it reduces
+// the present one, and adds the column sums of the weights' gradients in registers; a second kernel adds the CTAs'
+// sums in order, so that results do not depend on timing. All sums are fp32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace nf4 {
+
+// VEC values of a type as they lie in memory.
+template <typename T, int VEC> struct SwRaw;
+
+template <> struct SwRaw<float, 4> {
+    float4 v;
+    __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)); }
+    __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+    static __device__ __forceinline__ void store(void* p, long long i, const float (&f)[4]) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(f[0], f[1], f[2], f[3]);
+    }
+};
+template <> struct SwRaw<__half, 4> {
+    uint2 v;
+    __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(p) + i)); }
+    __device__ __forceinline__ void get(float (&f)[4]) const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    }
+    static __device__ __forceinline__ void store(void* p, long long i, const float (&f)[4]) {
+        const __half2 a = __floats2half2_rn(f[0], f[1]), b = __floats2half2_rn(f[2], f[3]);
+        *reinterpret_cast<uint2*>(static_cast<__half*>(p) + i) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+};
+template <> struct SwRaw<__nv_bfloat16, 4> {
+    uint2 v;
+    __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i)); }
+    __device__ __forceinline__ void get(float (&f)[4]) const {
+        f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+        f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ void store(void* p, long long i, const float (&f)[4]) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + i) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+};
+__device__ __forceinline__ float sw_float(float x) { return x; }
+__device__ __forceinline__ float sw_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float sw_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void sw_round(float x, float& y) { y = x; }
+__device__ __forceinline__ void sw_round(float x, __half& y) { y = __float2half_rn(x); }
+__device__ __forceinline__ void sw_round(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
+template <typename T> struct SwRaw<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const void* p, long long i) { v = static_cast<const T*>(p)[i]; }
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = sw_float(v); }
+    static __device__ __forceinline__ void store(void* p, long long i, const float (&f)[1]) { sw_round(f[0], static_cast<T*>(p)[i]); }
+};
+
+// Sums of N values over the CTA, the same in every thread. `part` has two halves that successive calls take in
+// turn: who writes a half again has passed the barrier behind which everybody had read it.
+template <int N>
+__device__ __forceinline__ void sw_block_sum(float (&v)[N], float (*part)[N][32], int& turn) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps > 1) {
+        if (lane == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) part[turn][n][threadIdx.x >> 5] = v[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = lane < warps ? part[turn][n][lane] : 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+        turn ^= 1;
+    }
+}
+
+template <int NV, int VEC>
+__device__ __forceinline__ void sw_weights(const float* p, int hidden, float fill, float (&w)[NV][VEC]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (threadIdx.x + i * blockDim.x) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[i][e] = fill;
+        if (p != nullptr && c < hidden) {
+            SwRaw<float, VEC> raw;
+            raw.load(p, c);
+            raw.get(w[i]);
+        }
+    }
+}
+
+template <int NV, int VEC, typename TD, typename TY>
+__global__ void __launch_bounds__(1024)
+sandwich_fwd_kernel(const SandwichArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ float part[2][1][32];
+    int turn = 0;
+    const int hidden = a.hidden;
+    const float inv_h = 1.f / (float)hidden;
+    float post[NV][VEC], pre[NV][VEC];
+    sw_weights<NV, VEC>(a.post, hidden, 0.f, post);
+    sw_weights<NV, VEC>(a.pre, hidden, 0.f, pre);
+    if (a.gates == 1) {
+        float gate[NV][VEC];
+        sw_weights<NV, VEC>(a.gate, hidden, 0.f, gate);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) post[i][e] *= gate[i][e];
+    }
+    SwRaw<float, VEC> next_r[NV];
+    SwRaw<TD, VEC> next_d[NV];
+    const auto fetch = [&](long long row) {
+        if (row >= a.rows) return;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            if (c < hidden) {
+                next_d[i].load(a.delta, row * hidden + c);
+                next_r[i].load(a.residual, row * hidden + c);
+            }
+        }
+    };
+    long long row = blockIdx.x;
+    fetch(row);
+    for (; row < a.rows; row += gridDim.x) {
+        float d[NV][VEC], s[NV][VEC], sum[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) d[i][e] = s[i][e] = 0.f;
+            if (c < hidden) {
+                next_d[i].get(d[i]);
+                next_r[i].get(s[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum[0] += d[i][e] * d[i][e];
+        }
+        fetch(row + gridDim.x);
+        sw_block_sum<1>(sum, part, turn);
+        const float rd = 1.f / sqrtf(sum[0] * inv_h + a.eps);
+        sum[0] = 0.f;
+        const float* gate_row = a.gates > 1 ? a.gate + row / a.group_rows * hidden : nullptr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            float n[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) n[e] = d[i][e] * rd * post[i][e];
+            if (gate_row != nullptr && c < hidden) {
+                SwRaw<float, VEC> raw;
+                float gate[VEC];
+                raw.load(gate_row, c);
+                raw.get(gate);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) n[e] *= gate[e];
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s[i][e] = fmaf(a.scale, s[i][e], n[e]);
+                sum[0] += s[i][e] * s[i][e];
+            }
+            if (c < hidden) SwRaw<float, VEC>::store(a.stream, row * hidden + c, s[i]);
+        }
+        sw_block_sum<1>(sum, part, turn);
+        const float rs = 1.f / sqrtf(sum[0] * inv_h + a.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            float y[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[e] = pre[i][e] * (s[i][e] * rs);
+            if (c < hidden) SwRaw<TY, VEC>::store(a.normed, row * hidden + c, y);
+        }
+        if (threadIdx.x == 0 && a.rstd != nullptr) {
+            a.rstd[2 * row] = rd;
+            a.rstd[2 * row + 1] = rs;
+        }
+    }
+}
+
+// A unit is a share of the rows that one gate row serves; a CTA takes units blockIdx.x, + gridDim.x, ...
+template <int NV, int VEC, typename TD, typename TY>
+__global__ void __launch_bounds__(1024)
+sandwich_bwd_kernel(const SandwichArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ float part[2][3][32];
+    int turn = 0;
+    const int hidden = a.hidden;
+    const float inv_h = 1.f / (float)hidden;
+    float post[NV][VEC], pre[NV][VEC], gate[NV][VEC], sum_post[NV][VEC], sum_pre[NV][VEC], sum_unit[NV][VEC];
+    sw_weights<NV, VEC>(a.post, hidden, 0.f, post);
+    sw_weights<NV, VEC>(a.pre, hidden, 0.f, pre);
+    sw_weights<NV, VEC>(a.gates == 1 ? a.gate : nullptr, hidden, 1.f, gate);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum_post[i][e] = sum_pre[i][e] = sum_unit[i][e] = 0.f;
+
+    SwRaw<float, VEC> next_s[NV], next_t[NV];
+    SwRaw<TD, VEC> next_d[NV];
+    SwRaw<TY, VEC> next_y[NV];
+    float next_rd = 0.f, next_rs = 0.f;
+    const auto fetch = [&](long long row) {
+        next_rd = a.rstd[2 * row];
+        next_rs = a.rstd[2 * row + 1];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            if (c < hidden) {
+                next_s[i].load(a.stream, row * hidden + c);
+                next_d[i].load(a.delta, row * hidden + c);
+                next_y[i].load(a.d_normed, row * hidden + c);
+                if (a.d_stream != nullptr) next_t[i].load(a.d_stream, row * hidden + c);
+            }
+        }
+    };
+    const auto first_row = [&](long long unit) { return unit / a.shares * a.group_rows + unit % a.shares * a.share_rows; };
+    const auto end_row = [&](long long unit) {
+        const long long group = unit / a.shares;
+        return min(group * a.group_rows + (unit % a.shares + 1) * a.share_rows, (group + 1) * a.group_rows);
+    };
+    long long unit = blockIdx.x;   // (gridDim.x <= units)
+    long long row = first_row(unit), end = end_row(unit);
+    fetch(row);
+    while (true) {
+        if (a.gates > 1 && row == first_row(unit))
+            sw_weights<NV, VEC>(a.gate + unit / a.shares * hidden, hidden, 0.f, gate);
+        float s[NV][VEC], t[NV][VEC], d[NV][VEC], y[NV][VEC], sum[3] = {0.f, 0.f, 0.f};
+        const float rd = next_rd, rs = next_rs;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s[i][e] = t[i][e] = d[i][e] = y[i][e] = 0.f;
+            if (c < hidden) {
+                next_s[i].get(s[i]);
+                next_d[i].get(d[i]);
+                next_y[i].get(y[i]);
+                if (a.d_stream != nullptr) next_t[i].get(t[i]);
+            }
+        }
+        const long long at = row * hidden;
+        bool unit_done = false, done = false;
+        const long long this_unit = unit;
+        if (++row == end) {
+            unit_done = true;
+            unit += gridDim.x;
+            if (unit < a.units) {
+                row = first_row(unit);
+                end = end_row(unit);
+            } else {
+                done = true;
+            }
+        }
+        if (!done) fetch(row);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s[i][e] *= rs;                                      // sh
+                d[i][e] *= rd;                                      // dh
+                const float w = y[i][e] * pre[i][e], gd = gate[i][e] * post[i][e] * d[i][e];
+                t[i][e] = fmaf(rs, w, t[i][e]);                     // ds but for the mean
+                sum[0] += w * s[i][e];
+                sum[1] += gd * t[i][e];
+                sum[2] += gd * s[i][e];
+                sum_pre[i][e] += y[i][e] * s[i][e];
+            }
+        sw_block_sum<3>(sum, part, turn);
+        const float m1 = rs * (sum[0] * inv_h);
+        const float m2 = (sum[1] - m1 * sum[2]) * inv_h;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            float dr[VEC], dd[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float ds = fmaf(-m1, s[i][e], t[i][e]);
+                dr[e] = a.scale * ds;
+                dd[e] = rd * (ds * (gate[i][e] * post[i][e]) - d[i][e] * m2);
+                sum_unit[i][e] = fmaf(ds, d[i][e], sum_unit[i][e]);
+            }
+            if (c < hidden) {
+                if (a.d_residual != nullptr) SwRaw<float, VEC>::store(a.d_residual, at + c, dr);
+                if (a.d_delta != nullptr) SwRaw<TD, VEC>::store(a.d_delta, at + c, dd);
+            }
+        }
+        if (unit_done) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (threadIdx.x + i * blockDim.x) * VEC;
+                float dg[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    dg[e] = post[i][e] * sum_unit[i][e];
+                    sum_post[i][e] = fmaf(gate[i][e], sum_unit[i][e], sum_post[i][e]);
+                    sum_unit[i][e] = 0.f;
+                }
+                // (one share per gate row: the row itself; otherwise the shares' plane)
+                if (a.d_gate != nullptr && c < hidden)
+                    SwRaw<float, VEC>::store(a.shares == 1 ? a.d_gate : a.planes_gate, this_unit * hidden + c, dg);
+            }
+        }
+        if (done) break;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (threadIdx.x + i * blockDim.x) * VEC;
+        if (c >= hidden) continue;
+        if (a.d_post != nullptr) SwRaw<float, VEC>::store(a.planes_post, (long long)blockIdx.x * hidden + c, sum_post[i]);
+        if (a.d_pre != nullptr) SwRaw<float, VEC>::store(a.planes_pre, (long long)blockIdx.x * hidden + c, sum_pre[i]);
+    }
+}
+
+// Adds the planes in order: blockIdx.y 0 d_post, 1 d_pre, then a gate row each. 32 columns by 32 shares of the planes.
+__global__ void __launch_bounds__(1024)
+sandwich_sum_kernel(const SandwichArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ float part[32][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    for (long long job = blockIdx.y; job < 2 + (a.shares > 1 ? a.groups : 0); job += gridDim.y) {
+        const float* planes = job == 0 ? a.planes_post : job == 1 ? a.planes_pre : a.planes_gate + (job - 2) * a.shares * a.hidden;
+        float* out = job == 0 ? a.d_post : job == 1 ? a.d_pre : a.d_gate == nullptr ? nullptr : a.d_gate + (job - 2) * a.hidden;
+        const long long count = job < 2 ? a.grid : a.shares;
+        float v = 0.f;
+        if (out != nullptr && col < a.hidden) {
+#pragma unroll 4
+            for (long long p = threadIdx.y; p < count; p += 32) v += planes[p * a.hidden + col];
+        }
+        part[threadIdx.y][threadIdx.x] = v;
+        __syncthreads();
+        float t = part[threadIdx.x][threadIdx.y];   // transposed: a warp holds one column's shares
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        const int c = blockIdx.x * 32 + threadIdx.y;
+        if (out != nullptr && threadIdx.x == 0 && c < a.hidden) out[c] = t;
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------- host side
+struct SandwichShape {
+    int vec, nv, threads;
+};
+
+// Columns per thread: one float4 as far as a CTA reaches, then two and four; single values for rows that are
+// no whole float4 or not aligned.
+static SandwichShape sandwich_shape(int hidden, bool vec) {
+    SandwichShape s;
+    s.vec = vec && hidden % 4 == 0 ? 4 : 1;
+    const int items = (hidden + s.vec - 1) / s.vec;
+    if (s.vec == 4) s.nv = items <= 1024 ? 1 : items <= 2048 ? 2 : 4;
+    else            s.nv = items <= 4096 ? 4 : 16;
+    s.threads = ((items + s.nv - 1) / s.nv + 31) / 32 * 32;
+    return s;
+}
+
+// Backward: CTAs, and how the rows of a gate row are shared among them.
+static void sandwich_plan(SandwichArgs& a, int threads) {
+    a.groups = a.gates > 0 ? a.gates : 1;
+    a.group_rows = a.rows / a.groups;
+    long long target = (long long)a.sm_count * (threads >= 1024 ? 1 : threads > 512 ? 2 : threads > 128 ? 1024 / threads : 8);
+    long long shares = target / a.groups;
+    if (shares > a.group_rows) shares = a.group_rows;
+    if (shares < 1) shares = 1;
+    a.share_rows = (a.group_rows + shares - 1) / shares;
+    a.shares = (a.group_rows + a.share_rows - 1) / a.share_rows;
+    a.units = a.groups * a.shares;
+    a.grid = a.units < target ? a.units : target;
+}
+
+long long sandwich_workspace_floats(long long rows, int hidden, long long gates, int sm_count) {
+    long long most = 0;
+    for (int vec = 0; vec < 2; ++vec) {   // (alignment is not known yet)
+        SandwichArgs a = {};
+        a.rows = rows; a.hidden = hidden; a.gates = gates; a.sm_count = sm_count;
+        sandwich_plan(a, sandwich_shape(hidden, vec != 0).threads);
+        const long long planes = 2 * a.grid + (a.gates > 0 && a.shares > 1 ? a.units : 0);
+        if (planes > most) most = planes;
+    }
+    return most * hidden;
+}
+
+template <typename TD, typename TY>
+static cudaError_t sandwich_as(const SandwichArgs& a, const SandwichShape& s, bool backward, unsigned grid, cudaStream_t stream) {
+    const dim3 g(grid), b((unsigned)s.threads);
+#define NF4_SANDWICH(NV, VEC) \
+    return backward ? launch_pdl(sandwich_bwd_kernel<NV, VEC, TD, TY>, g, b, 0, stream, a) \
+                    : launch_pdl(sandwich_fwd_kernel<NV, VEC, TD, TY>, g, b, 0, stream, a)
+    if (s.vec == 4) {
+        if (s.nv == 1) NF4_SANDWICH(1, 4);
+        if (s.nv == 2) NF4_SANDWICH(2, 4);
+        NF4_SANDWICH(4, 4);
+    }
+    if (s.nv == 4) NF4_SANDWICH(4, 1);
+    NF4_SANDWICH(16, 1);
+#undef NF4_SANDWICH
+}
+
+cudaError_t launch_sandwich(const SandwichArgs& a_in, bool backward, cudaStream_t stream) {
+    SandwichArgs a = a_in;
+    if (a.rows <= 0) return cudaSuccess;
+    uintptr_t bits = 0;
+    for (const void* p : {(const void*)a.residual, a.delta, (const void*)a.post, (const void*)a.pre, (const void*)a.gate,
+                          (const void*)a.stream, (const void*)a.normed, (const void*)a.d_stream, a.d_normed,
+                          (const void*)a.d_residual, (const void*)a.d_delta, (const void*)a.d_post, (const void*)a.d_pre,
+                          (const void*)a.d_gate, (const void*)a.planes_post})
+        bits |= reinterpret_cast<uintptr_t>(p);
+    const SandwichShape s = sandwich_shape(a.hidden, (bits & 15) == 0);
+    sandwich_plan(a, s.threads);
+    unsigned grid;
+    if (backward) {
+        a.planes_pre = a.planes_post + a.grid * a.hidden;
+        a.planes_gate = a.planes_pre + a.grid * a.hidden;
+        grid = (unsigned)a.grid;
+    } else {
+        const long long target = (long long)a.sm_count * (2048 / s.threads > 8 ? 8 : 2048 / s.threads);
+        grid = (unsigned)(a.rows < target ? a.rows : target);
+    }
+    cudaError_t e;
+    if (a.delta_type == 0)
+        e = a.normed_type == 2 ? sandwich_as<__half, float>(a, s, backward, grid, stream)
+                               : sandwich_as<__half, __half>(a, s, backward, grid, stream);
+    else if (a.delta_type == 1)
+        e = a.normed_type == 2 ? sandwich_as<__nv_bfloat16, float>(a, s, backward, grid, stream)
+                               : sandwich_as<__nv_bfloat16, __nv_bfloat16>(a, s, backward, grid, stream);
+    else
+        e = sandwich_as<float, float>(a, s, backward, grid, stream);
+    if (e != cudaSuccess || !backward) return e;
+    const bool gate_planes = a.d_gate != nullptr && a.shares > 1;
+    if (a.d_post == nullptr && a.d_pre == nullptr && !gate_planes) return e;
+    long long jobs = 2 + (a.shares > 1 ? a.groups : 0);
+    if (jobs > 4096) jobs = 4096;
+    return launch_pdl(sandwich_sum_kernel, dim3((unsigned)((a.hidden + 31) / 32), (unsigned)jobs), dim3(32, 32), 0, stream, a);
+}
+
+}  // namespace nf4

@@ -19,6 +19,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
+from .act8 import Act8, act8_quantize, lora_grad_act8
 from .lora import RANK, grad_buffer, lora_grad_batch, lora_side
 from .nf4 import _require, _rows, scratch_bytes, streams, weight_ref
 
@@ -92,6 +93,10 @@ class NF4LinearGroup(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, projs, *params):
+        return NF4LinearGroup.run(ctx, False, x, projs, params)
+
+    @staticmethod
+    def run(ctx, keep8, x, projs, params):
         n = len(projs)
         biases, las, lbs = params[0::3], params[1::3], params[2::3]
         xas, b16 = [None] * n, [None] * n
@@ -110,6 +115,12 @@ class NF4LinearGroup(torch.autograd.Function):
         ctx.has_lora = [a is not None for a in las]
         if any(ctx.needs_input_grad):
             saved = [x]
+            ctx.kept8 = None
+            ctx.x_info = (tuple(x.shape), x.device)
+            if keep8:       # only the gradients of the first factors read x
+                q = act8_quantize(x) if any(ctx.needs_input_grad[3 + 3 * i] for i in with_lora) else None
+                saved = [] if q is None else [q.codes, q.steps]
+                ctx.kept8 = () if q is None else (q.shape, q.dtype)
             for i in with_lora:
                 saved += [las[i], lbs[i], xas[i], *kept[i]]
             ctx.save_for_backward(*saved)
@@ -118,24 +129,29 @@ class NF4LinearGroup(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         saved = list(ctx.saved_tensors)
-        x = saved.pop(0)
+        x = kept = None
+        if ctx.kept8 is None:
+            x = saved.pop(0)
+        elif ctx.kept8:
+            kept = Act8(saved.pop(0), saved.pop(0), *ctx.kept8)
+        x_shape, device = ctx.x_info
         projs = ctx.projs
         lora = []
         for has in ctx.has_lora:
             lora.append(tuple(saved.pop(0) for _ in range(5)) if has else None)   # A, B, xa, A16, Bᵀ16
         grads = [g if g is not None else
-                 torch.zeros(*x.shape[:-1], pr.state.shape[0], dtype=torch.float16, device=x.device)
+                 torch.zeros(*x_shape[:-1], pr.state.shape[0], dtype=torch.float16, device=device)
                  for g, pr in zip(grads, projs)]
         us, a16 = [None] * len(projs), [None] * len(projs)
         with_lora = [i for i, lo in enumerate(lora) if lo is not None]
         # all LoRA weight gradients of the group in one launch, summed into a zeroed buffer
         jobs = []  # (z, s or None for u, rank-major output, projection, "a" | "b")
         for i in with_lora:
-            if ctx.needs_input_grad[3 + 3 * i]:
+            if ctx.needs_input_grad[3 + 3 * i] and kept is None:
                 jobs.append((x, None, True, i, "a"))
             if ctx.needs_input_grad[4 + 3 * i]:
                 jobs.append((grads[i], lora[i][2], False, i, "b"))
-        flat = grad_buffer(jobs, x.device) if jobs else None
+        flat = grad_buffer(jobs, device) if jobs else None
         if with_lora:  # every adapter's scaling * dy . B in one launch
             downs, *_ = lora_side([grads[i] for i in with_lora], [lora[i][4] for i in with_lora],
                                   [projs[i].scaling for i in with_lora], zero=flat)
@@ -151,6 +167,10 @@ class NF4LinearGroup(torch.autograd.Function):
                                   [j[2] for j in jobs], flat)
             for j, r in zip(jobs, res):
                 wgrads[j[3:]] = r
+        if kept is not None:
+            for i in with_lora:
+                if ctx.needs_input_grad[3 + 3 * i]:
+                    wgrads[(i, "a")] = lora_grad_act8(kept, us[i])
         out = [grad_x, None]
         for i, (g, pr, lo) in enumerate(zip(grads, projs, lora)):
             gb = ga = gbb = None
@@ -165,8 +185,17 @@ class NF4LinearGroup(torch.autograd.Function):
         return tuple(out)
 
 
-def nf4_linear_group(x, projections: Sequence[Projection]):
-    """Outputs of all `projections` applied to the same x, computed by one grouped launch."""
+class NF4LinearGroupAct8(NF4LinearGroup):
+    """The same with x kept once, in 8 bits, where a first factor's gradient needs it."""
+
+    @staticmethod
+    def forward(ctx, x, projs, *params):
+        return NF4LinearGroup.run(ctx, True, x, projs, params)
+
+
+def nf4_linear_group(x, projections: Sequence[Projection], keep8=False):
+    """Outputs of all `projections` applied to the same x, computed by one grouped launch. With `keep8`, x is
+    kept once, in 8 bits, for the gradients of the LoRA pairs' first factors (act8.py)."""
     params = []
     for pr in projections:
         if (pr.lora_a is None) != (pr.lora_b is None):
@@ -174,4 +203,4 @@ def nf4_linear_group(x, projections: Sequence[Projection]):
         if pr.lora_a is not None and pr.lora_a.shape[0] != RANK:
             raise ValueError(f"LoRA rank must be {RANK}")
         params += [pr.bias, pr.lora_a, pr.lora_b]
-    return NF4LinearGroup.apply(x, list(projections), *params)
+    return (NF4LinearGroupAct8 if keep8 else NF4LinearGroup).apply(x, list(projections), *params)

@@ -16,6 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .act8 import Act8, act8_quantize, lora_grad_act8
 from .nf4 import _rows_view, _stream_ptr, linear_backward_dx, linear_forward
 
 RANK = 16
@@ -126,10 +127,11 @@ def lora_grad_batch(zs, ss, rank_major_outs, flat=None):
 
 class NF4LoRALinear(torch.autograd.Function):
     """Frozen NF4 base weight + trainable rank-16 A, B. `x_lora` is the input of the LoRA branch:
-    pass `x` itself when there is no dropout (then the input gradient is one fused GEMM)."""
+    pass `x` itself when there is no dropout (then the input gradient is one fused GEMM). `keep8`: what the
+    gradient of A reads of `x_lora` is kept in 8 bits (act8.py)."""
 
     @staticmethod
-    def forward(ctx, x, x_lora, packed, bias, state, lora_a, lora_b, scaling):
+    def forward(ctx, x, x_lora, packed, bias, state, lora_a, lora_b, scaling, keep8=False):
         same = x_lora is x or (x_lora.data_ptr() == x.data_ptr() and x_lora.shape == x.shape
                                and x_lora.stride() == x.stride())
         if x_lora.numel() != x.numel():
@@ -140,20 +142,28 @@ class NF4LoRALinear(torch.autograd.Function):
         y = linear_forward(x, packed, bias, state, xa=xa, lora_b=b16)
         ctx.packed, ctx.state, ctx.scaling, ctx.same = packed, state, float(scaling), same
         ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.kept8 = None
         if b16t is not None:
-            ctx.save_for_backward(x_lora, xa, lora_a, lora_b, a16, b16t)
+            kept = [x_lora]
+            if keep8:
+                kept = []
+                if ctx.needs_input_grad[5]:
+                    q = act8_quantize(x_lora)
+                    kept, ctx.kept8 = [q.codes, q.steps], (q.shape, q.dtype)
+            ctx.x_shape = x_lora.shape
+            ctx.save_for_backward(*kept, xa, lora_a, lora_b, a16, b16t)
         return y
 
     @staticmethod
     def backward(ctx, grad_output):
-        x_lora, xa, lora_a, lora_b, a16, b16t = ctx.saved_tensors
+        *kept, xa, lora_a, lora_b, a16, b16t = ctx.saved_tensors
         need_x, need_xl = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         need_a, need_b = ctx.needs_input_grad[5], ctx.needs_input_grad[6]
         grad_x = grad_xl = grad_bias = grad_a = grad_b = None
         u = None
         jobs = []   # (z, s, rank-major output): the two factors' gradients in one launch
-        if need_a:
-            jobs.append((x_lora, None, True))
+        if need_a and ctx.kept8 is None:
+            jobs.append((kept[0], None, True))
         if need_b:
             jobs.append((grad_output, xa, False))
         flat = grad_buffer(jobs, grad_output.device) if jobs else None
@@ -168,21 +178,24 @@ class NF4LoRALinear(torch.autograd.Function):
             if need_x:
                 grad_x = linear_backward_dx(grad_output, ctx.packed, ctx.state)
             if need_xl:  # the dropout branch keeps its own gradient: u . A
-                grad_xl = (u.reshape(-1, RANK) @ a16).reshape(x_lora.shape)
+                grad_xl = (u.reshape(-1, RANK) @ a16).reshape(ctx.x_shape)
         if jobs:
             res = lora_grad_batch([j[0] for j in jobs], [u if j[1] is None else j[1] for j in jobs],
                                   [j[2] for j in jobs], flat)
-            if need_a:
+            if need_a and ctx.kept8 is None:
                 grad_a = res[0].to(lora_a.dtype)
             if need_b:
                 grad_b = res[-1].to(lora_b.dtype)
+        if need_a and ctx.kept8 is not None:
+            grad_a = lora_grad_act8(Act8(*kept, *ctx.kept8), u).to(lora_a.dtype)
         if ctx.needs_input_grad[3]:
             grad_bias = grad_output.reshape(-1, grad_output.shape[-1]).sum(0, dtype=ctx.bias_dtype)
-        return grad_x, grad_xl, None, grad_bias, None, grad_a, grad_b, None
+        return grad_x, grad_xl, None, grad_bias, None, grad_a, grad_b, None, None
 
 
-def nf4_lora_linear(x, packed, bias, state, lora_a, lora_b, scaling, x_lora=None):
-    """y = x . Wᵀ + bias + scaling * (x_lora . Aᵀ) . Bᵀ; x_lora defaults to x."""
+def nf4_lora_linear(x, packed, bias, state, lora_a, lora_b, scaling, x_lora=None, keep8=False):
+    """y = x . Wᵀ + bias + scaling * (x_lora . Aᵀ) . Bᵀ; x_lora defaults to x. With `keep8`, x_lora is kept in 8
+    bits for the gradient of A (act8.py)."""
     if x_lora is None:
         x_lora = x
-    return NF4LoRALinear.apply(x, x_lora, packed.reshape(-1), bias, state, lora_a, lora_b, scaling)
+    return NF4LoRALinear.apply(x, x_lora, packed.reshape(-1), bias, state, lora_a, lora_b, scaling, bool(keep8))

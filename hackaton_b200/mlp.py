@@ -19,8 +19,9 @@ import ctypes
 import torch
 
 from . import _lib
+from .act8 import _rows as _act8_rows, act8_quantize
 from .group import Projection, _refs, linear_backward_dx_group
-from .nf4 import _rows_view, _stream_ptr, scratch
+from .nf4 import _rows_view, _stream_ptr, linear_backward_dx, scratch
 
 
 def swiglu_forward(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -71,8 +72,26 @@ class SiluMul(torch.autograd.Function):
         return swiglu_backward(d_hidden, gate, up)
 
 
-def silu_mul(gate, up):
-    """solution/kernels.py:94-96."""
+class SiluMulAct8(torch.autograd.Function):
+    """silu(gate) * up; keeps gate and up in 8 bits (act8.py), written in the pass that forms the product."""
+
+    @staticmethod
+    def forward(ctx, gate, up):
+        _check_pair(gate, up)
+        hidden, *kept = _lib.host().act8_swiglu_fwd(_act8_rows(gate), _act8_rows(up))
+        ctx.save_for_backward(*kept)
+        return hidden.reshape(gate.shape)
+
+    @staticmethod
+    def backward(ctx, d_hidden):
+        d_gate, d_up = _lib.host().act8_swiglu_bwd(_act8_rows(d_hidden), *ctx.saved_tensors)
+        return d_gate.reshape(d_hidden.shape), d_up.reshape(d_hidden.shape)
+
+
+def silu_mul(gate, up, keep8=False):
+    """solution/kernels.py:94-96. With `keep8`, gate and up are kept in 8 bits for the backward (act8.py)."""
+    if keep8 and torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+        return SiluMulAct8.apply(gate, up)
     return SiluMul.apply(gate, up)
 
 
@@ -153,51 +172,62 @@ def linear_backward_dx_swiglu(grad_out, down_w, gate, up):
 class NF4SwiGLUMLP(torch.autograd.Function):
     """y = (silu(x . Wgᵀ) * (x . Wuᵀ)) . Wdᵀ on three frozen NF4 weights: two kernels forward
     (gate/up/product, down), two backward (down's dX with the SwiGLU backward in its epilogue,
-    then the grouped dX of gate and up). Keeps gate and up for the backward, not the product."""
+    then the grouped dX of gate and up). Keeps gate and up for the backward, not the product. With
+    `keep8` it keeps them in 8 bits: two more kernels forward, and down's dX and the SwiGLU backward apart."""
 
     @staticmethod
-    def forward(ctx, x, gate_w, up_w, down_w):
+    def forward(ctx, x, gate_w, up_w, down_w, keep8=False):
         from .nf4 import linear_forward
         keep = ctx.needs_input_grad[0]
         hidden, gate, up = gate_up_swiglu_forward(x, gate_w, up_w, keep)
         y = linear_forward(hidden, down_w[0], None, down_w[1])
         if keep:
-            ctx.save_for_backward(gate, up)
-            ctx.weights = (gate_w, up_w, down_w)
+            if keep8:
+                kept = [act8_quantize(t) for t in (gate, up)]
+                ctx.save_for_backward(*[t for k in kept for t in (k.codes, k.steps)])
+            else:
+                ctx.save_for_backward(gate, up)
+            ctx.weights, ctx.keep8 = (gate_w, up_w, down_w), keep8
         return y
 
     @staticmethod
     def backward(ctx, grad_out):
-        gate, up = ctx.saved_tensors
         gate_w, up_w, down_w = ctx.weights
-        d_gate, d_up = linear_backward_dx_swiglu(grad_out.contiguous(), down_w, gate, up)
+        if ctx.keep8:
+            d_hidden = linear_backward_dx(grad_out.contiguous(), *down_w)
+            grads = _lib.host().act8_swiglu_bwd(_act8_rows(d_hidden), *ctx.saved_tensors)
+            d_gate, d_up = (g.reshape(d_hidden.shape) for g in grads)
+        else:
+            gate, up = ctx.saved_tensors
+            d_gate, d_up = linear_backward_dx_swiglu(grad_out.contiguous(), down_w, gate, up)
         dx = linear_backward_dx_group([d_gate, d_up], [gate_w, up_w])
-        return dx, None, None, None
+        return dx, None, None, None, None
 
 
-def nf4_swiglu_mlp(x, gate_proj: Projection, up_proj: Projection, down_proj: Projection):
+def nf4_swiglu_mlp(x, gate_proj: Projection, up_proj: Projection, down_proj: Projection, keep8=False):
     """The whole SwiGLU MLP of a Qwen2 block (solution/patches.py:32-41) on NF4 weights without
     bias or LoRA pairs; other configurations go through `nf4_gate_up_swiglu` and the ordinary
-    linear."""
+    linear. With `keep8`, gate, up and the inputs of LoRA projections are kept in 8 bits for the backward (act8.py)."""
     projs = (gate_proj, up_proj, down_proj)
     if all(p.bias is None and p.lora_a is None and p.lora_b is None for p in projs):
-        return NF4SwiGLUMLP.apply(x, *[(p.packed, p.state) for p in projs])
+        return NF4SwiGLUMLP.apply(x, *[(p.packed, p.state) for p in projs], bool(keep8))
     from .lora import nf4_lora_linear
     from .nf4 import nf4_linear
-    hidden = nf4_gate_up_swiglu(x, gate_proj, up_proj)
+    hidden = nf4_gate_up_swiglu(x, gate_proj, up_proj, keep8)
     d = down_proj
     if d.lora_a is not None:
-        return nf4_lora_linear(hidden, d.packed, d.bias, d.state, d.lora_a, d.lora_b, d.scaling)
+        return nf4_lora_linear(hidden, d.packed, d.bias, d.state, d.lora_a, d.lora_b, d.scaling, keep8=keep8)
     return nf4_linear(hidden, d.packed, d.bias, d.state)
 
 
-def nf4_gate_up_swiglu(x, gate_proj: Projection, up_proj: Projection):
+def nf4_gate_up_swiglu(x, gate_proj: Projection, up_proj: Projection, keep8=False):
     """The front half of a SwiGLU MLP on NF4 weights. Projections with a bias or a LoRA pair are
-    not covered by the fused kernel: they take the grouped launch followed by `silu_mul`."""
+    not covered by the fused kernel: they take the grouped launch followed by `silu_mul`; so does `keep8` (gate,
+    up and the LoRA pairs' input kept in 8 bits for the backward)."""
     plain = all(p.bias is None and p.lora_a is None and p.lora_b is None for p in (gate_proj, up_proj))
-    if not plain:
+    if not plain or (keep8 and torch.is_grad_enabled() and x.requires_grad):
         from .group import nf4_linear_group
-        gate, up = nf4_linear_group(x, [gate_proj, up_proj])
-        return silu_mul(gate, up)
+        gate, up = nf4_linear_group(x, [gate_proj, up_proj], keep8)
+        return silu_mul(gate, up, keep8)
     return NF4GateUpSwiGLU.apply(x, (gate_proj.packed, gate_proj.state),
                                  (up_proj.packed, up_proj.state))

@@ -247,6 +247,52 @@ int nf4b200_gate_up_swiglu_fwd(const nf4b200_weight* gate_w, const nf4b200_weigh
                                void* hidden, void* workspace, size_t workspace_bytes, void* stream);
 int64_t nf4b200_gate_up_swiglu_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t m, int keep);
 /*
+ * Activations kept in 8 bits for the backward pass. 32 consecutive values of a row share one power of two as
+ * their step: step 2^e with e = floor(log2 max|x|) - 6 (at least -126), code rint(x / 2^e) within -127 .. 127. Codes
+ * int8 [rows, 32 * blocks], blocks = ceil(cols / 32), the last block of a row filled up with zeros; steps uint8
+ * [rows, blocks] = e + 127, 255 for a block that held an infinity or a NaN and is read back as NaN.
+ * nf4b200_act8_quantize / _dequantize: a contiguous [rows, cols] tensor of `dtype` (NF4B200_F16, _BF16 or _F32).
+ * nf4b200_act8_swiglu_fwd: hidden = silu(gate) * up (fp16, from the values as given) and both operands' codes and
+ *   steps in the same pass; nf4b200_act8_swiglu_bwd: nf4b200_swiglu_bwd from those.
+ * nf4b200_act8_lora_grad: out[r, k] = sum over rows of s[row, r] * x[row, k] (fp32 [16, cols], overwritten) for an
+ *   input that was kept in 8 bits from fp16, s fp16 [rows, 16]. Scratch as _workspace_bytes says; the sums are made
+ *   in a fixed order. Codes and scratch 16-byte aligned.
+ * No counterpart in the reference, which moves such tensors to host memory instead (solution/kernels.py:60-91).
+ */
+int nf4b200_act8_quantize(const void* x, int dtype, void* codes, void* steps, int64_t rows, int64_t cols, void* stream);
+int nf4b200_act8_dequantize(const void* codes, const void* steps, void* x, int dtype, int64_t rows, int64_t cols,
+                            void* stream);
+int nf4b200_act8_swiglu_fwd(const void* gate, const void* up, void* hidden, void* gate_codes, void* gate_steps,
+                            void* up_codes, void* up_steps, int64_t rows, int64_t cols, void* stream);
+int nf4b200_act8_swiglu_bwd(const void* d_hidden, const void* gate_codes, const void* gate_steps, const void* up_codes,
+                            const void* up_steps, void* d_gate, void* d_up, int64_t rows, int64_t cols, void* stream);
+int64_t nf4b200_act8_lora_grad_workspace_bytes(int64_t rows, int64_t cols);
+int nf4b200_act8_lora_grad(const void* codes, const void* steps, const void* s, void* out, int64_t rows, int64_t cols,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The norm behind a block, its gate, the scaled residual and the norm before the next block:
+ *   n = delta * rsqrt(mean(delta^2) + eps) * post;  stream = scale * residual + gate * n
+ *   normed = stream * rsqrt(mean(stream^2) + eps) * pre
+ * residual, stream fp32 and delta of delta_dtype [rows, hidden]; post, pre fp32 [hidden]; gate fp32 [gates, hidden]
+ * or NULL with gates = 0: gate row g serves rows g * rows / gates onwards (gates divides rows). normed is of
+ * normed_dtype: delta's, or NF4B200_F32. hidden up to 16384. rstd [rows, 2] fp32 is what the backward needs, or NULL.
+ * Backward: d_stream (fp32, or NULL) is the gradient that reaches the stream directly, d_normed of normed_dtype;
+ * d_residual fp32, d_delta, d_post, d_pre and d_gate ([gates, hidden]) may each be NULL. Scratch as
+ * _workspace_bytes says, 16-byte aligned; the weights' sums are made in a fixed order. The reference has the pre-norm
+ * alone (solution/rmsnorm.py:17-49).
+ */
+int nf4b200_sandwich_norm_fwd(const void* residual, const void* delta, int delta_dtype, const void* post, const void* pre,
+                              const void* gate, int64_t gates, void* stream_out, void* normed, int normed_dtype, void* rstd,
+                              int64_t rows, int64_t hidden, float scale, float eps, void* stream);
+int64_t nf4b200_sandwich_norm_workspace_bytes(int64_t rows, int64_t hidden, int64_t gates);
+int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delta_dtype, const void* post, const void* pre,
+                              const void* gate, int64_t gates, const void* rstd, const void* d_stream, const void* d_normed,
+                              int normed_dtype, void* d_residual, void* d_delta, void* d_post, void* d_pre, void* d_gate,
+                              int64_t rows, int64_t hidden, float scale, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/*
  * Backward of the projection that consumes the product (down_proj: d_hidden = dy . W_down) with the
  * SwiGLU backward applied to every tile as it is drained: d_gate and d_up ([m, n_cols], no
  * padding) are written instead of d_hidden, from the gate / up arrays the forward kept. One
