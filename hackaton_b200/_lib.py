@@ -26,6 +26,8 @@ EXPORTS = (
     "nf4b200_act8_quantize", "nf4b200_act8_dequantize", "nf4b200_act8_swiglu_fwd", "nf4b200_act8_swiglu_bwd",
     "nf4b200_act8_lora_grad", "nf4b200_act8_lora_grad_workspace_bytes", "nf4b200_sandwich_norm_fwd",
     "nf4b200_sandwich_norm_bwd", "nf4b200_sandwich_norm_workspace_bytes",
+    "nf4b200_vocab_loss_fwd", "nf4b200_vocab_loss_bwd", "nf4b200_vocab_loss_kept_bytes",
+    "nf4b200_vocab_loss_workspace_bytes",
     "nf4b200_qkv_rotate", "nf4b200_ce_stats", "nf4b200_ce_grad", "nf4b200_selftest_wait", "nf4b200_fp16_linear",
 )
 
@@ -149,9 +151,18 @@ def lib() -> ctypes.CDLL:
                                                      c_int64, c_int64, c_float, c_void_p, c_size_t, c_void_p]
     handle.nf4b200_sandwich_norm_workspace_bytes.argtypes = [c_int64, c_int64, c_int64]
     handle.nf4b200_sandwich_norm_workspace_bytes.restype = c_int64
+    handle.nf4b200_vocab_loss_kept_bytes.argtypes = [c_int64, c_int64]
+    handle.nf4b200_vocab_loss_kept_bytes.restype = c_int64
+    handle.nf4b200_vocab_loss_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
+    handle.nf4b200_vocab_loss_workspace_bytes.restype = c_int64
+    handle.nf4b200_vocab_loss_fwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                              c_int64, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
+    handle.nf4b200_vocab_loss_bwd.argtypes = [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                              c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
     for name in EXPORTS:
         if name not in ("nf4b200_last_error", "nf4b200_workspace_bytes",
                         "nf4b200_workspace_bytes_group", "nf4b200_scales16_bytes",
+                        "nf4b200_vocab_loss_kept_bytes", "nf4b200_vocab_loss_workspace_bytes",
                         "nf4b200_act8_lora_grad_workspace_bytes", "nf4b200_sandwich_norm_workspace_bytes",
                         "nf4b200_gate_up_swiglu_workspace_bytes",
                         "nf4b200_linear_bwd_dx_swiglu_workspace_bytes"):

@@ -20,7 +20,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libnf4b200.so"
 HOST = PKG / "_host.so"
-SOURCES = ["act8.cu", "capi.cu", "cross_entropy.cu", "dequant.cu", "gemm.cu", "gemv.cu", "lora.cu", "rmsnorm.cu", "rope.cu", "sandwich.cu", "selftest.cu", "static_scratch.cu", "swiglu.cu"]
+SOURCES = ["act8.cu", "capi.cu", "cross_entropy.cu", "dequant.cu", "gemm.cu", "gemv.cu", "lora.cu", "rmsnorm.cu", "rope.cu", "sandwich.cu", "selftest.cu", "static_scratch.cu", "swiglu.cu", "vocab_loss.cu"]
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",

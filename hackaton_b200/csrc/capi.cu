@@ -1020,6 +1020,93 @@ int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delt
     return NF4B200_OK;
 }
 
+static int vocab_loss_check(const char* what, int64_t rows, int64_t vocab, int64_t hidden) {
+    // (tile counts, coordinates and a slice's step count are 32-bit)
+    if (rows < 0 || rows > 0x7FFFFF00 / 4 || vocab <= 0 || vocab > 0x7FFFFF00 / 4 || hidden <= 0 || hidden > 65536 ||
+        ((rows + 255) / 256) * ((vocab + 255) / 256) > 0x7FFFFFFF)
+        return fail(NF4B200_EINVAL, "%s: bad shape (%lld rows, %lld words, %lld features)", what, (long long)rows,
+                    (long long)vocab, (long long)hidden);
+    if (hidden % 8 != 0) return fail(NF4B200_EINVAL, "%s: %lld features are not a multiple of 8", what, (long long)hidden);
+    return NF4B200_OK;
+}
+
+static int vocab_loss_weight(const char* what, const void* weight, int64_t ld_w, int64_t hidden, int dtype) {
+    if (dtype != NF4B200_F16 && dtype != NF4B200_BF16) return fail(NF4B200_EINVAL, "%s: dtype %d", what, dtype);
+    if (!weight || !aligned16(weight) || ld_w < hidden || ld_w % 8 != 0)
+        return fail(NF4B200_EINVAL, "%s: weight is NULL, not 16-byte aligned or has a row pitch that is no multiple of 8", what);
+    return NF4B200_OK;
+}
+
+int64_t nf4b200_vocab_loss_kept_bytes(int64_t rows, int64_t hidden) {
+    const int rc = vocab_loss_check("vocab_loss_kept_bytes", rows, 1, hidden);
+    return rc != NF4B200_OK ? rc : (int64_t)nf4::vocab_loss_kept_bytes(rows, hidden);
+}
+
+int64_t nf4b200_vocab_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int backward) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = vocab_loss_check("vocab_loss_workspace_bytes", rows, vocab, hidden);
+    if (rc != NF4B200_OK) return rc;
+    if (rows == 0) return 0;
+    nf4::VocabLossArgs a = {};
+    a.rows = rows; a.vocab = vocab; a.hidden = hidden; a.sm_count = gemm_sms(d);
+    a.d_x = (backward & 1) ? &a : nullptr;            // (only whether they are there)
+    a.d_weight = (backward & 2) ? &a : nullptr;
+    return (int64_t)nf4::vocab_loss_workspace_bytes(a, backward != 0);
+}
+
+int nf4b200_vocab_loss_fwd(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, int dtype, const void* targets,
+                           void* losses, void* lse, int64_t rows, int64_t vocab, int64_t hidden, void* kept,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = vocab_loss_check("vocab_loss_fwd", rows, vocab, hidden);
+    if (rc == NF4B200_OK) rc = vocab_loss_weight("vocab_loss_fwd", weight, ld_w, hidden, dtype);
+    if (rc != NF4B200_OK || rows == 0) return rc;
+    if (!x || !targets || !losses || !lse || !kept || !workspace) return fail(NF4B200_EINVAL, "vocab_loss_fwd: NULL argument");
+    if (!aligned16(x) || ld_x < hidden || ld_x % 8 != 0)
+        return fail(NF4B200_EINVAL, "vocab_loss_fwd: x is not 16-byte aligned or has a row pitch that is no multiple of 8");
+    nf4::VocabLossArgs a = {};
+    a.x = x; a.ld_x = ld_x; a.weight = weight; a.ld_w = ld_w; a.bf16 = dtype == NF4B200_BF16;
+    a.targets = static_cast<const long long*>(targets);
+    a.losses = static_cast<float*>(losses); a.lse = static_cast<float*>(lse);
+    a.kept = kept; a.workspace = workspace; a.rows = rows; a.vocab = vocab; a.hidden = hidden;
+    a.sm_count = gemm_sms(d); a.status = nf4::device_status_word();
+    if (workspace_bytes < nf4::vocab_loss_workspace_bytes(a, false) ||
+        ((reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) & 255) != 0)
+        return fail(NF4B200_EINVAL, "vocab_loss_fwd: %zu bytes of scratch, or buffers that are not 256-byte aligned", workspace_bytes);
+    const char* why = "";
+    cudaError_t e = nf4::launch_vocab_loss_fwd(a, static_cast<cudaStream_t>(stream), &why);
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "vocab_loss_fwd (%s): %s", why, cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
+int nf4b200_vocab_loss_bwd(const void* weight, int64_t ld_w, int dtype, const void* d_losses, int64_t d_losses_stride,
+                           const void* d_lse, int64_t d_lse_stride, void* d_x, void* d_weight, int64_t rows, int64_t vocab,
+                           int64_t hidden, void* kept, void* workspace, size_t workspace_bytes, void* stream) {
+    DeviceInfo* d = nullptr;
+    int rc = require_sm100(&d);
+    if (rc == NF4B200_OK) rc = vocab_loss_check("vocab_loss_bwd", rows, vocab, hidden);
+    if (rc == NF4B200_OK) rc = vocab_loss_weight("vocab_loss_bwd", weight, ld_w, hidden, dtype);
+    if (rc != NF4B200_OK || rows == 0 || (!d_x && !d_weight)) return rc;
+    if (!kept || !workspace) return fail(NF4B200_EINVAL, "vocab_loss_bwd: NULL argument");
+    if (!aligned16(d_x) || !aligned16(d_weight)) return fail(NF4B200_EINVAL, "vocab_loss_bwd: gradients are not 16-byte aligned");
+    nf4::VocabLossArgs a = {};
+    a.weight = weight; a.ld_w = ld_w; a.bf16 = dtype == NF4B200_BF16;
+    a.d_losses = static_cast<const float*>(d_losses); a.d_losses_stride = d_losses_stride;
+    a.d_lse = static_cast<const float*>(d_lse); a.d_lse_stride = d_lse_stride;
+    a.d_x = d_x; a.d_weight = d_weight;
+    a.kept = kept; a.workspace = workspace; a.rows = rows; a.vocab = vocab; a.hidden = hidden;
+    a.sm_count = gemm_sms(d); a.status = nf4::device_status_word();
+    if (workspace_bytes < nf4::vocab_loss_workspace_bytes(a, true) ||
+        ((reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) & 255) != 0)
+        return fail(NF4B200_EINVAL, "vocab_loss_bwd: %zu bytes of scratch, or buffers that are not 256-byte aligned", workspace_bytes);
+    const char* why = "";
+    cudaError_t e = nf4::launch_vocab_loss_bwd(a, static_cast<cudaStream_t>(stream), &why);
+    if (e != cudaSuccess) return fail(NF4B200_ECUDA, "vocab_loss_bwd (%s): %s", why, cudaGetErrorString(e));
+    return NF4B200_OK;
+}
+
 int64_t nf4b200_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t m, int backward) {
     DeviceInfo* d = nullptr;
     int rc = require_sm100(&d);

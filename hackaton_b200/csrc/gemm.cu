@@ -1267,7 +1267,7 @@ static EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
-static bool make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner,
+bool make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner,
                         uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
                         CUtensorMapSwizzle swz) {
     EncodeTiledFn fn = encode_tiled_fn();

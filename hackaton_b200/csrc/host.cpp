@@ -419,6 +419,59 @@ std::vector<Opt> sandwich_bwd(const Tensor& s2, const Tensor& d2, const Tensor& 
     return g;
 }
 
+// Weight of the vocabulary loss as the kernels read it.
+Tensor head_view(const Tensor& w) {
+    if (w.stride(1) == 1 && w.stride(0) % 8 == 0 && w.stride(0) >= w.size(1) &&
+        (reinterpret_cast<uintptr_t>(w.const_data_ptr()) & 15) == 0)
+        return w;
+    return w.clone(at::MemoryFormat::Contiguous);
+}
+
+int64_t sized(int64_t bytes) {
+    if (bytes < 0) check((int)bytes);
+    return bytes;
+}
+
+// (losses, logsumexps, what the gradient needs)
+std::tuple<Tensor, Tensor, Tensor> vocab_loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& targets) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t hidden = weight.size(1), vocab = weight.size(0);
+    const Tensor x2 = rows_view(x, hidden), w = head_view(weight), t = targets.reshape({-1}).contiguous();
+    const int64_t rows = x2.size(0);
+    const auto options = x.options().dtype(at::kFloat).memory_format(c10::nullopt);
+    Tensor losses = at::empty({rows}, options), lse = at::empty({rows}, options);
+    Tensor kept = at::empty({sized(nf4b200_vocab_loss_kept_bytes(rows, hidden))}, options.dtype(at::kByte));
+    const int64_t need = sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, 0));
+    const Scratch ws(need, x2);
+    check(nf4b200_vocab_loss_fwd(x2.const_data_ptr(), x2.stride(0), w.const_data_ptr(), w.stride(0), type_code(x.scalar_type()),
+                                 t.const_data_ptr(), losses.data_ptr(), lse.data_ptr(), rows, vocab, hidden, kept.data_ptr(),
+                                 ws.get(), (size_t)need, stream_of(x)));
+    return {losses, lse, kept};
+}
+
+// (gradient of the hidden states [rows, hidden], of the weight), as far as they are wanted
+std::tuple<Opt, Opt> vocab_loss_bwd(const Tensor& weight, const Tensor& kept, const Opt& d_losses, const Opt& d_lse,
+                                    int64_t rows, bool want_x, bool want_weight) {
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const int64_t hidden = weight.size(1), vocab = weight.size(0);
+    const Tensor w = head_view(weight);
+    const auto options = weight.options().memory_format(c10::nullopt);
+    const auto flat = [](const Opt& g) { return g.has_value() ? Opt(g->reshape({-1}).to(at::kFloat)) : Opt(); };
+    const Opt dl = flat(d_losses), dz = flat(d_lse);
+    const bool none = rows == 0 || (!dl.has_value() && !dz.has_value());
+    Opt dx, dw;
+    if (want_x) dx = none ? at::zeros({rows, hidden}, options) : at::empty({rows, hidden}, options);
+    if (want_weight) dw = none ? at::zeros({vocab, hidden}, options) : at::empty({vocab, hidden}, options);
+    if (none || (!want_x && !want_weight)) return {dx, dw};
+    const int64_t need = sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, (want_x ? 1 : 0) | (want_weight ? 2 : 0)));
+    const Scratch ws(need, w);
+    const auto step = [](const Opt& g) { return g.has_value() && g->size(0) > 1 ? g->stride(0) : (int64_t)0; };
+    check(nf4b200_vocab_loss_bwd(w.const_data_ptr(), w.stride(0), type_code(w.scalar_type()), ptr(dl), step(dl), ptr(dz), step(dz),
+                                 dx.has_value() ? dx->data_ptr() : nullptr, dw.has_value() ? dw->data_ptr() : nullptr, rows,
+                                 vocab, hidden, const_cast<void*>(kept.const_data_ptr()), ws.get(), (size_t)need, stream_of(w)));
+    return {dx, dw};
+}
+
 struct Rotation {   // everything about one rotation that is not a tensor
     int64_t tokens, seq, heads, kv_heads, dim, batch_stride;
     bool padded, f32;
@@ -495,6 +548,8 @@ PYBIND11_MODULE(_host, m) {
     m.def("act8_lora_grad", &act8_lora_grad, unlocked());
     m.def("sandwich_fwd", &sandwich_fwd, unlocked());
     m.def("sandwich_bwd", &sandwich_bwd, unlocked());
+    m.def("vocab_loss_fwd", &vocab_loss_fwd, unlocked());
+    m.def("vocab_loss_bwd", &vocab_loss_bwd, unlocked());
     m.def("rotate_fwd", &rotate_fwd, unlocked());
     m.def("rotate_bwd", &rotate_bwd, unlocked());
 }

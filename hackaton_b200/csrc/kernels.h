@@ -30,6 +30,10 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// 2-D tensor map for TMA (gemm.cu); strides and base 16-byte aligned.
+bool make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
+                 uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz);
+
 struct DequantArgs {
     const void* codes;
     const void* absmax;
@@ -278,6 +282,48 @@ struct CeArgs {
     int* status;                 // device status word (a target beyond the vocabulary is recorded there)
 };
 cudaError_t launch_ce(const CeArgs& a, cudaStream_t stream);
+
+// Cross-entropy from the hidden states in pieces of the vocabulary (vocab_loss.cu).
+struct VocabLossArgs {
+    const void* x;               // forward: [rows, hidden] fp16 or bf16, row pitch ld_x
+    long long ld_x;
+    const void* weight;          // [vocab, hidden], the same type, row pitch ld_w
+    long long ld_w;
+    int bf16;
+    const long long* targets;    // forward: [rows], negative = the row takes no part
+    float* losses;               // forward: [rows]
+    float* lse;
+    const float* d_losses;       // backward: [rows] with a stride, or null
+    long long d_losses_stride;
+    const float* d_lse;
+    long long d_lse_stride;
+    void* d_x;                   // backward: [rows, hidden] contiguous, or null
+    void* d_weight;              // [vocab, hidden] contiguous, or null
+    void* kept;                  // what the forward leaves for the backward (vocab_loss_kept_bytes)
+    void* workspace;             // (vocab_loss_workspace_bytes)
+    long long rows, vocab, hidden;
+    int sm_count;
+    int* status;
+    // set by the launcher, parts of `kept` and `workspace`
+    long long rows_pad;
+    int* count;                  // rows that take part
+    int* place;                  // [rows]: where among them, or -1
+    int* target;                 // per such row
+    float* target_logit;
+    float* lse_rows;             // in the base-2 domain
+    float* rest;                 // 1 - p of the target
+    void* gathered;              // the rows themselves
+    float2* parts;
+    float2* loss_rows;
+    float4* coef;
+    float* scales;
+    void* scaled;
+    float* planes;
+};
+size_t vocab_loss_kept_bytes(long long rows, long long hidden);
+size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward);
+cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a, cudaStream_t stream, const char** why);
+cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a, cudaStream_t stream, const char** why);
 
 // Weight-streaming kernels for a handful of token rows (gemv.cu); launch_gemm* route eligible
 // calls to them: forward for M <= 64 (a whole group in one launch), backward for M <= 16.

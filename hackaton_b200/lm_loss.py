@@ -176,3 +176,50 @@ def linear_cross_entropy(hidden, weight, targets, denom):
     """(loss, per-row losses, entropy, argmax) of hidden @ weightᵀ against `targets`
     (solution/lm_loss.py:65-67)."""
     return call(_HeadAndLoss(), hidden.contiguous(), weight, targets, denom)
+
+
+class _VocabLoss:
+    """lm_head + loss in pieces of the vocabulary (csrc/vocab_loss.cu). Next to the weight it keeps the rows that
+    take part and four numbers for each."""
+
+    materialize = False
+
+    def run(self, keep, hidden, weight, targets):
+        losses, lse, kept = _lib.host().vocab_loss_fwd(hidden, weight, targets)
+        keep(weight, kept, shape=hidden.shape, rows=targets.numel())
+        return losses.reshape(targets.shape), lse.reshape(targets.shape)
+
+    def grad(self, kept, d_losses, d_lse):
+        weight, state = kept.tensors
+        d_hidden, d_weight = _lib.host().vocab_loss_bwd(weight, state, d_losses, d_lse, kept.rows, kept.wants[0],
+                                                        kept.wants[1])
+        return None if d_hidden is None else d_hidden.reshape(kept.shape), d_weight, None
+
+
+def vocab_cross_entropy(hidden, weight, targets):
+    """(losses, lse), both fp32 in the shape of `targets`: lse = logsumexp(hidden @ weightᵀ), loss = lse - the target's
+    logit, without keeping the logits. hidden [..., features] and weight [vocab, features] are both fp16 or both
+    bf16 with a multiple of 8 features; targets int64 [...]. Rows with a negative target (-100) take no part: their
+    loss and lse are 0, they get no gradient, and what they hold is not read, nor are operations spent on them. A
+    target beyond the vocabulary is treated the same and reported by `device_status`.
+
+    Both outputs are differentiable row by row, with respect to hidden and weight: sums, means, weights per token,
+    differences of sequences' log probabilities, and a penalty on lse are plain torch on top of them. Next to
+    `linear_cross_entropy` (fp16, frozen head, one loss with its gradient made in the forward) this one takes bf16, gives
+    the head's gradient and holds no block of logits."""
+    if not (hidden.is_cuda and weight.is_cuda and targets.is_cuda):
+        raise ValueError("hackaton_b200: vocab_cross_entropy needs CUDA tensors (there is no CPU path)")
+    if not hidden.device == weight.device == targets.device:
+        raise ValueError("hackaton_b200: vocab_cross_entropy: tensors on different devices")
+    if hidden.dtype != weight.dtype or hidden.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("hackaton_b200: vocab_cross_entropy computes on fp16 or bf16 tensors of one type, got "
+                        f"{hidden.dtype} and {weight.dtype}")
+    if targets.dtype != torch.int64:
+        raise TypeError("hackaton_b200: targets must be int64")
+    if weight.dim() != 2 or hidden.dim() == 0 or hidden.shape[-1] != weight.shape[1] or hidden.shape[:-1] != targets.shape:
+        raise ValueError(f"hackaton_b200: vocab_cross_entropy: hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}, "
+                         f"targets {tuple(targets.shape)}")
+    if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8 != 0:
+        raise ValueError(f"hackaton_b200: vocab_cross_entropy: {weight.shape[0]} words of {weight.shape[1]} features (a "
+                         "multiple of 8)")
+    return call(_VocabLoss(), hidden, weight, targets)

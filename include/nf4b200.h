@@ -293,6 +293,28 @@ int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delt
                               void* stream);
 
 /*
+ * Softmax cross-entropy over the vocabulary from the hidden states, in pieces of the vocabulary, without keeping the
+ * logits: losses[r] = lse[r] - x_r . w_target, lse[r] = log sum_v exp(x_r . w_v), both fp32. Rows whose target is
+ * negative take no part (loss = lse = 0, no gradient, never read); a target beyond the vocabulary is treated the same
+ * and recorded in the device status word (200). x [rows, hidden] and weight [vocab, hidden] are both NF4B200_F16 or both
+ * NF4B200_BF16, 16-byte aligned, row pitches and hidden multiples of 8; targets int64.
+ * Backward, from the gradients of losses and lse (fp32 with an element stride, 0 for one number; either may be NULL):
+ * d_x [rows, hidden] and d_weight [vocab, hidden] in x's type, contiguous, either may be NULL. `kept` is what the
+ * forward left (_kept_bytes), scratch as _workspace_bytes says (backward: 0 forward, 1 d_x, 2 d_weight, 3 both); both
+ * 256-byte aligned. No sum depends on timing.
+ * The reference walks the rows in chunks and holds a chunk's logits (solution/lm_loss.py:27-67), with no gradient of
+ * the weight.
+ */
+int64_t nf4b200_vocab_loss_kept_bytes(int64_t rows, int64_t hidden);
+int64_t nf4b200_vocab_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int backward);
+int nf4b200_vocab_loss_fwd(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, int dtype, const void* targets,
+                           void* losses, void* lse, int64_t rows, int64_t vocab, int64_t hidden, void* kept,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int nf4b200_vocab_loss_bwd(const void* weight, int64_t ld_w, int dtype, const void* d_losses, int64_t d_losses_stride,
+                           const void* d_lse, int64_t d_lse_stride, void* d_x, void* d_weight, int64_t rows, int64_t vocab,
+                           int64_t hidden, void* kept, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Backward of the projection that consumes the product (down_proj: d_hidden = dy . W_down) with the
  * SwiGLU backward applied to every tile as it is drained: d_gate and d_up ([m, n_cols], no
  * padding) are written instead of d_hidden, from the gate / up arrays the forward kept. One
