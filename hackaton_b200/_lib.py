@@ -151,14 +151,15 @@ def lib() -> ctypes.CDLL:
                                                      c_int64, c_int64, c_float, c_void_p, c_size_t, c_void_p]
     handle.nf4b200_sandwich_norm_workspace_bytes.argtypes = [c_int64, c_int64, c_int64]
     handle.nf4b200_sandwich_norm_workspace_bytes.restype = c_int64
-    handle.nf4b200_vocab_loss_kept_bytes.argtypes = [c_int64, c_int64]
+    handle.nf4b200_vocab_loss_kept_bytes.argtypes = [c_int64, c_int64, c_int]
     handle.nf4b200_vocab_loss_kept_bytes.restype = c_int64
-    handle.nf4b200_vocab_loss_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
+    handle.nf4b200_vocab_loss_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int, c_int]
     handle.nf4b200_vocab_loss_workspace_bytes.restype = c_int64
     handle.nf4b200_vocab_loss_fwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
-                                              c_int64, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
+                                              c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_size_t, c_void_p]
     handle.nf4b200_vocab_loss_bwd.argtypes = [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                                              c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
+                                              c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_size_t,
+                                              c_void_p]
     for name in EXPORTS:
         if name not in ("nf4b200_last_error", "nf4b200_workspace_bytes",
                         "nf4b200_workspace_bytes_group", "nf4b200_scales16_bytes",

@@ -1037,26 +1037,26 @@ static int vocab_loss_weight(const char* what, const void* weight, int64_t ld_w,
     return NF4B200_OK;
 }
 
-int64_t nf4b200_vocab_loss_kept_bytes(int64_t rows, int64_t hidden) {
+int64_t nf4b200_vocab_loss_kept_bytes(int64_t rows, int64_t hidden, int grads) {
     const int rc = vocab_loss_check("vocab_loss_kept_bytes", rows, 1, hidden);
-    return rc != NF4B200_OK ? rc : (int64_t)nf4::vocab_loss_kept_bytes(rows, hidden);
+    return rc != NF4B200_OK ? rc : (int64_t)nf4::vocab_loss_kept_bytes(rows, hidden, grads);
 }
 
-int64_t nf4b200_vocab_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int backward) {
+int64_t nf4b200_vocab_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int grads, int backward) {
     DeviceInfo* d = nullptr;
     int rc = require_sm100(&d);
     if (rc == NF4B200_OK) rc = vocab_loss_check("vocab_loss_workspace_bytes", rows, vocab, hidden);
     if (rc != NF4B200_OK) return rc;
     if (rows == 0) return 0;
     nf4::VocabLossArgs a = {};
-    a.rows = rows; a.vocab = vocab; a.hidden = hidden; a.sm_count = gemm_sms(d);
-    a.d_x = (backward & 1) ? &a : nullptr;            // (only whether they are there)
-    a.d_weight = (backward & 2) ? &a : nullptr;
+    a.rows = rows; a.vocab = vocab; a.hidden = hidden; a.sm_count = gemm_sms(d); a.grads = grads;
+    a.d_x = (grads & 1) ? &a : nullptr;            // (only whether they are there)
+    a.d_weight = (grads & 2) ? &a : nullptr;
     return (int64_t)nf4::vocab_loss_workspace_bytes(a, backward != 0);
 }
 
 int nf4b200_vocab_loss_fwd(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, int dtype, const void* targets,
-                           void* losses, void* lse, int64_t rows, int64_t vocab, int64_t hidden, void* kept,
+                           void* losses, void* lse, int64_t rows, int64_t vocab, int64_t hidden, int grads, void* kept,
                            void* workspace, size_t workspace_bytes, void* stream) {
     DeviceInfo* d = nullptr;
     int rc = require_sm100(&d);
@@ -1070,7 +1070,7 @@ int nf4b200_vocab_loss_fwd(const void* x, int64_t ld_x, const void* weight, int6
     a.x = x; a.ld_x = ld_x; a.weight = weight; a.ld_w = ld_w; a.bf16 = dtype == NF4B200_BF16;
     a.targets = static_cast<const long long*>(targets);
     a.losses = static_cast<float*>(losses); a.lse = static_cast<float*>(lse);
-    a.kept = kept; a.workspace = workspace; a.rows = rows; a.vocab = vocab; a.hidden = hidden;
+    a.grads = grads; a.kept = kept; a.workspace = workspace; a.rows = rows; a.vocab = vocab; a.hidden = hidden;
     a.sm_count = gemm_sms(d); a.status = nf4::device_status_word();
     if (workspace_bytes < nf4::vocab_loss_workspace_bytes(a, false) ||
         ((reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) & 255) != 0)
@@ -1083,20 +1083,22 @@ int nf4b200_vocab_loss_fwd(const void* x, int64_t ld_x, const void* weight, int6
 
 int nf4b200_vocab_loss_bwd(const void* weight, int64_t ld_w, int dtype, const void* d_losses, int64_t d_losses_stride,
                            const void* d_lse, int64_t d_lse_stride, void* d_x, void* d_weight, int64_t rows, int64_t vocab,
-                           int64_t hidden, void* kept, void* workspace, size_t workspace_bytes, void* stream) {
+                           int64_t hidden, int grads, void* kept, void* workspace, size_t workspace_bytes, void* stream) {
     DeviceInfo* d = nullptr;
     int rc = require_sm100(&d);
     if (rc == NF4B200_OK) rc = vocab_loss_check("vocab_loss_bwd", rows, vocab, hidden);
     if (rc == NF4B200_OK) rc = vocab_loss_weight("vocab_loss_bwd", weight, ld_w, hidden, dtype);
     if (rc != NF4B200_OK || rows == 0 || (!d_x && !d_weight)) return rc;
-    if (!kept || !workspace) return fail(NF4B200_EINVAL, "vocab_loss_bwd: NULL argument");
+    if (!kept || (d_weight && !workspace)) return fail(NF4B200_EINVAL, "vocab_loss_bwd: NULL argument");
+    if ((d_x && !(grads & 1)) || (d_weight && !(grads & 2)))
+        return fail(NF4B200_EINVAL, "vocab_loss_bwd: a gradient that the forward was not told of (%d)", grads);
     if (!aligned16(d_x) || !aligned16(d_weight)) return fail(NF4B200_EINVAL, "vocab_loss_bwd: gradients are not 16-byte aligned");
     nf4::VocabLossArgs a = {};
     a.weight = weight; a.ld_w = ld_w; a.bf16 = dtype == NF4B200_BF16;
     a.d_losses = static_cast<const float*>(d_losses); a.d_losses_stride = d_losses_stride;
     a.d_lse = static_cast<const float*>(d_lse); a.d_lse_stride = d_lse_stride;
     a.d_x = d_x; a.d_weight = d_weight;
-    a.kept = kept; a.workspace = workspace; a.rows = rows; a.vocab = vocab; a.hidden = hidden;
+    a.grads = grads; a.kept = kept; a.workspace = workspace; a.rows = rows; a.vocab = vocab; a.hidden = hidden;
     a.sm_count = gemm_sms(d); a.status = nf4::device_status_word();
     if (workspace_bytes < nf4::vocab_loss_workspace_bytes(a, true) ||
         ((reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) & 255) != 0)

@@ -433,25 +433,25 @@ int64_t sized(int64_t bytes) {
 }
 
 // (losses, logsumexps, what the gradient needs)
-std::tuple<Tensor, Tensor, Tensor> vocab_loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& targets) {
+std::tuple<Tensor, Tensor, Tensor> vocab_loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t grads) {
     const c10::cuda::CUDAGuard guard(x.device());
     const int64_t hidden = weight.size(1), vocab = weight.size(0);
     const Tensor x2 = rows_view(x, hidden), w = head_view(weight), t = targets.reshape({-1}).contiguous();
     const int64_t rows = x2.size(0);
     const auto options = x.options().dtype(at::kFloat).memory_format(c10::nullopt);
     Tensor losses = at::empty({rows}, options), lse = at::empty({rows}, options);
-    Tensor kept = at::empty({sized(nf4b200_vocab_loss_kept_bytes(rows, hidden))}, options.dtype(at::kByte));
-    const int64_t need = sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, 0));
+    Tensor kept = at::empty({sized(nf4b200_vocab_loss_kept_bytes(rows, hidden, (int)grads))}, options.dtype(at::kByte));
+    const int64_t need = sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, (int)grads, 0));
     const Scratch ws(need, x2);
     check(nf4b200_vocab_loss_fwd(x2.const_data_ptr(), x2.stride(0), w.const_data_ptr(), w.stride(0), type_code(x.scalar_type()),
-                                 t.const_data_ptr(), losses.data_ptr(), lse.data_ptr(), rows, vocab, hidden, kept.data_ptr(),
+                                 t.const_data_ptr(), losses.data_ptr(), lse.data_ptr(), rows, vocab, hidden, (int)grads, kept.data_ptr(),
                                  ws.get(), (size_t)need, stream_of(x)));
     return {losses, lse, kept};
 }
 
 // (gradient of the hidden states [rows, hidden], of the weight), as far as they are wanted
 std::tuple<Opt, Opt> vocab_loss_bwd(const Tensor& weight, const Tensor& kept, const Opt& d_losses, const Opt& d_lse,
-                                    int64_t rows, bool want_x, bool want_weight) {
+                                    int64_t rows, int64_t grads, bool want_x, bool want_weight) {
     const c10::cuda::CUDAGuard guard(weight.device());
     const int64_t hidden = weight.size(1), vocab = weight.size(0);
     const Tensor w = head_view(weight);
@@ -463,12 +463,12 @@ std::tuple<Opt, Opt> vocab_loss_bwd(const Tensor& weight, const Tensor& kept, co
     if (want_x) dx = none ? at::zeros({rows, hidden}, options) : at::empty({rows, hidden}, options);
     if (want_weight) dw = none ? at::zeros({vocab, hidden}, options) : at::empty({vocab, hidden}, options);
     if (none || (!want_x && !want_weight)) return {dx, dw};
-    const int64_t need = sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, (want_x ? 1 : 0) | (want_weight ? 2 : 0)));
+    const int64_t need = want_weight ? sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, (int)grads, 1)) : 0;
     const Scratch ws(need, w);
     const auto step = [](const Opt& g) { return g.has_value() && g->size(0) > 1 ? g->stride(0) : (int64_t)0; };
     check(nf4b200_vocab_loss_bwd(w.const_data_ptr(), w.stride(0), type_code(w.scalar_type()), ptr(dl), step(dl), ptr(dz), step(dz),
                                  dx.has_value() ? dx->data_ptr() : nullptr, dw.has_value() ? dw->data_ptr() : nullptr, rows,
-                                 vocab, hidden, const_cast<void*>(kept.const_data_ptr()), ws.get(), (size_t)need, stream_of(w)));
+                                 vocab, hidden, (int)grads, const_cast<void*>(kept.const_data_ptr()), ws.get(), (size_t)need, stream_of(w)));
     return {dx, dw};
 }
 

@@ -299,6 +299,7 @@ struct VocabLossArgs {
     long long d_lse_stride;
     void* d_x;                   // backward: [rows, hidden] contiguous, or null
     void* d_weight;              // [vocab, hidden] contiguous, or null
+    int grads;                   // what the backward will be asked for: 1 of x, 2 of the weight, 3 both, 0 none
     void* kept;                  // what the forward leaves for the backward (vocab_loss_kept_bytes)
     void* workspace;             // (vocab_loss_workspace_bytes)
     long long rows, vocab, hidden;
@@ -308,19 +309,25 @@ struct VocabLossArgs {
     long long rows_pad;
     int* count;                  // rows that take part
     int* place;                  // [rows]: where among them, or -1
-    int* target;                 // per such row
+    int* source;                 // per such row: whose it is
+    int* target;
     float* target_logit;
     float* lse_rows;             // in the base-2 domain
     float* rest;                 // 1 - p of the target
+    float* norm;
     void* gathered;              // the rows themselves
+    float* mean;                 // [rows that take part, hidden]: sum of p_v w_v over v other than the target
     float2* parts;
-    float2* loss_rows;
-    float4* coef;
-    float* scales;
-    void* scaled;
+    float* refs;
+    int* flags;
+    long long n_flags;
+    void* piece;
+    int capacity, slots;
     float* planes;
+    float4* coef;
+    float* weight_scale;
 };
-size_t vocab_loss_kept_bytes(long long rows, long long hidden);
+size_t vocab_loss_kept_bytes(long long rows, long long hidden, int grads);
 size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward);
 cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a, cudaStream_t stream, const char** why);
 cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a, cudaStream_t stream, const char** why);

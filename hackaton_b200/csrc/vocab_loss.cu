@@ -1,21 +1,26 @@
 // Softmax cross-entropy over the vocabulary straight from the hidden states, in pieces of the vocabulary: the logits
-// l = h . w_v exist only in tensor memory, a tile at a time, and of their gradient there is one piece at a time.
+// l = h . w_v exist only in tensor memory, a tile at a time, and of the softmax there is one piece at a time.
 //   forward    lse = log sum_v exp(l_v),  loss = lse - l_t = log(1 + sum_{v != t} exp(l_v - l_t))
 //   backward   with b = d loss, c = d lse:  dl_v = (b + c) p_v - b [v = t];  dH = dl . W,  dW = dl^T . H
 // Rows whose target is negative take no part: the others are gathered first, everything behind that works on as many
 // rows as there are (the count stays on the device), and what an ignored row holds is never read.
 //
-// Four matrix products of 2 R V K operations each (R rows, V words, K features): the logits for the statistics,
-// once more for the gradient, then dH and dW. All run in one kernel, vl_gemm_kernel, in four modes that differ in
-// the operands' layouts and the epilogue; it is bound by the tensor cores. CTA pairs (tcgen05.mma.cta_group::2) own a
-// 256 x 256 tile, 128 rows by 256 columns of fp32 in each CTA's tensor memory, twice: while eight warps work on one
-// tile's values the next one is being multiplied. Operands come by TMA in 64-deep steps through a ring of six.
-//   statistics: a thread has a row's 128 columns; running maximum and sum of exponentials in the base-2 domain, the
-//     target left out, so that 1 - p_t and a loss near zero keep their digits; one pair of numbers per row and half
-//     tile goes out, which vl_merge_kernel joins in order. The target's own logit is a dot product in fp32 (vl_gather).
-//   gradient: dl in 16 bits, each row scaled by a power of two (exact) so that fp16 keeps small probabilities
-//   dH: fp32 planes, one per slice of the piece, added to from piece to piece; vl_hidden_kernel joins them in order
-//   dW: the rows of the piece, in 16 bits
+// dH is linear in two things that the forward knows up to a row's factors:
+//   dH = (b + c) U + (c p_t - b (1 - p_t)) w_t,   U = sum_{v != t} p_v w_v
+// so the forward forms U in the same sweep over the vocabulary as the statistics, two matrix products of 2 R V K
+// operations (R rows, V words, K features) instead of three: a piece's exponentials are taken relative to a reference
+// per row that is fixed before the sweep (from the first words and the target's own logit), and the sum's 1 / s comes
+// at the end. The target is left out of U and of the sums, so that 1 - p_t and a loss near zero keep their digits, and its
+// share is added in fp32. A row that meets a logit too far above its reference for the 16-bit type has its piece done
+// again with a new one (its sums so far scaled by a power of two); launches for that look at a flag and leave. dW needs
+// the final lse: the logits once more, in 16-bit dl this time, and one product.
+//
+// All products run in one kernel, vl_gemm_kernel, in modes that differ in the operands' layouts and the epilogue; it
+// is bound by the tensor cores. CTA pairs (tcgen05.mma.cta_group::2) own a 256 x 256 tile, 128 rows by 256 columns of
+// fp32 in each CTA's tensor memory, twice: while eight warps work on one tile's values the next one is being
+// multiplied. Operands come by TMA in 64-deep steps through a ring of six. The 16-bit piece is laid out in blocks of
+// [rows][64 words], which is how TMA reads it along either side, and its size is chosen on the device: whole waves of
+// tiles for the rows there are, within a buffer that stays in L2.
 // Nothing is added atomically: results do not depend on timing.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -31,6 +36,12 @@ constexpr float VL_LOG2E = 1.4426950408889634f;
 constexpr float VL_LN2 = 0.6931471805599453f;
 constexpr float VL_NEG = -1.0e30f;         // a finite "minus infinity"
 constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 2^13, down to 2^-24 / 2^13
+// A row's reference for its exponentials (base 2): the larger of the first words' maximum less VL_BELOW and the
+// target's logit less VL_BELOW_TARGET; fp16 takes what lies up to 2^15 above it, bf16 2^100.
+constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
+constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
+constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
+constexpr int VL_PIECE_UNITS = 512;        // tiles of 256 x 256 that a piece may have: 64 MiB
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
@@ -43,10 +54,11 @@ constexpr int VL_EPI_WARPS = 8;
 constexpr int VL_THREADS = 64 + VL_EPI_WARPS * 32;
 
 enum VlMode {
-    VL_STATS = 0,    // A = gathered rows [R, K], B = W [V, K]                  -> maximum and sum per row and half tile
-    VL_GRAD = 1,     // the same operands, one piece                            -> dl in 16 bits [R, piece]
-    VL_HIDDEN = 2,   // A = dl [R, piece], B = W rows of the piece, N along K   -> fp32 planes [slices][R, K]
-    VL_WEIGHT = 3    // A = dl^T, B = scaled rows [R, K], N along K             -> 16-bit rows of the piece [piece, K]
+    VL_STATS = 0,    // A = gathered rows [R, K], B = W [V, K]                -> maximum and sum per row and half tile
+    VL_SOFT = 1,     // the same operands, one piece                          -> exponentials in 16 bits, the same statistics
+    VL_GRAD = 2,     // the same                                              -> dl in 16 bits
+    VL_HIDDEN = 3,   // A = the piece [R, words], B = its rows of W, N along K   -> fp32 planes [slices][R, K]
+    VL_WEIGHT = 4    // A = the piece transposed, B = gathered rows, N along K   -> 16-bit dW rows of the piece
 };
 
 struct VlMaps {
@@ -56,34 +68,46 @@ struct VlMaps {
 struct VlParams {
     const int* count;        // rows that take part
     int* status;
-    int mode_bf16;
+    int bf16;
     int vocab, hidden;
-    int v0, piece;           // first word of the piece, its words (a multiple of 256 unless it is the last)
-    int n_tiles;             // tiles along the words (VL_STATS, VL_GRAD, VL_WEIGHT: as M) or features
-    int slots;               // pairs that the slices are planned for
-    // VL_STATS
-    float2* parts;           // [2 * n_tiles][rows_pad]
-    long long rows_pad;
+    int word_tiles;          // of the whole vocabulary (VL_STATS: of what is to be looked at)
+    int index;               // of the piece
+    int capacity;            // tiles that a piece may have
+    int slots;               // pairs that pieces and slices are planned for
     const int* target;       // per gathered row
+    // VL_STATS, VL_SOFT
+    float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum (relative to it; VL_SOFT: to the reference)
+    long long rows_pad;
+    // VL_SOFT, VL_HIDDEN
+    float* refs;             // [pieces + 1][rows_pad]: a row's reference before each piece and after the last
+    int* flags;              // [pieces][1 + row tiles]: whether any row, and which tiles' rows, need the piece again
+    int flags_pitch;
+    int again;               // VL_SOFT: this launch does flagged pieces again
     // VL_GRAD
     const float* lse2;
     const float* rest;       // 1 - p of the target
-    const float4* coef;      // (b + c, b, c, -) over the row's scale, times VL_P_SCALE
-    void* dl;
-    long long ld_dl;
+    const float4* coef;      // ((b + c), b, c) over the common power of two, times VL_P_SCALE
+    // VL_SOFT, VL_GRAD: the 16-bit piece, [block of 64 words][rows of the tiles][64]
+    void* piece;
     // VL_HIDDEN
-    float* planes;           // [slices][row tiles * 256][hidden]
-    int first;               // the piece that fills the planes
-    int first_steps;         // its steps, which decide on the slices
+    float* planes;           // [slices][rows of the tiles][hidden]
     // VL_WEIGHT
-    void* d_weight;
-    long long ld_dw;
+    void* d_weight;          // [vocab, hidden]
     const float* weight_scale;
 };
 
 __host__ __device__ inline int vl_div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Slices of a piece's words for dH: as many as keep the pairs busiest, with at least eight steps each; none is empty.
+// Tiles of words in a piece: what the buffer holds for so many row tiles, cut to whole waves of the pairs.
+__host__ __device__ inline int vl_piece_tiles(int row_tiles, int word_tiles, int capacity, int slots) {
+    int t = capacity / row_tiles;
+    if (t >= word_tiles) return word_tiles;
+    const int waves = row_tiles * t / slots;
+    if (waves > 0) t = waves * slots / row_tiles;
+    return t > 0 ? t : 1;
+}
+
+// Slices of a piece's words for U: as many as keep the pairs busiest, with at least eight steps each; none is empty.
 constexpr int VL_MAX_SLICES = 16;
 __host__ __device__ inline int vl_slices(int tiles, int steps, int slots) {
     int best = 1, best_cost = 0x7FFFFFFF;
@@ -110,29 +134,41 @@ __device__ __forceinline__ uint32_t vl_pack(float a, float b, int bf16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-struct VlPlan {      // what a mode's units are, from the device's row count
+struct VlPlan {      // what a launch's units are, from the device's row count
+    int rows, row_tiles, v0, tiles;            // first word and tiles of the piece
     int m_tiles, units, steps, slices, per_slice;
 };
 
 template <int MODE>
 __device__ __forceinline__ VlPlan vl_plan(const VlParams& p, int rows) {
     VlPlan w;
-    const int row_tiles = vl_div_up(rows, VL_TILE);
+    w.rows = rows;
+    w.row_tiles = vl_div_up(rows, VL_TILE);
     w.slices = 1;
+    const int feature_tiles = vl_div_up(p.hidden, VL_TILE);
+    w.v0 = 0;
+    w.tiles = p.word_tiles;
+    int first_tiles = p.word_tiles;
+    if (MODE != VL_STATS) {
+        first_tiles = vl_piece_tiles(max(w.row_tiles, 1), p.word_tiles, p.capacity, p.slots);
+        const int before = min((long long)first_tiles * p.index, (long long)p.word_tiles);
+        w.v0 = before * VL_TILE;
+        w.tiles = min(first_tiles, p.word_tiles - before);
+    }
     if (MODE == VL_WEIGHT) {
-        w.m_tiles = p.n_tiles;                                  // words of the piece
+        w.m_tiles = w.tiles;
         w.steps = vl_div_up(rows, VL_BK);
-        w.units = w.m_tiles * vl_div_up(p.hidden, VL_TILE);
+        w.units = w.tiles * feature_tiles;
     } else if (MODE == VL_HIDDEN) {
-        w.m_tiles = row_tiles;
-        w.steps = vl_div_up(p.piece, VL_BK);
-        const int tiles = row_tiles * vl_div_up(p.hidden, VL_TILE);
-        w.slices = rows > 0 ? vl_slices(tiles, p.first_steps, p.slots) : 1;
-        w.units = tiles * w.slices;
+        w.m_tiles = w.row_tiles;
+        w.steps = w.tiles * (VL_TILE / VL_BK);
+        const int tiles = w.row_tiles * feature_tiles;
+        if (rows > 0) w.slices = vl_slices(tiles, first_tiles * (VL_TILE / VL_BK), p.slots);
+        w.units = w.tiles > 0 ? tiles * w.slices : 0;
     } else {
-        w.m_tiles = row_tiles;
+        w.m_tiles = w.row_tiles;
         w.steps = vl_div_up(p.hidden, VL_BK);
-        w.units = row_tiles * p.n_tiles;
+        w.units = w.row_tiles * w.tiles;
     }
     w.per_slice = vl_div_up(w.steps, w.slices);
     return w;
@@ -162,6 +198,7 @@ template <int MODE>
 __global__ void __launch_bounds__(VL_THREADS, 1)
 vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
     constexpr bool A_MN = MODE == VL_WEIGHT, B_MN = MODE >= VL_HIDDEN;
+    constexpr bool A_PIECE = MODE >= VL_HIDDEN;      // A comes from the 16-bit piece
     extern __shared__ uint8_t vl_smem[];
     const uint32_t base = (smem_u32(vl_smem) + 1023u) & ~1023u;
     uint8_t* gen = vl_smem + (base - smem_u32(vl_smem));
@@ -177,6 +214,11 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+    const int* flags = p.flags + (long long)p.index * p.flags_pitch;
+    if (MODE == VL_SOFT && p.again) {     // nearly always there is nothing to do again
+        grid_dep_wait();
+        if (flags[0] == 0) return;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < VL_STAGES; ++s) {
@@ -208,6 +250,11 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     const uint32_t tmem = *tmem_slot;
     const int rows = *p.count;
     const VlPlan plan = vl_plan<MODE>(p, rows);
+    const int rows_dev = plan.row_tiles * VL_TILE;
+    // (what all roles leave out: slices that the last piece has no steps for, row tiles that need not be done again)
+    const auto skip = [&](const VlUnit& w) {
+        return w.steps <= 0 || (MODE == VL_SOFT && p.again && flags[1 + w.mt] == 0);
+    };
     int fail = 0;
 
     if (warp == 0) {
@@ -215,6 +262,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             uint32_t g = 0;
             for (int u = pair; u < plan.units && !fail; u += pairs) {
                 const VlUnit w = vl_unit<MODE>(u, plan);
+                if (skip(w)) continue;
                 for (int it = 0; it < w.steps; ++it, ++g) {
                     const int s = (int)(g % VL_STAGES);
                     const uint32_t ph = (g / VL_STAGES) & 1u;
@@ -224,18 +272,20 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                     const int k = (w.begin + it) * VL_BK;
                     const int am = w.mt * VL_TILE + (int)rank * 128, bn = w.nt * VL_TILE + (int)rank * 128;
                     mbar_arrive_expect_tx(landed, VL_STAGE_BYTES);
-                    if (A_MN) {     // (the piece's words as M: columns of dl)
-                        tma_load_2d(sa, &maps.a, am, k, landed);
-                        tma_load_2d(sa + 8192, &maps.a, am + 64, k, landed);
+                    if (A_MN) {             // words as M, rows as steps
+                        tma_load_2d(sa, &maps.a, 0, (am >> 6) * rows_dev + k, landed);
+                        tma_load_2d(sa + 8192, &maps.a, 0, ((am >> 6) + 1) * rows_dev + k, landed);
+                    } else if (A_PIECE) {   // rows as M, words as steps
+                        tma_load_2d(sa, &maps.a, 0, (k >> 6) * rows_dev + am, landed);
                     } else {
                         tma_load_2d(sa, &maps.a, k, am, landed);
                     }
                     if (B_MN) {     // VL_HIDDEN: rows of W from the piece's first word on; VL_WEIGHT: gathered rows
-                        const int y = MODE == VL_HIDDEN ? p.v0 + k : k;
+                        const int y = MODE == VL_HIDDEN ? plan.v0 + k : k;
                         tma_load_2d(sb, &maps.b, bn, y, landed);
                         tma_load_2d(sb + 8192, &maps.b, bn + 64, y, landed);
                     } else {
-                        tma_load_2d(sb, &maps.b, k, p.v0 + bn, landed);
+                        tma_load_2d(sb, &maps.b, k, plan.v0 + bn, landed);
                     }
                 }
             }
@@ -249,12 +299,12 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             constexpr uint64_t A_DESC = A_MN ? MN_MAJOR : K_MAJOR, B_DESC = B_MN ? MN_MAJOR : K_MAJOR;
             constexpr uint32_t A_STEP = (A_MN ? 16 * 128 : 32) >> 4, B_STEP = (B_MN ? 16 * 128 : 32) >> 4;
             const uint32_t idesc = make_idesc_f16(VL_TILE, A_MN ? 1u : 0u, B_MN ? 1u : 0u, VL_TILE) |
-                                   (p.mode_bf16 ? (1u << 7) | (1u << 10) : 0u);
+                                   (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
             const uint32_t base4 = (base & 0x3FFFFu) >> 4;
             uint32_t g = 0, n = 0;
             for (int u = pair; u < plan.units && !fail; u += pairs) {
                 const VlUnit w = vl_unit<MODE>(u, plan);
-                if (w.steps <= 0) continue;
+                if (skip(w)) continue;
                 const int b = (int)(n & 1u);
                 if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
                 tc_fence_after_sync();
@@ -279,6 +329,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             uint32_t g = 0;
             for (int u = pair; u < plan.units && !fail; u += pairs) {
                 const VlUnit w = vl_unit<MODE>(u, plan);
+                if (skip(w)) continue;
                 for (int it = 0; it < w.steps; ++it, ++g) {
                     const int s = (int)(g % VL_STAGES);
                     if (!mbar_wait(bar_landed(s), (g / VL_STAGES) & 1u, abort_flag)) { fail = 8; break; }
@@ -295,24 +346,46 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             const VlUnit w = vl_unit<MODE>(u, plan);
             const int row = w.mt * VL_TILE + (int)rank * 128 + q * 32 + lane;     // VL_WEIGHT: word of the piece
             const int col0 = w.nt * VL_TILE + half * 128;
-            if (w.steps <= 0) {
-                // no rows take part: the gradient of the head is zero (other modes have no units then)
-                if (MODE == VL_WEIGHT && p.v0 + row < p.vocab && row < p.piece)
+            if (MODE == VL_WEIGHT && plan.steps <= 0) {
+                // no row takes part: the gradient of the head is zero
+                if (plan.v0 + row < p.vocab)
                     for (int c = col0; c < col0 + 128 && c < p.hidden; ++c)
-                        static_cast<unsigned short*>(p.d_weight)[(long long)(p.v0 + row) * p.ld_dw + c] = 0;
+                        static_cast<unsigned short*>(p.d_weight)[(long long)(plan.v0 + row) * p.hidden + c] = 0;
+                continue;
+            }
+            const bool live = row < rows;
+            float scale = 1.f;
+            if (MODE == VL_HIDDEN && live && p.index > 0)
+                scale = exp2f(p.refs[p.index * p.rows_pad + row] - p.refs[(p.index + 1) * p.rows_pad + row]);
+            if (skip(w)) {
+                if (MODE == VL_HIDDEN && live && scale != 1.f) {     // nothing to add, but the reference has moved
+                    float* plane = p.planes + ((long long)w.slice * rows_dev + row) * p.hidden;
+                    for (int c = col0; c < col0 + 128 && c < p.hidden; ++c) plane[c] *= scale;
+                }
                 continue;
             }
             const int b = (int)(n & 1u);
             // what the values meet, asked for before the tile is complete
             int target = -1;
-            float lse2 = 0.f, rest = 0.f, scale = 1.f;
+            float lse2 = 0.f, rest = 0.f, ref = 0.f;
             float4 coef = make_float4(0.f, 0.f, 0.f, 0.f);
-            const bool live = row < rows;
-            if (MODE <= VL_GRAD && live) target = p.target[row] - p.v0 - col0;   // column of this thread's share
+            if (MODE <= VL_GRAD && live) target = p.target[row] - plan.v0 - col0;   // column of this thread's share
             if (MODE == VL_GRAD && live) {
                 lse2 = p.lse2[row];
                 rest = p.rest[row];
                 coef = p.coef[row];
+            }
+            if (MODE == VL_SOFT && live) {
+                ref = p.refs[p.index * p.rows_pad + row];
+                if (p.again) {
+                    // the piece's largest decides whether this row changes its reference (the sums are not read:
+                    // they may have overflowed, and other units replace them)
+                    float top = VL_NEG;
+                    for (int i = 0; i < 2 * plan.tiles; ++i)
+                        top = fmaxf(top, p.parts[(plan.v0 / VL_TILE * 2 + i) * p.rows_pad + row].x);
+                    if (top > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) ref = ceilf(top) - 6.f;
+                }
+                if (w.nt == 0 && half == 0) p.refs[(p.index + 1) * p.rows_pad + row] = ref;
             }
             if (MODE == VL_WEIGHT) scale = *p.weight_scale;
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
@@ -323,6 +396,15 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
             };
+            // 32 values of the row's part of the 16-bit piece (columns col0 + c ..)
+            auto store_piece = [&](const float (&v)[32], int c) {
+                uint4* out = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.piece) +
+                                                      ((long long)((col0 + c) >> 6) * rows_dev + row) * 64 + (c & 32));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    out[i] = make_uint4(vl_pack(v[8 * i], v[8 * i + 1], p.bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.bf16),
+                                        vl_pack(v[8 * i + 4], v[8 * i + 5], p.bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.bf16));
+            };
             float m2 = VL_NEG, sum = 0.f;
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
@@ -330,8 +412,8 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 tmem_ld_32x32(at + c, r);
                 tmem_ld_wait();
                 if (c == 96) release();
-                if (MODE == VL_STATS) {
-                    const int words = p.vocab - p.v0 - col0 - c;       // words there are in this chunk
+                if (MODE <= VL_SOFT) {
+                    const int words = p.vocab - plan.v0 - col0 - c;       // words there are in this chunk
                     const bool cut = words < 32 || (unsigned)(target - c) < 32u;
                     if (__any_sync(0xffffffffu, cut)) {
 #pragma unroll
@@ -342,16 +424,27 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
 #pragma unroll
                     for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
                     const float top2 = top * VL_LOG2E;
-                    if (top2 > m2) {
-                        sum *= vl_ex2(m2 - top2);
-                        m2 = top2;
-                    }
                     float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (MODE == VL_STATS) {
+                        if (top2 > m2) {
+                            sum *= vl_ex2(m2 - top2);
+                            m2 = top2;
+                        }
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) part[e & 3] += vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -m2));
+                        for (int e = 0; e < 32; ++e) part[e & 3] += vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -m2));
+                    } else {
+                        m2 = fmaxf(m2, top2);
+                        float v[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            v[e] = live ? vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -ref)) : 0.f;
+                            part[e & 3] += v[e];
+                        }
+                        store_piece(v, c);
+                    }
                     sum += (part[0] + part[1]) + (part[2] + part[3]);
                 } else if (MODE == VL_GRAD) {
-                    const int words = p.vocab - p.v0 - col0 - c;
+                    const int words = p.vocab - plan.v0 - col0 - c;
                     float v[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -lse2)) * coef.x;
@@ -364,30 +457,27 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                             if (e >= words || !live) v[e] = 0.f;
                         }
                     }
-                    uint4* out = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.dl) + (long long)row * p.ld_dl + col0 + c);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        out[i] = make_uint4(vl_pack(v[8 * i], v[8 * i + 1], p.mode_bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.mode_bf16),
-                                            vl_pack(v[8 * i + 4], v[8 * i + 5], p.mode_bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.mode_bf16));
+                    store_piece(v, c);
                 } else if (MODE == VL_HIDDEN) {
                     if (live && col0 + c < p.hidden) {
-                        float4* out = reinterpret_cast<float4*>(p.planes + ((long long)w.slice * plan.m_tiles * VL_TILE + row) * p.hidden + col0 + c);
+                        float4* out = reinterpret_cast<float4*>(p.planes + ((long long)w.slice * rows_dev + row) * p.hidden + col0 + c);
                         const int n4 = min(8, (p.hidden - col0 - c) >> 2);       // (hidden is a multiple of 8)
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             if (i >= n4) break;
                             float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
                                                    __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-                            if (!p.first) {
+                            if (p.index > 0) {
                                 const float4 o = out[i];
-                                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                                v.x = fmaf(o.x, scale, v.x); v.y = fmaf(o.y, scale, v.y);
+                                v.z = fmaf(o.z, scale, v.z); v.w = fmaf(o.w, scale, v.w);
                             }
                             out[i] = v;
                         }
                     }
                 } else {
-                    if (p.v0 + row < p.vocab && row < p.piece && col0 + c < p.hidden) {
-                        unsigned short* out = static_cast<unsigned short*>(p.d_weight) + (long long)(p.v0 + row) * p.ld_dw + col0 + c;
+                    if (plan.v0 + row < p.vocab && col0 + c < p.hidden) {
+                        unsigned short* out = static_cast<unsigned short*>(p.d_weight) + (long long)(plan.v0 + row) * p.hidden + col0 + c;
                         const int n8 = min(4, (p.hidden - col0 - c) >> 3);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -395,13 +485,20 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                             uint32_t o[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                o[j] = vl_pack(__uint_as_float(r[8 * i + 2 * j]) * scale, __uint_as_float(r[8 * i + 2 * j + 1]) * scale, p.mode_bf16);
+                                o[j] = vl_pack(__uint_as_float(r[8 * i + 2 * j]) * scale, __uint_as_float(r[8 * i + 2 * j + 1]) * scale, p.bf16);
                             reinterpret_cast<uint4*>(out)[i] = make_uint4(o[0], o[1], o[2], o[3]);
                         }
                     }
                 }
             }
-            if (MODE == VL_STATS) p.parts[(long long)(2 * w.nt + half) * p.rows_pad + row] = make_float2(m2, sum);
+            if (MODE <= VL_SOFT) {
+                p.parts[(long long)(plan.v0 / VL_TILE * 2 + 2 * w.nt + half) * p.rows_pad + row] = make_float2(m2, sum);
+                if (MODE == VL_SOFT && live && !p.again && m2 > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) {
+                    int* f = p.flags + (long long)p.index * p.flags_pitch;      // (several threads write the same)
+                    f[0] = 1;
+                    f[1 + w.mt] = 1;
+                }
+            }
             ++n;
         }
     }
@@ -446,28 +543,35 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
     for (long long i = threadIdx.x; i < row0; i += VL_GATHER_WARPS * 32) n += takes_part(a.targets[i]) ? 1 : 0;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) before[warp] = n;
+    if (a.flags != nullptr)
+        for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_flags; i += (long long)gridDim.x * blockDim.x)
+            a.flags[i] = 0;
     __syncthreads();
     if (warp == 0) {
         int start = 0;
         for (int i = 0; i < VL_GATHER_WARPS; ++i) start += before[i];
-        for (int c = 0; c < per; c += 32) {
-            const long long row = row0 + c + lane;
-            const bool in = c + lane < per && row < a.rows;
-            const long long t = in ? a.targets[row] : -1;
-            const bool part = in && takes_part(t);
-            if (in && t >= a.vocab) atomicCAS(a.status, 0, STATUS_CE_TARGET_RANGE);   // treated as ignored, and recorded
-            const unsigned mask = __ballot_sync(0xffffffffu, part);
-            const int at = start + __popc(mask & ((1u << lane) - 1u));
-            if (c + lane < per) place[c + lane] = part ? at : -1;
-            if (in) {
-                a.place[row] = part ? at : -1;
-                if (part) a.target[at] = (int)t;
-                else { a.losses[row] = 0.f; a.lse[row] = 0.f; }
+        const long long row = row0 + lane;
+        const bool in = lane < per && row < a.rows;
+        const long long t = in ? a.targets[row] : -1;
+        const bool part = in && takes_part(t);
+        if (in && t >= a.vocab) atomicCAS(a.status, 0, STATUS_CE_TARGET_RANGE);   // treated as ignored, and recorded
+        const unsigned mask = __ballot_sync(0xffffffffu, part);
+        const int at = start + __popc(mask & ((1u << lane) - 1u));
+        place[lane] = part ? at : -1;
+        if (in) {
+            a.place[row] = part ? at : -1;
+            if (part) {
+                a.target[at] = (int)t;
+                a.source[at] = (int)row;
+            } else {
+                a.losses[row] = 0.f;
+                a.lse[row] = 0.f;
             }
-            start += __popc(mask);
         }
-        if (lane == 0 && row0 + per >= a.rows) *a.count = start;      // (the last CTA)
-        if (lane == 0) total = start;
+        if (lane == 0) {
+            total = start + __popc(mask);
+            if (row0 + per >= a.rows) *a.count = total;      // (the last CTA)
+        }
     }
     __syncthreads();
     const int vecs = (int)(a.hidden / 8);
@@ -499,26 +603,31 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
     }
     // the last CTA fills the last tile's empty rows with zeros: they meet the others' in sums over rows
     if (row0 + per >= a.rows) {
-        const int count = total, end = vl_div_up(count, VL_TILE) * VL_TILE;
+        const int end = vl_div_up(total, VL_TILE) * VL_TILE;
         uint4* out = reinterpret_cast<uint4*>(a.gathered);
-        for (long long i = (long long)count * vecs + threadIdx.x; i < (long long)end * vecs; i += VL_GATHER_WARPS * 32)
+        for (long long i = (long long)total * vecs + threadIdx.x; i < (long long)end * vecs; i += VL_GATHER_WARPS * 32)
             out[i] = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
-// Joins a row's maxima and sums: 32 rows by 32 shares of the parts per CTA.
+// Joins a row's statistics, 32 rows by 32 shares of the parts per CTA. PROBE: the first words' maxima give the row's
+// reference. Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's references,
+// of which the parts of `piece` word tiles each had one.
+template <bool PROBE>
 __global__ void __launch_bounds__(1024)
-vl_merge_kernel(const VocabLossArgs a, int n_parts) {
+vl_merge_kernel(const VocabLossArgs a, int word_tiles, int soft) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float2 join[32][33];
     const int rows = *a.count, row = blockIdx.x * 32 + threadIdx.x;
     if (blockIdx.x * 32 >= rows) return;
+    const int piece = soft ? vl_piece_tiles(vl_div_up(rows, VL_TILE), word_tiles, a.capacity, a.slots) : 1;
     float m = VL_NEG, s = 0.f;
     if (row < rows) {
 #pragma unroll 4
-        for (int i = threadIdx.y; i < n_parts; i += 32) {
-            const float2 x = a.parts[(long long)i * a.rows_pad + row];
+        for (int i = threadIdx.y; i < 2 * word_tiles; i += 32) {
+            float2 x = a.parts[(long long)i * a.rows_pad + row];
+            if (soft) x.x = a.refs[(long long)(i / 2 / piece + 1) * a.rows_pad + row];
             const float top = fmaxf(m, x.x);
             s = s * vl_ex2(m - top) + x.y * vl_ex2(x.x - top);
             m = top;
@@ -537,37 +646,57 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts) {
     }
     const int at = blockIdx.x * 32 + threadIdx.y;
     if (threadIdx.x != 0 || at >= rows) return;
-    const float logit = a.target_logit[at], d = x.x - logit * VL_LOG2E;    // log2 of the others' largest over the target's
-    float loss, rest;
+    const float logit = a.target_logit[at], logit2 = logit * VL_LOG2E;
+    if (PROBE) {
+        // (fmaxf leaves out a NaN; within what a float keeps whole numbers of)
+        const float ref = fmaxf(fmaxf(x.x - VL_BELOW, logit2 - VL_BELOW_TARGET), -1.0e6f);
+        a.refs[at] = floorf(fminf(ref, 1.0e6f));
+        return;
+    }
+    const float d = x.x - logit2;      // log2 of what the others' sum is relative to, over the target's
+    float loss, rest, norm;
     if (d <= 0.f) {
-        const float r = x.y * exp2f(d);
+        const float f = exp2f(d), r = x.y * f;
         loss = log1pf(r);
         rest = r / (1.f + r);
+        norm = f / (1.f + r);
     } else {
         const float t = x.y + exp2f(-d);
         loss = d * VL_LN2 + logf(t);
         rest = x.y / t;
+        norm = 1.f / t;
     }
-    a.lse_rows[at] = logit * VL_LOG2E + loss * VL_LOG2E;
+    a.lse_rows[at] = logit2 + loss * VL_LOG2E;
     a.rest[at] = rest;
-    a.loss_rows[at] = make_float2(loss, logit + loss);
+    if (soft) a.norm[at] = norm;
+    a.losses[a.source[at]] = loss;
+    a.lse[a.source[at]] = logit + loss;
 }
 
-// To where the caller's rows are.
+// U: the planes' sum over the row's sum of exponentials.
 __global__ void __launch_bounds__(256)
-vl_scatter_kernel(const VocabLossArgs a) {
+vl_mean_kernel(const VocabLossArgs a, int word_tiles) {
     grid_dep_wait();
     grid_dep_launch();
-    const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (row >= a.rows) return;
-    const int at = a.place[row];
-    if (at < 0) return;
-    const float2 x = a.loss_rows[at];
-    a.losses[row] = x.x;
-    a.lse[row] = x.y;
+    const int rows = *a.count, quads = (int)(a.hidden / 4);
+    if (rows == 0) return;
+    const int row_tiles = vl_div_up(rows, VL_TILE);
+    const int steps = vl_piece_tiles(row_tiles, word_tiles, a.capacity, a.slots) * (VL_TILE / VL_BK);
+    const int slices = vl_slices(row_tiles * vl_div_up((int)a.hidden, VL_TILE), steps, a.slots);
+    const long long plane = (long long)row_tiles * VL_TILE * a.hidden;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * quads; i += (long long)gridDim.x * 256) {
+        const float norm = a.norm[i / quads];
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int z = 0; z < slices; ++z) {
+            const float4 x = *reinterpret_cast<const float4*>(a.planes + z * plane + i * 4);
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        reinterpret_cast<float4*>(a.mean)[i] = make_float4(v.x * norm, v.y * norm, v.z * norm, v.w * norm);
+    }
 }
 
-// ------------------------------------------------------------------------------------- backward's row factors
+// ------------------------------------------------------------------------------------- backward
 // Power of two at or above x >= 0, from 2^-95 to 2^126: 0 for zero, 1 for what is not finite.
 __device__ __forceinline__ float vl_power(float x) {
     const uint32_t bits = __float_as_uint(x);
@@ -575,92 +704,63 @@ __device__ __forceinline__ float vl_power(float x) {
     return __uint_as_float(min(max((bits + 0x007FFFFFu) >> 23, 32u), 253u) << 23);
 }
 
-// One CTA: per row that takes part (b + c, b, c) over the row's power of two, times VL_P_SCALE; the largest power.
+__device__ __forceinline__ float vl_upstream(const float* g, long long stride, long long row) {
+    return g == nullptr ? 0.f : g[row * stride];
+}
+
+// One CTA: per row that takes part (b + c, b, c) over the power of two above the largest |b|, |c|, times VL_P_SCALE. (A
+// row far below the largest keeps its digits down to 2^-27 of it, and adds nothing that the others' rounding would not
+// cover below.)
 __global__ void __launch_bounds__(1024)
 vl_coef_kernel(const VocabLossArgs a) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float part[32];
     float top = 0.f;
-    for (long long row = threadIdx.x; row < a.rows; row += 1024) {
-        const int at = a.place[row];
-        if (at < 0) continue;
-        const float b = a.d_losses == nullptr ? 0.f : a.d_losses[row * a.d_losses_stride];
-        const float c = a.d_lse == nullptr ? 0.f : a.d_lse[row * a.d_lse_stride];
-        const float power = vl_power(fmaxf(fabsf(b), fabsf(c)));
-        const float inv = power > 0.f ? VL_P_SCALE / power : 0.f;
-        a.coef[at] = make_float4((b + c) * inv, b * inv, c * inv, power);
-        top = fmaxf(top, power);
+    const int rows = *a.count;
+    for (int at = threadIdx.x; at < rows; at += 1024) {
+        const long long row = a.source[at];
+        top = fmaxf(top, fmaxf(fabsf(vl_upstream(a.d_losses, a.d_losses_stride, row)), fabsf(vl_upstream(a.d_lse, a.d_lse_stride, row))));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        top = part[threadIdx.x];
+    top = part[threadIdx.x & 31];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (threadIdx.x == 0) {
-            a.scales[0] = top;
-            a.scales[1] = top / VL_P_SCALE;
-        }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float power = vl_power(top), inv = power > 0.f ? VL_P_SCALE / power : 0.f;
+    for (int at = threadIdx.x; at < rows; at += 1024) {
+        const long long row = a.source[at];
+        const float b = vl_upstream(a.d_losses, a.d_losses_stride, row), c = vl_upstream(a.d_lse, a.d_lse_stride, row);
+        a.coef[at] = make_float4((b + c) * inv, b * inv, c * inv, 0.f);
     }
+    if (threadIdx.x == 0) *a.weight_scale = power / VL_P_SCALE;
 }
 
-// The rows times their power over the largest one, exact but for what falls out of the type's range below.
+// dH of the caller's rows; zeros where the row took no part.
 __global__ void __launch_bounds__(256)
-vl_scale_rows_kernel(const VocabLossArgs a) {
+vl_hidden_kernel(const VocabLossArgs a) {
     grid_dep_wait();
     grid_dep_launch();
-    const int rows = *a.count, vecs = (int)(a.hidden / 8), end = vl_div_up(rows, VL_TILE) * VL_TILE;
-    const float top = a.scales[0];
-    const uint4* in = reinterpret_cast<const uint4*>(a.gathered);
-    uint4* out = reinterpret_cast<uint4*>(a.scaled);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)end * vecs; i += (long long)gridDim.x * 256) {
-        const int row = (int)(i / vecs);
-        const float power = row < rows ? a.coef[row].w : 0.f;
-        uint4 v = in[i];
-        if (power != top) {
-            const float f = power > 0.f ? power / top : 0.f;
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 x = vl_two(w[e], a.bf16);
-                w[e] = f > 0.f ? vl_pack(x.x * f, x.y * f, a.bf16) : 0u;
-            }
-            v = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        out[i] = v;
-    }
-}
-
-// dH of the caller's rows: the planes' sum times the row's power; zeros where the row took no part.
-__global__ void __launch_bounds__(256)
-vl_hidden_kernel(const VocabLossArgs a, int steps, int slots) {
-    grid_dep_wait();
-    grid_dep_launch();
-    const int rows = *a.count, vecs = (int)(a.hidden / 8);
-    const int row_tiles = vl_div_up(rows, VL_TILE);
-    const int slices = rows > 0 ? vl_slices(row_tiles * vl_div_up((int)a.hidden, VL_TILE), steps, slots) : 1;
-    const long long plane = (long long)row_tiles * VL_TILE * a.hidden;
+    const int vecs = (int)(a.hidden / 8);
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.rows * vecs; i += (long long)gridDim.x * 256) {
         const long long row = i / vecs;
-        const int c = (int)(i - row * vecs) * 8, at = a.place[row];
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const int c = (int)(i - row * vecs), at = a.place[row];
+        uint4 out = make_uint4(0u, 0u, 0u, 0u);
         if (at >= 0) {
-            const float power = a.coef[at].w * (1.f / VL_P_SCALE);
-            const float* src = a.planes + (long long)at * a.hidden + c;
-#pragma unroll 4
-            for (int z = 0; z < slices; ++z) {
-                const float4 x = *reinterpret_cast<const float4*>(src + z * plane), y = *reinterpret_cast<const float4*>(src + z * plane + 4);
-                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-                v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= power;
+            const float b = vl_upstream(a.d_losses, a.d_losses_stride, row), z = vl_upstream(a.d_lse, a.d_lse_stride, row);
+            const float rest = a.rest[at], mean = b + z, hit = z * (1.f - rest) - b * rest;
+            const float4* u = reinterpret_cast<const float4*>(a.mean + (long long)at * a.hidden) + 2 * c;
+            const float4 x = u[0], y = u[1];
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.weight) + (long long)a.target[at] * a.ld_w) + c);
+            const float2 w0 = vl_two(w.x, a.bf16), w1 = vl_two(w.y, a.bf16), w2 = vl_two(w.z, a.bf16), w3 = vl_two(w.w, a.bf16);
+            out = make_uint4(vl_pack(fmaf(mean, x.x, hit * w0.x), fmaf(mean, x.y, hit * w0.y), a.bf16),
+                             vl_pack(fmaf(mean, x.z, hit * w1.x), fmaf(mean, x.w, hit * w1.y), a.bf16),
+                             vl_pack(fmaf(mean, y.x, hit * w2.x), fmaf(mean, y.y, hit * w2.y), a.bf16),
+                             vl_pack(fmaf(mean, y.z, hit * w3.x), fmaf(mean, y.w, hit * w3.y), a.bf16));
         }
-        reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.d_x) + row * a.hidden)[c / 8] =
-            make_uint4(vl_pack(v[0], v[1], a.bf16), vl_pack(v[2], v[3], a.bf16), vl_pack(v[4], v[5], a.bf16), vl_pack(v[6], v[7], a.bf16));
+        reinterpret_cast<uint4*>(a.d_x)[i] = out;
     }
 }
 
@@ -669,47 +769,55 @@ static size_t vl_align(size_t n) { return (n + 255) / 256 * 256; }
 
 static long long vl_rows_pad(long long rows) { return (rows + VL_TILE - 1) / VL_TILE * VL_TILE; }
 
+static int vl_word_tiles(long long vocab) { return (int)((vocab + VL_TILE - 1) / VL_TILE); }
+
+// Tiles that the 16-bit piece has room for, the most pieces that any number of rows up to `rows` makes of the
+// vocabulary, and the planes of U they need, in units of rows_pad rows.
+struct VlRoom {
+    int capacity, pieces, planes;
+};
+static VlRoom vl_room(long long rows, long long vocab, long long hidden, int slots) {
+    VlRoom r = {VL_PIECE_UNITS, 1, 1};
+    const long long row_tiles = vl_rows_pad(rows) / VL_TILE;
+    const int word_tiles = vl_word_tiles(vocab), feature_tiles = vl_div_up((int)hidden, VL_TILE);
+    if (r.capacity < 4 * row_tiles) r.capacity = (int)(4 * row_tiles);
+    if (r.capacity > row_tiles * word_tiles) r.capacity = (int)(row_tiles * word_tiles);
+    long long most = row_tiles;
+    for (long long t = 1; t <= row_tiles; ++t) {
+        const int tiles = vl_piece_tiles((int)t, word_tiles, r.capacity, slots), pieces = vl_div_up(word_tiles, tiles);
+        if (pieces > r.pieces) r.pieces = pieces;
+        const long long planes = t * vl_slices((int)t * feature_tiles, tiles * (VL_TILE / VL_BK), slots);
+        if (planes > most) most = planes;
+    }
+    r.planes = (int)((most + row_tiles - 1) / row_tiles);
+    return r;
+}
+
 // What the forward keeps for the backward.
 struct VlKept {
-    size_t count, place, target, lse, rest, gathered, bytes;
+    size_t count, place, source, target, lse, rest, gathered, mean, bytes;
 };
-static VlKept vl_kept(long long rows, long long hidden) {
-    VlKept k;
+static VlKept vl_kept(long long rows, long long hidden, int grads) {
+    VlKept k = {};
     const size_t pad = (size_t)vl_rows_pad(rows);
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t r = at; at += vl_align(n); return r; };
     k.count = take(4);
     k.place = take((size_t)rows * 4);
+    k.source = take(pad * 4);
     k.target = take(pad * 4);
     k.lse = take(pad * 4);
     k.rest = take(pad * 4);
-    k.gathered = take(pad * (size_t)hidden * 2);
+    if (grads & 1) k.mean = take((size_t)rows * (size_t)hidden * 4);
+    k.gathered = at;                       // last: without a gradient of the weight it is scratch of the forward
+    if (grads & 2) take(pad * (size_t)hidden * 2);
     k.bytes = at;
     return k;
 }
 
-// Words of a piece: its 16-bit gradient takes at most 64 MiB (it is read back from L2), in whole tiles.
-static int vl_piece(long long rows, long long vocab) {
-    const long long pad = vl_rows_pad(rows), all = (vocab + VL_TILE - 1) / VL_TILE * VL_TILE;
-    long long piece = (64ll << 20) / 2 / pad / VL_TILE * VL_TILE;
-    if (piece < 1024) piece = 1024;
-    return (int)(piece < all ? piece : all);
-}
-
-// Planes of dH in units of rows_pad rows: what any count of rows up to `rows` asks for.
-static int vl_planes(long long rows, long long hidden, int piece, int slots) {
-    const long long tiles = vl_rows_pad(rows) / VL_TILE;
-    long long most = tiles;
-    for (long long t = 1; t <= tiles && t <= 4096; ++t) {     // (more tiles than that are one slice)
-        const long long n = t * vl_slices((int)t * vl_div_up((int)hidden, VL_TILE), vl_div_up(piece, VL_BK), slots);
-        if (n > most) most = n;
-    }
-    return (int)((most + tiles - 1) / tiles);
-}
-
 struct VlScratch {
-    size_t parts, loss_rows, target_logit, coef, scales, scaled, dl, planes, bytes;
-    int piece;
+    size_t parts, target_logit, norm, refs, flags, gathered, coef, weight_scale, piece, planes, bytes;
+    VlRoom room;
 };
 
 static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
@@ -717,24 +825,29 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
     const size_t pad = (size_t)vl_rows_pad(a.rows);
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t r = at; at += vl_align(n); return r; };
+    if ((backward && a.d_weight != nullptr) || (!backward && (a.grads & 1)))
+        s.room = vl_room(a.rows, a.vocab, a.hidden, a.sm_count / 2);
     if (!backward) {
-        s.parts = take((size_t)((a.vocab + VL_TILE - 1) / VL_TILE) * 2 * 8 * pad);
-        s.loss_rows = take(pad * 8);
+        s.parts = take((size_t)vl_word_tiles(a.vocab) * 2 * 8 * pad);
         s.target_logit = take(pad * 4);
-    } else {
-        s.piece = vl_piece(a.rows, a.vocab);
+        if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
+        if (a.grads & 1) {
+            s.norm = take(pad * 4);
+            s.refs = take((size_t)(s.room.pieces + 1) * pad * 4);
+            s.flags = take((size_t)s.room.pieces * (1 + pad / VL_TILE) * 4);
+            s.piece = take((size_t)s.room.capacity * VL_TILE * VL_TILE * 2);
+            s.planes = take((size_t)s.room.planes * pad * (size_t)a.hidden * 4);
+        }
+    } else if (a.d_weight != nullptr) {
         s.coef = take(pad * 16);
-        s.scales = take(16);
-        s.dl = take(pad * (size_t)s.piece * 2);
-        if (a.d_x != nullptr)
-            s.planes = take((size_t)vl_planes(a.rows, a.hidden, s.piece, a.sm_count / 2) * pad * (size_t)a.hidden * 4);
-        if (a.d_weight != nullptr) s.scaled = take(pad * (size_t)a.hidden * 2);
+        s.weight_scale = take(4);
+        s.piece = take((size_t)s.room.capacity * VL_TILE * VL_TILE * 2);
     }
     s.bytes = at;
     return s;
 }
 
-size_t vocab_loss_kept_bytes(long long rows, long long hidden) { return vl_kept(rows, hidden).bytes; }
+size_t vocab_loss_kept_bytes(long long rows, long long hidden, int grads) { return vl_kept(rows, hidden, grads).bytes; }
 
 size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward) { return vl_scratch(a, backward).bytes; }
 
@@ -764,6 +877,7 @@ static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long un
     }();
     long long pairs = sm_count / 2 < most ? sm_count / 2 : most;
     if (units < pairs) pairs = units;
+    if (pairs < 1) pairs = 1;
     cfg.gridDim = dim3((unsigned)(2 * pairs));
     return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
@@ -774,15 +888,30 @@ static bool vl_map(CUtensorMap* map, int bf16, const void* base, long long inner
 }
 
 static void vl_use_kept(VocabLossArgs& a) {
-    const VlKept k = vl_kept(a.rows, a.hidden);
+    const VlKept k = vl_kept(a.rows, a.hidden, a.grads);
     char* base = static_cast<char*>(a.kept);
     a.count = reinterpret_cast<int*>(base + k.count);
     a.place = reinterpret_cast<int*>(base + k.place);
+    a.source = reinterpret_cast<int*>(base + k.source);
     a.target = reinterpret_cast<int*>(base + k.target);
     a.lse_rows = reinterpret_cast<float*>(base + k.lse);
     a.rest = reinterpret_cast<float*>(base + k.rest);
+    a.mean = reinterpret_cast<float*>(base + k.mean);
     a.gathered = base + k.gathered;
     a.rows_pad = vl_rows_pad(a.rows);
+    a.slots = a.sm_count / 2;
+}
+
+static VlParams vl_params(const VocabLossArgs& a) {
+    VlParams p = {};
+    p.count = a.count; p.status = a.status; p.bf16 = a.bf16;
+    p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab);
+    p.capacity = a.capacity; p.slots = a.slots;
+    p.target = a.target; p.parts = a.parts; p.rows_pad = a.rows_pad;
+    p.refs = a.refs; p.flags = a.flags; p.flags_pitch = 1 + (int)(a.rows_pad / VL_TILE);
+    p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef;
+    p.piece = a.piece; p.planes = a.planes; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
+    return p;
 }
 
 cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream, const char** why) {
@@ -793,29 +922,56 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     const VlScratch s = vl_scratch(a, false);
     char* ws = static_cast<char*>(a.workspace);
     a.parts = reinterpret_cast<float2*>(ws + s.parts);
-    a.loss_rows = reinterpret_cast<float2*>(ws + s.loss_rows);
     a.target_logit = reinterpret_cast<float*>(ws + s.target_logit);
+    if (!(a.grads & 2)) a.gathered = ws + s.gathered;
+    const bool soft = (a.grads & 1) != 0;
+    if (soft) {
+        a.norm = reinterpret_cast<float*>(ws + s.norm);
+        a.refs = reinterpret_cast<float*>(ws + s.refs);
+        a.flags = reinterpret_cast<int*>(ws + s.flags);
+        a.n_flags = s.room.pieces * (1 + a.rows_pad / VL_TILE);
+        a.piece = ws + s.piece;
+        a.planes = reinterpret_cast<float*>(ws + s.planes);
+        a.capacity = s.room.capacity;
+    }
     const int per = a.rows <= 4096 ? 8 : 32;
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
-    VlMaps maps;
-    if (!vl_map(&maps.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
-        !vl_map(&maps.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128)) {
-        *why = "cuTensorMapEncodeTiled";
-        return cudaErrorInvalidValue;
+    VlMaps logits, hidden;
+    bool ok = vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
+              vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
+    if (ok && soft)
+        ok = vl_map(&hidden.a, a.bf16, a.piece, VL_BK, (long long)a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, 128) &&
+             vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64);
+    if (!ok) { *why = "cuTensorMapEncodeTiled"; return cudaErrorInvalidValue; }
+    const VlParams base = vl_params(a);
+    const long long row_tiles = a.rows_pad / VL_TILE;
+    const dim3 merge_grid((unsigned)((a.rows + 31) / 32)), merge_block(32, 32);
+    if (!soft) {
+        e = vl_launch<VL_STATS>(logits, base, row_tiles * base.word_tiles, a.sm_count, stream);
+        if (e != cudaSuccess) { *why = "statistics"; return e; }
+    } else {
+        VlParams probe = base;
+        if (probe.word_tiles > VL_PROBE_TILES) probe.word_tiles = VL_PROBE_TILES;
+        e = vl_launch<VL_STATS>(logits, probe, row_tiles * probe.word_tiles, a.sm_count, stream);
+        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, probe.word_tiles, 0);
+        if (e != cudaSuccess) { *why = "references"; return e; }
+        const long long units = row_tiles * base.word_tiles < a.capacity ? row_tiles * base.word_tiles : a.capacity;
+        for (int i = 0; i < s.room.pieces; ++i) {
+            VlParams p = base;
+            p.index = i;
+            e = vl_launch<VL_SOFT>(logits, p, units, a.sm_count, stream);
+            p.again = 1;
+            if (e == cudaSuccess) e = vl_launch<VL_SOFT>(logits, p, units, a.sm_count, stream);
+            if (e != cudaSuccess) { *why = "softmax"; return e; }
+            e = vl_launch<VL_HIDDEN>(hidden, p, row_tiles * vl_div_up(p.hidden, VL_TILE) * VL_MAX_SLICES, a.sm_count, stream);
+            if (e != cudaSuccess) { *why = "gradient of the hidden states"; return e; }
+        }
     }
-    VlParams p = {};
-    p.count = a.count; p.status = a.status; p.mode_bf16 = a.bf16;
-    p.vocab = (int)a.vocab; p.hidden = (int)a.hidden;
-    p.v0 = 0; p.piece = (int)a.vocab;
-    p.n_tiles = (int)((a.vocab + VL_TILE - 1) / VL_TILE);
-    p.parts = a.parts; p.rows_pad = a.rows_pad; p.target = a.target;
-    e = vl_launch<VL_STATS>(maps, p, a.rows_pad / VL_TILE * p.n_tiles, a.sm_count, stream);
-    if (e != cudaSuccess) { *why = "statistics"; return e; }
-    e = launch_pdl(vl_merge_kernel, dim3((unsigned)((a.rows + 31) / 32)), dim3(32, 32), 0, stream, a, 2 * p.n_tiles);
-    if (e != cudaSuccess) { *why = "merge"; return e; }
-    e = launch_pdl(vl_scatter_kernel, dim3((unsigned)((a.rows + 255) / 256)), dim3(256), 0, stream, a);
-    if (e != cudaSuccess) *why = "scatter";
+    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, base.word_tiles, soft ? 1 : 0);
+    if (e == cudaSuccess && soft)
+        e = launch_pdl(vl_mean_kernel, dim3((unsigned)(a.sm_count * 8)), dim3(256), 0, stream, a, base.word_tiles);
+    if (e != cudaSuccess) *why = "merge";
     return e;
 }
 
@@ -826,56 +982,33 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     vl_use_kept(a);
     const VlScratch s = vl_scratch(a, true);
     char* ws = static_cast<char*>(a.workspace);
-    a.coef = reinterpret_cast<float4*>(ws + s.coef);
-    a.scales = reinterpret_cast<float*>(ws + s.scales);
-    a.scaled = ws + s.scaled;
-    a.planes = reinterpret_cast<float*>(ws + s.planes);
-    void* dl = ws + s.dl;
-    cudaError_t e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
-    if (e != cudaSuccess) { *why = "row factors"; return e; }
-    if (a.d_weight != nullptr) {
-        e = launch_pdl(vl_scale_rows_kernel, dim3((unsigned)(a.sm_count * 8)), dim3(256), 0, stream, a);
-        if (e != cudaSuccess) { *why = "row scales"; return e; }
+    cudaError_t e = cudaSuccess;
+    if (a.d_x != nullptr) {
+        e = launch_pdl(vl_hidden_kernel, dim3((unsigned)(a.sm_count * 8)), dim3(256), 0, stream, a);
+        if (e != cudaSuccess) { *why = "gradient of the hidden states"; return e; }
     }
-    const int feature_tiles = (int)((a.hidden + VL_TILE - 1) / VL_TILE);
-    VlMaps logits, hidden, weight;
+    if (a.d_weight == nullptr) return e;
+    a.coef = reinterpret_cast<float4*>(ws + s.coef);
+    a.weight_scale = reinterpret_cast<float*>(ws + s.weight_scale);
+    a.piece = ws + s.piece;
+    a.capacity = s.room.capacity;
+    e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
+    if (e != cudaSuccess) { *why = "row factors"; return e; }
+    VlMaps logits, weight;
     if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
         !vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) ||
-        !vl_map(&hidden.a, a.bf16, dl, s.piece, a.rows_pad, s.piece, 128) ||
-        !vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) ||
-        !vl_map(&weight.a, a.bf16, dl, s.piece, a.rows_pad, s.piece, 64) ||
-        !vl_map(&weight.b, a.bf16, a.d_weight != nullptr ? a.scaled : a.gathered, a.hidden, a.rows_pad, a.hidden, 64)) {
+        !vl_map(&weight.a, a.bf16, a.piece, VL_BK, (long long)a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, 64) ||
+        !vl_map(&weight.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64)) {
         *why = "cuTensorMapEncodeTiled";
         return cudaErrorInvalidValue;
     }
-    VlParams p = {};
-    p.count = a.count; p.status = a.status; p.mode_bf16 = a.bf16;
-    p.vocab = (int)a.vocab; p.hidden = (int)a.hidden;
-    p.rows_pad = a.rows_pad; p.target = a.target;
-    p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef; p.dl = dl; p.ld_dl = s.piece;
-    p.planes = a.planes; p.slots = a.sm_count / 2; p.first_steps = vl_div_up((int)(a.vocab < s.piece ? a.vocab : s.piece), VL_BK);
-    p.d_weight = a.d_weight; p.ld_dw = a.hidden; p.weight_scale = a.scales + 1;
-    for (long long v0 = 0; v0 < a.vocab; v0 += s.piece) {
-        p.v0 = (int)v0;
-        p.piece = (int)(a.vocab - v0 < s.piece ? a.vocab - v0 : s.piece);
-        p.n_tiles = vl_div_up(p.piece, VL_TILE);
-        const long long row_tiles = a.rows_pad / VL_TILE;
-        e = vl_launch<VL_GRAD>(logits, p, row_tiles * p.n_tiles, a.sm_count, stream);
+    VlParams p = vl_params(a);
+    const long long units = a.rows_pad / VL_TILE * p.word_tiles < a.capacity ? a.rows_pad / VL_TILE * p.word_tiles : a.capacity;
+    for (p.index = 0; p.index < s.room.pieces; ++p.index) {
+        e = vl_launch<VL_GRAD>(logits, p, units, a.sm_count, stream);
         if (e != cudaSuccess) { *why = "gradient of the logits"; return e; }
-        if (a.d_x != nullptr) {
-            p.first = v0 == 0 ? 1 : 0;
-            e = vl_launch<VL_HIDDEN>(hidden, p, row_tiles * feature_tiles * VL_MAX_SLICES, a.sm_count, stream);
-            if (e != cudaSuccess) { *why = "gradient of the hidden states"; return e; }
-        }
-        if (a.d_weight != nullptr) {
-            e = vl_launch<VL_WEIGHT>(weight, p, (long long)p.n_tiles * feature_tiles, a.sm_count, stream);
-            if (e != cudaSuccess) { *why = "gradient of the head"; return e; }
-        }
-    }
-    if (a.d_x != nullptr) {
-        e = launch_pdl(vl_hidden_kernel, dim3((unsigned)(a.sm_count * 8)), dim3(256), 0, stream, a,
-                       p.first_steps, p.slots);
-        if (e != cudaSuccess) *why = "sum of the planes";
+        e = vl_launch<VL_WEIGHT>(weight, p, (long long)p.word_tiles * vl_div_up(p.hidden, VL_TILE), a.sm_count, stream);
+        if (e != cudaSuccess) { *why = "gradient of the head"; return e; }
     }
     return e;
 }

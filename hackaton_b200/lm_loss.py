@@ -179,20 +179,24 @@ def linear_cross_entropy(hidden, weight, targets, denom):
 
 
 class _VocabLoss:
-    """lm_head + loss in pieces of the vocabulary (csrc/vocab_loss.cu). Next to the weight it keeps the rows that
-    take part and four numbers for each."""
+    """lm_head + loss in pieces of the vocabulary (csrc/vocab_loss.cu). Next to the weight it keeps, for each row that
+    takes part, a few numbers, the softmax's mean of the weight (fp32) where the hidden states want a gradient, and the row
+    itself where the weight does."""
 
     materialize = False
 
+    def __init__(self, grads):
+        self.grads = grads
+
     def run(self, keep, hidden, weight, targets):
-        losses, lse, kept = _lib.host().vocab_loss_fwd(hidden, weight, targets)
+        losses, lse, kept = _lib.host().vocab_loss_fwd(hidden, weight, targets, self.grads)
         keep(weight, kept, shape=hidden.shape, rows=targets.numel())
         return losses.reshape(targets.shape), lse.reshape(targets.shape)
 
     def grad(self, kept, d_losses, d_lse):
         weight, state = kept.tensors
-        d_hidden, d_weight = _lib.host().vocab_loss_bwd(weight, state, d_losses, d_lse, kept.rows, kept.wants[0],
-                                                        kept.wants[1])
+        d_hidden, d_weight = _lib.host().vocab_loss_bwd(weight, state, d_losses, d_lse, kept.rows, self.grads,
+                                                        kept.wants[0], kept.wants[1])
         return None if d_hidden is None else d_hidden.reshape(kept.shape), d_weight, None
 
 
@@ -222,4 +226,10 @@ def vocab_cross_entropy(hidden, weight, targets):
     if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8 != 0:
         raise ValueError(f"hackaton_b200: vocab_cross_entropy: {weight.shape[0]} words of {weight.shape[1]} features (a "
                          "multiple of 8)")
-    return call(_VocabLoss(), hidden, weight, targets)
+    grads = 0
+    if torch.is_grad_enabled():
+        grads = (1 if hidden.requires_grad else 0) | (2 if weight.requires_grad else 0)
+    if grads:
+        return call(_VocabLoss(grads), hidden, weight, targets)
+    losses, lse, _ = _lib.host().vocab_loss_fwd(hidden, weight, targets, 0)
+    return losses.reshape(targets.shape), lse.reshape(targets.shape)

@@ -300,19 +300,20 @@ int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delt
  * NF4B200_BF16, 16-byte aligned, row pitches and hidden multiples of 8; targets int64.
  * Backward, from the gradients of losses and lse (fp32 with an element stride, 0 for one number; either may be NULL):
  * d_x [rows, hidden] and d_weight [vocab, hidden] in x's type, contiguous, either may be NULL. `kept` is what the
- * forward left (_kept_bytes), scratch as _workspace_bytes says (backward: 0 forward, 1 d_x, 2 d_weight, 3 both); both
- * 256-byte aligned. No sum depends on timing.
+ * forward left (_kept_bytes), scratch as _workspace_bytes says; both 256-byte aligned. `grads` says in all of them what the
+ * backward will be asked for: 1 d_x, 2 d_weight, 3 both, 0 no backward. d_x costs the forward one more product of the
+ * logits' size and the backward next to nothing; d_weight costs the backward two. No sum depends on timing.
  * The reference walks the rows in chunks and holds a chunk's logits (solution/lm_loss.py:27-67), with no gradient of
  * the weight.
  */
-int64_t nf4b200_vocab_loss_kept_bytes(int64_t rows, int64_t hidden);
-int64_t nf4b200_vocab_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int backward);
+int64_t nf4b200_vocab_loss_kept_bytes(int64_t rows, int64_t hidden, int grads);
+int64_t nf4b200_vocab_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int grads, int backward);
 int nf4b200_vocab_loss_fwd(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, int dtype, const void* targets,
-                           void* losses, void* lse, int64_t rows, int64_t vocab, int64_t hidden, void* kept,
+                           void* losses, void* lse, int64_t rows, int64_t vocab, int64_t hidden, int grads, void* kept,
                            void* workspace, size_t workspace_bytes, void* stream);
 int nf4b200_vocab_loss_bwd(const void* weight, int64_t ld_w, int dtype, const void* d_losses, int64_t d_losses_stride,
                            const void* d_lse, int64_t d_lse_stride, void* d_x, void* d_weight, int64_t rows, int64_t vocab,
-                           int64_t hidden, void* kept, void* workspace, size_t workspace_bytes, void* stream);
+                           int64_t hidden, int grads, void* kept, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Backward of the projection that consumes the product (down_proj: d_hidden = dy . W_down) with the
