@@ -48,9 +48,11 @@ constexpr int VL_BK = 64;
 constexpr int VL_STAGES = 6;
 constexpr int VL_HALF_BYTES = 128 * VL_BK * 2;      // one CTA's share of either operand
 constexpr int VL_STAGE_BYTES = 2 * VL_HALF_BYTES;
-constexpr int VL_BAR_OFF = VL_STAGES * VL_STAGE_BYTES;
-constexpr int VL_SMEM = VL_BAR_OFF + 256 + 1024;    // + slack for 1024-byte alignment
 constexpr int VL_EPI_WARPS = 8;
+constexpr int VL_STAGING_OFF = VL_STAGES * VL_STAGE_BYTES;      // a box of 32 rows x 128 bytes per warp, on its way out
+constexpr int VL_BAR_OFF = VL_STAGING_OFF + VL_EPI_WARPS * 4096;
+constexpr int VL_SMEM = VL_BAR_OFF + 256 + 1024;    // + slack for 1024-byte alignment
+static_assert(VL_SMEM <= 232448, "exceeds the 227 KB of shared memory per CTA");
 constexpr int VL_THREADS = 64 + VL_EPI_WARPS * 32;
 
 enum VlMode {
@@ -62,7 +64,7 @@ enum VlMode {
 };
 
 struct VlMaps {
-    CUtensorMap a, b;
+    CUtensorMap a, b, c;     // c: where the epilogue's boxes go (not VL_STATS)
 };
 
 struct VlParams {
@@ -132,6 +134,10 @@ __device__ __forceinline__ uint32_t vl_pack(float a, float b, int bf16) {
     }
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void vl_sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
 struct VlPlan {      // what a launch's units are, from the device's row count
@@ -236,6 +242,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&maps.a);
         tma_prefetch_desc(&maps.b);
+        if (MODE != VL_STATS) tma_prefetch_desc(&maps.c);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -341,6 +348,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
         // ------------------------------------------------------------------ epilogue: a row's half tile per thread
         const int q = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
+        const uint32_t staging = base + VL_STAGING_OFF + (uint32_t)(warp - 2) * 4096u;
         uint32_t n = 0;
         for (int u = pair; u < plan.units && !fail; u += pairs) {
             const VlUnit w = vl_unit<MODE>(u, plan);
@@ -396,14 +404,36 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
             };
-            // 32 values of the row's part of the 16-bit piece (columns col0 + c ..)
-            auto store_piece = [&](const float (&v)[32], int c) {
-                uint4* out = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.piece) +
-                                                      ((long long)((col0 + c) >> 6) * rows_dev + row) * 64 + (c & 32));
+            // The box's memory is free again once the store before has read it; what is in it goes out as 32 whole lines.
+            auto box_begin = [&]() {
+                if (lane == 0) bulk_wait_read();
+                __syncwarp();
+            };
+            auto box_put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t t) {    // 16 bytes of this lane's row
+                vl_sts128(staging + lane * 128 + ((chunk ^ (lane & 7)) << 4), x, y, z, t);
+            };
+            auto box_end = [&](int x, int y, bool add) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (add) tma_reduce_add_2d(&maps.c, staging, x, y);
+                    else     tma_store_2d(&maps.c, staging, x, y);
+                    bulk_commit();
+                }
+            };
+            const int row0 = row - lane;
+            // 32 values in 16 bits: half a box
+            auto put16 = [&](const float (&v)[32], int c) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    out[i] = make_uint4(vl_pack(v[8 * i], v[8 * i + 1], p.bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.bf16),
-                                        vl_pack(v[8 * i + 4], v[8 * i + 5], p.bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.bf16));
+                    box_put((c & 32) / 8 + i, vl_pack(v[8 * i], v[8 * i + 1], p.bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.bf16),
+                            vl_pack(v[8 * i + 4], v[8 * i + 5], p.bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.bf16));
+            };
+            // values of the 16-bit piece (columns col0 + c ..)
+            auto store_piece = [&](const float (&v)[32], int c) {
+                if ((c & 32) == 0) box_begin();
+                put16(v, c);
+                if ((c & 32) != 0) box_end(0, ((col0 + c) >> 6) * rows_dev + row0, false);
             };
             float m2 = VL_NEG, sum = 0.f;
 #pragma unroll 1
@@ -459,36 +489,26 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                     }
                     store_piece(v, c);
                 } else if (MODE == VL_HIDDEN) {
-                    if (live && col0 + c < p.hidden) {
-                        float4* out = reinterpret_cast<float4*>(p.planes + ((long long)w.slice * rows_dev + row) * p.hidden + col0 + c);
-                        const int n4 = min(8, (p.hidden - col0 - c) >> 2);       // (hidden is a multiple of 8)
+                    if (col0 + c >= p.hidden) continue;
+                    if (__any_sync(0xffffffffu, scale != 1.f)) {       // a reference has moved: sums so far go along
+                        float* out = p.planes + ((long long)w.slice * rows_dev + row) * p.hidden + col0 + c;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (i >= n4) break;
-                            float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
-                                                   __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-                            if (p.index > 0) {
-                                const float4 o = out[i];
-                                v.x = fmaf(o.x, scale, v.x); v.y = fmaf(o.y, scale, v.y);
-                                v.z = fmaf(o.z, scale, v.z); v.w = fmaf(o.w, scale, v.w);
-                            }
-                            out[i] = v;
-                        }
+                        for (int e = 0; e < 32; ++e)
+                            if (col0 + c + e < p.hidden) out[e] = fmaf(out[e], scale, __uint_as_float(r[e]));
+                        continue;
                     }
+                    box_begin();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) box_put(i, r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                    box_end(col0 + c, w.slice * rows_dev + row0, p.index > 0);
                 } else {
-                    if (plan.v0 + row < p.vocab && col0 + c < p.hidden) {
-                        unsigned short* out = static_cast<unsigned short*>(p.d_weight) + (long long)(plan.v0 + row) * p.hidden + col0 + c;
-                        const int n8 = min(4, (p.hidden - col0 - c) >> 3);
+                    if (col0 + (c & 64) >= p.hidden) continue;
+                    if ((c & 32) == 0) box_begin();
+                    float v[32];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (i >= n8) break;
-                            uint32_t o[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                o[j] = vl_pack(__uint_as_float(r[8 * i + 2 * j]) * scale, __uint_as_float(r[8 * i + 2 * j + 1]) * scale, p.bf16);
-                            reinterpret_cast<uint4*>(out)[i] = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
-                    }
+                    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * scale;
+                    put16(v, c);
+                    if ((c & 32) != 0) box_end(col0 + (c & 64), plan.v0 + row0, false);
                 }
             }
             if (MODE <= VL_SOFT) {
@@ -501,6 +521,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             }
             ++n;
         }
+        if (MODE != VL_STATS && lane == 0) bulk_wait();
     }
 
     if (fail) {
@@ -887,6 +908,11 @@ static bool vl_map(CUtensorMap* map, int bf16, const void* base, long long inner
                        (uint64_t)outer, (uint64_t)pitch * 2, VL_BK, (uint32_t)box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// The 16-bit piece: blocks of [rows][64 words], read in boxes of 128 rows (rows as M) or 64 (as steps), written in 32.
+static bool vl_piece_map(CUtensorMap* map, const VocabLossArgs& a, int box_outer) {
+    return vl_map(map, a.bf16, a.piece, VL_BK, (long long)a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, box_outer);
+}
+
 static void vl_use_kept(VocabLossArgs& a) {
     const VlKept k = vl_kept(a.rows, a.hidden, a.grads);
     char* base = static_cast<char*>(a.kept);
@@ -937,12 +963,14 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     const int per = a.rows <= 4096 ? 8 : 32;
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
-    VlMaps logits, hidden;
+    VlMaps logits = {}, hidden = {};
     bool ok = vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
               vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
     if (ok && soft)
-        ok = vl_map(&hidden.a, a.bf16, a.piece, VL_BK, (long long)a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, 128) &&
-             vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64);
+        ok = vl_piece_map(&logits.c, a, 32) && vl_piece_map(&hidden.a, a, 128) &&
+             vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) &&
+             make_map_2d(&hidden.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.planes, (uint64_t)a.hidden,
+                         (uint64_t)s.room.planes * (uint64_t)a.rows_pad, (uint64_t)a.hidden * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!ok) { *why = "cuTensorMapEncodeTiled"; return cudaErrorInvalidValue; }
     const VlParams base = vl_params(a);
     const long long row_tiles = a.rows_pad / VL_TILE;
@@ -994,11 +1022,12 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     a.capacity = s.room.capacity;
     e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) { *why = "row factors"; return e; }
-    VlMaps logits, weight;
+    VlMaps logits = {}, weight = {};
     if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
         !vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) ||
-        !vl_map(&weight.a, a.bf16, a.piece, VL_BK, (long long)a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, 64) ||
-        !vl_map(&weight.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64)) {
+        !vl_piece_map(&logits.c, a, 32) || !vl_piece_map(&weight.a, a, 64) ||
+        !vl_map(&weight.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64) ||
+        !vl_map(&weight.c, a.bf16, a.d_weight, a.hidden, a.vocab, a.hidden, 32)) {
         *why = "cuTensorMapEncodeTiled";
         return cudaErrorInvalidValue;
     }
