@@ -10,8 +10,6 @@ attributes:
                              `kept.tensors` are the stored tensors, `kept.<fact>` the stored facts,
                              `kept.wants[i]` says whether input i needs a gradient at all
 
-An operation with `materialize = False` is given None, not zeros, for outputs that nothing was computed from.
-
 `call(op, *tensors)` runs the operation under autograd. Tensors are the only things that travel
 through `torch.autograd.Function.apply`; sizes, flags and dtypes live on the operation object, so
 an operation's `grad` never returns placeholders for them.
@@ -48,7 +46,6 @@ class _Node(torch.autograd.Function):
     def forward(ctx, op, *tensors):
         ctx.op = op
         ctx.facts = {}
-        ctx.set_materialize_grads(getattr(op, "materialize", True))
 
         def keep(*saved, **facts):
             ctx.save_for_backward(*saved)

@@ -1,11 +1,14 @@
 // The host side of the calls that training and decoding make most: views, output tensors, device
 // and stream look-ups and the call into the C ABI, in one step out of Python. The same work through
 // ctypes costs several times the kernels of a small call (q/k/v with LoRA at 810 tokens: 16 launches
-// of 86 us GPU time in all took 668 us from Python). Argument checks that need the quant state, and the
-// autograd functions, stay in Python; nothing is kept here between calls.
+// of 86 us GPU time in all took 668 us from Python). Argument checks that need the quant state, and most
+// autograd functions, stay in Python; nothing is kept here between calls. The newer operators have their autograd
+// functions here too: a node of Python costs a backward pass about 40 us of interpreter and thread hand-over (a SwiGLU of
+// 333 x 1000 both ways took 96 us that way). What one of those calls refuses comes back as None, and Python says why.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -18,6 +21,8 @@ namespace py = pybind11;
 using at::Tensor;
 using Opt = std::optional<Tensor>;
 using Opts = std::vector<Opt>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 namespace {
 
@@ -361,6 +366,32 @@ std::tuple<Tensor, Tensor> act8_swiglu_bwd(const Tensor& d2, const Tensor& gc, c
     return {dg, du};
 }
 
+// [..., cols] as contiguous [rows, cols].
+Tensor flat_rows(const Tensor& t) {
+    const int64_t cols = t.dim() == 0 ? 1 : t.size(-1);
+    return t.reshape({cols > 0 ? t.numel() / cols : 0, cols}).contiguous();
+}
+
+struct SiluMulAct8 : torch::autograd::Function<SiluMulAct8> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up) {
+        auto [hidden, gc, gs, uc, us] = act8_swiglu_fwd(flat_rows(gate), flat_rows(up));
+        ctx->save_for_backward({gc, gs, uc, us});
+        return hidden.view(gate.sizes());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto kept = ctx->get_saved_variables();
+        auto [dg, du] = act8_swiglu_bwd(flat_rows(grads[0]), kept[0], kept[1], kept[2], kept[3]);
+        return {dg.view(grads[0].sizes()), du.view(grads[0].sizes())};
+    }
+};
+
+Opt silu_mul_act8(const Tensor& gate, const Tensor& up) {
+    if (!gate.is_cuda() || gate.device() != up.device() || gate.scalar_type() != at::kHalf || up.scalar_type() != at::kHalf ||
+        gate.sizes() != up.sizes())
+        return {};
+    return SiluMulAct8::apply(gate, up);
+}
+
 Tensor act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s2, int64_t cols) {
     const c10::cuda::CUDAGuard guard(codes.device());
     const int64_t rows = codes.size(0);
@@ -375,48 +406,106 @@ Tensor act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s2
     return out;
 }
 
-// (stream, normed rows, what the gradient needs or None)
-std::tuple<Tensor, Tensor, Opt> sandwich_fwd(const Tensor& r2, const Tensor& d2, const Tensor& post, const Tensor& pre,
-                                             const Opt& gate2, double scale, double eps, bool f32_out, bool train) {
-    const c10::cuda::CUDAGuard guard(r2.device());
-    const int64_t rows = r2.size(0), hidden = r2.size(1);
-    Tensor out = at::empty_like(r2);
-    Tensor normed = at::empty({rows, hidden}, d2.options().dtype(f32_out ? at::kFloat : d2.scalar_type()));
+struct SandwichRows {   // the operands as the kernels read them
+    Tensor residual, delta, post, pre;
+    Opt gate;
+    int64_t rows, hidden;
+};
+
+SandwichRows sandwich_rows(const Tensor& residual, const Tensor& delta, const Tensor& post, const Tensor& pre, const Opt& gate) {
+    SandwichRows r{residual.contiguous(), delta.contiguous(), post.contiguous(), pre.contiguous(), {}, 0, residual.size(-1)};
+    r.rows = residual.numel() / r.hidden;
+    if (gate.has_value() && r.rows > 0) r.gate = gate->contiguous();
+    return r;
+}
+
+// (stream, normed, what the gradient needs or None)
+std::tuple<Tensor, Tensor, Opt> sandwich_fwd(const SandwichRows& r, double scale, double eps, bool f32_out, bool train) {
+    const c10::cuda::CUDAGuard guard(r.residual.device());
+    Tensor out = at::empty_like(r.residual);
+    Tensor normed = at::empty(r.residual.sizes(), r.delta.options().dtype(f32_out ? at::kFloat : r.delta.scalar_type()));
     Opt rstd;
-    if (train) rstd = at::empty({rows, 2}, r2.options());
-    check(nf4b200_sandwich_norm_fwd(r2.const_data_ptr(), d2.const_data_ptr(), type_code(d2.scalar_type()),
-                                    post.const_data_ptr(), pre.const_data_ptr(), ptr(gate2),
-                                    gate2.has_value() ? gate2->size(0) : 0, out.data_ptr(), normed.data_ptr(),
-                                    type_code(normed.scalar_type()), train ? rstd->data_ptr() : nullptr, rows, hidden,
-                                    (float)scale, (float)eps, stream_of(r2)));
+    if (train) rstd = at::empty({r.rows, 2}, r.residual.options());
+    check(nf4b200_sandwich_norm_fwd(r.residual.const_data_ptr(), r.delta.const_data_ptr(), type_code(r.delta.scalar_type()),
+                                    r.post.const_data_ptr(), r.pre.const_data_ptr(), ptr(r.gate),
+                                    r.gate.has_value() ? r.gate->numel() / r.hidden : 0, out.data_ptr(), normed.data_ptr(),
+                                    type_code(normed.scalar_type()), train ? rstd->data_ptr() : nullptr, r.rows, r.hidden,
+                                    (float)scale, (float)eps, stream_of(r.residual)));
     return {out, normed, rstd};
 }
 
-// Gradients of residual, delta, post, pre and gate, as far as they are wanted.
-std::vector<Opt> sandwich_bwd(const Tensor& s2, const Tensor& d2, const Tensor& post, const Tensor& pre, const Opt& gate2,
-                              const Tensor& rstd, const Tensor& d_stream, const Tensor& d_normed, double scale,
-                              const std::vector<bool>& wants) {
-    const c10::cuda::CUDAGuard guard(s2.device());
-    TORCH_CHECK(wants.size() == 5, "sandwich_bwd: five wishes");
-    const int64_t rows = s2.size(0), hidden = s2.size(1), gates = gate2.has_value() ? gate2->size(0) : 0;
-    std::vector<Opt> g(5);
-    const Tensor* like[] = {&s2, &d2, &post, &pre, gate2.has_value() ? &*gate2 : nullptr};
-    void* at_[5];
-    for (int i = 0; i < 5; ++i) {
-        if (wants[i] && like[i] != nullptr)
-            g[i] = rows == 0 ? at::zeros_like(*like[i]) : at::empty_like(*like[i]);
-        at_[i] = g[i].has_value() ? g[i]->data_ptr() : nullptr;
+struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& residual, const Tensor& delta, const Tensor& post,
+                                 const Tensor& pre, const Opt& gate, double scale, double eps, bool f32_out) {
+        const SandwichRows r = sandwich_rows(residual, delta, post, pre, gate);
+        auto [stream, normed, rstd] = sandwich_fwd(r, scale, eps, f32_out, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({stream, r.delta, r.post, r.pre, r.gate.has_value() ? *r.gate : Tensor(), *rstd});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["normed"] = (int64_t)normed.scalar_type();
+        ctx->saved_data["no rows"] = gate.has_value() && r.rows == 0;
+        if (gate.has_value()) ctx->saved_data["gate"] = gate->sizes().vec();
+        return {stream, normed};
     }
-    if (rows == 0) return g;
-    const int64_t need = nf4b200_sandwich_norm_workspace_bytes(rows, hidden, gates);
-    if (need < 0) check((int)need);
-    const Scratch ws(need, s2);
-    check(nf4b200_sandwich_norm_bwd(s2.const_data_ptr(), d2.const_data_ptr(), type_code(d2.scalar_type()),
-                                    post.const_data_ptr(), pre.const_data_ptr(), ptr(gate2), gates, rstd.const_data_ptr(),
-                                    d_stream.const_data_ptr(), d_normed.const_data_ptr(), type_code(d_normed.scalar_type()),
-                                    at_[0], at_[1], at_[2], at_[3], at_[4], rows, hidden, (float)scale, ws.get(),
-                                    (size_t)need, stream_of(s2)));
-    return g;
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto kept = ctx->get_saved_variables();
+        const Tensor &s = kept[0], &d = kept[1], &post = kept[2], &pre = kept[3], &gate = kept[4], &rstd = kept[5];
+        variable_list g(8);
+        if (!grads[0].defined() && !grads[1].defined()) return g;
+        const c10::cuda::CUDAGuard guard(s.device());
+        const int64_t hidden = s.size(-1), rows = s.numel() / hidden, gates = gate.defined() ? gate.numel() / hidden : 0;
+        const Tensor* like[] = {&s, &d, &post, &pre, &gate};
+        void* at_[5] = {};
+        for (int i = 0; i < 5; ++i) {
+            if (!like[i]->defined() || !ctx->needs_input_grad(i)) continue;
+            g[i] = rows == 0 ? at::zeros_like(*like[i]) : at::empty_like(*like[i]);
+            at_[i] = g[i].data_ptr();
+        }
+        if (rows == 0) {
+            if (ctx->saved_data["no rows"].toBool() && ctx->needs_input_grad(4))
+                g[4] = at::zeros(ctx->saved_data["gate"].toIntVector(), s.options());
+            return g;
+        }
+        const Tensor d_stream = grads[0].defined() ? grads[0].to(at::kFloat).contiguous() : Tensor();
+        const auto normed = (at::ScalarType)ctx->saved_data["normed"].toInt();
+        const Tensor d_normed = grads[1].defined() ? grads[1].to(normed).contiguous() : at::zeros(s.sizes(), s.options().dtype(normed));
+        const int64_t need = nf4b200_sandwich_norm_workspace_bytes(rows, hidden, gates);
+        if (need < 0) check((int)need);
+        const Scratch ws(need, s);
+        check(nf4b200_sandwich_norm_bwd(s.const_data_ptr(), d.const_data_ptr(), type_code(d.scalar_type()),
+                                        post.const_data_ptr(), pre.const_data_ptr(),
+                                        gate.defined() ? gate.const_data_ptr() : nullptr, gates, rstd.const_data_ptr(),
+                                        d_stream.defined() ? d_stream.const_data_ptr() : nullptr, d_normed.const_data_ptr(),
+                                        type_code(d_normed.scalar_type()), at_[0], at_[1], at_[2], at_[3], at_[4], rows, hidden,
+                                        (float)ctx->saved_data["scale"].toDouble(), ws.get(), (size_t)need, stream_of(s)));
+        return g;
+    }
+};
+
+// (stream, normed); gate: [hidden] or [gates, hidden] over the stream's rows. None for what it does not take.
+std::optional<std::tuple<Tensor, Tensor>> sandwich_norm(const Tensor& residual, const Tensor& delta, const Tensor& post,
+                                                        const Tensor& pre, const Opt& gate, double scale, double eps, bool f32_out) {
+    if (!residual.is_cuda() || residual.scalar_type() != at::kFloat || residual.dim() == 0 || delta.sizes() != residual.sizes() ||
+        delta.device() != residual.device())
+        return {};
+    const auto type = delta.scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) return {};
+    const int64_t hidden = residual.size(-1);
+    if (hidden < 1 || hidden > 16384) return {};
+    const int64_t rows = residual.numel() / hidden;
+    const auto weight = [&](const Tensor& w) { return w.scalar_type() == at::kFloat && w.device() == residual.device(); };
+    const auto row = [&](const Tensor& w) { return weight(w) && w.dim() == 1 && w.size(0) == hidden; };
+    if (!row(post) || !row(pre)) return {};
+    if (gate.has_value() && (!weight(*gate) || gate->dim() == 0 || gate->dim() > 2 || gate->size(-1) != hidden ||
+                             (rows > 0 && (gate->numel() == 0 || rows % (gate->numel() / hidden) != 0))))
+        return {};
+    if (at::GradMode::is_enabled() && (residual.requires_grad() || delta.requires_grad() || post.requires_grad() ||
+                                       pre.requires_grad() || (gate.has_value() && gate->requires_grad()))) {
+        const variable_list out = SandwichNorm::apply(residual, delta, post, pre, gate, scale, eps, f32_out);
+        return std::make_tuple(out[0], out[1]);
+    }
+    auto [stream, normed, rstd] = sandwich_fwd(sandwich_rows(residual, delta, post, pre, gate), scale, eps, f32_out, false);
+    return std::make_tuple(stream, normed);
 }
 
 // Weight of the vocabulary loss as the kernels read it.
@@ -470,6 +559,48 @@ std::tuple<Opt, Opt> vocab_loss_bwd(const Tensor& weight, const Tensor& kept, co
                                  dx.has_value() ? dx->data_ptr() : nullptr, dw.has_value() ? dw->data_ptr() : nullptr, rows,
                                  vocab, hidden, (int)grads, const_cast<void*>(kept.const_data_ptr()), ws.get(), (size_t)need, stream_of(w)));
     return {dx, dw};
+}
+
+struct VocabLoss : torch::autograd::Function<VocabLoss> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets,
+                                 int64_t grads) {
+        auto [losses, lse, kept] = vocab_loss_fwd(hidden, weight, targets, grads);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({weight, kept});
+        ctx->saved_data["grads"] = grads;
+        ctx->saved_data["rows"] = targets.numel();
+        ctx->saved_data["shape"] = hidden.sizes().vec();
+        return {losses.view(targets.sizes()), lse.view(targets.sizes())};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list g(4);
+        if (!grads[0].defined() && !grads[1].defined()) return g;
+        const auto kept = ctx->get_saved_variables();
+        const auto opt = [](const Tensor& t) { return t.defined() ? Opt(t) : Opt(); };
+        auto [dx, dw] = vocab_loss_bwd(kept[0], kept[1], opt(grads[0]), opt(grads[1]), ctx->saved_data["rows"].toInt(),
+                                       ctx->saved_data["grads"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        if (dx.has_value()) g[0] = dx->view(ctx->saved_data["shape"].toIntVector());
+        if (dw.has_value()) g[1] = *dw;
+        return g;
+    }
+};
+
+// (losses, logsumexps), or None for what it does not take.
+std::optional<std::tuple<Tensor, Tensor>> vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& targets) {
+    const auto type = hidden.scalar_type();
+    if (!hidden.is_cuda() || weight.device() != hidden.device() || targets.device() != hidden.device() ||
+        (type != at::kHalf && type != at::kBFloat16) || weight.scalar_type() != type || targets.scalar_type() != at::kLong ||
+        weight.dim() != 2 || hidden.dim() != targets.dim() + 1 || weight.size(0) == 0 || weight.size(1) == 0 ||
+        weight.size(1) % 8 != 0 || hidden.size(-1) != weight.size(1) || hidden.sizes().slice(0, targets.dim()) != targets.sizes())
+        return {};
+    int64_t grads = 0;
+    if (at::GradMode::is_enabled()) grads = (hidden.requires_grad() ? 1 : 0) | (weight.requires_grad() ? 2 : 0);
+    if (grads != 0) {
+        const variable_list out = VocabLoss::apply(hidden, weight, targets, grads);
+        return std::make_tuple(out[0], out[1]);
+    }
+    auto [losses, lse, kept] = vocab_loss_fwd(hidden, weight, targets, 0);
+    return std::make_tuple(losses.view(targets.sizes()), lse.view(targets.sizes()));
 }
 
 struct Rotation {   // everything about one rotation that is not a tensor
@@ -543,13 +674,11 @@ PYBIND11_MODULE(_host, m) {
     m.def("rmsnorm_bwd", &rmsnorm_bwd, unlocked());
     m.def("act8_quantize", &act8_quantize, unlocked());
     m.def("act8_dequantize", &act8_dequantize, unlocked());
-    m.def("act8_swiglu_fwd", &act8_swiglu_fwd, unlocked());
+    m.def("silu_mul_act8", &silu_mul_act8, unlocked());
     m.def("act8_swiglu_bwd", &act8_swiglu_bwd, unlocked());
     m.def("act8_lora_grad", &act8_lora_grad, unlocked());
-    m.def("sandwich_fwd", &sandwich_fwd, unlocked());
-    m.def("sandwich_bwd", &sandwich_bwd, unlocked());
-    m.def("vocab_loss_fwd", &vocab_loss_fwd, unlocked());
-    m.def("vocab_loss_bwd", &vocab_loss_bwd, unlocked());
+    m.def("sandwich_norm", &sandwich_norm, unlocked());
+    m.def("vocab_loss", &vocab_loss, unlocked());
     m.def("rotate_fwd", &rotate_fwd, unlocked());
     m.def("rotate_bwd", &rotate_bwd, unlocked());
 }

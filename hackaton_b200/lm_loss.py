@@ -178,28 +178,6 @@ def linear_cross_entropy(hidden, weight, targets, denom):
     return call(_HeadAndLoss(), hidden.contiguous(), weight, targets, denom)
 
 
-class _VocabLoss:
-    """lm_head + loss in pieces of the vocabulary (csrc/vocab_loss.cu). Next to the weight it keeps, for each row that
-    takes part, a few numbers, the softmax's mean of the weight (fp32) where the hidden states want a gradient, and the row
-    itself where the weight does."""
-
-    materialize = False
-
-    def __init__(self, grads):
-        self.grads = grads
-
-    def run(self, keep, hidden, weight, targets):
-        losses, lse, kept = _lib.host().vocab_loss_fwd(hidden, weight, targets, self.grads)
-        keep(weight, kept, shape=hidden.shape, rows=targets.numel())
-        return losses.reshape(targets.shape), lse.reshape(targets.shape)
-
-    def grad(self, kept, d_losses, d_lse):
-        weight, state = kept.tensors
-        d_hidden, d_weight = _lib.host().vocab_loss_bwd(weight, state, d_losses, d_lse, kept.rows, self.grads,
-                                                        kept.wants[0], kept.wants[1])
-        return None if d_hidden is None else d_hidden.reshape(kept.shape), d_weight, None
-
-
 def vocab_cross_entropy(hidden, weight, targets):
     """(losses, lse), both fp32 in the shape of `targets`: lse = logsumexp(hidden @ weightᵀ), loss = lse - the target's
     logit, without keeping the logits. hidden [..., features] and weight [vocab, features] are both fp16 or both
@@ -211,6 +189,13 @@ def vocab_cross_entropy(hidden, weight, targets):
     differences of sequences' log probabilities, and a penalty on lse are plain torch on top of them. Next to
     `linear_cross_entropy` (fp16, frozen head, one loss with its gradient made in the forward) this one takes bf16, gives
     the head's gradient and holds no block of logits."""
+    out = _lib.host().vocab_loss(hidden, weight, targets)
+    if out is None:
+        _refuse_vocab(hidden, weight, targets)
+    return out
+
+
+def _refuse_vocab(hidden, weight, targets):
     if not (hidden.is_cuda and weight.is_cuda and targets.is_cuda):
         raise ValueError("hackaton_b200: vocab_cross_entropy needs CUDA tensors (there is no CPU path)")
     if not hidden.device == weight.device == targets.device:
@@ -226,10 +211,4 @@ def vocab_cross_entropy(hidden, weight, targets):
     if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8 != 0:
         raise ValueError(f"hackaton_b200: vocab_cross_entropy: {weight.shape[0]} words of {weight.shape[1]} features (a "
                          "multiple of 8)")
-    grads = 0
-    if torch.is_grad_enabled():
-        grads = (1 if hidden.requires_grad else 0) | (2 if weight.requires_grad else 0)
-    if grads:
-        return call(_VocabLoss(grads), hidden, weight, targets)
-    losses, lse, _ = _lib.host().vocab_loss_fwd(hidden, weight, targets, 0)
-    return losses.reshape(targets.shape), lse.reshape(targets.shape)
+    raise ValueError("hackaton_b200: vocab_cross_entropy does not take these tensors")

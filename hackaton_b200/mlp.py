@@ -72,26 +72,15 @@ class SiluMul(torch.autograd.Function):
         return swiglu_backward(d_hidden, gate, up)
 
 
-class SiluMulAct8(torch.autograd.Function):
-    """silu(gate) * up; keeps gate and up in 8 bits (act8.py), written in the pass that forms the product."""
-
-    @staticmethod
-    def forward(ctx, gate, up):
-        _check_pair(gate, up)
-        hidden, *kept = _lib.host().act8_swiglu_fwd(_act8_rows(gate), _act8_rows(up))
-        ctx.save_for_backward(*kept)
-        return hidden.reshape(gate.shape)
-
-    @staticmethod
-    def backward(ctx, d_hidden):
-        d_gate, d_up = _lib.host().act8_swiglu_bwd(_act8_rows(d_hidden), *ctx.saved_tensors)
-        return d_gate.reshape(d_hidden.shape), d_up.reshape(d_hidden.shape)
-
-
 def silu_mul(gate, up, keep8=False):
-    """solution/kernels.py:94-96. With `keep8`, gate and up are kept in 8 bits for the backward (act8.py)."""
+    """solution/kernels.py:94-96. With `keep8`, gate and up are kept in 8 bits for the backward (act8.py), written in
+    the pass that forms the product."""
     if keep8 and torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-        return SiluMulAct8.apply(gate, up)
+        hidden = _lib.host().silu_mul_act8(gate, up)
+        if hidden is None:
+            _check_pair(gate, up)
+            raise ValueError(f"hackaton_b200: SwiGLU operands on {gate.device} and {up.device}")
+        return hidden
     return SiluMul.apply(gate, up)
 
 

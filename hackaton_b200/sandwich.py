@@ -13,7 +13,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._autograd import call
 
 MAX_HIDDEN = 16384
 
@@ -65,50 +64,22 @@ def _validate(residual, delta, post_weight, pre_weight, gate, out_dtype):
         raise ValueError("hackaton_b200: sandwich_norm weights do not match the last dimension")
 
 
-def _launch(op, residual, delta, post_weight, pre_weight, gate, train):
-    hidden = residual.shape[-1]
-    r2, d2 = residual.reshape(-1, hidden).contiguous(), delta.reshape(-1, hidden).contiguous()
-    post, pre = post_weight.contiguous(), pre_weight.contiguous()
-    g2 = None if gate is None or r2.shape[0] == 0 else _gate_rows(gate, residual.shape)
-    stream, normed, rstd = _lib.host().sandwich_fwd(r2, d2, post, pre, g2, op.scale, op.eps,
-                                                    op.out_dtype == torch.float32, train)
-    return stream, normed, rstd, (d2, post, pre, g2)
-
-
-class _SandwichOp:
-    def __init__(self, eps, scale, out_dtype):
-        self.eps, self.scale, self.out_dtype = eps, scale, out_dtype
-
-    def run(self, keep, residual, delta, post_weight, pre_weight, gate):
-        stream, normed, rstd, read = _launch(self, residual, delta, post_weight, pre_weight, gate, True)
-        keep(stream, *read, rstd, shape=residual.shape, gate_shape=None if gate is None else gate.shape)
-        return stream.reshape(residual.shape), normed.reshape(residual.shape)
-
-    def grad(self, kept, d_stream, d_normed):
-        stream, d2, post, pre, g2, rstd = kept.tensors
-        grads = _lib.host().sandwich_bwd(stream, d2, post, pre, g2, rstd,
-                                         d_stream.reshape(stream.shape).float().contiguous(),
-                                         d_normed.reshape(stream.shape).contiguous(), self.scale, list(kept.wants))
-        shapes = [kept.shape, kept.shape, post.shape, pre.shape, kept.gate_shape]
-        out = [None if g is None else g.reshape(shape) for g, shape in zip(grads, shapes)]
-        if kept.gate_shape is not None and g2 is None and kept.wants[4]:     # (no rows)
-            out[4] = torch.zeros(kept.gate_shape, dtype=torch.float32, device=stream.device)
-        return tuple(out)
-
-
 def sandwich_norm(residual, delta, post_weight, pre_weight, eps, gate=None, residual_scale=1.0, out_dtype=None):
     """(stream, normed) as above. residual: fp32 [..., hidden]; delta: the block's output, fp16, bf16 or fp32 of the same
     shape; post_weight, pre_weight: fp32 [hidden]; gate: None, or fp32 [hidden], or leading dimensions of the stream's
     followed by ones ([batch, 1, hidden] over [batch, tokens, hidden]), or [gates, hidden] over [rows, hidden] with row g
     for the g-th share of consecutive rows; residual_scale: a number; out_dtype of `normed`: delta's type (the default)
     or fp32. Gradients flow to all five tensors."""
-    out_dtype = delta.dtype if out_dtype is None else out_dtype
-    _validate(residual, delta, post_weight, pre_weight, gate, out_dtype)
-    if gate is not None and residual.numel() > 0:
-        _gate_rows(gate, residual.shape)
-    op = _SandwichOp(float(eps), float(residual_scale), out_dtype)
-    tensors = (residual, delta, post_weight, pre_weight, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return call(op, *tensors)
-    stream, normed, *_ = _launch(op, *tensors, False)
-    return stream.reshape(residual.shape), normed.reshape(residual.shape)
+    given = gate
+    if gate is not None and residual.dim() != 2 and gate.dim() > 1 and gate.shape[-1] == residual.shape[-1]:
+        gate = _gate_rows(gate, residual.shape) if residual.numel() else gate.reshape(-1, gate.shape[-1])
+    out = None
+    if out_dtype is None or out_dtype in (delta.dtype, torch.float32):
+        out = _lib.host().sandwich_norm(residual, delta, post_weight, pre_weight, gate, float(residual_scale), float(eps),
+                                        out_dtype is torch.float32)
+    if out is None:
+        _validate(residual, delta, post_weight, pre_weight, given, delta.dtype if out_dtype is None else out_dtype)
+        if given is not None:
+            _gate_rows(given, residual.shape)
+        raise ValueError("hackaton_b200: sandwich_norm does not take these tensors")
+    return out
