@@ -237,6 +237,7 @@ struct SandwichArgs {
     float* planes_pre;
     float* planes_gate;
     long long groups, group_rows, shares, share_rows, units, grid;
+    int depth;               // rows ahead
 };
 constexpr int SANDWICH_MAX_HIDDEN = 16384;
 long long sandwich_workspace_floats(long long rows, int hidden, long long gates, int sm_count);

@@ -10,9 +10,11 @@
 // The backward's second mean is linear in ds, so that both means come out of one reduction of three sums:
 //   mean(g ds dh) = mean(g dh (d_stream + rs w)) - rs mean(w sh) mean(g dh sh)
 // Memory bound: 4 + 4 bytes per value of the stream and 2 + 2 of 16-bit delta and y forward (12), 18 backward. A CTA
-// keeps a thread's columns of the weights in registers over all its rows, asks for the next row before it reduces
-// the present one, and adds the column sums of the weights' gradients in registers; a second kernel adds the CTAs'
-// sums in order, so that results do not depend on timing. All sums are fp32.
+// keeps a thread's columns of the weights in registers over all its rows; rows to come are on their way to shared
+// memory, each thread's own columns into slots that nobody else reads (cp.async, no barrier), four rows ahead forward and
+// three backward, since two or three CTAs of an SM with one row each in flight leave most of the bandwidth idle (one row
+// ahead in registers: 16,384 x 1536 82 and 129 us). Column sums of the weights' gradients stay in registers; a second
+// kernel adds the CTAs' sums in order, so that results do not depend on timing. All sums are fp32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -25,6 +27,7 @@ namespace nf4 {
 template <typename T, int VEC> struct SwRaw;
 
 template <> struct SwRaw<float, 4> {
+    static __device__ __forceinline__ void copy(uint32_t dst, const void* p, long long i) { cp_async16(dst, static_cast<const float*>(p) + i); }
     float4 v;
     __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)); }
     __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
@@ -33,6 +36,7 @@ template <> struct SwRaw<float, 4> {
     }
 };
 template <> struct SwRaw<__half, 4> {
+    static __device__ __forceinline__ void copy(uint32_t dst, const void* p, long long i) { cp_async8(dst, static_cast<const __half*>(p) + i); }
     uint2 v;
     __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(p) + i)); }
     __device__ __forceinline__ void get(float (&f)[4]) const {
@@ -45,6 +49,7 @@ template <> struct SwRaw<__half, 4> {
     }
 };
 template <> struct SwRaw<__nv_bfloat16, 4> {
+    static __device__ __forceinline__ void copy(uint32_t dst, const void* p, long long i) { cp_async8(dst, static_cast<const __nv_bfloat16*>(p) + i); }
     uint2 v;
     __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i)); }
     __device__ __forceinline__ void get(float (&f)[4]) const {
@@ -68,6 +73,47 @@ template <typename T> struct SwRaw<T, 1> {
     __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = sw_float(v); }
     static __device__ __forceinline__ void store(void* p, long long i, const float (&f)[1]) { sw_round(f[0], static_cast<T*>(p)[i]); }
 };
+
+// Rows on their way: `depth` slots of what a thread's columns take of one array, [slot][i][thread]. Rows of single
+// values (VEC = 1) go through registers, one row ahead.
+template <typename T, int NV, int VEC>
+struct SwRing {
+    SwRaw<T, VEC> next[VEC == 4 ? 1 : NV];
+    uint32_t base;     // this thread's place in slot 0
+    // Bytes of the ring; `at` moves behind it.
+    __device__ __forceinline__ void place(uint32_t& at, int depth) {
+        if (VEC != 4) return;
+        base = at + threadIdx.x * (4 * sizeof(T));
+        at += depth * NV * blockDim.x * (4 * sizeof(T));
+    }
+    __device__ __forceinline__ void ask(int slot, int i, const void* p, long long index) {
+        if constexpr (VEC == 4) SwRaw<T, 4>::copy(base + (slot * NV + i) * blockDim.x * (4 * sizeof(T)), p, index);
+        else                    next[i].load(p, index);
+    }
+    __device__ __forceinline__ void get(int slot, int i, float (&f)[VEC]) const {
+        if constexpr (VEC == 4) {
+            const uint32_t a = base + (slot * NV + i) * blockDim.x * (4 * sizeof(T));
+            SwRaw<T, 4> raw;
+            if constexpr (sizeof(T) == 4)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(raw.v.x), "=f"(raw.v.y), "=f"(raw.v.z), "=f"(raw.v.w) : "r"(a));
+            else
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(raw.v.x), "=r"(raw.v.y) : "r"(a));
+            raw.get(f);
+        } else {
+            next[i].get(f);
+        }
+    }
+};
+
+constexpr int SW_FWD_DEPTH = 4, SW_BWD_DEPTH = 3;      // where shared memory allows
+
+// Waits for this thread's copies of the oldest of `depth` rows.
+__device__ __forceinline__ void sw_oldest(int depth) {
+    if (depth >= 4)      cp_async_wait<3>();
+    else if (depth == 3) cp_async_wait<2>();
+    else if (depth == 2) cp_async_wait<1>();
+    else                 cp_async_wait<0>();
+}
 
 // Sums of N values over the CTA, the same in every thread. `part` has two halves that successive calls take in
 // turn: who writes a half again has passed the barrier behind which everybody had read it.
@@ -108,8 +154,8 @@ __device__ __forceinline__ void sw_weights(const float* p, int hidden, float fil
     }
 }
 
-template <int NV, int VEC, typename TD, typename TY>
-__global__ void __launch_bounds__(1024)
+template <int NV, int VEC, typename TD, typename TY, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1)
 sandwich_fwd_kernel(const SandwichArgs a) {
     grid_dep_wait();
     grid_dep_launch();
@@ -128,22 +174,30 @@ sandwich_fwd_kernel(const SandwichArgs a) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) post[i][e] *= gate[i][e];
     }
-    SwRaw<float, VEC> next_r[NV];
-    SwRaw<TD, VEC> next_d[NV];
-    const auto fetch = [&](long long row) {
-        if (row >= a.rows) return;
+    const int depth = VEC == 4 ? a.depth : 1;
+    extern __shared__ uint4 sw_smem[];
+    uint32_t room = smem_u32(sw_smem);
+    SwRing<float, NV, VEC> ring_r;
+    SwRing<TD, NV, VEC> ring_d;
+    ring_r.place(room, depth);
+    ring_d.place(room, depth);
+    const auto fetch = [&](long long row, int slot) {
+        if (row < a.rows) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            if (c < hidden) {
-                next_d[i].load(a.delta, row * hidden + c);
-                next_r[i].load(a.residual, row * hidden + c);
+            for (int i = 0; i < NV; ++i) {
+                const int c = (threadIdx.x + i * blockDim.x) * VEC;
+                if (c < hidden) {
+                    ring_d.ask(slot, i, a.delta, row * hidden + c);
+                    ring_r.ask(slot, i, a.residual, row * hidden + c);
+                }
             }
         }
+        if (VEC == 4) cp_async_commit();
     };
     long long row = blockIdx.x;
-    fetch(row);
-    for (; row < a.rows; row += gridDim.x) {
+    for (int k = 0; k < depth; ++k) fetch(row + (long long)k * gridDim.x, k);
+    for (int slot = 0; row < a.rows; row += gridDim.x, slot = slot + 1 == depth ? 0 : slot + 1) {
+        if (VEC == 4) sw_oldest(depth);
         float d[NV][VEC], s[NV][VEC], sum[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -151,15 +205,16 @@ sandwich_fwd_kernel(const SandwichArgs a) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) d[i][e] = s[i][e] = 0.f;
             if (c < hidden) {
-                next_d[i].get(d[i]);
-                next_r[i].get(s[i]);
+                ring_d.get(slot, i, d[i]);
+                ring_r.get(slot, i, s[i]);
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) sum[0] += d[i][e] * d[i][e];
         }
-        fetch(row + gridDim.x);
+        if (VEC != 4) fetch(row + gridDim.x, 0);
         sw_block_sum<1>(sum, part, turn);
         const float rd = 1.f / sqrtf(sum[0] * inv_h + a.eps);
+        if (VEC == 4) fetch(row + (long long)depth * gridDim.x, slot);    // (behind the barrier: the slot has been read)
         sum[0] = 0.f;
         const float* gate_row = a.gates > 1 ? a.gate + row / a.group_rows * hidden : nullptr;
 #pragma unroll
@@ -201,8 +256,8 @@ sandwich_fwd_kernel(const SandwichArgs a) {
 }
 
 // A unit is a share of the rows that one gate row serves; a CTA takes units blockIdx.x, + gridDim.x, ...
-template <int NV, int VEC, typename TD, typename TY>
-__global__ void __launch_bounds__(1024)
+template <int NV, int VEC, typename TD, typename TY, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1)
 sandwich_bwd_kernel(const SandwichArgs a) {
     grid_dep_wait();
     grid_dep_launch();
@@ -219,63 +274,89 @@ sandwich_bwd_kernel(const SandwichArgs a) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sum_post[i][e] = sum_pre[i][e] = sum_unit[i][e] = 0.f;
 
-    SwRaw<float, VEC> next_s[NV], next_t[NV];
-    SwRaw<TD, VEC> next_d[NV];
-    SwRaw<TY, VEC> next_y[NV];
-    float next_rd = 0.f, next_rs = 0.f;
-    const auto fetch = [&](long long row) {
-        next_rd = a.rstd[2 * row];
-        next_rs = a.rstd[2 * row + 1];
+    const int depth = VEC == 4 ? a.depth : 1;
+    extern __shared__ uint4 sw_smem[];
+    uint32_t room = smem_u32(sw_smem);
+    SwRing<float, NV, VEC> ring_s, ring_t;
+    SwRing<TD, NV, VEC> ring_d;
+    SwRing<TY, NV, VEC> ring_y;
+    ring_s.place(room, depth);
+    ring_t.place(room, depth);
+    ring_d.place(room, depth);
+    ring_y.place(room, depth);
+    const uint32_t ring_rstd = room + threadIdx.x * 8;      // (a copy for every thread)
+    float2 next_rstd = make_float2(0.f, 0.f);
+    const auto fetch = [&](int row, int slot) {      // (a negative row: nothing)
+        if (row >= 0) {
+            const long long at = (long long)row * hidden;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            if (c < hidden) {
-                next_s[i].load(a.stream, row * hidden + c);
-                next_d[i].load(a.delta, row * hidden + c);
-                next_y[i].load(a.d_normed, row * hidden + c);
-                if (a.d_stream != nullptr) next_t[i].load(a.d_stream, row * hidden + c);
+            for (int i = 0; i < NV; ++i) {
+                const int c = (threadIdx.x + i * blockDim.x) * VEC;
+                if (c < hidden) {
+                    ring_s.ask(slot, i, a.stream, at + c);
+                    ring_d.ask(slot, i, a.delta, at + c);
+                    ring_y.ask(slot, i, a.d_normed, at + c);
+                    if (a.d_stream != nullptr) ring_t.ask(slot, i, a.d_stream, at + c);
+                }
             }
+            if (VEC == 4) cp_async8(ring_rstd + slot * blockDim.x * 8, a.rstd + 2ll * row);
+            else          next_rstd = *reinterpret_cast<const float2*>(a.rstd + 2ll * row);
         }
+        if (VEC == 4) cp_async_commit();
     };
-    const auto first_row = [&](long long unit) { return unit / a.shares * a.group_rows + unit % a.shares * a.share_rows; };
-    const auto end_row = [&](long long unit) {
-        const long long group = unit / a.shares;
-        return min(group * a.group_rows + (unit % a.shares + 1) * a.share_rows, (group + 1) * a.group_rows);
+    // two walks over this CTA's rows: the one that asks for them is depth rows ahead of the one that works on them
+    const int shares = (int)a.shares, share_rows = (int)a.share_rows, group_rows = (int)a.group_rows, units = (int)a.units;
+    struct Walk {
+        int unit, row, end;
     };
-    long long unit = blockIdx.x;   // (gridDim.x <= units)
-    long long row = first_row(unit), end = end_row(unit);
-    fetch(row);
-    while (true) {
-        if (a.gates > 1 && row == first_row(unit))
-            sw_weights<NV, VEC>(a.gate + unit / a.shares * hidden, hidden, 0.f, gate);
+    const auto enter = [&](Walk& w) {
+        const int group = w.unit / shares, share = w.unit - group * shares;
+        w.row = group * group_rows + share * share_rows;
+        w.end = min(w.row + share_rows, (group + 1) * group_rows);
+    };
+    const auto step = [&](Walk& w) {     // row -1 behind the last one
+        if (w.row < 0 || ++w.row < w.end) return;
+        w.unit += gridDim.x;
+        if (w.unit < units) enter(w);
+        else                w.row = -1;
+    };
+    Walk ahead;
+    ahead.unit = blockIdx.x;   // (gridDim.x <= units)
+    enter(ahead);
+    Walk now = ahead;
+    for (int k = 0; k < depth; ++k) {
+        fetch(ahead.row, k);
+        step(ahead);
+    }
+    bool new_unit = true;
+    for (int slot = 0; now.row >= 0; slot = slot + 1 == depth ? 0 : slot + 1) {
+        if (VEC == 4) sw_oldest(depth);
+        if (a.gates > 1 && new_unit) sw_weights<NV, VEC>(a.gate + (long long)(now.unit / shares) * hidden, hidden, 0.f, gate);
+        float2 rstd = next_rstd;
+        if (VEC == 4) asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(rstd.x), "=f"(rstd.y) : "r"(ring_rstd + slot * blockDim.x * 8));
+        const float rd = rstd.x, rs = rstd.y;
         float s[NV][VEC], t[NV][VEC], d[NV][VEC], y[NV][VEC], sum[3] = {0.f, 0.f, 0.f};
-        const float rd = next_rd, rs = next_rs;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (threadIdx.x + i * blockDim.x) * VEC;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s[i][e] = t[i][e] = d[i][e] = y[i][e] = 0.f;
             if (c < hidden) {
-                next_s[i].get(s[i]);
-                next_d[i].get(d[i]);
-                next_y[i].get(y[i]);
-                if (a.d_stream != nullptr) next_t[i].get(t[i]);
+                ring_s.get(slot, i, s[i]);
+                ring_d.get(slot, i, d[i]);
+                ring_y.get(slot, i, y[i]);
+                if (a.d_stream != nullptr) ring_t.get(slot, i, t[i]);
             }
         }
-        const long long at = row * hidden;
-        bool unit_done = false, done = false;
-        const long long this_unit = unit;
-        if (++row == end) {
-            unit_done = true;
-            unit += gridDim.x;
-            if (unit < a.units) {
-                row = first_row(unit);
-                end = end_row(unit);
-            } else {
-                done = true;
-            }
+        const long long at = (long long)now.row * hidden;
+        const int this_unit = now.unit;
+        step(now);
+        const bool unit_done = now.row < 0 || now.unit != this_unit;
+        new_unit = unit_done;
+        if (VEC != 4) {
+            fetch(ahead.row, 0);
+            step(ahead);
         }
-        if (!done) fetch(row);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -290,6 +371,10 @@ sandwich_bwd_kernel(const SandwichArgs a) {
                 sum_pre[i][e] += y[i][e] * s[i][e];
             }
         sw_block_sum<3>(sum, part, turn);
+        if (VEC == 4) {       // (behind the barrier: the slot has been read)
+            fetch(ahead.row, slot);
+            step(ahead);
+        }
         const float m1 = rs * (sum[0] * inv_h);
         const float m2 = (sum[1] - m1 * sum[2]) * inv_h;
 #pragma unroll
@@ -321,10 +406,9 @@ sandwich_bwd_kernel(const SandwichArgs a) {
                 }
                 // (one share per gate row: the row itself; otherwise the shares' plane)
                 if (a.d_gate != nullptr && c < hidden)
-                    SwRaw<float, VEC>::store(a.shares == 1 ? a.d_gate : a.planes_gate, this_unit * hidden + c, dg);
+                    SwRaw<float, VEC>::store(shares == 1 ? a.d_gate : a.planes_gate, (long long)this_unit * hidden + c, dg);
             }
         }
-        if (done) break;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -364,26 +448,47 @@ sandwich_sum_kernel(const SandwichArgs a) {
 
 // ------------------------------------------------------------------------------------------- host side
 struct SandwichShape {
-    int vec, nv, threads;
+    int vec, nv, threads, depth;
+    size_t smem;      // of the rings
 };
 
 // Columns per thread: one float4 as far as a CTA reaches, then two and four; single values for rows that are
-// no whole float4 or not aligned.
-static SandwichShape sandwich_shape(int hidden, bool vec) {
-    SandwichShape s;
+// no whole float4, not aligned, or too long for one of them in shared memory.
+static SandwichShape sandwich_shape(int hidden, bool vec, bool backward, int delta_type, int normed_type) {
+    const size_t room = (227 << 10) - 2048;
+    SandwichShape s = {};
     s.vec = vec && hidden % 4 == 0 ? 4 : 1;
-    const int items = (hidden + s.vec - 1) / s.vec;
-    if (s.vec == 4) s.nv = items <= 1024 ? 1 : items <= 2048 ? 2 : 4;
-    else            s.nv = items <= 4096 ? 4 : 16;
-    s.threads = ((items + s.nv - 1) / s.nv + 31) / 32 * 32;
-    return s;
+    for (;;) {
+        const int items = (hidden + s.vec - 1) / s.vec;
+        if (s.vec == 4) s.nv = items <= 1024 ? 1 : items <= 2048 ? 2 : 4;
+        else            s.nv = items <= 4096 ? 4 : 16;
+        s.threads = ((items + s.nv - 1) / s.nv + 31) / 32 * 32;
+        if (s.vec != 4) return s;
+        const size_t d = delta_type == 2 ? 16 : 8, y = normed_type == 2 ? 16 : 8;
+        const size_t row = (size_t)s.nv * s.threads * (backward ? 32 + d + y : 16 + d) + (backward ? (size_t)s.threads * 8 : 0);
+        s.depth = backward ? SW_BWD_DEPTH : SW_FWD_DEPTH;
+        while (s.depth > 0 && s.depth * row > room) --s.depth;
+        s.smem = s.depth * row;
+        if (s.depth > 0) return s;
+        s.vec = 1;
+        s.smem = 0;
+    }
+}
+
+// CTAs that an SM holds: up to 56 registers a thread forward, 80 backward (64 where a CTA has more than SW_FEW threads),
+// the rings.
+constexpr int SW_FEW = 384;
+static long long sandwich_resident(const SandwichShape& s, bool backward) {
+    long long n = backward ? (s.threads <= SW_FEW ? 768 / s.threads : 1) : 1152 / s.threads;
+    if (s.smem > 0 && (long long)((227 << 10) / (s.smem + 2048)) < n) n = (long long)((227 << 10) / (s.smem + 2048));
+    return n < 1 ? 1 : n > 16 ? 16 : n;
 }
 
 // Backward: CTAs, and how the rows of a gate row are shared among them.
-static void sandwich_plan(SandwichArgs& a, int threads) {
+static void sandwich_plan(SandwichArgs& a, const SandwichShape& s) {
     a.groups = a.gates > 0 ? a.gates : 1;
     a.group_rows = a.rows / a.groups;
-    long long target = (long long)a.sm_count * (threads >= 1024 ? 1 : threads > 512 ? 2 : threads > 128 ? 1024 / threads : 8);
+    const long long target = a.sm_count * sandwich_resident(s, true);
     long long shares = target / a.groups;
     if (shares > a.group_rows) shares = a.group_rows;
     if (shares < 1) shares = 1;
@@ -395,30 +500,38 @@ static void sandwich_plan(SandwichArgs& a, int threads) {
 
 long long sandwich_workspace_floats(long long rows, int hidden, long long gates, int sm_count) {
     long long most = 0;
-    for (int vec = 0; vec < 2; ++vec) {   // (alignment is not known yet)
+    for (int k = 0; k < 8; ++k) {   // (alignment and types are not known yet)
         SandwichArgs a = {};
         a.rows = rows; a.hidden = hidden; a.gates = gates; a.sm_count = sm_count;
-        sandwich_plan(a, sandwich_shape(hidden, vec != 0).threads);
+        a.delta_type = k & 2; a.normed_type = k & 4 ? 2 : 0;
+        sandwich_plan(a, sandwich_shape(hidden, (k & 1) != 0, true, a.delta_type, a.normed_type));
         const long long planes = 2 * a.grid + (a.gates > 0 && a.shares > 1 ? a.units : 0);
         if (planes > most) most = planes;
     }
     return most * hidden;
 }
 
+template <int NV, int VEC, typename TD, typename TY>
+static cudaError_t sandwich_with(const SandwichArgs& a, const SandwichShape& s, bool backward, unsigned grid, cudaStream_t stream) {
+    constexpr int MANY = 1024, FEW = SW_FEW;      // what a kernel may take in registers goes by its threads
+    auto kernel = backward ? (s.threads > FEW ? sandwich_bwd_kernel<NV, VEC, TD, TY, MANY> : sandwich_bwd_kernel<NV, VEC, TD, TY, FEW>)
+                           : (s.threads > FEW ? sandwich_fwd_kernel<NV, VEC, TD, TY, MANY> : sandwich_fwd_kernel<NV, VEC, TD, TY, FEW>);
+    if (s.smem > (40 << 10)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(kernel, dim3(grid), dim3((unsigned)s.threads), s.smem, stream, a);
+}
+
 template <typename TD, typename TY>
 static cudaError_t sandwich_as(const SandwichArgs& a, const SandwichShape& s, bool backward, unsigned grid, cudaStream_t stream) {
-    const dim3 g(grid), b((unsigned)s.threads);
-#define NF4_SANDWICH(NV, VEC) \
-    return backward ? launch_pdl(sandwich_bwd_kernel<NV, VEC, TD, TY>, g, b, 0, stream, a) \
-                    : launch_pdl(sandwich_fwd_kernel<NV, VEC, TD, TY>, g, b, 0, stream, a)
     if (s.vec == 4) {
-        if (s.nv == 1) NF4_SANDWICH(1, 4);
-        if (s.nv == 2) NF4_SANDWICH(2, 4);
-        NF4_SANDWICH(4, 4);
+        if (s.nv == 1) return sandwich_with<1, 4, TD, TY>(a, s, backward, grid, stream);
+        if (s.nv == 2) return sandwich_with<2, 4, TD, TY>(a, s, backward, grid, stream);
+        return sandwich_with<4, 4, TD, TY>(a, s, backward, grid, stream);
     }
-    if (s.nv == 4) NF4_SANDWICH(4, 1);
-    NF4_SANDWICH(16, 1);
-#undef NF4_SANDWICH
+    if (s.nv == 4) return sandwich_with<4, 1, TD, TY>(a, s, backward, grid, stream);
+    return sandwich_with<16, 1, TD, TY>(a, s, backward, grid, stream);
 }
 
 cudaError_t launch_sandwich(const SandwichArgs& a_in, bool backward, cudaStream_t stream) {
@@ -430,15 +543,16 @@ cudaError_t launch_sandwich(const SandwichArgs& a_in, bool backward, cudaStream_
                           (const void*)a.d_residual, (const void*)a.d_delta, (const void*)a.d_post, (const void*)a.d_pre,
                           (const void*)a.d_gate, (const void*)a.planes_post})
         bits |= reinterpret_cast<uintptr_t>(p);
-    const SandwichShape s = sandwich_shape(a.hidden, (bits & 15) == 0);
-    sandwich_plan(a, s.threads);
+    const SandwichShape s = sandwich_shape(a.hidden, (bits & 15) == 0, backward, a.delta_type, a.normed_type);
+    a.depth = s.depth;
+    sandwich_plan(a, s);
     unsigned grid;
     if (backward) {
         a.planes_pre = a.planes_post + a.grid * a.hidden;
         a.planes_gate = a.planes_pre + a.grid * a.hidden;
         grid = (unsigned)a.grid;
     } else {
-        const long long target = (long long)a.sm_count * (2048 / s.threads > 8 ? 8 : 2048 / s.threads);
+        const long long target = a.sm_count * sandwich_resident(s, false);
         grid = (unsigned)(a.rows < target ? a.rows : target);
     }
     cudaError_t e;
