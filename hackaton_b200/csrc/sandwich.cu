@@ -105,6 +105,8 @@ struct SwRing {
     }
 };
 
+// Threads up to which a kernel may take 80 registers each forward and 128 backward.
+constexpr int SW_FEW_FWD = 256, SW_FEW_BWD = 512;
 constexpr int SW_FWD_DEPTH = 4, SW_BWD_DEPTH = 3;      // where shared memory allows
 
 // Waits for this thread's copies of the oldest of `depth` rows.
@@ -115,8 +117,10 @@ __device__ __forceinline__ void sw_oldest(int depth) {
     else                 cp_async_wait<0>();
 }
 
-// Sums of N values over the CTA, the same in every thread. `part` has two halves that successive calls take in
-// turn: who writes a half again has passed the barrier behind which everybody had read it.
+// Sums of N values over the CTA, the same in every thread: a warp's by shuffles, the warps' by every thread for itself
+// (a broadcast load per four warps; shuffles are what a row of few columns per thread spends its time on). `part` has two
+// halves that successive calls take in turn: who writes a half again has passed the barrier behind which everybody
+// had read it. What belongs to warps that are not there is zero from the start.
 template <int N>
 __device__ __forceinline__ void sw_block_sum(float (&v)[N], float (*part)[N][32], int& turn) {
 #pragma unroll
@@ -130,13 +134,22 @@ __device__ __forceinline__ void sw_block_sum(float (&v)[N], float (*part)[N][32]
             for (int n = 0; n < N; ++n) part[turn][n][threadIdx.x >> 5] = v[n];
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < N; ++n) v[n] = lane < warps ? part[turn][n][lane] : 0.f;
+        for (int n = 0; n < N; ++n) v[n] = 0.f;
+        for (int w = 0; w < warps; w += 4)
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+            for (int n = 0; n < N; ++n) {
+                const float4 x = *reinterpret_cast<const float4*>(&part[turn][n][w]);
+                v[n] += (x.x + x.y) + (x.z + x.w);
+            }
         turn ^= 1;
     }
+}
+
+// (the barrier in the first sum comes behind this for every half that is read)
+template <int N>
+__device__ __forceinline__ void sw_clear(float (*part)[N][32]) {
+    for (int i = threadIdx.x; i < 2 * N * 32; i += blockDim.x)
+        if ((i & 31) >= (int)(blockDim.x >> 5)) (&part[0][0][0])[i] = 0.f;
 }
 
 template <int NV, int VEC>
@@ -155,12 +168,13 @@ __device__ __forceinline__ void sw_weights(const float* p, int hidden, float fil
 }
 
 template <int NV, int VEC, typename TD, typename TY, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1)
+__global__ void __launch_bounds__(MAXT, MAXT <= SW_FEW_FWD ? 3 : 1)
 sandwich_fwd_kernel(const SandwichArgs a) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ float part[2][1][32];
+    __shared__ __align__(16) float part[2][1][32];
     int turn = 0;
+    sw_clear<1>(part);
     const int hidden = a.hidden;
     const float inv_h = 1.f / (float)hidden;
     float post[NV][VEC], pre[NV][VEC];
@@ -257,12 +271,13 @@ sandwich_fwd_kernel(const SandwichArgs a) {
 
 // A unit is a share of the rows that one gate row serves; a CTA takes units blockIdx.x, + gridDim.x, ...
 template <int NV, int VEC, typename TD, typename TY, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1)
+__global__ void __launch_bounds__(MAXT, 1)
 sandwich_bwd_kernel(const SandwichArgs a) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ float part[2][3][32];
+    __shared__ __align__(16) float part[2][3][32];
     int turn = 0;
+    sw_clear<3>(part);
     const int hidden = a.hidden;
     const float inv_h = 1.f / (float)hidden;
     float post[NV][VEC], pre[NV][VEC], gate[NV][VEC], sum_post[NV][VEC], sum_pre[NV][VEC], sum_unit[NV][VEC];
@@ -452,15 +467,17 @@ struct SandwichShape {
     size_t smem;      // of the rings
 };
 
-// Columns per thread: one float4 as far as a CTA reaches, then two and four; single values for rows that are
-// no whole float4, not aligned, or too long for one of them in shared memory.
-static SandwichShape sandwich_shape(int hidden, bool vec, bool backward, int delta_type, int normed_type) {
+// Columns per thread: two or four float4 where a row is then left to eight warps or fewer (its sums cost every warp ten
+// shuffles and more: 16,384 x 1536 with one float4 74 and 97 us, PLACEHOLDER), as many as registers hold backward; one where there
+// are few rows and latency counts; single values for rows that are no whole float4, not aligned, or too long for one of
+// them in shared memory.
+static SandwichShape sandwich_shape(int hidden, bool vec, bool few, bool backward, int delta_type, int normed_type) {
     const size_t room = (227 << 10) - 2048;
     SandwichShape s = {};
     s.vec = vec && hidden % 4 == 0 ? 4 : 1;
     for (;;) {
         const int items = (hidden + s.vec - 1) / s.vec;
-        if (s.vec == 4) s.nv = items <= 1024 ? 1 : items <= 2048 ? 2 : 4;
+        if (s.vec == 4) s.nv = items <= (few ? 1024 : backward ? 192 : 256) ? 1 : items <= (few ? 2048 : backward ? 1024 : 512) ? 2 : 4;
         else            s.nv = items <= 4096 ? 4 : 16;
         s.threads = ((items + s.nv - 1) / s.nv + 31) / 32 * 32;
         if (s.vec != 4) return s;
@@ -475,11 +492,9 @@ static SandwichShape sandwich_shape(int hidden, bool vec, bool backward, int del
     }
 }
 
-// CTAs that an SM holds: up to 56 registers a thread forward, 80 backward (64 where a CTA has more than SW_FEW threads),
-// the rings.
-constexpr int SW_FEW = 384;
+// CTAs that an SM holds, by registers and the rings.
 static long long sandwich_resident(const SandwichShape& s, bool backward) {
-    long long n = backward ? (s.threads <= SW_FEW ? 768 / s.threads : 1) : 1152 / s.threads;
+    long long n = backward ? (s.threads <= SW_FEW_BWD ? SW_FEW_BWD / s.threads : 1) : (s.threads <= SW_FEW_FWD ? 768 : 1024) / s.threads;
     if (s.smem > 0 && (long long)((227 << 10) / (s.smem + 2048)) < n) n = (long long)((227 << 10) / (s.smem + 2048));
     return n < 1 ? 1 : n > 16 ? 16 : n;
 }
@@ -500,11 +515,12 @@ static void sandwich_plan(SandwichArgs& a, const SandwichShape& s) {
 
 long long sandwich_workspace_floats(long long rows, int hidden, long long gates, int sm_count) {
     long long most = 0;
+    const bool few = rows <= 2 * sm_count;
     for (int k = 0; k < 8; ++k) {   // (alignment and types are not known yet)
         SandwichArgs a = {};
         a.rows = rows; a.hidden = hidden; a.gates = gates; a.sm_count = sm_count;
         a.delta_type = k & 2; a.normed_type = k & 4 ? 2 : 0;
-        sandwich_plan(a, sandwich_shape(hidden, (k & 1) != 0, true, a.delta_type, a.normed_type));
+        sandwich_plan(a, sandwich_shape(hidden, (k & 1) != 0, few, true, a.delta_type, a.normed_type));
         const long long planes = 2 * a.grid + (a.gates > 0 && a.shares > 1 ? a.units : 0);
         if (planes > most) most = planes;
     }
@@ -513,9 +529,8 @@ long long sandwich_workspace_floats(long long rows, int hidden, long long gates,
 
 template <int NV, int VEC, typename TD, typename TY>
 static cudaError_t sandwich_with(const SandwichArgs& a, const SandwichShape& s, bool backward, unsigned grid, cudaStream_t stream) {
-    constexpr int MANY = 1024, FEW = SW_FEW;      // what a kernel may take in registers goes by its threads
-    auto kernel = backward ? (s.threads > FEW ? sandwich_bwd_kernel<NV, VEC, TD, TY, MANY> : sandwich_bwd_kernel<NV, VEC, TD, TY, FEW>)
-                           : (s.threads > FEW ? sandwich_fwd_kernel<NV, VEC, TD, TY, MANY> : sandwich_fwd_kernel<NV, VEC, TD, TY, FEW>);
+    auto kernel = backward ? (s.threads > SW_FEW_BWD ? sandwich_bwd_kernel<NV, VEC, TD, TY, 1024> : sandwich_bwd_kernel<NV, VEC, TD, TY, SW_FEW_BWD>)
+                           : (s.threads > SW_FEW_FWD ? sandwich_fwd_kernel<NV, VEC, TD, TY, 1024> : sandwich_fwd_kernel<NV, VEC, TD, TY, SW_FEW_FWD>);
     if (s.smem > (40 << 10)) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem);
         if (e != cudaSuccess) return e;
@@ -543,7 +558,7 @@ cudaError_t launch_sandwich(const SandwichArgs& a_in, bool backward, cudaStream_
                           (const void*)a.d_residual, (const void*)a.d_delta, (const void*)a.d_post, (const void*)a.d_pre,
                           (const void*)a.d_gate, (const void*)a.planes_post})
         bits |= reinterpret_cast<uintptr_t>(p);
-    const SandwichShape s = sandwich_shape(a.hidden, (bits & 15) == 0, backward, a.delta_type, a.normed_type);
+    const SandwichShape s = sandwich_shape(a.hidden, (bits & 15) == 0, a.rows <= 2 * a.sm_count, backward, a.delta_type, a.normed_type);
     a.depth = s.depth;
     sandwich_plan(a, s);
     unsigned grid;
