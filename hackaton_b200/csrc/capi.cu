@@ -976,7 +976,7 @@ int nf4b200_sandwich_norm_fwd(const void* residual, const void* delta, int delta
     a.post = static_cast<const float*>(post); a.pre = static_cast<const float*>(pre); a.gate = static_cast<const float*>(gate);
     a.stream = static_cast<float*>(stream_out); a.normed = normed; a.rstd = static_cast<float*>(rstd);
     a.rows = rows; a.hidden = (int)hidden; a.gates = gates; a.scale = scale; a.eps = eps;
-    a.delta_type = delta_dtype; a.normed_type = normed_dtype; a.sm_count = d->sms;
+    a.delta_type = delta_dtype; a.normed_type = normed_dtype; a.sm_count = d->sms; a.status = nf4::device_status_word();
     cudaError_t e = nf4::launch_sandwich(a, false, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(NF4B200_ECUDA, "sandwich_norm_fwd: %s", cudaGetErrorString(e));
     return NF4B200_OK;
@@ -1014,7 +1014,7 @@ int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delt
     a.d_post = static_cast<float*>(d_post); a.d_pre = static_cast<float*>(d_pre); a.d_gate = static_cast<float*>(d_gate);
     a.planes_post = static_cast<float*>(workspace);
     a.rows = rows; a.hidden = (int)hidden; a.gates = gates; a.scale = scale;
-    a.delta_type = delta_dtype; a.normed_type = normed_dtype; a.sm_count = d->sms;
+    a.delta_type = delta_dtype; a.normed_type = normed_dtype; a.sm_count = d->sms; a.status = nf4::device_status_word();
     cudaError_t e = nf4::launch_sandwich(a, true, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(NF4B200_ECUDA, "sandwich_norm_bwd: %s", cudaGetErrorString(e));
     return NF4B200_OK;

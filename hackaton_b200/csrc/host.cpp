@@ -425,7 +425,7 @@ std::tuple<Tensor, Tensor, Opt> sandwich_fwd(const SandwichRows& r, double scale
     Tensor out = at::empty_like(r.residual);
     Tensor normed = at::empty(r.residual.sizes(), r.delta.options().dtype(f32_out ? at::kFloat : r.delta.scalar_type()));
     Opt rstd;
-    if (train) rstd = at::empty({r.rows, 2}, r.residual.options());
+    if (train) rstd = at::empty({r.rows, 4}, r.residual.options());
     check(nf4b200_sandwich_norm_fwd(r.residual.const_data_ptr(), r.delta.const_data_ptr(), type_code(r.delta.scalar_type()),
                                     r.post.const_data_ptr(), r.pre.const_data_ptr(), ptr(r.gate),
                                     r.gate.has_value() ? r.gate->numel() / r.hidden : 0, out.data_ptr(), normed.data_ptr(),

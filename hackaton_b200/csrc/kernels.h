@@ -218,7 +218,7 @@ struct SandwichArgs {
     const float* gate;       // [gates, hidden], or null (gates = 0)
     float* stream;           // [rows, hidden]: written by the forward, read by the backward
     void* normed;            // forward, of normed_type
-    float* rstd;             // [rows, 2]: of delta and of the stream; forward: may be null
+    float* rstd;             // [rows, 4]: of delta, of the stream (two unused); forward: may be null
     const float* d_stream;   // backward: gradient that reaches the stream directly, or null
     const void* d_normed;    // backward: of normed_type
     float* d_residual;       // backward: each may be null
@@ -233,10 +233,11 @@ struct SandwichArgs {
     float scale, eps;
     int delta_type, normed_type;   // 0 fp16, 1 bf16, 2 fp32; the second is the first or fp32
     int sm_count;
+    int* status;
     // set by the launcher
     float* planes_pre;
     float* planes_gate;
-    long long groups, group_rows, shares, share_rows, units, grid;
+    long long groups, group_rows, shares, units, grid;
     int depth;               // rows ahead
 };
 constexpr int SANDWICH_MAX_HIDDEN = 16384;
@@ -419,9 +420,11 @@ int set_error(int code, const char* fmt, ...);
 
 // Device-side status word: 0, or the first code a kernel recorded since it was last read:
 //   100 + role   a bounded wait of the fused GEMM ran out (role = which wait)
+//   190          the norms around a block: the bounded wait for a row ran out
 //   200          cross-entropy: a target index beyond the vocabulary (row treated as ignored)
 //   300          scale table: a block scale outside fp16's normal range (inf, subnormal or zero)
 //   400          the self-test kernel's bounded wait ran out (what nf4b200_selftest_wait asks for)
+constexpr int STATUS_ROW_WAIT = 190;
 constexpr int STATUS_CE_TARGET_RANGE = 200;
 constexpr int STATUS_SCALE_RANGE = 300;
 constexpr int STATUS_SELFTEST_WAIT = 400;

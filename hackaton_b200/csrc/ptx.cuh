@@ -157,15 +157,18 @@ __device__ __forceinline__ void prefetch_l2(const void* gptr) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() {
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// `bytes` (a multiple of 16) from a 16-byte aligned global address to shared memory; they count towards `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* gptr, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_dst), "l"(gptr), "r"(bytes), "r"(bar) : "memory");
 }
 
 // Asks for `bytes` (multiple of 16) at a 16-byte aligned global address to be brought into L2.

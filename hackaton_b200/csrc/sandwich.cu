@@ -10,11 +10,12 @@
 // The backward's second mean is linear in ds, so that both means come out of one reduction of three sums:
 //   mean(g ds dh) = mean(g dh (d_stream + rs w)) - rs mean(w sh) mean(g dh sh)
 // Memory bound: 4 + 4 bytes per value of the stream and 2 + 2 of 16-bit delta and y forward (12), 18 backward. A CTA
-// keeps a thread's columns of the weights in registers over all its rows; rows to come are on their way to shared
-// memory, each thread's own columns into slots that nobody else reads (cp.async, no barrier), four rows ahead forward and
-// three backward, since two or three CTAs of an SM with one row each in flight leave most of the bandwidth idle (one row
-// ahead in registers: 16,384 x 1536 82 and 129 us). Column sums of the weights' gradients stay in registers; a second
-// kernel adds the CTAs' sums in order, so that results do not depend on timing. All sums are fp32.
+// keeps a thread's columns of the weights in registers over all its rows. Rows to come are on their way to shared
+// memory, four ahead forward and three backward, a bulk copy per array and row that one thread asks for: two or three CTAs
+// of an SM with one row each in flight leave most of the bandwidth idle, and every instruction that a thread spends
+// on addresses counts where it has eight values of a row (PLACEHOLDER). Column sums of the weights'
+// gradients stay in registers; a second kernel adds the CTAs' sums in order, so that results do not depend on timing.
+// All sums are fp32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -27,7 +28,6 @@ namespace nf4 {
 template <typename T, int VEC> struct SwRaw;
 
 template <> struct SwRaw<float, 4> {
-    static __device__ __forceinline__ void copy(uint32_t dst, const void* p, long long i) { cp_async16(dst, static_cast<const float*>(p) + i); }
     float4 v;
     __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)); }
     __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
@@ -36,7 +36,6 @@ template <> struct SwRaw<float, 4> {
     }
 };
 template <> struct SwRaw<__half, 4> {
-    static __device__ __forceinline__ void copy(uint32_t dst, const void* p, long long i) { cp_async8(dst, static_cast<const __half*>(p) + i); }
     uint2 v;
     __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(p) + i)); }
     __device__ __forceinline__ void get(float (&f)[4]) const {
@@ -49,7 +48,6 @@ template <> struct SwRaw<__half, 4> {
     }
 };
 template <> struct SwRaw<__nv_bfloat16, 4> {
-    static __device__ __forceinline__ void copy(uint32_t dst, const void* p, long long i) { cp_async8(dst, static_cast<const __nv_bfloat16*>(p) + i); }
     uint2 v;
     __device__ __forceinline__ void load(const void* p, long long i) { v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i)); }
     __device__ __forceinline__ void get(float (&f)[4]) const {
@@ -74,33 +72,30 @@ template <typename T> struct SwRaw<T, 1> {
     static __device__ __forceinline__ void store(void* p, long long i, const float (&f)[1]) { sw_round(f[0], static_cast<T*>(p)[i]); }
 };
 
-// Rows on their way: `depth` slots of what a thread's columns take of one array, [slot][i][thread]. Rows of single
-// values (VEC = 1) go through registers, one row ahead.
+// What a thread's columns take of one array's rows. VEC = 4: from a slot in shared memory, where the row lies as in memory;
+// VEC = 1: through registers, one row ahead.
 template <typename T, int NV, int VEC>
-struct SwRing {
+struct SwRow {
     SwRaw<T, VEC> next[VEC == 4 ? 1 : NV];
-    uint32_t base;     // this thread's place in slot 0
-    // Bytes of the ring; `at` moves behind it.
-    __device__ __forceinline__ void place(uint32_t& at, int depth) {
-        if (VEC != 4) return;
-        base = at + threadIdx.x * (4 * sizeof(T));
-        at += depth * NV * blockDim.x * (4 * sizeof(T));
+    __device__ __forceinline__ void ask(const T* row, const int (&cols)[NV]) {      // (VEC = 1)
+        if constexpr (VEC == 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) next[i].load(row, cols[i]);
     }
-    __device__ __forceinline__ void ask(int slot, int i, const void* p, long long index) {
-        if constexpr (VEC == 4) SwRaw<T, 4>::copy(base + (slot * NV + i) * blockDim.x * (4 * sizeof(T)), p, index);
-        else                    next[i].load(p, index);
-    }
-    __device__ __forceinline__ void get(int slot, int i, float (&f)[VEC]) const {
-        if constexpr (VEC == 4) {
-            const uint32_t a = base + (slot * NV + i) * blockDim.x * (4 * sizeof(T));
-            SwRaw<T, 4> raw;
-            if constexpr (sizeof(T) == 4)
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(raw.v.x), "=f"(raw.v.y), "=f"(raw.v.z), "=f"(raw.v.w) : "r"(a));
-            else
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(raw.v.x), "=r"(raw.v.y) : "r"(a));
-            raw.get(f);
-        } else {
-            next[i].get(f);
+    __device__ __forceinline__ void get(uint32_t slot, const int (&cols)[NV], float (&f)[NV][VEC]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (VEC == 4) {
+                const uint32_t x = slot + cols[i] * (int)sizeof(T);
+                SwRaw<T, 4> raw;
+                if constexpr (sizeof(T) == 4)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(raw.v.x), "=f"(raw.v.y), "=f"(raw.v.z), "=f"(raw.v.w) : "r"(x));
+                else
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(raw.v.x), "=r"(raw.v.y) : "r"(x));
+                raw.get(f[i]);
+            } else {
+                next[i].get(f[i]);
+            }
         }
     }
 };
@@ -109,268 +104,313 @@ struct SwRing {
 constexpr int SW_FEW_FWD = 256, SW_FEW_BWD = 512;
 constexpr int SW_FWD_DEPTH = 4, SW_BWD_DEPTH = 3;      // where shared memory allows
 
-// Waits for this thread's copies of the oldest of `depth` rows.
-__device__ __forceinline__ void sw_oldest(int depth) {
-    if (depth >= 4)      cp_async_wait<3>();
-    else if (depth == 3) cp_async_wait<2>();
-    else if (depth == 2) cp_async_wait<1>();
-    else                 cp_async_wait<0>();
-}
+// The slots' barriers: a slot's copies count towards its own.
+struct SwBars {
+    uint32_t first;
+    volatile int* abort_flag;
+    __device__ __forceinline__ void init(unsigned long long* room, int* flag, int depth) {
+        first = smem_u32(room);
+        abort_flag = flag;
+        if (threadIdx.x == 0) {
+            for (int k = 0; k < depth; ++k) mbar_init(first + 8 * k, 1);
+            *flag = 0;
+            fence_barrier_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ uint32_t operator[](int slot) const { return first + 8 * slot; }
+};
 
-// Sums of N values over the CTA, the same in every thread: a warp's by shuffles, the warps' by every thread for itself
-// (a broadcast load per four warps; shuffles are what a row of few columns per thread spends its time on). `part` has two
-// halves that successive calls take in turn: who writes a half again has passed the barrier behind which everybody
-// had read it. What belongs to warps that are not there is zero from the start.
+// Sums of N values over the CTA, the same in every thread: a warp's by shuffles; of the warps' every fourth by each
+// lane (a load that is mostly a broadcast), the four shares by shuffles again. `part` has two halves that successive calls
+// take in turn: who writes a half again has passed the barrier behind which everybody had read it.
 template <int N>
-__device__ __forceinline__ void sw_block_sum(float (&v)[N], float (*part)[N][32], int& turn) {
+__device__ __forceinline__ void sw_block_sum(float (&v)[N], float4 (*part)[32], int& turn) {
+    static_assert(N <= 4, "one float4 per warp");
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     if (warps > 1) {
-        if (lane == 0)
-#pragma unroll
-            for (int n = 0; n < N; ++n) part[turn][n][threadIdx.x >> 5] = v[n];
+        if (lane == 0) part[turn][threadIdx.x >> 5] = make_float4(v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f, 0.f);
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < N; ++n) v[n] = 0.f;
-        for (int w = 0; w < warps; w += 4)
+        for (int w = lane & 3; w < warps; w += 4) {
+            const float4 x = part[turn][w];
+            v[0] += x.x;
+            if (N > 1) v[N > 1 ? 1 : 0] += x.y;
+            if (N > 2) v[N > 2 ? 2 : 0] += x.z;
+        }
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const float4 x = *reinterpret_cast<const float4*>(&part[turn][n][w]);
-                v[n] += (x.x + x.y) + (x.z + x.w);
-            }
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int o = 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
         turn ^= 1;
     }
 }
 
-// (the barrier in the first sum comes behind this for every half that is read)
-template <int N>
-__device__ __forceinline__ void sw_clear(float (*part)[N][32]) {
-    for (int i = threadIdx.x; i < 2 * N * 32; i += blockDim.x)
-        if ((i & 31) >= (int)(blockDim.x >> 5)) (&part[0][0][0])[i] = 0.f;
-}
-
+// A thread's columns. Where a row ends before them they stand for its last ones, with weights of zero: nothing needs
+// a guard but what is added up or written.
 template <int NV, int VEC>
-__device__ __forceinline__ void sw_weights(const float* p, int hidden, float fill, float (&w)[NV][VEC]) {
+__device__ __forceinline__ void sw_columns(int hidden, int (&cols)[NV], bool (&in)[NV]) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) w[i][e] = fill;
-        if (p != nullptr && c < hidden) {
-            SwRaw<float, VEC> raw;
-            raw.load(p, c);
-            raw.get(w[i]);
-        }
+        in[i] = c < hidden;
+        cols[i] = in[i] ? c : hidden - VEC;
     }
 }
+
+template <int NV, int VEC>
+__device__ __forceinline__ void sw_weights(const float* p, const int (&cols)[NV], const bool (&in)[NV], float (&w)[NV][VEC]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        SwRaw<float, VEC> raw;
+        raw.load(p, cols[i]);
+        raw.get(w[i]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[i][e] = in[i] ? w[i][e] : 0.f;
+    }
+}
+
+// Weights behind the block with their gate row.
+template <int NV, int VEC>
+__device__ __forceinline__ void sw_gated(const SandwichArgs& a, long long gate_row, const int (&cols)[NV], const bool (&in)[NV],
+                                         float (&w)[NV][VEC]) {
+    sw_weights<NV, VEC>(a.post, cols, in, w);
+    if (a.gates == 0) return;
+    float gate[NV][VEC];
+    sw_weights<NV, VEC>(a.gate + gate_row * a.hidden, cols, in, gate);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[i][e] *= gate[i][e];
+}
+
+// A CTA's rows: units (gate row, share) blockIdx.x, + gridDim.x, ...; of a gate row's rows a share is every shares-th, so
+// that what the CTAs read at a time lies together (shares of consecutive rows: 16,384 x 1536 forward 55 us, so 48).
+struct SwWalk {
+    int unit, row, end;      // row -1 behind the last one
+    __device__ __forceinline__ void enter(const SandwichArgs& a) {
+        if (unit >= (int)a.units) {
+            row = -1;
+            return;
+        }
+        const int group = unit / (int)a.shares;
+        row = group * (int)a.group_rows + unit - group * (int)a.shares;
+        end = (group + 1) * (int)a.group_rows;
+    }
+    __device__ __forceinline__ void step(const SandwichArgs& a) {
+        if (row < 0) return;
+        row += (int)a.shares;
+        if (row < end) return;
+        unit += gridDim.x;
+        enter(a);
+    }
+};
 
 template <int NV, int VEC, typename TD, typename TY, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT <= SW_FEW_FWD ? 3 : 1)
 sandwich_fwd_kernel(const SandwichArgs a) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ __align__(16) float part[2][1][32];
+    __shared__ float4 part[2][32];
+    __shared__ unsigned long long bar_room[4];
+    __shared__ int abort_room;
     int turn = 0;
-    sw_clear<1>(part);
     const int hidden = a.hidden;
     const float inv_h = 1.f / (float)hidden;
-    float post[NV][VEC], pre[NV][VEC];
-    sw_weights<NV, VEC>(a.post, hidden, 0.f, post);
-    sw_weights<NV, VEC>(a.pre, hidden, 0.f, pre);
-    if (a.gates == 1) {
-        float gate[NV][VEC];
-        sw_weights<NV, VEC>(a.gate, hidden, 0.f, gate);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) post[i][e] *= gate[i][e];
-    }
+    int cols[NV];
+    bool in[NV];
+    sw_columns<NV, VEC>(hidden, cols, in);
+    float post[NV][VEC], pre[NV][VEC];      // post: times the gate
+    sw_weights<NV, VEC>(a.pre, cols, in, pre);
     const int depth = VEC == 4 ? a.depth : 1;
     extern __shared__ uint4 sw_smem[];
-    uint32_t room = smem_u32(sw_smem);
-    SwRing<float, NV, VEC> ring_r;
-    SwRing<TD, NV, VEC> ring_d;
-    ring_r.place(room, depth);
-    ring_d.place(room, depth);
-    const auto fetch = [&](long long row, int slot) {
-        if (row < a.rows) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (threadIdx.x + i * blockDim.x) * VEC;
-                if (c < hidden) {
-                    ring_d.ask(slot, i, a.delta, row * hidden + c);
-                    ring_r.ask(slot, i, a.residual, row * hidden + c);
-                }
-            }
+    const uint32_t room = smem_u32(sw_smem), bytes_r = hidden * 4, bytes_d = hidden * (int)sizeof(TD), slot_bytes = bytes_r + bytes_d;
+    SwBars bars;
+    SwRow<float, NV, VEC> in_r;
+    SwRow<TD, NV, VEC> in_d;
+    if (VEC == 4) bars.init(bar_room, &abort_room, depth);
+    const auto fetch = [&](int r, int slot) {      // (a negative row: nothing)
+        if (r < 0) return;
+        const long long at = (long long)r * hidden;
+        const TD* const d_row = static_cast<const TD*>(a.delta) + at;
+        if (VEC == 1) {
+            in_d.ask(d_row, cols);
+            in_r.ask(a.residual + at, cols);
+        } else if (threadIdx.x == 0) {
+            const uint32_t to = room + slot * slot_bytes;
+            mbar_arrive_expect_tx(bars[slot], slot_bytes);
+            bulk_load(to, a.residual + at, bytes_r, bars[slot]);
+            bulk_load(to + bytes_r, d_row, bytes_d, bars[slot]);
         }
-        if (VEC == 4) cp_async_commit();
     };
-    long long row = blockIdx.x;
-    for (int k = 0; k < depth; ++k) fetch(row + (long long)k * gridDim.x, k);
-    for (int slot = 0; row < a.rows; row += gridDim.x, slot = slot + 1 == depth ? 0 : slot + 1) {
-        if (VEC == 4) sw_oldest(depth);
-        float d[NV][VEC], s[NV][VEC], sum[1] = {0.f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d[i][e] = s[i][e] = 0.f;
-            if (c < hidden) {
-                ring_d.get(slot, i, d[i]);
-                ring_r.get(slot, i, s[i]);
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum[0] += d[i][e] * d[i][e];
+    SwWalk ahead = {(int)blockIdx.x, 0, 0};      // asks for rows, `depth` of them before the one that works on them
+    ahead.enter(a);
+    SwWalk now = ahead;
+    for (int k = 0; k < depth; ++k) {
+        fetch(ahead.row, k);
+        ahead.step(a);
+    }
+    uint32_t phase = 0;
+    int unit = -1;
+    for (int slot = 0; now.row >= 0; now.step(a)) {
+        const uint32_t from = room + slot * slot_bytes;
+        const int row = now.row;
+        if (VEC == 4 && !mbar_wait(bars[slot], phase, bars.abort_flag)) {
+            if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_ROW_WAIT);
+            return;
         }
-        if (VEC != 4) fetch(row + gridDim.x, 0);
+        if (now.unit != unit) {
+            unit = now.unit;
+            sw_gated<NV, VEC>(a, unit / (int)a.shares, cols, in, post);
+        }
+        float d[NV][VEC], s[NV][VEC], sum[1] = {0.f};
+        in_d.get(from + bytes_r, cols, d);
+        in_r.get(from, cols, s);
+        if (VEC != 4) {
+            fetch(ahead.row, 0);
+            ahead.step(a);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (in[i])
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum[0] = fmaf(d[i][e], d[i][e], sum[0]);
         sw_block_sum<1>(sum, part, turn);
         const float rd = 1.f / sqrtf(sum[0] * inv_h + a.eps);
-        if (VEC == 4) fetch(row + (long long)depth * gridDim.x, slot);    // (behind the barrier: the slot has been read)
+        if (VEC == 4) {       // (behind the barrier: the slot has been read)
+            fetch(ahead.row, slot);
+            ahead.step(a);
+            if (++slot == depth) {
+                slot = 0;
+                phase ^= 1u;
+            }
+        }
         sum[0] = 0.f;
-        const float* gate_row = a.gates > 1 ? a.gate + row / a.group_rows * hidden : nullptr;
+        const long long at = (long long)row * hidden;
+        float* const out = a.stream + at;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            float n[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) n[e] = d[i][e] * rd * post[i][e];
-            if (gate_row != nullptr && c < hidden) {
-                SwRaw<float, VEC> raw;
-                float gate[VEC];
-                raw.load(gate_row, c);
-                raw.get(gate);
+            for (int e = 0; e < VEC; ++e) s[i][e] = fmaf(d[i][e] * rd, post[i][e], a.scale * s[i][e]);
+            if (in[i]) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) n[e] *= gate[e];
+                for (int e = 0; e < VEC; ++e) sum[0] = fmaf(s[i][e], s[i][e], sum[0]);
+                SwRaw<float, VEC>::store(out, cols[i], s[i]);
             }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                s[i][e] = fmaf(a.scale, s[i][e], n[e]);
-                sum[0] += s[i][e] * s[i][e];
-            }
-            if (c < hidden) SwRaw<float, VEC>::store(a.stream, row * hidden + c, s[i]);
         }
         sw_block_sum<1>(sum, part, turn);
         const float rs = 1.f / sqrtf(sum[0] * inv_h + a.eps);
+        TY* const normed = static_cast<TY*>(a.normed) + at;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
             float y[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) y[e] = pre[i][e] * (s[i][e] * rs);
-            if (c < hidden) SwRaw<TY, VEC>::store(a.normed, row * hidden + c, y);
+            if (in[i]) SwRaw<TY, VEC>::store(normed, cols[i], y);
         }
-        if (threadIdx.x == 0 && a.rstd != nullptr) {
-            a.rstd[2 * row] = rd;
-            a.rstd[2 * row + 1] = rs;
-        }
+        if (threadIdx.x == 0 && a.rstd != nullptr) *reinterpret_cast<float4*>(a.rstd + 4ll * row) = make_float4(rd, rs, 0.f, 0.f);
     }
 }
 
-// A unit is a share of the rows that one gate row serves; a CTA takes units blockIdx.x, + gridDim.x, ...
 template <int NV, int VEC, typename TD, typename TY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1)
 sandwich_bwd_kernel(const SandwichArgs a) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ __align__(16) float part[2][3][32];
+    __shared__ float4 part[2][32];
+    __shared__ unsigned long long bar_room[4];
+    __shared__ int abort_room;
     int turn = 0;
-    sw_clear<3>(part);
     const int hidden = a.hidden;
     const float inv_h = 1.f / (float)hidden;
-    float post[NV][VEC], pre[NV][VEC], gate[NV][VEC], sum_post[NV][VEC], sum_pre[NV][VEC], sum_unit[NV][VEC];
-    sw_weights<NV, VEC>(a.post, hidden, 0.f, post);
-    sw_weights<NV, VEC>(a.pre, hidden, 0.f, pre);
-    sw_weights<NV, VEC>(a.gates == 1 ? a.gate : nullptr, hidden, 1.f, gate);
+    int cols[NV];
+    bool in[NV];
+    sw_columns<NV, VEC>(hidden, cols, in);
+    float post[NV][VEC], pre[NV][VEC], sum_post[NV][VEC], sum_pre[NV][VEC], sum_unit[NV][VEC];   // post: times the gate
+    sw_weights<NV, VEC>(a.pre, cols, in, pre);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sum_post[i][e] = sum_pre[i][e] = sum_unit[i][e] = 0.f;
 
     const int depth = VEC == 4 ? a.depth : 1;
+    const bool direct = a.d_stream != nullptr;
     extern __shared__ uint4 sw_smem[];
-    uint32_t room = smem_u32(sw_smem);
-    SwRing<float, NV, VEC> ring_s, ring_t;
-    SwRing<TD, NV, VEC> ring_d;
-    SwRing<TY, NV, VEC> ring_y;
-    ring_s.place(room, depth);
-    ring_t.place(room, depth);
-    ring_d.place(room, depth);
-    ring_y.place(room, depth);
-    const uint32_t ring_rstd = room + threadIdx.x * 8;      // (a copy for every thread)
+    const uint32_t room = smem_u32(sw_smem), bytes_s = hidden * 4, bytes_t = direct ? bytes_s : 0, bytes_d = hidden * (int)sizeof(TD),
+                   bytes_y = hidden * (int)sizeof(TY), at_t = bytes_s, at_d = at_t + bytes_t, at_y = at_d + bytes_d,
+                   at_rstd = at_y + bytes_y, slot_bytes = at_rstd + 16;
+    SwBars bars;
+    SwRow<float, NV, VEC> in_s, in_t;
+    SwRow<TD, NV, VEC> in_d;
+    SwRow<TY, NV, VEC> in_y;
+    if (VEC == 4) bars.init(bar_room, &abort_room, depth);
     float2 next_rstd = make_float2(0.f, 0.f);
     const auto fetch = [&](int row, int slot) {      // (a negative row: nothing)
-        if (row >= 0) {
-            const long long at = (long long)row * hidden;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (threadIdx.x + i * blockDim.x) * VEC;
-                if (c < hidden) {
-                    ring_s.ask(slot, i, a.stream, at + c);
-                    ring_d.ask(slot, i, a.delta, at + c);
-                    ring_y.ask(slot, i, a.d_normed, at + c);
-                    if (a.d_stream != nullptr) ring_t.ask(slot, i, a.d_stream, at + c);
-                }
-            }
-            if (VEC == 4) cp_async8(ring_rstd + slot * blockDim.x * 8, a.rstd + 2ll * row);
-            else          next_rstd = *reinterpret_cast<const float2*>(a.rstd + 2ll * row);
+        if (row < 0) return;
+        const long long at = (long long)row * hidden;
+        const TD* const d_row = static_cast<const TD*>(a.delta) + at;
+        const TY* const y_row = static_cast<const TY*>(a.d_normed) + at;
+        if (VEC == 1) {
+            in_s.ask(a.stream + at, cols);
+            in_d.ask(d_row, cols);
+            in_y.ask(y_row, cols);
+            if (direct) in_t.ask(a.d_stream + at, cols);
+            next_rstd = *reinterpret_cast<const float2*>(a.rstd + 4ll * row);
+        } else if (threadIdx.x == 0) {
+            const uint32_t to = room + slot * slot_bytes, bar = bars[slot];
+            mbar_arrive_expect_tx(bar, slot_bytes);
+            bulk_load(to, a.stream + at, bytes_s, bar);
+            if (direct) bulk_load(to + at_t, a.d_stream + at, bytes_t, bar);
+            bulk_load(to + at_d, d_row, bytes_d, bar);
+            bulk_load(to + at_y, y_row, bytes_y, bar);
+            bulk_load(to + at_rstd, a.rstd + 4ll * row, 16, bar);
         }
-        if (VEC == 4) cp_async_commit();
     };
-    // two walks over this CTA's rows: the one that asks for them is depth rows ahead of the one that works on them
-    const int shares = (int)a.shares, share_rows = (int)a.share_rows, group_rows = (int)a.group_rows, units = (int)a.units;
-    struct Walk {
-        int unit, row, end;
-    };
-    const auto enter = [&](Walk& w) {
-        const int group = w.unit / shares, share = w.unit - group * shares;
-        w.row = group * group_rows + share * share_rows;
-        w.end = min(w.row + share_rows, (group + 1) * group_rows);
-    };
-    const auto step = [&](Walk& w) {     // row -1 behind the last one
-        if (w.row < 0 || ++w.row < w.end) return;
-        w.unit += gridDim.x;
-        if (w.unit < units) enter(w);
-        else                w.row = -1;
-    };
-    Walk ahead;
-    ahead.unit = blockIdx.x;   // (gridDim.x <= units)
-    enter(ahead);
-    Walk now = ahead;
+    const int shares = (int)a.shares;
+    SwWalk ahead = {(int)blockIdx.x, 0, 0};      // as in the forward   (gridDim.x <= units)
+    ahead.enter(a);
+    SwWalk now = ahead;
     for (int k = 0; k < depth; ++k) {
         fetch(ahead.row, k);
-        step(ahead);
+        ahead.step(a);
     }
     bool new_unit = true;
-    for (int slot = 0; now.row >= 0; slot = slot + 1 == depth ? 0 : slot + 1) {
-        if (VEC == 4) sw_oldest(depth);
-        if (a.gates > 1 && new_unit) sw_weights<NV, VEC>(a.gate + (long long)(now.unit / shares) * hidden, hidden, 0.f, gate);
+    uint32_t phase = 0;
+    for (int slot = 0; now.row >= 0;) {
+        const uint32_t from = room + slot * slot_bytes;
+        if (VEC == 4 && !mbar_wait(bars[slot], phase, bars.abort_flag)) {
+            if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_ROW_WAIT);
+            return;
+        }
+        if (new_unit) sw_gated<NV, VEC>(a, now.unit / shares, cols, in, post);
         float2 rstd = next_rstd;
-        if (VEC == 4) asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(rstd.x), "=f"(rstd.y) : "r"(ring_rstd + slot * blockDim.x * 8));
+        if (VEC == 4) asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(rstd.x), "=f"(rstd.y) : "r"(from + at_rstd));
         const float rd = rstd.x, rs = rstd.y;
         float s[NV][VEC], t[NV][VEC], d[NV][VEC], y[NV][VEC], sum[3] = {0.f, 0.f, 0.f};
+        in_s.get(from, cols, s);
+        in_d.get(from + at_d, cols, d);
+        in_y.get(from + at_y, cols, y);
+        if (direct) {
+            in_t.get(from + at_t, cols, t);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s[i][e] = t[i][e] = d[i][e] = y[i][e] = 0.f;
-            if (c < hidden) {
-                ring_s.get(slot, i, s[i]);
-                ring_d.get(slot, i, d[i]);
-                ring_y.get(slot, i, y[i]);
-                if (a.d_stream != nullptr) ring_t.get(slot, i, t[i]);
-            }
+                for (int e = 0; e < VEC; ++e) t[i][e] = 0.f;
         }
         const long long at = (long long)now.row * hidden;
         const int this_unit = now.unit;
-        step(now);
+        now.step(a);
         const bool unit_done = now.row < 0 || now.unit != this_unit;
         new_unit = unit_done;
         if (VEC != 4) {
             fetch(ahead.row, 0);
-            step(ahead);
+            ahead.step(a);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -378,59 +418,66 @@ sandwich_bwd_kernel(const SandwichArgs a) {
             for (int e = 0; e < VEC; ++e) {
                 s[i][e] *= rs;                                      // sh
                 d[i][e] *= rd;                                      // dh
-                const float w = y[i][e] * pre[i][e], gd = gate[i][e] * post[i][e] * d[i][e];
+                const float w = y[i][e] * pre[i][e], gd = post[i][e] * d[i][e];      // (both zero behind the row)
                 t[i][e] = fmaf(rs, w, t[i][e]);                     // ds but for the mean
-                sum[0] += w * s[i][e];
-                sum[1] += gd * t[i][e];
-                sum[2] += gd * s[i][e];
-                sum_pre[i][e] += y[i][e] * s[i][e];
+                sum[0] = fmaf(w, s[i][e], sum[0]);
+                sum[1] = fmaf(gd, t[i][e], sum[1]);
+                sum[2] = fmaf(gd, s[i][e], sum[2]);
+                sum_pre[i][e] = fmaf(y[i][e], s[i][e], sum_pre[i][e]);
             }
         sw_block_sum<3>(sum, part, turn);
         if (VEC == 4) {       // (behind the barrier: the slot has been read)
             fetch(ahead.row, slot);
-            step(ahead);
+            ahead.step(a);
+            if (++slot == depth) {
+                slot = 0;
+                phase ^= 1u;
+            }
         }
         const float m1 = rs * (sum[0] * inv_h);
-        const float m2 = (sum[1] - m1 * sum[2]) * inv_h;
+        const float m2 = (sum[1] - m1 * sum[2]) * inv_h, rd_m2 = rd * m2;
+        float* const d_residual = a.d_residual + at;
+        TD* const d_delta = static_cast<TD*>(a.d_delta) + at;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
             float dr[VEC], dd[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float ds = fmaf(-m1, s[i][e], t[i][e]);
                 dr[e] = a.scale * ds;
-                dd[e] = rd * (ds * (gate[i][e] * post[i][e]) - d[i][e] * m2);
+                dd[e] = rd * (ds * post[i][e]) - d[i][e] * rd_m2;
                 sum_unit[i][e] = fmaf(ds, d[i][e], sum_unit[i][e]);
             }
-            if (c < hidden) {
-                if (a.d_residual != nullptr) SwRaw<float, VEC>::store(a.d_residual, at + c, dr);
-                if (a.d_delta != nullptr) SwRaw<TD, VEC>::store(a.d_delta, at + c, dd);
+            if (in[i]) {
+                if (a.d_residual != nullptr) SwRaw<float, VEC>::store(d_residual, cols[i], dr);
+                if (a.d_delta != nullptr) SwRaw<TD, VEC>::store(d_delta, cols[i], dd);
             }
         }
         if (unit_done) {
+            float own[NV][VEC], gate[NV][VEC];
+            sw_weights<NV, VEC>(a.post, cols, in, own);
+            if (a.gates > 0) sw_weights<NV, VEC>(a.gate + (long long)(this_unit / shares) * hidden, cols, in, gate);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (threadIdx.x + i * blockDim.x) * VEC;
                 float dg[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    dg[e] = post[i][e] * sum_unit[i][e];
-                    sum_post[i][e] = fmaf(gate[i][e], sum_unit[i][e], sum_post[i][e]);
+                    dg[e] = own[i][e] * sum_unit[i][e];
+                    sum_post[i][e] = fmaf(a.gates > 0 ? gate[i][e] : 1.f, sum_unit[i][e], sum_post[i][e]);
                     sum_unit[i][e] = 0.f;
                 }
                 // (one share per gate row: the row itself; otherwise the shares' plane)
-                if (a.d_gate != nullptr && c < hidden)
-                    SwRaw<float, VEC>::store(shares == 1 ? a.d_gate : a.planes_gate, (long long)this_unit * hidden + c, dg);
+                if (a.d_gate != nullptr && in[i])
+                    SwRaw<float, VEC>::store(shares == 1 ? a.d_gate : a.planes_gate, (long long)this_unit * hidden + cols[i], dg);
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (threadIdx.x + i * blockDim.x) * VEC;
-        if (c >= hidden) continue;
-        if (a.d_post != nullptr) SwRaw<float, VEC>::store(a.planes_post, (long long)blockIdx.x * hidden + c, sum_post[i]);
-        if (a.d_pre != nullptr) SwRaw<float, VEC>::store(a.planes_pre, (long long)blockIdx.x * hidden + c, sum_pre[i]);
+        if (!in[i]) continue;
+        const long long at = (long long)blockIdx.x * hidden + cols[i];
+        if (a.d_post != nullptr) SwRaw<float, VEC>::store(a.planes_post, at, sum_post[i]);
+        if (a.d_pre != nullptr) SwRaw<float, VEC>::store(a.planes_pre, at, sum_pre[i]);
     }
 }
 
@@ -474,15 +521,15 @@ struct SandwichShape {
 static SandwichShape sandwich_shape(int hidden, bool vec, bool few, bool backward, int delta_type, int normed_type) {
     const size_t room = (227 << 10) - 2048;
     SandwichShape s = {};
-    s.vec = vec && hidden % 4 == 0 ? 4 : 1;
+    s.vec = vec && hidden % (delta_type == 2 && normed_type == 2 ? 4 : 8) == 0 ? 4 : 1;     // (rows of whole 16 bytes)
     for (;;) {
         const int items = (hidden + s.vec - 1) / s.vec;
         if (s.vec == 4) s.nv = items <= (few ? 1024 : backward ? 192 : 256) ? 1 : items <= (few ? 2048 : backward ? 1024 : 512) ? 2 : 4;
         else            s.nv = items <= 4096 ? 4 : 16;
         s.threads = ((items + s.nv - 1) / s.nv + 31) / 32 * 32;
         if (s.vec != 4) return s;
-        const size_t d = delta_type == 2 ? 16 : 8, y = normed_type == 2 ? 16 : 8;
-        const size_t row = (size_t)s.nv * s.threads * (backward ? 32 + d + y : 16 + d) + (backward ? (size_t)s.threads * 8 : 0);
+        const size_t d = delta_type == 2 ? 4 : 2, y = normed_type == 2 ? 4 : 2;
+        const size_t row = backward ? (size_t)hidden * (8 + d + y) + 16 : (size_t)hidden * (4 + d);
         s.depth = backward ? SW_BWD_DEPTH : SW_FWD_DEPTH;
         while (s.depth > 0 && s.depth * row > room) --s.depth;
         s.smem = s.depth * row;
@@ -499,16 +546,14 @@ static long long sandwich_resident(const SandwichShape& s, bool backward) {
     return n < 1 ? 1 : n > 16 ? 16 : n;
 }
 
-// Backward: CTAs, and how the rows of a gate row are shared among them.
-static void sandwich_plan(SandwichArgs& a, const SandwichShape& s) {
+// CTAs, and how the rows of a gate row are shared among them.
+static void sandwich_plan(SandwichArgs& a, const SandwichShape& s, bool backward) {
     a.groups = a.gates > 0 ? a.gates : 1;
     a.group_rows = a.rows / a.groups;
-    const long long target = a.sm_count * sandwich_resident(s, true);
+    const long long target = a.sm_count * sandwich_resident(s, backward);
     long long shares = target / a.groups;
     if (shares > a.group_rows) shares = a.group_rows;
-    if (shares < 1) shares = 1;
-    a.share_rows = (a.group_rows + shares - 1) / shares;
-    a.shares = (a.group_rows + a.share_rows - 1) / a.share_rows;
+    a.shares = shares < 1 ? 1 : shares;
     a.units = a.groups * a.shares;
     a.grid = a.units < target ? a.units : target;
 }
@@ -520,7 +565,7 @@ long long sandwich_workspace_floats(long long rows, int hidden, long long gates,
         SandwichArgs a = {};
         a.rows = rows; a.hidden = hidden; a.gates = gates; a.sm_count = sm_count;
         a.delta_type = k & 2; a.normed_type = k & 4 ? 2 : 0;
-        sandwich_plan(a, sandwich_shape(hidden, (k & 1) != 0, few, true, a.delta_type, a.normed_type));
+        sandwich_plan(a, sandwich_shape(hidden, (k & 1) != 0, few, true, a.delta_type, a.normed_type), true);
         const long long planes = 2 * a.grid + (a.gates > 0 && a.shares > 1 ? a.units : 0);
         if (planes > most) most = planes;
     }
@@ -556,19 +601,15 @@ cudaError_t launch_sandwich(const SandwichArgs& a_in, bool backward, cudaStream_
     for (const void* p : {(const void*)a.residual, a.delta, (const void*)a.post, (const void*)a.pre, (const void*)a.gate,
                           (const void*)a.stream, (const void*)a.normed, (const void*)a.d_stream, a.d_normed,
                           (const void*)a.d_residual, (const void*)a.d_delta, (const void*)a.d_post, (const void*)a.d_pre,
-                          (const void*)a.d_gate, (const void*)a.planes_post})
+                          (const void*)a.d_gate, (const void*)a.planes_post, (const void*)a.rstd})
         bits |= reinterpret_cast<uintptr_t>(p);
     const SandwichShape s = sandwich_shape(a.hidden, (bits & 15) == 0, a.rows <= 2 * a.sm_count, backward, a.delta_type, a.normed_type);
     a.depth = s.depth;
-    sandwich_plan(a, s);
-    unsigned grid;
+    sandwich_plan(a, s, backward);
+    const unsigned grid = (unsigned)a.grid;
     if (backward) {
         a.planes_pre = a.planes_post + a.grid * a.hidden;
         a.planes_gate = a.planes_pre + a.grid * a.hidden;
-        grid = (unsigned)a.grid;
-    } else {
-        const long long target = a.sm_count * sandwich_resident(s, false);
-        grid = (unsigned)(a.rows < target ? a.rows : target);
     }
     cudaError_t e;
     if (a.delta_type == 0)
