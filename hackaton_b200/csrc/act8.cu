@@ -259,142 +259,168 @@ act8_swiglu_any_kernel(const Act8Swiglu a, const A8Rows g, int backward) {
 
 // ---------------------------------------------------------------------------------------- LoRA gradient
 // out[r, k] = sum_m s[m, r] * x[m, k] as mma.sync m16n8k16 with the 16 ranks as M, 8 columns as N and 16 rows
-// as the contraction: bound by reading the codes once, so the warp-level instruction is ample. A warp walks
-// 16 rows x 64 columns per step: lane (g = lane / 4, t = lane % 4) reads 8 codes, columns 8g .. 8g + 7, of rows
-// 2t, 2t + 1, 2t + 8 and 2t + 9, and column 8g + j of them is its part of the j-th of 8 products. The values go in as bf16, which holds a code times a power of two exactly, over
-// fp32's range (fp16 would lose blocks below 2^-18); s, fp16 with 11 significant bits, as the sum of two bf16 numbers,
-// also exact. Sums are fp32 throughout: a warp's in its accumulators, the CTA's warps' in shared memory, row
+// as the contraction: bound by reading the codes once and by the instructions that make operands of them, so the
+// warp-level instruction is ample. A warp walks 16 rows x 128 columns per step; its steps' codes, rows of s and step
+// bytes are on their way to shared memory, four steps ahead and nobody else's (one step ahead in registers, 64
+// columns: 16,384 x 3584 40 us, PLACEHOLDER). Lane (g = lane / 4, t = lane % 4) takes 16 codes, columns 16g .. 16g + 15, of rows
+// t, t + 4, t + 8 and t + 12, and column 16g + j of them is its part of the j-th of 16 products. (The contraction may
+// visit the rows in any order that both operands share; this one reads shared memory without conflicts.) The values
+// are fp16 numbers: a code under the exponent of 1024, less 1152, times the step, every operation exact. (Steps below
+// 2^-24, of blocks below 2^-18, go in as two factors; what they hold are multiples of 2^-24 like their source. s and
+// x as bf16 need no such care but two products for the 11 bits of s, and the warp-level products are what bounds this: 32
+// us at 16,384 x 3584.) Sums are fp32 throughout: a warp's in its accumulators, the CTA's warps' in shared memory, row
 // shares' in planes that a second kernel adds in order, so that results do not depend on timing.
 constexpr int A8G_WARPS = 8;
-constexpr int A8G_COLS = 64;
+constexpr int A8G_COLS = 128;
+constexpr int A8G_DEPTH = 4;
+constexpr int A8G_CODES = 16 * A8G_COLS, A8G_STEP_BYTES = A8G_CODES + 16 * 32 + 64;      // codes, s, step bytes
+constexpr int A8G_SMEM = A8G_WARPS * A8G_DEPTH * A8G_STEP_BYTES;
+static_assert(A8G_SMEM >= A8G_WARPS / 2 * 16 * (A8G_COLS + 4) * 4, "the warps' sums meet in the same memory");
 
 __device__ __forceinline__ void a8_mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two fp16 numbers as the sum of two pairs of bf16 numbers.
-__device__ __forceinline__ void a8_split(uint32_t x0, uint32_t x1, uint32_t& hi, uint32_t& lo) {
-    const float2 f = A8Source<__half>::two(x0 | x1 << 16);
-    hi = A8Source<__nv_bfloat16>::pack(f.x, f.y);
-    const float2 h = A8Source<__nv_bfloat16>::two(hi);
-    lo = A8Source<__nv_bfloat16>::pack(f.x - h.x, f.y - h.y);
 }
 
 __global__ void __launch_bounds__(A8G_WARPS * 32, 2)
 act8_lora_grad_kernel(const Act8LoraGrad a) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ float sums[A8G_WARPS / 2][16][A8G_COLS + 4];
+    extern __shared__ uint4 a8_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int col0 = blockIdx.x * A8G_COLS, col = col0 + 8 * g;
-    const bool col_ok = col < a.pitch;
+    const int col0 = blockIdx.x * A8G_COLS;
     const long long row_begin = (long long)blockIdx.y * a.rows_per_split;
     const long long row_end = min(row_begin + a.rows_per_split, a.rows);
-    const uint2* codes = reinterpret_cast<const uint2*>(a.codes + col);
-    const long long pitch8 = a.pitch / 8, steps_pitch = a.pitch / A8_BLOCK;
-    const uint8_t* steps = a.steps + col / A8_BLOCK;
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(a.s) + g;
-    const int at[4] = {2 * t, 2 * t + 1, 2 * t + 8, 2 * t + 9};
-    float acc[8][4];
+    const long long blocks = a.pitch / A8_BLOCK;
+    const bool step_words = blocks % 4 == 0 && (reinterpret_cast<uintptr_t>(a.steps) & 3) == 0;
+    const uint32_t ring = smem_u32(a8_smem) + (uint32_t)warp * (A8G_DEPTH * A8G_STEP_BYTES);
+    float acc[16][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 16; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
 
-    struct Step {
-        uint2 q[4];
-        uint32_t st[4], lo[4], hi[4];
-    } next;
-    const auto fetch = [&](long long r0) {
+    const auto fetch = [&](long long r0, int slot) {
+        const uint32_t at = ring + (uint32_t)slot * A8G_STEP_BYTES;
+        if (r0 < row_end) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const long long r = r0 + at[i];
-            const bool ok = r < row_end;
-            next.q[i] = make_uint2(0u, 0u);
-            next.st[i] = 0u;
-            next.lo[i] = next.hi[i] = 0u;
-            if (ok && col_ok) {
-                next.q[i] = __ldcs(codes + r * pitch8);
-                next.st[i] = __ldg(steps + r * steps_pitch);
+            for (int i = 0; i < 4; ++i) {      // codes: 8 pieces of 16 bytes a row
+                const int row = i * 4 + (lane >> 3), piece = lane & 7;
+                const bool there = r0 + row < row_end && col0 + piece * 16 < a.pitch;
+                cp_async16_or_zero(at + row * A8G_COLS + piece * 16, a.codes + (there ? (r0 + row) * a.pitch + col0 + piece * 16 : 0), there);
             }
-            if (ok) {
-                next.lo[i] = __ldg(s + r * 16);
-                next.hi[i] = __ldg(s + r * 16 + 8);
+            const bool there = r0 + (lane >> 1) < row_end;
+            cp_async16_or_zero(at + A8G_CODES + lane * 16, reinterpret_cast<const char*>(a.s) + (there ? (r0 * 32 + lane * 16) : 0), there);
+            if (lane < 16 && step_words) {
+                const bool in = r0 + lane < row_end;       // (a tile begins at a multiple of four blocks)
+                cp_async4_or_zero(at + A8G_CODES + 512 + lane * 4, a.steps + (in ? (r0 + lane) * blocks + col0 / A8_BLOCK : 0), in);
             }
         }
+        cp_async_commit();
     };
     long long r0 = row_begin + warp * 16;
-    fetch(r0);
-    for (; r0 < row_end; r0 += A8G_WARPS * 16) {
-        const Step now = next;
-        fetch(r0 + A8G_WARPS * 16);
-        uint32_t hi[4], lo[4];
-        a8_split(now.lo[0], now.lo[1], hi[0], lo[0]);
-        a8_split(now.hi[0], now.hi[1], hi[1], lo[1]);
-        a8_split(now.lo[2], now.lo[3], hi[2], lo[2]);
-        a8_split(now.hi[2], now.hi[3], hi[3], lo[3]);
-        float scale[4], shift[4];
+    for (int k = 0; k < A8G_DEPTH; ++k) fetch(r0 + (long long)k * (A8G_WARPS * 16), k);
+    int slot = 0;
+    for (; r0 < row_end; r0 += A8G_WARPS * 16, slot = (slot + 1) & (A8G_DEPTH - 1)) {
+        cp_async_wait<A8G_DEPTH - 1>();
+        __syncwarp();
+        const uint32_t at = ring + (uint32_t)slot * A8G_STEP_BYTES;
+        uint4 q[4];
+        float large[4], small[4];      // the step's factors: at least 2^-24, and what that left out
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            scale[i] = a8_value_of_step(now.st[i]);
-            shift[i] = -8388736.f * scale[i];
+            const int row = t + 4 * i;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w)
+                         : "r"(at + row * A8G_COLS + g * 16));
+            uint32_t st;
+            if (step_words) {
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(st) : "r"(at + A8G_CODES + 512 + row * 4 + (g >> 1)));
+            } else {
+                const long long b = col0 / A8_BLOCK + (g >> 1);
+                st = r0 + row < row_end && b < blocks ? a.steps[(r0 + row) * blocks + b] : 0u;
+            }
+            const float step = a8_value_of_step(st);      // (NaN stays)
+            const bool tiny = step < 5.9604644775390625e-8f;
+            large[i] = tiny ? 5.9604644775390625e-8f : step;
+            small[i] = tiny ? step * 16777216.f : 1.f;
+        }
+        __half2 factor[2], scale[2], shift[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            factor[p] = __floats2half2_rn(large[2 * p], large[2 * p + 1]);
+            scale[p] = __floats2half2_rn(small[2 * p], small[2 * p + 1]);
+            shift[p] = __hmul2(__float2half2_rn(-1152.f), scale[p]);
+        }
+        // the fragment of s, rank-major: contraction index 2t is row t, 2t + 1 row t + 4, 2t + 8 and 2t + 9 rows t + 8, t + 12
+        uint32_t f[4];
+        {
+            const int k = (lane & 7) + (lane >= 16 ? 8 : 0);      // (matrices 0, 1: indices 0 .. 7; 2, 3: 8 .. 15)
+            const int row = ((k & 7) >> 1) + (k & 1) * 4 + (k & 8);
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+                         : "r"(at + A8G_CODES + row * 32 + ((lane >> 3) & 1) * 16));
         }
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
+        for (int w = 0; w < 4; ++w) {
             uint32_t word[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                word[i] = (w == 0 ? now.q[i].x : now.q[i].y) ^ 0x80808080u;
+                word[i] = (w == 0 ? q[i].x : w == 1 ? q[i].y : w == 2 ? q[i].z : q[i].w) ^ 0x80808080u;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                uint32_t v[4], b[2];
+                uint32_t b[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)   // (2^23 + 128 + q) * step - (2^23 + 128) * step: exact, seven bits
-                    v[i] = __float_as_uint(fmaf(__uint_as_float(__byte_perm(word[i], 0x4B000000u, 0x7440 + e)),
-                                                scale[i], shift[i]));
-                b[0] = __byte_perm(v[0], v[1], 0x7632);   // their upper halves are the bf16 numbers
-                b[1] = __byte_perm(v[2], v[3], 0x7632);
-                a8_mma16816(acc[4 * w + e], hi, b[0], b[1]);
-                a8_mma16816(acc[4 * w + e], lo, b[0], b[1]);
+                for (int p = 0; p < 2; ++p) {
+                    // the byte of each of two rows, each under 0x64
+                    const uint32_t two = __byte_perm(word[2 * p], word[2 * p + 1], (uint32_t)(e | (4 + e) << 4));
+                    const uint32_t raw = __byte_perm(two, 0x64646464u, 0x4140u);
+                    const __half2 v = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&raw), scale[p], shift[p]), factor[p]);
+                    b[p] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+                a8_mma16816(acc[4 * w + e], f, b[0], b[1]);
             }
         }
+        __syncwarp();      // (every lane has read the slot)
+        fetch(r0 + (long long)A8G_DEPTH * (A8G_WARPS * 16), slot);
     }
-    // acc[j]: ranks g, g, g + 8, g + 8 of columns 8 * (2t) + j and 8 * (2t + 1) + j (N index n stands for the column
+    cp_async_wait<0>();
+    __syncthreads();
+    // acc[j]: ranks g, g, g + 8, g + 8 of columns 16 * (2t) + j and 16 * (2t + 1) + j (N index n stands for the column
     // group of the lanes with g = n)
+    float (*sums)[16][A8G_COLS + 4] = reinterpret_cast<float (*)[16][A8G_COLS + 4]>(a8_smem);
     for (int half = A8G_WARPS / 2; half >= 1; half >>= 1) {
         if (warp >= half && warp < 2 * half) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sums[warp - half][g][16 * t + j] = acc[j][0];
-                sums[warp - half][g][16 * t + 8 + j] = acc[j][1];
-                sums[warp - half][g + 8][16 * t + j] = acc[j][2];
-                sums[warp - half][g + 8][16 * t + 8 + j] = acc[j][3];
+            for (int j = 0; j < 16; ++j) {
+                sums[warp - half][g][32 * t + j] = acc[j][0];
+                sums[warp - half][g][32 * t + 16 + j] = acc[j][1];
+                sums[warp - half][g + 8][32 * t + j] = acc[j][2];
+                sums[warp - half][g + 8][32 * t + 16 + j] = acc[j][3];
             }
         }
         __syncthreads();
         if (warp < half) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                acc[j][0] += sums[warp][g][16 * t + j];
-                acc[j][1] += sums[warp][g][16 * t + 8 + j];
-                acc[j][2] += sums[warp][g + 8][16 * t + j];
-                acc[j][3] += sums[warp][g + 8][16 * t + 8 + j];
+            for (int j = 0; j < 16; ++j) {
+                acc[j][0] += sums[warp][g][32 * t + j];
+                acc[j][1] += sums[warp][g][32 * t + 16 + j];
+                acc[j][2] += sums[warp][g + 8][32 * t + j];
+                acc[j][3] += sums[warp][g + 8][32 * t + 16 + j];
             }
         }
         __syncthreads();
     }
     if (warp == 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            sums[0][g][16 * t + j] = acc[j][0];
-            sums[0][g][16 * t + 8 + j] = acc[j][1];
-            sums[0][g + 8][16 * t + j] = acc[j][2];
-            sums[0][g + 8][16 * t + 8 + j] = acc[j][3];
+        for (int j = 0; j < 16; ++j) {
+            sums[0][g][32 * t + j] = acc[j][0];
+            sums[0][g][32 * t + 16 + j] = acc[j][1];
+            sums[0][g + 8][32 * t + j] = acc[j][2];
+            sums[0][g + 8][32 * t + 16 + j] = acc[j][3];
         }
     }
     __syncthreads();
@@ -483,7 +509,7 @@ cudaError_t launch_act8_swiglu(const Act8Swiglu& a, bool backward, cudaStream_t 
     return launch_pdl(act8_swiglu_any_kernel, a8_grid(g, a.sm_count), dim3(A8_THREADS), 0, stream, a, g, backward ? 1 : 0);
 }
 
-// Row shares: about two CTAs per SM, each of at least a step of every warp.
+// Row shares: two CTAs per SM as far as that goes without a third wave, each of at least a step of every warp.
 int act8_lora_grad_splits(long long rows, long long cols, int sm_count) {
     const long long tiles = (cols + A8G_COLS - 1) / A8G_COLS, step = A8G_WARPS * 16;
     long long splits = 2ll * sm_count / tiles;
@@ -501,7 +527,9 @@ cudaError_t launch_act8_lora_grad(const Act8LoraGrad& a_in, cudaStream_t stream)
     a.rows_per_split = (a.rows_per_split + step - 1) / step * step;
     a.splits = (int)((a.rows + a.rows_per_split - 1) / a.rows_per_split);   // no empty share
     const dim3 grid((unsigned)((a.cols + A8G_COLS - 1) / A8G_COLS), (unsigned)a.splits);
-    cudaError_t e = launch_pdl(act8_lora_grad_kernel, grid, dim3(A8G_WARPS * 32), 0, stream, a);
+    cudaError_t e = cudaFuncSetAttribute(act8_lora_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A8G_SMEM);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(act8_lora_grad_kernel, grid, dim3(A8G_WARPS * 32), A8G_SMEM, stream, a);
     if (e != cudaSuccess || a.splits == 1) return e;
     const long long n = 16 * a.cols;
     return launch_pdl(act8_lora_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream,
