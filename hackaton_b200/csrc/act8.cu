@@ -265,7 +265,7 @@ act8_swiglu_any_kernel(const Act8Swiglu a, const A8Rows g, int backward) {
 // columns: 16,384 x 3584 40 us, PLACEHOLDER). Lane (g = lane / 4, t = lane % 4) takes 16 codes, columns 16g .. 16g + 15, of rows
 // t, t + 4, t + 8 and t + 12, and column 16g + j of them is its part of the j-th of 16 products. (The contraction may
 // visit the rows in any order that both operands share; this one reads shared memory without conflicts.) The values
-// are fp16 numbers: a code under the exponent of 1024, less 1152, times the step, every operation exact. (Steps below
+// are fp16 numbers: a code on top of 1536, less that, times the step, every operation exact. (Steps below
 // 2^-24, of blocks below 2^-18, go in as two factors; what they hold are multiples of 2^-24 like their source. s and
 // x as bf16 need no such care but two products for the 11 bits of s, and the warp-level products are what bounds this: 32
 // us at 16,384 x 3584.) Sums are fp32 throughout: a warp's in its accumulators, the CTA's warps' in shared memory, row
@@ -304,81 +304,106 @@ act8_lora_grad_kernel(const Act8LoraGrad a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
 
+    // where this lane's copies come from in the step at row 0, and go to
+    const int piece = lane & 7, prow = lane >> 3;
+    const bool piece_ok = col0 + piece * 16 < a.pitch;
+    const int8_t* const from_codes = a.codes + prow * a.pitch + (piece_ok ? col0 + piece * 16 : 0);
+    const uint32_t to_codes = ring + prow * A8G_COLS + piece * 16;
+    const char* const from_s = reinterpret_cast<const char*>(a.s) + lane * 16;
+    const uint8_t* const from_steps = a.steps + (lane & 15) * blocks + col0 / A8_BLOCK;    // (a tile begins at a multiple of four blocks)
     const auto fetch = [&](long long r0, int slot) {
-        const uint32_t at = ring + (uint32_t)slot * A8G_STEP_BYTES;
-        if (r0 < row_end) {
+        const uint32_t off = (uint32_t)slot * A8G_STEP_BYTES;
+        if (r0 + 16 <= row_end && piece_ok) {
+            const int8_t* p = from_codes + r0 * a.pitch;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {      // codes: 8 pieces of 16 bytes a row
-                const int row = i * 4 + (lane >> 3), piece = lane & 7;
-                const bool there = r0 + row < row_end && col0 + piece * 16 < a.pitch;
-                cp_async16_or_zero(at + row * A8G_COLS + piece * 16, a.codes + (there ? (r0 + row) * a.pitch + col0 + piece * 16 : 0), there);
+                cp_async16(to_codes + off + i * 4 * A8G_COLS, p);
+                p += 4 * a.pitch;
             }
-            const bool there = r0 + (lane >> 1) < row_end;
-            cp_async16_or_zero(at + A8G_CODES + lane * 16, reinterpret_cast<const char*>(a.s) + (there ? (r0 * 32 + lane * 16) : 0), there);
-            if (lane < 16 && step_words) {
-                const bool in = r0 + lane < row_end;       // (a tile begins at a multiple of four blocks)
-                cp_async4_or_zero(at + A8G_CODES + 512 + lane * 4, a.steps + (in ? (r0 + lane) * blocks + col0 / A8_BLOCK : 0), in);
+        } else if (r0 < row_end) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool there = piece_ok && r0 + i * 4 + prow < row_end;
+                cp_async16_or_zero(to_codes + off + i * 4 * A8G_COLS, there ? from_codes + (r0 + i * 4) * a.pitch : a.codes, there);
             }
+        }
+        if (r0 < row_end) {
+            const bool there = r0 + (lane >> 1) < row_end, in = r0 + (lane & 15) < row_end;
+            cp_async16_or_zero(ring + off + A8G_CODES + lane * 16, there ? from_s + r0 * 32 : reinterpret_cast<const char*>(a.s), there);
+            if (lane < 16 && step_words)
+                cp_async4_or_zero(ring + off + A8G_CODES + 512 + lane * 4, in ? from_steps + r0 * blocks : a.steps, in);
         }
         cp_async_commit();
     };
     long long r0 = row_begin + warp * 16;
     for (int k = 0; k < A8G_DEPTH; ++k) fetch(r0 + (long long)k * (A8G_WARPS * 16), k);
+    // the fragment of s, rank-major: contraction index 2t is row t, 2t + 1 row t + 4, 2t + 8 and 2t + 9 rows t + 8, t + 12
+    const int k8 = (lane & 7) + (lane >= 16 ? 8 : 0);      // (matrices 0, 1: indices 0 .. 7; 2, 3: 8 .. 15)
+    const uint32_t at_s = ring + A8G_CODES + (((k8 & 7) >> 1) + (k8 & 1) * 4 + (k8 & 8)) * 32 + ((lane >> 3) & 1) * 16;
+    const uint32_t at_codes = ring + t * A8G_COLS + g * 16, at_steps = ring + A8G_CODES + 512 + t * 4 + (g >> 1);
+    const __half2 bias = __float2half2_rn(1536.f);
     int slot = 0;
     for (; r0 < row_end; r0 += A8G_WARPS * 16, slot = (slot + 1) & (A8G_DEPTH - 1)) {
         cp_async_wait<A8G_DEPTH - 1>();
         __syncwarp();
-        const uint32_t at = ring + (uint32_t)slot * A8G_STEP_BYTES;
+        const uint32_t off = (uint32_t)slot * A8G_STEP_BYTES;
         uint4 q[4];
-        float large[4], small[4];      // the step's factors: at least 2^-24, and what that left out
+        float step[4];
+        bool tiny = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = t + 4 * i;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w)
-                         : "r"(at + row * A8G_COLS + g * 16));
+                         : "r"(at_codes + off + i * 4 * A8G_COLS));
             uint32_t st;
             if (step_words) {
-                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(st) : "r"(at + A8G_CODES + 512 + row * 4 + (g >> 1)));
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(st) : "r"(at_steps + off + i * 16));
             } else {
-                const long long b = col0 / A8_BLOCK + (g >> 1);
-                st = r0 + row < row_end && b < blocks ? a.steps[(r0 + row) * blocks + b] : 0u;
+                const long long b = col0 / A8_BLOCK + (g >> 1), row = r0 + t + 4 * i;
+                st = row < row_end && b < blocks ? a.steps[row * blocks + b] : 0u;
             }
-            const float step = a8_value_of_step(st);      // (NaN stays)
-            const bool tiny = step < 5.9604644775390625e-8f;
-            large[i] = tiny ? 5.9604644775390625e-8f : step;
-            small[i] = tiny ? step * 16777216.f : 1.f;
+            step[i] = a8_value_of_step(st);      // (NaN stays)
+            tiny = tiny || step[i] < 5.9604644775390625e-8f;
         }
-        __half2 factor[2], scale[2], shift[2];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            factor[p] = __floats2half2_rn(large[2 * p], large[2 * p + 1]);
-            scale[p] = __floats2half2_rn(small[2 * p], small[2 * p + 1]);
-            shift[p] = __hmul2(__float2half2_rn(-1152.f), scale[p]);
-        }
-        // the fragment of s, rank-major: contraction index 2t is row t, 2t + 1 row t + 4, 2t + 8 and 2t + 9 rows t + 8, t + 12
         uint32_t f[4];
-        {
-            const int k = (lane & 7) + (lane >= 16 ? 8 : 0);      // (matrices 0, 1: indices 0 .. 7; 2, 3: 8 .. 15)
-            const int row = ((k & 7) >> 1) + (k & 1) * 4 + (k & 8);
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
-                         : "r"(at + A8G_CODES + row * 32 + ((lane >> 3) & 1) * 16));
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at_s + off));
+        // steps below 2^-24: that, and a second factor
+        __half2 large[2], small[2];
+        const bool any_tiny = __any_sync(0xffffffffu, tiny);
+        if (any_tiny) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                float s2[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float& x = step[2 * p + i];
+                    const bool below = x < 5.9604644775390625e-8f;
+                    s2[i] = below ? x * 16777216.f : 1.f;
+                    x = below ? 5.9604644775390625e-8f : x;
+                }
+                small[p] = __floats2half2_rn(s2[0], s2[1]);
+            }
         }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) large[p] = __floats2half2_rn(step[2 * p], step[2 * p + 1]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             uint32_t word[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                word[i] = (w == 0 ? q[i].x : w == 1 ? q[i].y : w == 2 ? q[i].z : q[i].w) ^ 0x80808080u;
+            for (int i = 0; i < 4; ++i) word[i] = w == 0 ? q[i].x : w == 1 ? q[i].y : w == 2 ? q[i].z : q[i].w;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 uint32_t b[2];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    // the byte of each of two rows, each under 0x64
-                    const uint32_t two = __byte_perm(word[2 * p], word[2 * p + 1], (uint32_t)(e | (4 + e) << 4));
-                    const uint32_t raw = __byte_perm(two, 0x64646464u, 0x4140u);
-                    const __half2 v = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&raw), scale[p], shift[p]), factor[p]);
+                    // a code of each of two rows, sign-extended; 0x6600 plus a number from -128 to 127 is 1536 plus it in fp16,
+                    // and the sum's upper byte is 0x66, or 0x65 where the number is negative
+                    uint32_t two;
+                    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(two) : "r"(word[2 * p]), "r"(word[2 * p + 1]), "r"(0xC480 + 0x1111 * e));
+                    const uint32_t raw = (two & 0x03FF03FFu) ^ 0x66006600u;
+                    __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raw), bias);
+                    if (any_tiny) v = __hmul2(v, small[p]);
+                    v = __hmul2(v, large[p]);
                     b[p] = *reinterpret_cast<const uint32_t*>(&v);
                 }
                 a8_mma16816(acc[4 * w + e], f, b[0], b[1]);
