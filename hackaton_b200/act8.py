@@ -17,8 +17,6 @@ Users: `silu_mul(..., keep8=True)`, `nf4_swiglu_mlp(..., keep8=True)`, `nf4_lora
 
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 from . import _lib
@@ -26,55 +24,52 @@ from . import _lib
 BLOCK = 32     # values of a row that share a step
 RANK = 16
 _TYPES = (torch.float16, torch.bfloat16, torch.float32)
+_LIKE = {t: torch.empty(0, dtype=t) for t in _TYPES}
 
 
-@dataclass(frozen=True)
 class Act8:
     """A tensor of `shape` and `dtype` in 8 bits: codes int8 [rows, ceil(cols / 32) * 32], steps uint8
     [rows, ceil(cols / 32)]."""
-    codes: torch.Tensor
-    steps: torch.Tensor
-    shape: tuple
-    dtype: torch.dtype
+
+    __slots__ = ("codes", "steps", "shape", "dtype")
+
+    def __init__(self, codes, steps, shape, dtype):
+        self.codes, self.steps, self.shape, self.dtype = codes, steps, shape, dtype
+
+    def __repr__(self):
+        return f"Act8({tuple(self.shape)}, {self.dtype}, {self.codes.device})"
 
     @property
     def nbytes(self):
         return self.codes.numel() + self.steps.numel()
 
 
-def _rows(t):
-    """[..., cols] as contiguous [rows, cols]."""
-    cols = t.shape[-1]
-    return t.reshape(t.numel() // cols if cols else 0, cols).contiguous()
-
-
 def act8_quantize(x):
     """`x` (fp16, bf16 or fp32, CUDA, at least one dimension) in 8 bits; blocks run along the last dimension."""
-    if x.dtype not in _TYPES:
-        raise TypeError(f"hackaton_b200: activations are kept from fp16, bf16 or fp32, got {x.dtype}")
-    if not x.is_cuda:
-        raise ValueError("hackaton_b200: act8_quantize needs a CUDA tensor (there is no CPU path)")
-    if x.dim() == 0:
+    kept = _lib.host().act8_quantize(x)
+    if kept is None:
+        if x.dtype not in _TYPES:
+            raise TypeError(f"hackaton_b200: activations are kept from fp16, bf16 or fp32, got {x.dtype}")
+        if not x.is_cuda:
+            raise ValueError("hackaton_b200: act8_quantize needs a CUDA tensor (there is no CPU path)")
         raise ValueError("hackaton_b200: act8_quantize needs at least one dimension")
-    codes, steps = _lib.host().act8_quantize(_rows(x.detach()))
-    return Act8(codes, steps, tuple(x.shape), x.dtype)
+    return Act8(*kept, x.shape, x.dtype)
 
 
 def act8_dequantize(kept):
     """The values that `kept` holds, in the shape and type it was made from."""
-    rows, cols = kept.codes.shape[0], kept.shape[-1]
-    out = torch.empty((rows, cols), dtype=kept.dtype, device=kept.codes.device)
-    return _lib.host().act8_dequantize(kept.codes, kept.steps, out).reshape(kept.shape)
+    return _lib.host().act8_dequantize(kept.codes, kept.steps, kept.shape, _LIKE[kept.dtype])
 
 
 def lora_grad_act8(kept, s):
     """sᵀ . x as fp32 [16, cols] for an fp16 input x kept in 8 bits and fp16 s [..., 16] with a row for each of
     its rows: the gradient of a LoRA pair's first factor (`lora.lora_grad` with rank-major output), in a fixed
     order of additions."""
-    if kept.dtype != torch.float16 or s.dtype != torch.float16:
-        raise TypeError(f"hackaton_b200: the LoRA gradient computes from fp16, got {kept.dtype} and {s.dtype}")
-    if s.device != kept.codes.device:
-        raise ValueError(f"hackaton_b200: operands on {kept.codes.device} and {s.device}")
-    if s.shape[-1] != RANK or s.numel() != kept.codes.shape[0] * RANK:
-        raise ValueError(f"hackaton_b200: {tuple(s.shape)} for an input of shape {kept.shape}")
-    return _lib.host().act8_lora_grad(kept.codes, kept.steps, s.reshape(-1, RANK).contiguous(), kept.shape[-1])
+    grad = _lib.host().act8_lora_grad(kept.codes, kept.steps, s, kept.shape[-1]) if kept.dtype is torch.float16 else None
+    if grad is None:
+        if kept.dtype != torch.float16 or s.dtype != torch.float16:
+            raise TypeError(f"hackaton_b200: the LoRA gradient computes from fp16, got {kept.dtype} and {s.dtype}")
+        if s.device != kept.codes.device:
+            raise ValueError(f"hackaton_b200: operands on {kept.codes.device} and {s.device}")
+        raise ValueError(f"hackaton_b200: {tuple(s.shape)} for an input of shape {tuple(kept.shape)}")
+    return grad

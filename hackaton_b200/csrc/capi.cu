@@ -938,7 +938,7 @@ int nf4b200_act8_lora_grad(const void* codes, const void* steps, const void* s, 
     if (rc != NF4B200_OK) return rc;
     if (rows <= 0 || cols <= 0) return fail(NF4B200_EINVAL, "act8_lora_grad: bad shape %lld x %lld", (long long)rows, (long long)cols);
     if (!codes || !steps || !s || !out) return fail(NF4B200_EINVAL, "act8_lora_grad: NULL argument");
-    if (!aligned16(codes)) return fail(NF4B200_EINVAL, "act8_lora_grad: codes are not 16-byte aligned");
+    if (!aligned16(codes) || !aligned16(s)) return fail(NF4B200_EINVAL, "act8_lora_grad: codes or s are not 16-byte aligned");
     const int64_t need = nf4b200_act8_lora_grad_workspace_bytes(rows, cols);
     if (need > 0 && (!workspace || workspace_bytes < (size_t)need || !aligned16(workspace)))
         return fail(NF4B200_EINVAL, "act8_lora_grad: needs %lld bytes of scratch", (long long)need);

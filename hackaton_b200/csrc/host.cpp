@@ -330,18 +330,29 @@ std::tuple<Tensor, Tensor> act8_room(const Tensor& like, int64_t rows, int64_t c
     return {at::empty({rows, blocks * 32}, options.dtype(at::kChar)), at::empty({rows, blocks}, options.dtype(at::kByte))};
 }
 
-std::tuple<Tensor, Tensor> act8_quantize(const Tensor& x2) {
-    const c10::cuda::CUDAGuard guard(x2.device());
-    auto [codes, steps] = act8_room(x2, x2.size(0), x2.size(1));
-    check(nf4b200_act8_quantize(x2.const_data_ptr(), type_code(x2.scalar_type()), codes.data_ptr(), steps.data_ptr(),
-                                x2.size(0), x2.size(1), stream_of(x2)));
-    return {codes, steps};
+// [..., cols] as contiguous [rows, cols].
+Tensor flat_rows(const Tensor& t) {
+    const int64_t cols = t.dim() == 0 ? 1 : t.size(-1);
+    if (t.dim() == 2 && t.is_contiguous()) return t;
+    return t.reshape({cols > 0 ? t.numel() / cols : 0, cols}).contiguous();
 }
 
-Tensor act8_dequantize(const Tensor& codes, const Tensor& steps, const Tensor& out) {
+std::optional<std::tuple<Tensor, Tensor>> act8_quantize(const Tensor& x) {
+    const auto type = x.scalar_type();
+    if (!x.is_cuda() || x.dim() == 0 || (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat)) return {};
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor x2 = flat_rows(x.requires_grad() ? x.detach() : x);
+    auto [codes, steps] = act8_room(x2, x2.size(0), x2.size(1));
+    check(nf4b200_act8_quantize(x2.const_data_ptr(), type_code(type), codes.data_ptr(), steps.data_ptr(), x2.size(0),
+                                x2.size(1), stream_of(x2)));
+    return std::make_tuple(codes, steps);
+}
+
+Tensor act8_dequantize(const Tensor& codes, const Tensor& steps, const std::vector<int64_t>& shape, const Tensor& like) {
     const c10::cuda::CUDAGuard guard(codes.device());
+    Tensor out = at::empty(shape, codes.options().dtype(like.scalar_type()));
     check(nf4b200_act8_dequantize(codes.const_data_ptr(), steps.const_data_ptr(), out.data_ptr(),
-                                  type_code(out.scalar_type()), out.size(0), out.size(1), stream_of(codes)));
+                                  type_code(out.scalar_type()), codes.size(0), shape.back(), stream_of(codes)));
     return out;
 }
 
@@ -366,12 +377,6 @@ std::tuple<Tensor, Tensor> act8_swiglu_bwd(const Tensor& d2, const Tensor& gc, c
     return {dg, du};
 }
 
-// [..., cols] as contiguous [rows, cols].
-Tensor flat_rows(const Tensor& t) {
-    const int64_t cols = t.dim() == 0 ? 1 : t.size(-1);
-    return t.reshape({cols > 0 ? t.numel() / cols : 0, cols}).contiguous();
-}
-
 struct SiluMulAct8 : torch::autograd::Function<SiluMulAct8> {
     static Tensor forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up) {
         auto [hidden, gc, gs, uc, us] = act8_swiglu_fwd(flat_rows(gate), flat_rows(up));
@@ -392,9 +397,14 @@ Opt silu_mul_act8(const Tensor& gate, const Tensor& up) {
     return SiluMulAct8::apply(gate, up);
 }
 
-Tensor act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s2, int64_t cols) {
-    const c10::cuda::CUDAGuard guard(codes.device());
+// None for an s that does not fit the kept input.
+Opt act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s, int64_t cols) {
     const int64_t rows = codes.size(0);
+    if (s.scalar_type() != at::kHalf || s.device() != codes.device() || s.dim() == 0 || s.size(-1) != RANK || s.numel() != rows * RANK)
+        return {};
+    const c10::cuda::CUDAGuard guard(codes.device());
+    Tensor s2 = flat_rows(s.requires_grad() ? s.detach() : s);
+    if ((reinterpret_cast<uintptr_t>(s2.const_data_ptr()) & 15) != 0) s2 = s2.clone();
     const auto options = s2.options().dtype(at::kFloat).memory_format(c10::nullopt);
     if (rows == 0 || cols == 0) return at::zeros({RANK, cols}, options);
     Tensor out = at::empty({RANK, cols}, options);

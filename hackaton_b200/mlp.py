@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .act8 import _rows as _act8_rows, act8_quantize
+from .act8 import act8_quantize
 from .group import Projection, _refs, linear_backward_dx_group
 from .nf4 import _rows_view, _stream_ptr, linear_backward_dx, scratch
 
@@ -184,7 +184,7 @@ class NF4SwiGLUMLP(torch.autograd.Function):
         gate_w, up_w, down_w = ctx.weights
         if ctx.keep8:
             d_hidden = linear_backward_dx(grad_out.contiguous(), *down_w)
-            grads = _lib.host().act8_swiglu_bwd(_act8_rows(d_hidden), *ctx.saved_tensors)
+            grads = _lib.host().act8_swiglu_bwd(d_hidden.reshape(-1, d_hidden.shape[-1]), *ctx.saved_tensors)
             d_gate, d_up = (g.reshape(d_hidden.shape) for g in grads)
         else:
             gate, up = ctx.saved_tensors

@@ -256,7 +256,7 @@ int64_t nf4b200_gate_up_swiglu_workspace_bytes(int64_t n_rows, int64_t n_cols, i
  *   steps in the same pass; nf4b200_act8_swiglu_bwd: nf4b200_swiglu_bwd from those.
  * nf4b200_act8_lora_grad: out[r, k] = sum over rows of s[row, r] * x[row, k] (fp32 [16, cols], overwritten) for an
  *   input that was kept in 8 bits from fp16, s fp16 [rows, 16]. Scratch as _workspace_bytes says; the sums are made
- *   in a fixed order. Codes and scratch 16-byte aligned.
+ *   in a fixed order. Codes, s and scratch 16-byte aligned.
  * No counterpart in the reference, which moves such tensors to host memory instead (solution/kernels.py:60-91).
  */
 int nf4b200_act8_quantize(const void* x, int dtype, void* codes, void* steps, int64_t rows, int64_t cols, void* stream);
