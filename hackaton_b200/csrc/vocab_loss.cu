@@ -45,14 +45,20 @@ constexpr int VL_PIECE_UNITS = 512;        // tiles of 256 x 256 that a piece ma
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
-constexpr int VL_STAGES = 6;
-constexpr int VL_HALF_BYTES = 128 * VL_BK * 2;      // one CTA's share of either operand
-constexpr int VL_STAGE_BYTES = 2 * VL_HALF_BYTES;
 constexpr int VL_EPI_WARPS = 8;
-constexpr int VL_STAGING_OFF = VL_STAGES * VL_STAGE_BYTES;      // a box of 32 rows x 128 bytes per warp, on its way out
-constexpr int VL_BAR_OFF = VL_STAGING_OFF + VL_EPI_WARPS * 4096;
-constexpr int VL_SMEM = VL_BAR_OFF + 256 + 1024;    // + slack for 1024-byte alignment
-static_assert(VL_SMEM <= 232448, "exceeds the 227 KB of shared memory per CTA");
+constexpr int VL_SMEM_MAX = 232448;
+// Shared memory of a CTA: the ring (ROWS rows of A and 128 of B per step), a box of 32 rows x 128 bytes per epilogue warp
+// on its way out (OUT), barriers.
+template <int ROWS, int STAGES_, bool OUT>
+struct VlSmem {
+    static constexpr int STAGES = STAGES_;
+    static constexpr int A_BYTES = ROWS * VL_BK * 2, B_BYTES = 128 * VL_BK * 2;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGING_OFF = STAGES * STAGE_BYTES;
+    static constexpr int BAR_OFF = STAGING_OFF + (OUT ? VL_EPI_WARPS * 4096 : 0);
+    static constexpr int TOTAL = BAR_OFF + 8 * (3 * STAGES + 4) + 8 + 1024;    // + slack for 1024-byte alignment
+    static_assert(TOTAL <= VL_SMEM_MAX && BAR_OFF % 8 == 0, "exceeds the 227 KB of shared memory per CTA");
+};
 constexpr int VL_THREADS = 64 + VL_EPI_WARPS * 32;
 
 enum VlMode {
@@ -76,6 +82,8 @@ struct VlParams {
     int index;               // of the piece
     int capacity;            // tiles that a piece may have
     int slots;               // pairs that pieces and slices are planned for
+    int width;               // words of a tile: 256; VL_STATS of a single row tile: what balances the pairs
+    int box_rows;            // gathered rows that a CTA brings per tile (128; fewer where there is one row tile of fewer)
     const int* target;       // per gathered row
     // VL_STATS, VL_SOFT
     float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum (relative to it; VL_SOFT: to the reference)
@@ -180,6 +188,9 @@ __device__ __forceinline__ VlPlan vl_plan(const VlParams& p, int rows) {
     return w;
 }
 
+template <int MODE, int ROWS>
+using VlSmemOf = VlSmem<ROWS, MODE != VL_STATS ? 6 : ROWS == 64 ? 9 : 7, MODE != VL_STATS>;
+
 struct VlUnit {
     int mt, nt, slice, begin, steps;
 };
@@ -200,22 +211,25 @@ __device__ __forceinline__ VlUnit vl_unit(int u, const VlPlan& w) {
     return r;
 }
 
-template <int MODE>
+// ROWS: 128, or 64 for the statistics of at most 64 rows, where the ring is deep instead.
+template <int MODE, int ROWS = 128>
 __global__ void __launch_bounds__(VL_THREADS, 1)
 vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
     constexpr bool A_MN = MODE == VL_WEIGHT, B_MN = MODE >= VL_HIDDEN;
     constexpr bool A_PIECE = MODE >= VL_HIDDEN;      // A comes from the 16-bit piece
+    using L = VlSmemOf<MODE, ROWS>;
+    constexpr int STAGES = L::STAGES;
     extern __shared__ uint8_t vl_smem[];
     const uint32_t base = (smem_u32(vl_smem) + 1023u) & ~1023u;
     uint8_t* gen = vl_smem + (base - smem_u32(vl_smem));
-    const uint32_t bar = base + VL_BAR_OFF;
+    const uint32_t bar = base + L::BAR_OFF;
     auto bar_full = [&](int s) { return bar + 8u * s; };                        // leader: both CTAs' operands
-    auto bar_landed = [&](int s) { return bar + 8u * (VL_STAGES + s); };        // peer: its own
-    auto bar_empty = [&](int s) { return bar + 8u * (2 * VL_STAGES + s); };
-    auto bar_done = [&](int b) { return bar + 8u * (3 * VL_STAGES + b); };      // accumulator complete
-    auto bar_drained = [&](int b) { return bar + 8u * (3 * VL_STAGES + 2 + b); };
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + VL_BAR_OFF + 8 * (3 * VL_STAGES + 4));
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + VL_BAR_OFF + 8 * (3 * VL_STAGES + 4) + 4);
+    auto bar_landed = [&](int s) { return bar + 8u * (STAGES + s); };        // peer: its own
+    auto bar_empty = [&](int s) { return bar + 8u * (2 * STAGES + s); };
+    auto bar_done = [&](int b) { return bar + 8u * (3 * STAGES + b); };      // accumulator complete
+    auto bar_drained = [&](int b) { return bar + 8u * (3 * STAGES + 2 + b); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BAR_OFF + 8 * (3 * STAGES + 4));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BAR_OFF + 8 * (3 * STAGES + 4) + 4);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -227,7 +241,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     }
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < VL_STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(bar_full(s), 2);       // the leader's expect_tx and the peer's word that its share is there
             mbar_init(bar_landed(s), 1);
             mbar_init(bar_empty(s), 1);
@@ -271,20 +285,23 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 const VlUnit w = vl_unit<MODE>(u, plan);
                 if (skip(w)) continue;
                 for (int it = 0; it < w.steps; ++it, ++g) {
-                    const int s = (int)(g % VL_STAGES);
-                    const uint32_t ph = (g / VL_STAGES) & 1u;
+                    const int s = (int)(g % STAGES);
+                    const uint32_t ph = (g / STAGES) & 1u;
                     if (!mbar_wait_cluster(bar_empty(s), ph ^ 1u, abort_flag)) { fail = 1; break; }
                     const uint32_t landed = rank == 0 ? bar_full(s) : bar_landed(s);
-                    const uint32_t sa = base + (uint32_t)s * VL_STAGE_BYTES, sb = sa + VL_HALF_BYTES;
+                    const uint32_t sa = base + (uint32_t)s * L::STAGE_BYTES, sb = sa + L::A_BYTES;
                     const int k = (w.begin + it) * VL_BK;
-                    const int am = w.mt * VL_TILE + (int)rank * 128, bn = w.nt * VL_TILE + (int)rank * 128;
-                    mbar_arrive_expect_tx(landed, VL_STAGE_BYTES);
+                    const int width = MODE == VL_STATS ? p.width : VL_TILE;
+                    const int am = w.mt * VL_TILE + (int)rank * 128, bn = w.nt * width + (int)rank * (width / 2);
+                    const bool bring = MODE > VL_GRAD || p.box_rows == 128 || rank == 0;
+                    mbar_arrive_expect_tx(landed, MODE > VL_GRAD ? L::STAGE_BYTES
+                                                                 : (bring ? p.box_rows * 128 : 0) + (MODE == VL_STATS ? p.width * 64 : L::B_BYTES));
                     if (A_MN) {             // words as M, rows as steps
                         tma_load_2d(sa, &maps.a, 0, (am >> 6) * rows_dev + k, landed);
                         tma_load_2d(sa + 8192, &maps.a, 0, ((am >> 6) + 1) * rows_dev + k, landed);
                     } else if (A_PIECE) {   // rows as M, words as steps
                         tma_load_2d(sa, &maps.a, 0, (k >> 6) * rows_dev + am, landed);
-                    } else {
+                    } else if (bring) {     // (rows that are not brought give rows of the tile that nobody reads)
                         tma_load_2d(sa, &maps.a, k, am, landed);
                     }
                     if (B_MN) {     // VL_HIDDEN: rows of W from the piece's first word on; VL_WEIGHT: gathered rows
@@ -305,7 +322,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             constexpr uint64_t MN_MAJOR = make_smem_desc(0, 8192, 1024, LAYOUT_SW128);
             constexpr uint64_t A_DESC = A_MN ? MN_MAJOR : K_MAJOR, B_DESC = B_MN ? MN_MAJOR : K_MAJOR;
             constexpr uint32_t A_STEP = (A_MN ? 16 * 128 : 32) >> 4, B_STEP = (B_MN ? 16 * 128 : 32) >> 4;
-            const uint32_t idesc = make_idesc_f16(VL_TILE, A_MN ? 1u : 0u, B_MN ? 1u : 0u, VL_TILE) |
+            const uint32_t idesc = make_idesc_f16(MODE == VL_STATS ? (uint32_t)p.width : VL_TILE, A_MN ? 1u : 0u, B_MN ? 1u : 0u, VL_TILE) |
                                    (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
             const uint32_t base4 = (base & 0x3FFFFu) >> 4;
             uint32_t g = 0, n = 0;
@@ -316,10 +333,10 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
                 tc_fence_after_sync();
                 for (int it = 0; it < w.steps; ++it, ++g) {
-                    const int s = (int)(g % VL_STAGES);
-                    if (!mbar_wait_cluster(bar_full(s), (g / VL_STAGES) & 1u, abort_flag)) { fail = 3; break; }
+                    const int s = (int)(g % STAGES);
+                    if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
                     tc_fence_after_sync();
-                    const uint32_t a4 = base4 + (uint32_t)s * (VL_STAGE_BYTES >> 4), b4 = a4 + (VL_HALF_BYTES >> 4);
+                    const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4), b4 = a4 + (L::A_BYTES >> 4);
 #pragma unroll
                     for (int k = 0; k < VL_BK / 16; ++k)
                         umma_f16_words<2>(tmem + b * VL_TILE, a4 + (uint32_t)(A_DESC & 0xFFFFFFFFu) + A_STEP * k,
@@ -338,8 +355,8 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 const VlUnit w = vl_unit<MODE>(u, plan);
                 if (skip(w)) continue;
                 for (int it = 0; it < w.steps; ++it, ++g) {
-                    const int s = (int)(g % VL_STAGES);
-                    if (!mbar_wait(bar_landed(s), (g / VL_STAGES) & 1u, abort_flag)) { fail = 8; break; }
+                    const int s = (int)(g % STAGES);
+                    if (!mbar_wait(bar_landed(s), (g / STAGES) & 1u, abort_flag)) { fail = 8; break; }
                     mbar_arrive_cluster(lead_full0 + 8u * s);
                 }
             }
@@ -348,12 +365,13 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
         // ------------------------------------------------------------------ epilogue: a row's half tile per thread
         const int q = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
-        const uint32_t staging = base + VL_STAGING_OFF + (uint32_t)(warp - 2) * 4096u;
+        const uint32_t staging = base + L::STAGING_OFF + (uint32_t)(warp - 2) * 4096u;
         uint32_t n = 0;
         for (int u = pair; u < plan.units && !fail; u += pairs) {
             const VlUnit w = vl_unit<MODE>(u, plan);
             const int row = w.mt * VL_TILE + (int)rank * 128 + q * 32 + lane;     // VL_WEIGHT: word of the piece
-            const int col0 = w.nt * VL_TILE + half * 128;
+            const int share = MODE == VL_STATS ? p.width / 2 : 128;      // columns of a thread
+            const int col0 = w.nt * (2 * share) + half * share;
             if (MODE == VL_WEIGHT && plan.steps <= 0) {
                 // no row takes part: the gradient of the head is zero
                 if (plan.v0 + row < p.vocab)
@@ -398,7 +416,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             if (MODE == VL_WEIGHT) scale = *p.weight_scale;
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
-            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * share;
             auto release = [&]() {
                 tc_fence_before_sync();
                 __syncwarp();
@@ -437,11 +455,11 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             };
             float m2 = VL_NEG, sum = 0.f;
 #pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
+            for (int c = 0; c < share; c += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(at + c, r);
                 tmem_ld_wait();
-                if (c == 96) release();
+                if (c == share - 32) release();
                 if (MODE <= VL_SOFT) {
                     const int words = p.vocab - plan.v0 - col0 - c;       // words there are in this chunk
                     const bool cut = words < 32 || (unsigned)(target - c) < 32u;
@@ -849,7 +867,7 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
     if ((backward && a.d_weight != nullptr) || (!backward && (a.grads & 1)))
         s.room = vl_room(a.rows, a.vocab, a.hidden, a.sm_count / 2);
     if (!backward) {
-        s.parts = take((size_t)vl_word_tiles(a.vocab) * 2 * 8 * pad);
+        s.parts = take((size_t)((a.vocab + 127) / 128) * 2 * 8 * pad);      // (tiles are 128 words or more)
         s.target_logit = take(pad * 4);
         if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
         if (a.grads & 1) {
@@ -872,9 +890,10 @@ size_t vocab_loss_kept_bytes(long long rows, long long hidden, int grads) { retu
 
 size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward) { return vl_scratch(a, backward).bytes; }
 
-template <int MODE>
+template <int MODE, int ROWS = 128>
 static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long units, int sm_count, cudaStream_t stream) {
-    auto kernel = vl_gemm_kernel<MODE>;
+    auto kernel = vl_gemm_kernel<MODE, ROWS>;
+    constexpr int VL_SMEM = VlSmemOf<MODE, ROWS>::TOTAL;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, VL_SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -928,8 +947,25 @@ static void vl_use_kept(VocabLossArgs& a) {
     a.slots = a.sm_count / 2;
 }
 
+// Rows that a CTA brings of a tile: fewer than 128 where all there are fit in the first CTA of one tile. (64 rows of 3584
+// features against 151,936 words: PLACEHOLDER)
+static int vl_box_rows(long long rows) { return rows <= 128 ? (int)((rows + 7) / 8 * 8) : 128; }
+
+// Words of a tile of the statistics: 256, unless the rows make one row tile and 192 or 128 leave the pairs less unequal.
+static int vl_width(const VocabLossArgs& a) {
+    if (a.rows > VL_TILE) return VL_TILE;
+    int best = VL_TILE;
+    long long best_cost = 0;
+    for (const int width : {256, 192, 128}) {
+        const long long tiles = (a.vocab + width - 1) / width, cost = (tiles + a.slots - 1) / a.slots * (width + 8);
+        if (best_cost == 0 || cost < best_cost) { best_cost = cost; best = width; }
+    }
+    return best;
+}
+
 static VlParams vl_params(const VocabLossArgs& a) {
     VlParams p = {};
+    p.width = VL_TILE; p.box_rows = vl_box_rows(a.rows);
     p.count = a.count; p.status = a.status; p.bf16 = a.bf16;
     p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab);
     p.capacity = a.capacity; p.slots = a.slots;
@@ -964,19 +1000,24 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
     VlMaps logits = {}, hidden = {};
-    bool ok = vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
-              vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
+    const int width = soft ? VL_TILE : vl_width(a);
+    bool ok = vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, vl_box_rows(a.rows)) &&
+              vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, width / 2);
     if (ok && soft)
         ok = vl_piece_map(&logits.c, a, 32) && vl_piece_map(&hidden.a, a, 128) &&
              vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) &&
              make_map_2d(&hidden.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.planes, (uint64_t)a.hidden,
                          (uint64_t)s.room.planes * (uint64_t)a.rows_pad, (uint64_t)a.hidden * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!ok) { *why = "cuTensorMapEncodeTiled"; return cudaErrorInvalidValue; }
-    const VlParams base = vl_params(a);
+    VlParams base = vl_params(a);
+    base.width = width;
+    base.word_tiles = (int)((a.vocab + width - 1) / width);
     const long long row_tiles = a.rows_pad / VL_TILE;
     const dim3 merge_grid((unsigned)((a.rows + 31) / 32)), merge_block(32, 32);
     if (!soft) {
-        e = vl_launch<VL_STATS>(logits, base, row_tiles * base.word_tiles, a.sm_count, stream);
+        const long long units = row_tiles * base.word_tiles;
+        e = a.rows <= 64 ? vl_launch<VL_STATS, 64>(logits, base, units, a.sm_count, stream)
+                         : vl_launch<VL_STATS>(logits, base, units, a.sm_count, stream);
         if (e != cudaSuccess) { *why = "statistics"; return e; }
     } else {
         VlParams probe = base;
@@ -1023,7 +1064,7 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) { *why = "row factors"; return e; }
     VlMaps logits = {}, weight = {};
-    if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
+    if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, vl_box_rows(a.rows)) ||
         !vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) ||
         !vl_piece_map(&logits.c, a, 32) || !vl_piece_map(&weight.a, a, 64) ||
         !vl_map(&weight.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64) ||
