@@ -47,12 +47,12 @@ constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
 constexpr int VL_EPI_WARPS = 8;
 constexpr int VL_SMEM_MAX = 232448;
-// Shared memory of a CTA: the ring (ROWS rows of A and 128 of B per step), a box of 32 rows x 128 bytes per epilogue warp
+// Shared memory of a CTA: the ring (128 rows of A and ROWS of B per step), a box of 32 rows x 128 bytes per epilogue warp
 // on its way out (OUT), barriers.
 template <int ROWS, int STAGES_, bool OUT>
 struct VlSmem {
     static constexpr int STAGES = STAGES_;
-    static constexpr int A_BYTES = ROWS * VL_BK * 2, B_BYTES = 128 * VL_BK * 2;
+    static constexpr int A_BYTES = 128 * VL_BK * 2, B_BYTES = ROWS * VL_BK * 2;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int STAGING_OFF = STAGES * STAGE_BYTES;
     static constexpr int BAR_OFF = STAGING_OFF + (OUT ? VL_EPI_WARPS * 4096 : 0);
@@ -66,7 +66,8 @@ enum VlMode {
     VL_SOFT = 1,     // the same operands, one piece                          -> exponentials in 16 bits, the same statistics
     VL_GRAD = 2,     // the same                                              -> dl in 16 bits
     VL_HIDDEN = 3,   // A = the piece [R, words], B = its rows of W, N along K   -> fp32 planes [slices][R, K]
-    VL_WEIGHT = 4    // A = the piece transposed, B = gathered rows, N along K   -> 16-bit dW rows of the piece
+    VL_WEIGHT = 4,   // A = the piece transposed, B = gathered rows, N along K   -> 16-bit dW rows of the piece
+    VL_FEW = 5       // A = W, B = at most 64 gathered rows, words as M                 -> maximum and sum per row and warp
 };
 
 struct VlMaps {
@@ -82,8 +83,7 @@ struct VlParams {
     int index;               // of the piece
     int capacity;            // tiles that a piece may have
     int slots;               // pairs that pieces and slices are planned for
-    int width;               // words of a tile: 256; VL_STATS of a single row tile: what balances the pairs
-    int box_rows;            // gathered rows that a CTA brings per tile (128; fewer where there is one row tile of fewer)
+    int n_rows;              // VL_FEW: columns of the accumulator, 32 or 64
     const int* target;       // per gathered row
     // VL_STATS, VL_SOFT
     float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum (relative to it; VL_SOFT: to the reference)
@@ -163,7 +163,7 @@ __device__ __forceinline__ VlPlan vl_plan(const VlParams& p, int rows) {
     w.v0 = 0;
     w.tiles = p.word_tiles;
     int first_tiles = p.word_tiles;
-    if (MODE != VL_STATS) {
+    if (MODE != VL_STATS && MODE != VL_FEW) {
         first_tiles = vl_piece_tiles(max(w.row_tiles, 1), p.word_tiles, p.capacity, p.slots);
         const int before = min((long long)first_tiles * p.index, (long long)p.word_tiles);
         w.v0 = before * VL_TILE;
@@ -179,6 +179,10 @@ __device__ __forceinline__ VlPlan vl_plan(const VlParams& p, int rows) {
         const int tiles = w.row_tiles * feature_tiles;
         if (rows > 0) w.slices = vl_slices(tiles, first_tiles * (VL_TILE / VL_BK), p.slots);
         w.units = w.tiles > 0 ? tiles * w.slices : 0;
+    } else if (MODE == VL_FEW) {
+        w.m_tiles = w.tiles;
+        w.steps = vl_div_up(p.hidden, VL_BK);
+        w.units = rows > 0 ? w.tiles : 0;
     } else {
         w.m_tiles = w.row_tiles;
         w.steps = vl_div_up(p.hidden, VL_BK);
@@ -188,8 +192,8 @@ __device__ __forceinline__ VlPlan vl_plan(const VlParams& p, int rows) {
     return w;
 }
 
-template <int MODE, int ROWS>
-using VlSmemOf = VlSmem<ROWS, MODE != VL_STATS ? 6 : ROWS == 64 ? 9 : 7, MODE != VL_STATS>;
+template <int MODE>
+using VlSmemOf = VlSmem<MODE == VL_FEW ? 32 : 128, MODE == VL_FEW ? 11 : MODE == VL_STATS ? 7 : 6, MODE != VL_STATS && MODE != VL_FEW>;
 
 struct VlUnit {
     int mt, nt, slice, begin, steps;
@@ -211,13 +215,12 @@ __device__ __forceinline__ VlUnit vl_unit(int u, const VlPlan& w) {
     return r;
 }
 
-// ROWS: 128, or 64 for the statistics of at most 64 rows, where the ring is deep instead.
-template <int MODE, int ROWS = 128>
+template <int MODE>
 __global__ void __launch_bounds__(VL_THREADS, 1)
 vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
-    constexpr bool A_MN = MODE == VL_WEIGHT, B_MN = MODE >= VL_HIDDEN;
-    constexpr bool A_PIECE = MODE >= VL_HIDDEN;      // A comes from the 16-bit piece
-    using L = VlSmemOf<MODE, ROWS>;
+    constexpr bool A_MN = MODE == VL_WEIGHT, B_MN = MODE == VL_HIDDEN || MODE == VL_WEIGHT;
+    constexpr bool A_PIECE = MODE == VL_HIDDEN || MODE == VL_WEIGHT;      // A comes from the 16-bit piece
+    using L = VlSmemOf<MODE>;
     constexpr int STAGES = L::STAGES;
     extern __shared__ uint8_t vl_smem[];
     const uint32_t base = (smem_u32(vl_smem) + 1023u) & ~1023u;
@@ -291,17 +294,15 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                     const uint32_t landed = rank == 0 ? bar_full(s) : bar_landed(s);
                     const uint32_t sa = base + (uint32_t)s * L::STAGE_BYTES, sb = sa + L::A_BYTES;
                     const int k = (w.begin + it) * VL_BK;
-                    const int width = MODE == VL_STATS ? p.width : VL_TILE;
-                    const int am = w.mt * VL_TILE + (int)rank * 128, bn = w.nt * width + (int)rank * (width / 2);
-                    const bool bring = MODE > VL_GRAD || p.box_rows == 128 || rank == 0;
-                    mbar_arrive_expect_tx(landed, MODE > VL_GRAD ? L::STAGE_BYTES
-                                                                 : (bring ? p.box_rows * 128 : 0) + (MODE == VL_STATS ? p.width * 64 : L::B_BYTES));
+                    const int am = w.mt * VL_TILE + (int)rank * 128;
+                    const int bn = MODE == VL_FEW ? (int)rank * (p.n_rows / 2) : w.nt * VL_TILE + (int)rank * 128;
+                    mbar_arrive_expect_tx(landed, L::A_BYTES + (MODE == VL_FEW ? p.n_rows * 64 : L::B_BYTES));
                     if (A_MN) {             // words as M, rows as steps
                         tma_load_2d(sa, &maps.a, 0, (am >> 6) * rows_dev + k, landed);
                         tma_load_2d(sa + 8192, &maps.a, 0, ((am >> 6) + 1) * rows_dev + k, landed);
                     } else if (A_PIECE) {   // rows as M, words as steps
                         tma_load_2d(sa, &maps.a, 0, (k >> 6) * rows_dev + am, landed);
-                    } else if (bring) {     // (rows that are not brought give rows of the tile that nobody reads)
+                    } else {
                         tma_load_2d(sa, &maps.a, k, am, landed);
                     }
                     if (B_MN) {     // VL_HIDDEN: rows of W from the piece's first word on; VL_WEIGHT: gathered rows
@@ -322,7 +323,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             constexpr uint64_t MN_MAJOR = make_smem_desc(0, 8192, 1024, LAYOUT_SW128);
             constexpr uint64_t A_DESC = A_MN ? MN_MAJOR : K_MAJOR, B_DESC = B_MN ? MN_MAJOR : K_MAJOR;
             constexpr uint32_t A_STEP = (A_MN ? 16 * 128 : 32) >> 4, B_STEP = (B_MN ? 16 * 128 : 32) >> 4;
-            const uint32_t idesc = make_idesc_f16(MODE == VL_STATS ? (uint32_t)p.width : VL_TILE, A_MN ? 1u : 0u, B_MN ? 1u : 0u, VL_TILE) |
+            const uint32_t idesc = make_idesc_f16(MODE == VL_FEW ? (uint32_t)p.n_rows : VL_TILE, A_MN ? 1u : 0u, B_MN ? 1u : 0u, VL_TILE) |
                                    (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
             const uint32_t base4 = (base & 0x3FFFFu) >> 4;
             uint32_t g = 0, n = 0;
@@ -361,6 +362,60 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
                 }
             }
         }
+    } else if constexpr (MODE == VL_FEW) {
+        // ------------------------------------------------------------------ epilogue: a word's values of half the rows
+        // A thread keeps maximum and sum of the words that come by its lane, for each of its 16 or 32 rows, over all tiles;
+        // the lanes of a warp meet at the end.
+        const int q = warp & 3, half = (warp - 2) >> 2, n = p.n_rows / 2, row0 = half * n;
+        const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
+        const int target = lane < n && row0 + lane < rows ? p.target[row0 + lane] : -1;
+        float m[32], s[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) { m[j] = VL_NEG; s[j] = 0.f; }
+        uint32_t it = 0;
+        for (int u = pair; u < plan.units && !fail; u += pairs, ++it) {
+            const int b = (int)(it & 1u);
+            if (!mbar_wait(bar_done(b), (it >> 1) & 1u, abort_flag)) { fail = 5; break; }
+            tc_fence_after_sync();
+            const int word0 = u * VL_TILE + (int)rank * 128 + q * 32;
+            uint32_t r[32];
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + row0;
+            if (n == 32) {
+                tmem_ld_32x32(at, r);
+            } else {
+                uint32_t h[16];
+                tmem_ld_32x16(at, h);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = j < 16 ? h[j] : 0u;
+            }
+            tmem_ld_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
+            const bool there = word0 + lane < p.vocab;
+            const unsigned hits = __ballot_sync(0xffffffffu, (unsigned)(target - word0) < 32u);    // rows whose target is here
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                if (j >= n) break;
+                float x2 = there ? __uint_as_float(r[j]) * VL_LOG2E : VL_NEG;
+                if (hits >> j & 1u) x2 = __shfl_sync(0xffffffffu, target, j) == word0 + lane ? VL_NEG : x2;
+                const float top = fmaxf(m[j], x2);
+                s[j] = fmaf(s[j], vl_ex2(m[j] - top), there && x2 != VL_NEG ? vl_ex2(x2 - top) : 0.f);
+                m[j] = top;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (j >= n) break;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const float om = __shfl_xor_sync(0xffffffffu, m[j], o), os = __shfl_xor_sync(0xffffffffu, s[j], o);
+                const float top = fmaxf(m[j], om);
+                s[j] = s[j] * vl_ex2(m[j] - top) + os * vl_ex2(om - top);
+                m[j] = top;
+            }
+            if (lane == 0) p.parts[(long long)(blockIdx.x * 4 + q) * p.rows_pad + row0 + j] = make_float2(m[j], s[j]);
+        }
     } else {
         // ------------------------------------------------------------------ epilogue: a row's half tile per thread
         const int q = warp & 3, half = (warp - 2) >> 2;
@@ -370,8 +425,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
         for (int u = pair; u < plan.units && !fail; u += pairs) {
             const VlUnit w = vl_unit<MODE>(u, plan);
             const int row = w.mt * VL_TILE + (int)rank * 128 + q * 32 + lane;     // VL_WEIGHT: word of the piece
-            const int share = MODE == VL_STATS ? p.width / 2 : 128;      // columns of a thread
-            const int col0 = w.nt * (2 * share) + half * share;
+            const int col0 = w.nt * VL_TILE + half * 128;
             if (MODE == VL_WEIGHT && plan.steps <= 0) {
                 // no row takes part: the gradient of the head is zero
                 if (plan.v0 + row < p.vocab)
@@ -416,7 +470,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             if (MODE == VL_WEIGHT) scale = *p.weight_scale;
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
-            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * share;
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
             auto release = [&]() {
                 tc_fence_before_sync();
                 __syncwarp();
@@ -455,11 +509,11 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             };
             float m2 = VL_NEG, sum = 0.f;
 #pragma unroll 1
-            for (int c = 0; c < share; c += 32) {
+            for (int c = 0; c < 128; c += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(at + c, r);
                 tmem_ld_wait();
-                if (c == share - 32) release();
+                if (c == 96) release();
                 if (MODE <= VL_SOFT) {
                     const int words = p.vocab - plan.v0 - col0 - c;       // words there are in this chunk
                     const bool cut = words < 32 || (unsigned)(target - c) < 32u;
@@ -654,7 +708,7 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
 // of which the parts of `piece` word tiles each had one.
 template <bool PROBE>
 __global__ void __launch_bounds__(1024)
-vl_merge_kernel(const VocabLossArgs a, int word_tiles, int soft) {
+vl_merge_kernel(const VocabLossArgs a, int n_parts, int word_tiles, int soft) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float2 join[32][33];
@@ -664,7 +718,7 @@ vl_merge_kernel(const VocabLossArgs a, int word_tiles, int soft) {
     float m = VL_NEG, s = 0.f;
     if (row < rows) {
 #pragma unroll 4
-        for (int i = threadIdx.y; i < 2 * word_tiles; i += 32) {
+        for (int i = threadIdx.y; i < n_parts; i += 32) {
             float2 x = a.parts[(long long)i * a.rows_pad + row];
             if (soft) x.x = a.refs[(long long)(i / 2 / piece + 1) * a.rows_pad + row];
             const float top = fmaxf(m, x.x);
@@ -867,7 +921,8 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
     if ((backward && a.d_weight != nullptr) || (!backward && (a.grads & 1)))
         s.room = vl_room(a.rows, a.vocab, a.hidden, a.sm_count / 2);
     if (!backward) {
-        s.parts = take((size_t)((a.vocab + 127) / 128) * 2 * 8 * pad);      // (tiles are 128 words or more)
+        const size_t n_parts = (size_t)vl_word_tiles(a.vocab) * 2, few_parts = (size_t)a.sm_count * 4;
+        s.parts = take((n_parts > few_parts ? n_parts : few_parts) * 8 * pad);
         s.target_logit = take(pad * 4);
         if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
         if (a.grads & 1) {
@@ -890,10 +945,11 @@ size_t vocab_loss_kept_bytes(long long rows, long long hidden, int grads) { retu
 
 size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward) { return vl_scratch(a, backward).bytes; }
 
-template <int MODE, int ROWS = 128>
-static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long units, int sm_count, cudaStream_t stream) {
-    auto kernel = vl_gemm_kernel<MODE, ROWS>;
-    constexpr int VL_SMEM = VlSmemOf<MODE, ROWS>::TOTAL;
+template <int MODE>
+static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long units, int sm_count, cudaStream_t stream,
+                             int* ctas = nullptr) {
+    auto kernel = vl_gemm_kernel<MODE>;
+    constexpr int VL_SMEM = VlSmemOf<MODE>::TOTAL;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, VL_SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -919,6 +975,7 @@ static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long un
     if (units < pairs) pairs = units;
     if (pairs < 1) pairs = 1;
     cfg.gridDim = dim3((unsigned)(2 * pairs));
+    if (ctas != nullptr) *ctas = (int)(2 * pairs);
     return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
 
@@ -947,25 +1004,8 @@ static void vl_use_kept(VocabLossArgs& a) {
     a.slots = a.sm_count / 2;
 }
 
-// Rows that a CTA brings of a tile: fewer than 128 where all there are fit in the first CTA of one tile. (64 rows of 3584
-// features against 151,936 words: PLACEHOLDER)
-static int vl_box_rows(long long rows) { return rows <= 128 ? (int)((rows + 7) / 8 * 8) : 128; }
-
-// Words of a tile of the statistics: 256, unless the rows make one row tile and 192 or 128 leave the pairs less unequal.
-static int vl_width(const VocabLossArgs& a) {
-    if (a.rows > VL_TILE) return VL_TILE;
-    int best = VL_TILE;
-    long long best_cost = 0;
-    for (const int width : {256, 192, 128}) {
-        const long long tiles = (a.vocab + width - 1) / width, cost = (tiles + a.slots - 1) / a.slots * (width + 8);
-        if (best_cost == 0 || cost < best_cost) { best_cost = cost; best = width; }
-    }
-    return best;
-}
-
 static VlParams vl_params(const VocabLossArgs& a) {
     VlParams p = {};
-    p.width = VL_TILE; p.box_rows = vl_box_rows(a.rows);
     p.count = a.count; p.status = a.status; p.bf16 = a.bf16;
     p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab);
     p.capacity = a.capacity; p.slots = a.slots;
@@ -1000,9 +1040,14 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
     VlMaps logits = {}, hidden = {};
-    const int width = soft ? VL_TILE : vl_width(a);
-    bool ok = vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, vl_box_rows(a.rows)) &&
-              vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, width / 2);
+    // Up to 64 rows without a gradient of x: the words take the tensor cores' long side. (64 rows of 3584 features against
+    // 151,936 words: 216 us with the rows there, which costs four times the products; the weight alone takes 168.)
+    const bool few = !soft && a.rows <= 64;
+    const int few_rows = a.rows <= 32 ? 32 : 64;
+    bool ok = few ? vl_map(&logits.a, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) &&
+                        vl_map(&logits.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, few_rows / 2)
+                  : vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
+                        vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
     if (ok && soft)
         ok = vl_piece_map(&logits.c, a, 32) && vl_piece_map(&hidden.a, a, 128) &&
              vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) &&
@@ -1010,20 +1055,21 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
                          (uint64_t)s.room.planes * (uint64_t)a.rows_pad, (uint64_t)a.hidden * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!ok) { *why = "cuTensorMapEncodeTiled"; return cudaErrorInvalidValue; }
     VlParams base = vl_params(a);
-    base.width = width;
-    base.word_tiles = (int)((a.vocab + width - 1) / width);
+    base.n_rows = few_rows;
+    int n_parts = 2 * base.word_tiles;
     const long long row_tiles = a.rows_pad / VL_TILE;
     const dim3 merge_grid((unsigned)((a.rows + 31) / 32)), merge_block(32, 32);
     if (!soft) {
-        const long long units = row_tiles * base.word_tiles;
-        e = a.rows <= 64 ? vl_launch<VL_STATS, 64>(logits, base, units, a.sm_count, stream)
-                         : vl_launch<VL_STATS>(logits, base, units, a.sm_count, stream);
+        int ctas = 0;
+        e = few ? vl_launch<VL_FEW>(logits, base, base.word_tiles, a.sm_count, stream, &ctas)
+                : vl_launch<VL_STATS>(logits, base, row_tiles * base.word_tiles, a.sm_count, stream);
+        if (few) n_parts = 4 * ctas;
         if (e != cudaSuccess) { *why = "statistics"; return e; }
     } else {
         VlParams probe = base;
         if (probe.word_tiles > VL_PROBE_TILES) probe.word_tiles = VL_PROBE_TILES;
         e = vl_launch<VL_STATS>(logits, probe, row_tiles * probe.word_tiles, a.sm_count, stream);
-        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, probe.word_tiles, 0);
+        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, probe.word_tiles, 0);
         if (e != cudaSuccess) { *why = "references"; return e; }
         const long long units = row_tiles * base.word_tiles < a.capacity ? row_tiles * base.word_tiles : a.capacity;
         for (int i = 0; i < s.room.pieces; ++i) {
@@ -1037,7 +1083,7 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
             if (e != cudaSuccess) { *why = "gradient of the hidden states"; return e; }
         }
     }
-    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, base.word_tiles, soft ? 1 : 0);
+    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, base.word_tiles, soft ? 1 : 0);
     if (e == cudaSuccess && soft)
         e = launch_pdl(vl_mean_kernel, dim3((unsigned)(a.sm_count * 8)), dim3(256), 0, stream, a, base.word_tiles);
     if (e != cudaSuccess) *why = "merge";
@@ -1064,7 +1110,7 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) { *why = "row factors"; return e; }
     VlMaps logits = {}, weight = {};
-    if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, vl_box_rows(a.rows)) ||
+    if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
         !vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) ||
         !vl_piece_map(&logits.c, a, 32) || !vl_piece_map(&weight.a, a, 64) ||
         !vl_map(&weight.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64) ||

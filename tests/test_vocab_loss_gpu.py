@@ -329,3 +329,39 @@ def test_agrees_with_the_chunked_loss(cuda_lib):
     (loss * 1024).backward()
     (mine * 1024).backward()
     assert (h1.grad.float() - h2.grad.float()).norm() <= 2.0 ** -7 * h2.grad.float().norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,hidden", [(1, 1, 8), (1, 40007, 64), (16, 300, 128), (17, 5000, 72), (32, 257, 64), (33, 1003, 320),
+                                               (64, 20000, 1536), (65, 1003, 128), (300, 5000, 64)])
+def test_without_gradients(cuda_lib, dtype, rows, vocab, hidden):
+    """Losses and logsumexps alone: up to 64 rows they come out of a product with the words on the long side."""
+    from hackaton_b200 import vocab_cross_entropy
+
+    h, w, t = make(rows, vocab, hidden, dtype, rows * 3 + vocab, ignored=0.2 if rows > 4 else 0.0)
+    if rows > 20:
+        t[3], t[9] = 0, vocab - 1
+    with torch.no_grad():
+        losses, lse = vocab_cross_entropy(h, w, t)
+        check({"losses": losses, "lse": lse}, exact(h, w, t))
+        again = vocab_cross_entropy(h, w, t)
+    assert torch.equal(losses, again[0]) and torch.equal(lse, again[1])
+    cuda_lib.device_status()
+
+
+def test_without_gradients_and_nan(cuda_lib):
+    from hackaton_b200 import vocab_cross_entropy
+
+    h, w, t = make(40, 3000, 64, torch.float16, 31)
+    clean = vocab_cross_entropy(h, w, t)
+    h[5, 1] = float("nan")
+    got = vocab_cross_entropy(h, w, t)
+    keep = [i for i in range(40) if i != 5]
+    assert all(torch.equal(g[keep], c[keep]) and g[5].isnan() for g, c in zip(got, clean))
+    h[5, 1] = 0
+    h[:, 0], w[:, 0] = 30000.0, 0.0
+    w[2999, 0] = 1.0                      # one word far above the rest, in the last tile
+    t[:] = torch.arange(40, device="cuda")
+    with torch.no_grad():
+        losses, lse = vocab_cross_entropy(h, w, t)
+        check({"losses": losses, "lse": lse}, exact(h, w, t))
