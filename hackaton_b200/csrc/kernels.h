@@ -316,16 +316,17 @@ struct VocabLossArgs {
     float* target_logit;
     float* lse_rows;             // in the base-2 domain
     float* rest;                 // 1 - p of the target
-    float* norm;
+    float* norm;                 // one over the sum that `sums` is relative to
+    float* sums;                 // [rows that take part, hidden]: sum of exp(l_v - reference) w_v over v other than the target
     void* gathered;              // the rows themselves
-    float* mean;                 // [rows that take part, hidden]: sum of p_v w_v over v other than the target
     float2* parts;
     float* refs;
+    int* counters;               // of the sweeps, and `flags` and `list` behind them
+    long long n_counters;
     int* flags;
-    long long n_flags;
+    int* list;
     void* piece;
-    int capacity, slots;
-    float* planes;
+    int capacity;
     float4* coef;
     float* weight_scale;
 };

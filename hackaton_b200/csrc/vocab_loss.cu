@@ -11,17 +11,22 @@
 // operations (R rows, V words, K features) instead of three: a piece's exponentials are taken relative to a reference
 // per row that is fixed before the sweep (from the first words and the target's own logit), and the sum's 1 / s comes
 // at the end. The target is left out of U and of the sums, so that 1 - p_t and a loss near zero keep their digits, and its
-// share is added in fp32. A row that meets a logit too far above its reference for the 16-bit type has its piece done
-// again with a new one (its sums so far scaled by a power of two); launches for that look at a flag and leave. dW needs
-// the final lse: the logits once more, in 16-bit dl this time, and one product.
+// share is added in fp32. Where a row meets a logit too far above its reference for the 16-bit type, its row tile's sweep
+// is done again with references from the maxima; the launch for that looks at a flag and leaves. dW needs the final
+// lse: the logits once more, in 16-bit dl this time, and one product.
 //
-// All products run in one kernel, vl_gemm_kernel, in modes that differ in the operands' layouts and the epilogue; it
-// is bound by the tensor cores. CTA pairs (tcgen05.mma.cta_group::2) own a 256 x 256 tile, 128 rows by 256 columns of
-// fp32 in each CTA's tensor memory, twice: while eight warps work on one tile's values the next one is being
-// multiplied. Operands come by TMA in 64-deep steps through a ring of six. The 16-bit piece is laid out in blocks of
-// [rows][64 words], which is how TMA reads it along either side, and its size is chosen on the device: whole waves of
-// tiles for the rows there are, within a buffer that stays in L2.
-// Nothing is added atomically: results do not depend on timing.
+// The tensor cores bound it, and their clock the power that the chip may take, so what counts is that they never pause
+// and that little moves. CTA pairs (tcgen05.mma.cta_group::2) own a 256 x 256 tile, 128 rows by 256 columns of fp32 in
+// each CTA's tensor memory, twice: while eight warps work on one tile's values the next one is being multiplied.
+// Operands come by TMA in 64-deep steps through a ring of six. A sweep is one kernel (vl_sweep_kernel): first logits, then
+// the product with the 16-bit piece, as units of one list that the pairs draw tickets from,
+//     P(0)  P(1) Q(0)  P(2) Q(1)  ...  Q(last)          P(i): logits tiles of piece i, Q(i): tiles of the product with it
+// each unit waiting, with counters in memory, for what it reads or overwrites; all of that has smaller tickets, which
+// running CTAs have drawn, so that nothing depends on how many CTAs are resident. (As a launch per piece and product, a
+// pair idled 11 of 66 us per launch: 2048 rows x 151,936 words x 1536, loss and dH 1586 us, PLACEHOLDER.) The 16-bit piece is laid
+// out in blocks of [rows][64 words], which is how TMA reads it along either side; three pieces are in the works at a
+// time, their size chosen on the device for the rows there are, so that they and their words stay in L2.
+// Nothing is added in an order that depends on timing: U's tiles take the pieces' products one after the other.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,12 +46,14 @@ constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 
 constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
-constexpr int VL_PIECE_UNITS = 512;        // tiles of 256 x 256 that a piece may have: 64 MiB
+// A piece: at most VL_PIECE_TILES tiles of words and VL_PIECE_UNITS tiles of 256 x 256 (22 MB), at least
+// VL_PIECE_LEAST tiles of words, whatever the rows.
+constexpr int VL_PIECE_UNITS = 170, VL_PIECE_TILES = 24, VL_PIECE_LEAST = 8, VL_BUFFERS = 3;
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
 constexpr int VL_EPI_WARPS = 8;
-constexpr int VL_SMEM_MAX = 232448;
+constexpr int VL_SMEM_MAX = 232448, VL_BAR_ROOM = 512;
 // Shared memory of a CTA: the ring (128 rows of A and ROWS of B per step), a box of 32 rows x 128 bytes per epilogue warp
 // on its way out (OUT), barriers.
 template <int ROWS, int STAGES_, bool OUT>
@@ -56,22 +63,19 @@ struct VlSmem {
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int STAGING_OFF = STAGES * STAGE_BYTES;
     static constexpr int BAR_OFF = STAGING_OFF + (OUT ? VL_EPI_WARPS * 4096 : 0);
-    static constexpr int TOTAL = BAR_OFF + 8 * (3 * STAGES + 4) + 8 + 1024;    // + slack for 1024-byte alignment
+    static constexpr int TOTAL = BAR_OFF + VL_BAR_ROOM + 1024;    // + slack for 1024-byte alignment
     static_assert(TOTAL <= VL_SMEM_MAX && BAR_OFF % 8 == 0, "exceeds the 227 KB of shared memory per CTA");
 };
 constexpr int VL_THREADS = 64 + VL_EPI_WARPS * 32;
 
+// Statistics alone (no gradient of the hidden states): one product, nothing to write but a maximum and a sum.
 enum VlMode {
-    VL_STATS = 0,    // A = gathered rows [R, K], B = W [V, K]                -> maximum and sum per row and half tile
-    VL_SOFT = 1,     // the same operands, one piece                          -> exponentials in 16 bits, the same statistics
-    VL_GRAD = 2,     // the same                                              -> dl in 16 bits
-    VL_HIDDEN = 3,   // A = the piece [R, words], B = its rows of W, N along K   -> fp32 planes [slices][R, K]
-    VL_WEIGHT = 4,   // A = the piece transposed, B = gathered rows, N along K   -> 16-bit dW rows of the piece
-    VL_FEW = 5       // A = W, B = at most 64 gathered rows, words as M                 -> maximum and sum per row and warp
+    VL_STATS = 0,    // A = gathered rows [R, K], B = W [V, K]         -> maximum and sum per row and half tile
+    VL_FEW = 1       // A = W, B = at most 64 gathered rows, words as M -> per row and warp
 };
 
 struct VlMaps {
-    CUtensorMap a, b, c;     // c: where the epilogue's boxes go (not VL_STATS)
+    CUtensorMap a, b;
 };
 
 struct VlParams {
@@ -79,60 +83,111 @@ struct VlParams {
     int* status;
     int bf16;
     int vocab, hidden;
-    int word_tiles;          // of the whole vocabulary (VL_STATS: of what is to be looked at)
-    int index;               // of the piece
-    int capacity;            // tiles that a piece may have
-    int slots;               // pairs that pieces and slices are planned for
+    int word_tiles;          // to be looked at
     int n_rows;              // VL_FEW: columns of the accumulator, 32 or 64
     const int* target;       // per gathered row
-    // VL_STATS, VL_SOFT
-    float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum (relative to it; VL_SOFT: to the reference)
+    float2* parts;           // [parts][rows_pad]: maximum (base 2), sum relative to it
     long long rows_pad;
-    // VL_SOFT, VL_HIDDEN
-    float* refs;             // [pieces + 1][rows_pad]: a row's reference before each piece and after the last
-    int* flags;              // [pieces][1 + row tiles]: whether any row, and which tiles' rows, need the piece again
-    int flags_pitch;
-    int again;               // VL_SOFT: this launch does flagged pieces again
-    // VL_GRAD
+};
+
+struct VlSweepMaps {
+    CUtensorMap rows, words;      // P: gathered rows, W
+    CUtensorMap piece_in;         // Q: the piece, as rows (forward) or as words (backward) of the product
+    CUtensorMap other;            // Q: W with features along N (forward), gathered rows with features along N (backward)
+    CUtensorMap piece_out;        // P writes the piece
+    CUtensorMap out;              // Q adds to U (forward, fp32), writes dW (backward)
+};
+
+struct VlSweepParams {
+    const int* count;
+    int* status;
+    int bf16;
+    int vocab, hidden;
+    int word_tiles;
+    int capacity;            // tiles that a piece may have
+    long long rows_pad;
+    const int* target;
+    void* piece;             // [buffer][block of 64 words][rows of the tiles][64]
+    // counters, zero before: units drawn; per piece and row tile (backward: word tile) warps that have written their
+    // part of the piece, units that have read it; per tile of U warps that have added theirs
+    int* ticket;
+    int* written;
+    int* read;
+    int* added;
+    int pitch;               // counters per piece
+    // forward
+    float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum relative to the reference
+    const float* refs;       // [rows_pad]
+    int* flags;              // [1 + row tiles]: whether any row, and which tiles' rows, outgrew their references
+    const int* list;         // a sweep done again: number of row tiles, their indexes
+    int again;
+    // backward
     const float* lse2;
     const float* rest;       // 1 - p of the target
     const float4* coef;      // ((b + c), b, c) over the common power of two, times VL_P_SCALE
-    // VL_SOFT, VL_GRAD: the 16-bit piece, [block of 64 words][rows of the tiles][64]
-    void* piece;
-    // VL_HIDDEN
-    float* planes;           // [slices][rows of the tiles][hidden]
-    // VL_WEIGHT
     void* d_weight;          // [vocab, hidden]
     const float* weight_scale;
 };
 
 __host__ __device__ inline int vl_div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Tiles of words in a piece: what the buffer holds for so many row tiles, cut to whole waves of the pairs.
-__host__ __device__ inline int vl_piece_tiles(int row_tiles, int word_tiles, int capacity, int slots) {
-    int t = capacity / row_tiles;
-    if (t >= word_tiles) return word_tiles;
-    const int waves = row_tiles * t / slots;
-    if (waves > 0) t = waves * slots / row_tiles;
-    return t > 0 ? t : 1;
-}
-
-// Slices of a piece's words for U: as many as keep the pairs busiest, with at least eight steps each; none is empty.
-constexpr int VL_MAX_SLICES = 16;
-__host__ __device__ inline int vl_slices(int tiles, int steps, int slots) {
-    int best = 1, best_cost = 0x7FFFFFFF;
-    for (int s = 1; s <= VL_MAX_SLICES && (s == 1 || steps / s >= 8); ++s) {
-        const int per = vl_div_up(steps, s);
-        const int cost = vl_div_up(tiles * vl_div_up(steps, per), slots) * (per + 6);
-        if (cost < best_cost) { best_cost = cost; best = s; }
-    }
-    return vl_div_up(steps, vl_div_up(steps, best));
+// Tiles of words in a piece for so many row tiles.
+__host__ __device__ inline int vl_piece_tiles(int row_tiles, int word_tiles, int capacity) {
+    int t = capacity / (row_tiles > 0 ? row_tiles : 1);
+    if (t > VL_PIECE_TILES) t = VL_PIECE_TILES;
+    return t < word_tiles ? t : word_tiles;
 }
 
 __device__ __forceinline__ float vl_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ void vl_sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// The largest of 32 accumulator values (a NaN left out).
+__device__ __forceinline__ float vl_top(const uint32_t (&r)[32]) {
+    float top = __uint_as_float(r[0]);
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
+    return top;
+}
+
+// Of 32 words' logits, what lies behind the vocabulary and the target's own count as nothing.
+__device__ __forceinline__ void vl_leave_out(uint32_t (&r)[32], int words, int target) {
+    if (!__any_sync(0xffffffffu, words < 32 || (unsigned)target < 32u)) return;
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+        if (e >= words || e == target) r[e] = __float_as_uint(VL_NEG);
+}
+
+// Arrival and wait that order memory over the cluster (tickets are written by the pair's other CTA).
+__device__ __forceinline__ void vl_mbar_arrive_release(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool vl_mbar_wait_acquire(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    unsigned long long t0 = 0;
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "}\n"
+            : "=r"(done) : "r"(bar), "r"(parity), "r"(TRY_WAIT_HINT_NS) : "memory");
+        if (done) return true;
+        const unsigned long long now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        if (*abort_flag) return false;
+        if (now - t0 > WAIT_TIMEOUT_NS) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
 }
 
 __device__ __forceinline__ uint32_t vl_pack(float a, float b, int bf16) {
@@ -144,82 +199,43 @@ __device__ __forceinline__ uint32_t vl_pack(float a, float b, int bf16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void vl_sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+template <int MODE>
+using VlSmemOf = VlSmem<MODE == VL_FEW ? 32 : 128, MODE == VL_FEW ? 11 : 7, false>;
+
+__device__ __forceinline__ float2 vl_join(float2 x, float2 y) {
+    const float top = fmaxf(x.x, y.x);
+    return make_float2(top, x.y * vl_ex2(x.x - top) + y.y * vl_ex2(y.x - top));
 }
 
-struct VlPlan {      // what a launch's units are, from the device's row count
-    int rows, row_tiles, v0, tiles;            // first word and tiles of the piece
-    int m_tiles, units, steps, slices, per_slice;
-};
+// tcgen05 descriptors: K-major tiles are rows of 128 bytes, eight rows 1024 bytes apart; MN-major ones 64 steps of 128
+// bytes (64 values along M or N), the next 64 values 8192 bytes on.
+constexpr uint64_t VL_K_MAJOR = make_smem_desc(0, 16, 1024, LAYOUT_SW128);
+constexpr uint64_t VL_MN_MAJOR = make_smem_desc(0, 8192, 1024, LAYOUT_SW128);
 
-template <int MODE>
-__device__ __forceinline__ VlPlan vl_plan(const VlParams& p, int rows) {
-    VlPlan w;
-    w.rows = rows;
-    w.row_tiles = vl_div_up(rows, VL_TILE);
-    w.slices = 1;
-    const int feature_tiles = vl_div_up(p.hidden, VL_TILE);
-    w.v0 = 0;
-    w.tiles = p.word_tiles;
-    int first_tiles = p.word_tiles;
-    if (MODE != VL_STATS && MODE != VL_FEW) {
-        first_tiles = vl_piece_tiles(max(w.row_tiles, 1), p.word_tiles, p.capacity, p.slots);
-        const int before = min((long long)first_tiles * p.index, (long long)p.word_tiles);
-        w.v0 = before * VL_TILE;
-        w.tiles = min(first_tiles, p.word_tiles - before);
-    }
-    if (MODE == VL_WEIGHT) {
-        w.m_tiles = w.tiles;
-        w.steps = vl_div_up(rows, VL_BK);
-        w.units = w.tiles * feature_tiles;
-    } else if (MODE == VL_HIDDEN) {
-        w.m_tiles = w.row_tiles;
-        w.steps = w.tiles * (VL_TILE / VL_BK);
-        const int tiles = w.row_tiles * feature_tiles;
-        if (rows > 0) w.slices = vl_slices(tiles, first_tiles * (VL_TILE / VL_BK), p.slots);
-        w.units = w.tiles > 0 ? tiles * w.slices : 0;
-    } else if (MODE == VL_FEW) {
-        w.m_tiles = w.tiles;
-        w.steps = vl_div_up(p.hidden, VL_BK);
-        w.units = rows > 0 ? w.tiles : 0;
-    } else {
-        w.m_tiles = w.row_tiles;
-        w.steps = vl_div_up(p.hidden, VL_BK);
-        w.units = w.row_tiles * w.tiles;
-    }
-    w.per_slice = vl_div_up(w.steps, w.slices);
-    return w;
+// One 64-deep step of a pair's tile.
+__device__ __forceinline__ void vl_mma_step(uint32_t d_tmem, uint32_t a4, uint32_t b4, bool a_mn, bool b_mn, uint32_t idesc, bool first) {
+    const uint32_t a_lo = a4 + (uint32_t)((a_mn ? VL_MN_MAJOR : VL_K_MAJOR) & 0xFFFFFFFFu), a_hi = (uint32_t)((a_mn ? VL_MN_MAJOR : VL_K_MAJOR) >> 32);
+    const uint32_t b_lo = b4 + (uint32_t)((b_mn ? VL_MN_MAJOR : VL_K_MAJOR) & 0xFFFFFFFFu), b_hi = (uint32_t)((b_mn ? VL_MN_MAJOR : VL_K_MAJOR) >> 32);
+    const uint32_t a_step = (a_mn ? 16 * 128 : 32) >> 4, b_step = (b_mn ? 16 * 128 : 32) >> 4;
+#pragma unroll
+    for (int k = 0; k < VL_BK / 16; ++k)
+        umma_f16_words<2>(d_tmem, a_lo + a_step * k, a_hi, b_lo + b_step * k, b_hi, idesc, first && k == 0 ? 0u : 1u);
 }
 
-template <int MODE>
-using VlSmemOf = VlSmem<MODE == VL_FEW ? 32 : 128, MODE == VL_FEW ? 11 : MODE == VL_STATS ? 7 : 6, MODE != VL_STATS && MODE != VL_FEW>;
+__device__ __forceinline__ uint32_t vl_idesc(int n, bool a_mn, bool b_mn, int bf16) {
+    return make_idesc_f16((uint32_t)n, a_mn ? 1u : 0u, b_mn ? 1u : 0u, VL_TILE) | (bf16 ? (1u << 7) | (1u << 10) : 0u);
+}
 
-struct VlUnit {
-    int mt, nt, slice, begin, steps;
-};
-
-template <int MODE>
-__device__ __forceinline__ VlUnit vl_unit(int u, const VlPlan& w) {
-    VlUnit r;
-    r.slice = 0;
-    if (MODE == VL_HIDDEN) {       // slices outermost: the units of a wave read the same words
-        const int tiles = w.units / w.slices;
-        r.slice = u / tiles;
-        u -= r.slice * tiles;
-    }
-    r.mt = u % w.m_tiles;
-    r.nt = u / w.m_tiles;
-    r.begin = r.slice * w.per_slice;
-    r.steps = min(w.per_slice, w.steps - r.begin);
-    return r;
+// On a failed wait: copies and MMAs in flight get time to land before shared memory and TMEM go away.
+__device__ __forceinline__ void vl_failed(int* status, int fail) {
+    atomicCAS(status, 0, 100 + fail);
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
 }
 
 template <int MODE>
 __global__ void __launch_bounds__(VL_THREADS, 1)
-vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
-    constexpr bool A_MN = MODE == VL_WEIGHT, B_MN = MODE == VL_HIDDEN || MODE == VL_WEIGHT;
-    constexpr bool A_PIECE = MODE == VL_HIDDEN || MODE == VL_WEIGHT;      // A comes from the 16-bit piece
+vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
     using L = VlSmemOf<MODE>;
     constexpr int STAGES = L::STAGES;
     extern __shared__ uint8_t vl_smem[];
@@ -227,9 +243,9 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     uint8_t* gen = vl_smem + (base - smem_u32(vl_smem));
     const uint32_t bar = base + L::BAR_OFF;
     auto bar_full = [&](int s) { return bar + 8u * s; };                        // leader: both CTAs' operands
-    auto bar_landed = [&](int s) { return bar + 8u * (STAGES + s); };        // peer: its own
+    auto bar_landed = [&](int s) { return bar + 8u * (STAGES + s); };           // peer: its own
     auto bar_empty = [&](int s) { return bar + 8u * (2 * STAGES + s); };
-    auto bar_done = [&](int b) { return bar + 8u * (3 * STAGES + b); };      // accumulator complete
+    auto bar_done = [&](int b) { return bar + 8u * (3 * STAGES + b); };         // accumulator complete
     auto bar_drained = [&](int b) { return bar + 8u * (3 * STAGES + 2 + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BAR_OFF + 8 * (3 * STAGES + 4));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BAR_OFF + 8 * (3 * STAGES + 4) + 4);
@@ -237,11 +253,6 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
-    const int* flags = p.flags + (long long)p.index * p.flags_pitch;
-    if (MODE == VL_SOFT && p.again) {     // nearly always there is nothing to do again
-        grid_dep_wait();
-        if (flags[0] == 0) return;
-    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -259,7 +270,6 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&maps.a);
         tma_prefetch_desc(&maps.b);
-        if (MODE != VL_STATS) tma_prefetch_desc(&maps.c);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -272,90 +282,52 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    const int rows = *p.count;
-    const VlPlan plan = vl_plan<MODE>(p, rows);
-    const int rows_dev = plan.row_tiles * VL_TILE;
-    // (what all roles leave out: slices that the last piece has no steps for, row tiles that need not be done again)
-    const auto skip = [&](const VlUnit& w) {
-        return w.steps <= 0 || (MODE == VL_SOFT && p.again && flags[1 + w.mt] == 0);
-    };
+    const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK);
+    const int units = rows == 0 ? 0 : MODE == VL_FEW ? p.word_tiles : row_tiles * p.word_tiles;
     int fail = 0;
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t g = 0;
-            for (int u = pair; u < plan.units && !fail; u += pairs) {
-                const VlUnit w = vl_unit<MODE>(u, plan);
-                if (skip(w)) continue;
-                for (int it = 0; it < w.steps; ++it, ++g) {
+            for (int u = pair; u < units && !fail; u += pairs) {
+                const int am = (MODE == VL_FEW ? u : u % row_tiles) * VL_TILE + (int)rank * 128;
+                const int bn = MODE == VL_FEW ? (int)rank * (p.n_rows / 2) : u / row_tiles * VL_TILE + (int)rank * 128;
+                for (int it = 0; it < steps; ++it, ++g) {
                     const int s = (int)(g % STAGES);
-                    const uint32_t ph = (g / STAGES) & 1u;
-                    if (!mbar_wait_cluster(bar_empty(s), ph ^ 1u, abort_flag)) { fail = 1; break; }
+                    if (!mbar_wait_cluster(bar_empty(s), ((g / STAGES) & 1u) ^ 1u, abort_flag)) { fail = 1; break; }
                     const uint32_t landed = rank == 0 ? bar_full(s) : bar_landed(s);
-                    const uint32_t sa = base + (uint32_t)s * L::STAGE_BYTES, sb = sa + L::A_BYTES;
-                    const int k = (w.begin + it) * VL_BK;
-                    const int am = w.mt * VL_TILE + (int)rank * 128;
-                    const int bn = MODE == VL_FEW ? (int)rank * (p.n_rows / 2) : w.nt * VL_TILE + (int)rank * 128;
+                    const uint32_t sa = base + (uint32_t)s * L::STAGE_BYTES;
                     mbar_arrive_expect_tx(landed, L::A_BYTES + (MODE == VL_FEW ? p.n_rows * 64 : L::B_BYTES));
-                    if (A_MN) {             // words as M, rows as steps
-                        tma_load_2d(sa, &maps.a, 0, (am >> 6) * rows_dev + k, landed);
-                        tma_load_2d(sa + 8192, &maps.a, 0, ((am >> 6) + 1) * rows_dev + k, landed);
-                    } else if (A_PIECE) {   // rows as M, words as steps
-                        tma_load_2d(sa, &maps.a, 0, (k >> 6) * rows_dev + am, landed);
-                    } else {
-                        tma_load_2d(sa, &maps.a, k, am, landed);
-                    }
-                    if (B_MN) {     // VL_HIDDEN: rows of W from the piece's first word on; VL_WEIGHT: gathered rows
-                        const int y = MODE == VL_HIDDEN ? plan.v0 + k : k;
-                        tma_load_2d(sb, &maps.b, bn, y, landed);
-                        tma_load_2d(sb + 8192, &maps.b, bn + 64, y, landed);
-                    } else {
-                        tma_load_2d(sb, &maps.b, k, plan.v0 + bn, landed);
-                    }
+                    tma_load_2d(sa, &maps.a, it * VL_BK, am, landed);
+                    tma_load_2d(sa + L::A_BYTES, &maps.b, it * VL_BK, bn, landed);
                 }
             }
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            // tcgen05 descriptors: K-major tiles are rows of 128 bytes, eight rows 1024 bytes apart; MN-major ones 64 steps
-            // of 128 bytes (64 values along M or N), the next 64 values 8192 bytes on
-            constexpr uint64_t K_MAJOR = make_smem_desc(0, 16, 1024, LAYOUT_SW128);
-            constexpr uint64_t MN_MAJOR = make_smem_desc(0, 8192, 1024, LAYOUT_SW128);
-            constexpr uint64_t A_DESC = A_MN ? MN_MAJOR : K_MAJOR, B_DESC = B_MN ? MN_MAJOR : K_MAJOR;
-            constexpr uint32_t A_STEP = (A_MN ? 16 * 128 : 32) >> 4, B_STEP = (B_MN ? 16 * 128 : 32) >> 4;
-            const uint32_t idesc = make_idesc_f16(MODE == VL_FEW ? (uint32_t)p.n_rows : VL_TILE, A_MN ? 1u : 0u, B_MN ? 1u : 0u, VL_TILE) |
-                                   (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
+            const uint32_t idesc = vl_idesc(MODE == VL_FEW ? p.n_rows : VL_TILE, false, false, p.bf16);
             const uint32_t base4 = (base & 0x3FFFFu) >> 4;
             uint32_t g = 0, n = 0;
-            for (int u = pair; u < plan.units && !fail; u += pairs) {
-                const VlUnit w = vl_unit<MODE>(u, plan);
-                if (skip(w)) continue;
+            for (int u = pair; u < units && !fail; u += pairs, ++n) {
                 const int b = (int)(n & 1u);
                 if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
                 tc_fence_after_sync();
-                for (int it = 0; it < w.steps; ++it, ++g) {
+                for (int it = 0; it < steps; ++it, ++g) {
                     const int s = (int)(g % STAGES);
                     if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
                     tc_fence_after_sync();
-                    const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4), b4 = a4 + (L::A_BYTES >> 4);
-#pragma unroll
-                    for (int k = 0; k < VL_BK / 16; ++k)
-                        umma_f16_words<2>(tmem + b * VL_TILE, a4 + (uint32_t)(A_DESC & 0xFFFFFFFFu) + A_STEP * k,
-                                          (uint32_t)(A_DESC >> 32), b4 + (uint32_t)(B_DESC & 0xFFFFFFFFu) + B_STEP * k,
-                                          (uint32_t)(B_DESC >> 32), idesc, it > 0 || k > 0 ? 1u : 0u);
+                    const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4);
+                    vl_mma_step(tmem + b * VL_TILE, a4, a4 + (L::A_BYTES >> 4), false, false, idesc, it == 0);
                     umma_commit_pair(bar_empty(s), (uint16_t)3);
                 }
                 if (fail) break;
                 umma_commit_pair(bar_done(b), (uint16_t)3);
-                ++n;
             }
         } else if (lane == 0) {
             const uint32_t lead_full0 = mapa_shared(bar_full(0), 0u);
             uint32_t g = 0;
-            for (int u = pair; u < plan.units && !fail; u += pairs) {
-                const VlUnit w = vl_unit<MODE>(u, plan);
-                if (skip(w)) continue;
-                for (int it = 0; it < w.steps; ++it, ++g) {
+            for (int u = pair; u < units && !fail; u += pairs) {
+                for (int it = 0; it < steps; ++it, ++g) {
                     const int s = (int)(g % STAGES);
                     if (!mbar_wait(bar_landed(s), (g / STAGES) & 1u, abort_flag)) { fail = 8; break; }
                     mbar_arrive_cluster(lead_full0 + 8u * s);
@@ -373,7 +345,7 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
 #pragma unroll
         for (int j = 0; j < 32; ++j) { m[j] = VL_NEG; s[j] = 0.f; }
         uint32_t it = 0;
-        for (int u = pair; u < plan.units && !fail; u += pairs, ++it) {
+        for (int u = pair; u < units && !fail; u += pairs, ++it) {
             const int b = (int)(it & 1u);
             if (!mbar_wait(bar_done(b), (it >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
@@ -409,10 +381,10 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
             if (j >= n) break;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
-                const float om = __shfl_xor_sync(0xffffffffu, m[j], o), os = __shfl_xor_sync(0xffffffffu, s[j], o);
-                const float top = fmaxf(m[j], om);
-                s[j] = s[j] * vl_ex2(m[j] - top) + os * vl_ex2(om - top);
-                m[j] = top;
+                const float2 x = vl_join(make_float2(m[j], s[j]), make_float2(__shfl_xor_sync(0xffffffffu, m[j], o),
+                                                                              __shfl_xor_sync(0xffffffffu, s[j], o)));
+                m[j] = x.x;
+                s[j] = x.y;
             }
             if (lane == 0) p.parts[(long long)(blockIdx.x * 4 + q) * p.rows_pad + row0 + j] = make_float2(m[j], s[j]);
         }
@@ -420,159 +392,432 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
         // ------------------------------------------------------------------ epilogue: a row's half tile per thread
         const int q = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
-        const uint32_t staging = base + L::STAGING_OFF + (uint32_t)(warp - 2) * 4096u;
         uint32_t n = 0;
-        for (int u = pair; u < plan.units && !fail; u += pairs) {
-            const VlUnit w = vl_unit<MODE>(u, plan);
-            const int row = w.mt * VL_TILE + (int)rank * 128 + q * 32 + lane;     // VL_WEIGHT: word of the piece
-            const int col0 = w.nt * VL_TILE + half * 128;
-            if (MODE == VL_WEIGHT && plan.steps <= 0) {
-                // no row takes part: the gradient of the head is zero
-                if (plan.v0 + row < p.vocab)
-                    for (int c = col0; c < col0 + 128 && c < p.hidden; ++c)
-                        static_cast<unsigned short*>(p.d_weight)[(long long)(plan.v0 + row) * p.hidden + c] = 0;
-                continue;
-            }
-            const bool live = row < rows;
-            float scale = 1.f;
-            if (MODE == VL_HIDDEN && live && p.index > 0)
-                scale = exp2f(p.refs[p.index * p.rows_pad + row] - p.refs[(p.index + 1) * p.rows_pad + row]);
-            if (skip(w)) {
-                if (MODE == VL_HIDDEN && live && scale != 1.f) {     // nothing to add, but the reference has moved
-                    float* plane = p.planes + ((long long)w.slice * rows_dev + row) * p.hidden;
-                    for (int c = col0; c < col0 + 128 && c < p.hidden; ++c) plane[c] *= scale;
-                }
-                continue;
-            }
-            const int b = (int)(n & 1u);
-            // what the values meet, asked for before the tile is complete
-            int target = -1;
-            float lse2 = 0.f, rest = 0.f, ref = 0.f;
-            float4 coef = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (MODE <= VL_GRAD && live) target = p.target[row] - plan.v0 - col0;   // column of this thread's share
-            if (MODE == VL_GRAD && live) {
-                lse2 = p.lse2[row];
-                rest = p.rest[row];
-                coef = p.coef[row];
-            }
-            if (MODE == VL_SOFT && live) {
-                ref = p.refs[p.index * p.rows_pad + row];
-                if (p.again) {
-                    // the piece's largest decides whether this row changes its reference (the sums are not read:
-                    // they may have overflowed, and other units replace them)
-                    float top = VL_NEG;
-                    for (int i = 0; i < 2 * plan.tiles; ++i)
-                        top = fmaxf(top, p.parts[(plan.v0 / VL_TILE * 2 + i) * p.rows_pad + row].x);
-                    if (top > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) ref = ceilf(top) - 6.f;
-                }
-                if (w.nt == 0 && half == 0) p.refs[(p.index + 1) * p.rows_pad + row] = ref;
-            }
-            if (MODE == VL_WEIGHT) scale = *p.weight_scale;
+        for (int u = pair; u < units && !fail; u += pairs, ++n) {
+            const int row = u % row_tiles * VL_TILE + (int)rank * 128 + q * 32 + lane, nt = u / row_tiles;
+            const int col0 = nt * VL_TILE + half * 128, b = (int)(n & 1u);
+            const int target = row < rows ? p.target[row] - col0 : -1;      // column of this thread's share
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
-            auto release = [&]() {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
-            };
-            // The box's memory is free again once the store before has read it; what is in it goes out as 32 whole lines.
-            auto box_begin = [&]() {
-                if (lane == 0) bulk_wait_read();
-                __syncwarp();
-            };
-            auto box_put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t t) {    // 16 bytes of this lane's row
-                vl_sts128(staging + lane * 128 + ((chunk ^ (lane & 7)) << 4), x, y, z, t);
-            };
-            auto box_end = [&](int x, int y, bool add) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    if (add) tma_reduce_add_2d(&maps.c, staging, x, y);
-                    else     tma_store_2d(&maps.c, staging, x, y);
-                    bulk_commit();
-                }
-            };
-            const int row0 = row - lane;
-            // 32 values in 16 bits: half a box
-            auto put16 = [&](const float (&v)[32], int c) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    box_put((c & 32) / 8 + i, vl_pack(v[8 * i], v[8 * i + 1], p.bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.bf16),
-                            vl_pack(v[8 * i + 4], v[8 * i + 5], p.bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.bf16));
-            };
-            // values of the 16-bit piece (columns col0 + c ..)
-            auto store_piece = [&](const float (&v)[32], int c) {
-                if ((c & 32) == 0) box_begin();
-                put16(v, c);
-                if ((c & 32) != 0) box_end(0, ((col0 + c) >> 6) * rows_dev + row0, false);
-            };
             float m2 = VL_NEG, sum = 0.f;
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(at + c, r);
                 tmem_ld_wait();
-                if (c == 96) release();
-                if (MODE <= VL_SOFT) {
-                    const int words = p.vocab - plan.v0 - col0 - c;       // words there are in this chunk
-                    const bool cut = words < 32 || (unsigned)(target - c) < 32u;
-                    if (__any_sync(0xffffffffu, cut)) {
+                if (c == 96) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
+                }
+                vl_leave_out(r, p.vocab - col0 - c, target - c);
+                const float top2 = vl_top(r) * VL_LOG2E;
+                if (top2 > m2) {
+                    sum *= vl_ex2(m2 - top2);
+                    m2 = top2;
+                }
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (e >= words || e == target - c) r[e] = __float_as_uint(VL_NEG);
+                for (int e = 0; e < 32; ++e) part[e & 3] += vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -m2));
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+            }
+            p.parts[(long long)(2 * nt + half) * p.rows_pad + row] = make_float2(m2, sum);
+        }
+    }
+
+    if (fail) vl_failed(p.status, fail);
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------------------------- the sweep
+struct VlUnit {
+    bool q;              // a tile of the product with the piece, not of the logits
+    int piece, tiles;    // the piece, its tiles of words
+    int mt;              // row tile (P, forward's Q)
+    int slot;            // where its counters are: row tile among those of the sweep (forward), word tile of the piece
+    int nt;              // P: word tile of the piece; Q: feature tile
+    int steps;
+};
+
+struct VlList {          // the list of units
+    int rows, row_tiles, active, feature_tiles, tiles, pieces, last_tiles, p, q, p_last, q_last, total;
+};
+
+template <bool BWD>
+__device__ __forceinline__ VlList vl_list(const VlSweepParams& p) {
+    VlList w;
+    w.rows = *p.count;
+    w.row_tiles = vl_div_up(w.rows, VL_TILE);
+    w.active = p.again ? p.list[0] : w.row_tiles;
+    w.feature_tiles = vl_div_up(p.hidden, VL_TILE);
+    w.tiles = vl_piece_tiles(w.row_tiles, p.word_tiles, p.capacity);
+    w.pieces = vl_div_up(p.word_tiles, w.tiles);
+    w.last_tiles = p.word_tiles - (w.pieces - 1) * w.tiles;
+    w.p = w.active * w.tiles;
+    w.p_last = w.active * w.last_tiles;
+    w.q = (BWD ? w.tiles : w.active) * w.feature_tiles;
+    w.q_last = (BWD ? w.last_tiles : w.active) * w.feature_tiles;
+    w.total = (w.pieces - 1) * (w.p + w.q) + w.p_last + w.q_last;
+    return w;
+}
+
+template <bool BWD>
+__device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const VlList& w) {
+    VlUnit r;
+    const int head = w.pieces == 1 ? w.p_last : w.p;
+    if (k < head) {
+        r.q = false;
+        r.piece = 0;
+    } else {
+        k -= head;
+        const int block = min(k / max(w.p + w.q, 1), max(w.pieces - 2, 0));
+        k -= block * (w.p + w.q);
+        r.piece = min(block + 1, w.pieces - 1);                 // P(piece), then Q(piece - 1); behind the last also Q(piece)
+        const int ps = w.pieces == 1 ? 0 : r.piece == w.pieces - 1 ? w.p_last : w.p;
+        r.q = k >= ps;
+        if (r.q) {
+            k -= ps;
+            if (w.pieces > 1 && k < w.q) r.piece -= 1;
+            else if (w.pieces > 1)       k -= w.q;
+        }
+    }
+    r.tiles = r.piece == w.pieces - 1 ? w.last_tiles : w.tiles;
+    const int width = r.q && BWD ? r.tiles : w.active, first = k % width;
+    r.nt = k / width;
+    r.mt = r.q && BWD ? 0 : p.again ? p.list[1 + first] : first;
+    r.slot = BWD ? (r.q ? first : r.nt) : first;
+    r.steps = !r.q ? vl_div_up(p.hidden, VL_BK) : BWD ? vl_div_up(w.rows, VL_BK) : r.tiles * (VL_TILE / VL_BK);
+    return r;
+}
+
+// Bounded wait for a counter in memory. What its writers wrote before is visible behind it, to TMA too.
+__device__ __forceinline__ bool vl_wait_count(const int* counter, int least, volatile int* abort_flag) {
+    if (least <= 0) return true;
+    unsigned long long t0 = 0;
+    for (;;) {
+        int v;
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
+        if (v >= least) break;
+        const unsigned long long now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        if (*abort_flag) return false;
+        if (now - t0 > WAIT_TIMEOUT_NS) {
+            *abort_flag = 1;
+            return false;
+        }
+        __nanosleep(100);
+    }
+    asm volatile("fence.proxy.async;" ::: "memory");
+    return true;
+}
+
+// Counts one more, behind everything this thread wrote or waited for, its TMA stores included.
+__device__ __forceinline__ void vl_count(int* counter) {
+    asm volatile("fence.proxy.async;" ::: "memory");
+    asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(counter) : "memory");
+}
+
+constexpr int VL_TICKETS = 4;        // units that a pair has drawn and not begun, at most
+constexpr int VL_SWEEP_THREADS = VL_THREADS + 32;
+
+template <bool BWD>
+__global__ void __launch_bounds__(VL_SWEEP_THREADS, 1)
+vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant__ VlSweepParams p) {
+    using L = VlSmem<128, 6, true>;
+    constexpr int STAGES = L::STAGES;
+    constexpr int BARS = 3 * STAGES + 4 + 2 * VL_TICKETS;
+    constexpr uint32_t ALL = 2 * (VL_EPI_WARPS + 2);      // who reads a ticket: both CTAs' TMA, MMA (peer: its word) and epilogue
+    extern __shared__ uint8_t vl_smem[];
+    const uint32_t base = (smem_u32(vl_smem) + 1023u) & ~1023u;
+    uint8_t* gen = vl_smem + (base - smem_u32(vl_smem));
+    const uint32_t bar = base + L::BAR_OFF;
+    auto bar_full = [&](int s) { return bar + 8u * s; };
+    auto bar_landed = [&](int s) { return bar + 8u * (STAGES + s); };
+    auto bar_empty = [&](int s) { return bar + 8u * (2 * STAGES + s); };
+    auto bar_done = [&](int b) { return bar + 8u * (3 * STAGES + b); };
+    auto bar_drained = [&](int b) { return bar + 8u * (3 * STAGES + 2 + b); };
+    auto bar_drawn = [&](int k) { return bar + 8u * (3 * STAGES + 4 + k); };                    // a ticket is there
+    auto bar_taken = [&](int k) { return bar + 8u * (3 * STAGES + 4 + VL_TICKETS + k); };       // leader: all have read it
+    static_assert(8 * BARS + 8 + 4 * VL_TICKETS <= VL_BAR_ROOM, "barrier area");
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BAR_OFF + 8 * BARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BAR_OFF + 8 * BARS + 4);
+    const uint32_t tickets = base + L::BAR_OFF + 8 * BARS + 8;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    if (!BWD && p.again) {     // nearly always there is nothing to do again
+        grid_dep_wait();
+        if (p.list[0] == 0) return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bar_full(s), 2);
+            mbar_init(bar_landed(s), 1);
+            mbar_init(bar_empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar_done(b), 1);
+            mbar_init(bar_drained(b), 2 * VL_EPI_WARPS);
+        }
+        for (int k = 0; k < VL_TICKETS; ++k) {
+            mbar_init(bar_drawn(k), 1);
+            mbar_init(bar_taken(k), ALL);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&maps.rows);
+        tma_prefetch_desc(&maps.words);
+        tma_prefetch_desc(&maps.piece_in);
+        tma_prefetch_desc(&maps.other);
+        tma_prefetch_desc(&maps.piece_out);
+        tma_prefetch_desc(&maps.out);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+        tmem_relinquish_pair();
+    }
+    grid_dep_wait();
+    grid_dep_launch();
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const VlList list = vl_list<BWD>(p);
+    const int rows = list.rows, rows_dev = list.row_tiles * VL_TILE;
+    const int buffer_rows = p.capacity * VL_TILE * (VL_TILE / 64);     // of 64 words, in one buffer
+    int fail = 0;
+
+    // The next unit's ticket, or -1 behind the last; every reader takes them in turn: one lane for itself, or a warp, of
+    // which all lanes have read before one says so.
+    const uint32_t lead_taken0 = mapa_shared(bar_taken(0), 0u);
+    uint32_t drawn = 0;
+    auto next_ticket = [&](bool whole_warp) -> int {
+        const int k = (int)(drawn % VL_TICKETS);
+        if (!vl_mbar_wait_acquire(bar_drawn(k), (drawn / VL_TICKETS) & 1u, abort_flag)) { fail = 9; return -1; }
+        int t;
+        asm volatile("ld.shared.s32 %0, [%1];" : "=r"(t) : "r"(tickets + 4u * k) : "memory");
+        if (whole_warp) __syncwarp();
+        if (!whole_warp || lane == 0) vl_mbar_arrive_release(lead_taken0 + 8u * k);
+        ++drawn;
+        return t;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t g = 0;
+            for (int t; !fail && (t = next_ticket(false)) >= 0;) {
+                const VlUnit w = vl_unit<BWD>(t, p, list);
+                const int in_buffer = w.piece % VL_BUFFERS * buffer_rows, v0 = w.piece * list.tiles * VL_TILE;
+                if (w.q) {     // the piece has to be there
+                    const int least = 2 * VL_EPI_WARPS * (BWD ? list.active : w.tiles);
+                    if (!vl_wait_count(p.written + w.piece * p.pitch + w.slot, least, abort_flag)) { fail = 10; break; }
+                }
+                const int am = (w.q && BWD ? w.slot : w.mt) * VL_TILE + (int)rank * 128, bn = w.nt * VL_TILE + (int)rank * 128;
+                for (int it = 0; it < w.steps; ++it, ++g) {
+                    const int s = (int)(g % STAGES);
+                    if (!mbar_wait_cluster(bar_empty(s), ((g / STAGES) & 1u) ^ 1u, abort_flag)) { fail = 1; break; }
+                    const uint32_t landed = rank == 0 ? bar_full(s) : bar_landed(s);
+                    const uint32_t sa = base + (uint32_t)s * L::STAGE_BYTES, sb = sa + L::A_BYTES;
+                    mbar_arrive_expect_tx(landed, L::STAGE_BYTES);
+                    if (!w.q) {
+                        tma_load_2d(sa, &maps.rows, it * VL_BK, am, landed);
+                        tma_load_2d(sb, &maps.words, it * VL_BK, v0 + bn, landed);
+                    } else if (!BWD) {       // rows as M, words as steps; features as N
+                        tma_load_2d(sa, &maps.piece_in, 0, in_buffer + it * rows_dev + am, landed);
+                        tma_load_2d(sb, &maps.other, bn, v0 + it * VL_BK, landed);
+                        tma_load_2d(sb + 8192, &maps.other, bn + 64, v0 + it * VL_BK, landed);
+                    } else {                 // words as M, rows as steps; features as N
+                        tma_load_2d(sa, &maps.piece_in, 0, in_buffer + (am >> 6) * rows_dev + it * VL_BK, landed);
+                        tma_load_2d(sa + 8192, &maps.piece_in, 0, in_buffer + ((am >> 6) + 1) * rows_dev + it * VL_BK, landed);
+                        tma_load_2d(sb, &maps.other, bn, it * VL_BK, landed);
+                        tma_load_2d(sb + 8192, &maps.other, bn + 64, it * VL_BK, landed);
                     }
-                    float top = __uint_as_float(r[0]);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc_p = vl_idesc(VL_TILE, false, false, p.bf16), idesc_q = vl_idesc(VL_TILE, BWD, true, p.bf16);
+            const uint32_t base4 = (base & 0x3FFFFu) >> 4;
+            uint32_t g = 0, n = 0;
+            for (int t; !fail && (t = next_ticket(false)) >= 0;) {
+                const VlUnit w = vl_unit<BWD>(t, p, list);
+                if (w.steps <= 0) continue;
+                const int b = (int)(n & 1u);
+                if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
+                tc_fence_after_sync();
+                for (int it = 0; it < w.steps; ++it, ++g) {
+                    const int s = (int)(g % STAGES);
+                    if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
+                    tc_fence_after_sync();
+                    const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4), b4 = a4 + (L::A_BYTES >> 4);
+                    if (w.q) vl_mma_step(tmem + b * VL_TILE, a4, b4, BWD, true, idesc_q, it == 0);
+                    else     vl_mma_step(tmem + b * VL_TILE, a4, b4, false, false, idesc_p, it == 0);
+                    umma_commit_pair(bar_empty(s), (uint16_t)3);
+                }
+                if (fail) break;
+                umma_commit_pair(bar_done(b), (uint16_t)3);
+                ++n;
+            }
+        } else if (lane == 0) {
+            const uint32_t lead_full0 = mapa_shared(bar_full(0), 0u);
+            uint32_t g = 0;
+            for (int t; !fail && (t = next_ticket(false)) >= 0;) {
+                const VlUnit w = vl_unit<BWD>(t, p, list);
+                for (int it = 0; it < w.steps; ++it, ++g) {
+                    const int s = (int)(g % STAGES);
+                    if (!mbar_wait(bar_landed(s), (g / STAGES) & 1u, abort_flag)) { fail = 8; break; }
+                    mbar_arrive_cluster(lead_full0 + 8u * s);
+                }
+            }
+        }
+    } else if (warp == VL_EPI_WARPS + 2) {
+        // ------------------------------------------------------------------ draws the pair's tickets
+        if (lane == 0 && rank == 0) {
+            const uint32_t peer_tickets = mapa_shared(tickets, 1u), peer_drawn0 = mapa_shared(bar_drawn(0), 1u);
+            const uint32_t own_drawn0 = mapa_shared(bar_drawn(0), 0u);
+            for (uint32_t n = 0;; ++n) {
+                const int k = (int)(n % VL_TICKETS);
+                if (!vl_mbar_wait_acquire(bar_taken(k), ((n / VL_TICKETS) & 1u) ^ 1u, abort_flag)) { fail = 11; break; }
+                int t = atomicAdd(p.ticket, 1);
+                if (t >= list.total) t = -1;
+                asm volatile("st.shared.s32 [%0], %1;" ::"r"(tickets + 4u * k), "r"(t) : "memory");
+                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(peer_tickets + 4u * k), "r"(t) : "memory");
+                vl_mbar_arrive_release(own_drawn0 + 8u * k);
+                vl_mbar_arrive_release(peer_drawn0 + 8u * k);
+                if (t < 0) break;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue: a row's half tile per thread
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
+        const uint32_t staging = base + L::STAGING_OFF + (uint32_t)(warp - 2) * 4096u;
+        // The box's memory is free again once the store before has read it; what is in it goes out as 32 whole lines.
+        auto box_begin = [&]() {
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();
+        };
+        auto box_put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t t) {    // 16 bytes of this lane's row
+            vl_sts128(staging + lane * 128 + ((chunk ^ (lane & 7)) << 4), x, y, z, t);
+        };
+        auto box_end = [&](const CUtensorMap* map, int x, int y, bool add) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (add) tma_reduce_add_2d(map, staging, x, y);
+                else     tma_store_2d(map, staging, x, y);
+                bulk_commit();
+            }
+        };
+        // 32 values in 16 bits: half a box
+        auto put16 = [&](const float (&v)[32], int c) {
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
-                    const float top2 = top * VL_LOG2E;
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (MODE == VL_STATS) {
-                        if (top2 > m2) {
-                            sum *= vl_ex2(m2 - top2);
-                            m2 = top2;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) part[e & 3] += vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -m2));
-                    } else {
-                        m2 = fmaxf(m2, top2);
-                        float v[32];
+            for (int i = 0; i < 4; ++i)
+                box_put((c & 32) / 8 + i, vl_pack(v[8 * i], v[8 * i + 1], p.bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.bf16),
+                        vl_pack(v[8 * i + 4], v[8 * i + 5], p.bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.bf16));
+        };
+        // Lane 0 waits for a counter, everybody for lane 0.
+        auto wait_count = [&](const int* counter, int least) -> bool {
+            int ok = 1;
+            if (lane == 0) ok = vl_wait_count(counter, least, abort_flag) ? 1 : 0;
+            return __shfl_sync(0xffffffffu, ok, 0) != 0;
+        };
+        uint32_t n = 0;
+        for (int t; !fail && (t = next_ticket(true)) >= 0;) {
+            const VlUnit w = vl_unit<BWD>(t, p, list);
+            const int v0 = w.piece * list.tiles * VL_TILE;
+            const int row0 = (w.q && BWD ? w.slot : w.mt) * VL_TILE + (int)rank * 128 + q * 32, row = row0 + lane;   // backward's Q: word of the piece
+            const int col0 = w.nt * VL_TILE + half * 128;      // word of the piece, feature
+            if (BWD && w.q && w.steps <= 0) {
+                // no row takes part: the gradient of the head is zero
+                if (v0 + row < p.vocab)
+                    for (int c = col0; c < col0 + 128 && c < p.hidden; ++c)
+                        static_cast<unsigned short*>(p.d_weight)[(long long)(v0 + row) * p.hidden + c] = 0;
+                continue;
+            }
+            const int b = (int)(n & 1u);
+            // what the values meet, asked for before the tile is complete
+            int target = -1;
+            float lse2 = 0.f, rest = 0.f, ref = 0.f, scale = 1.f;
+            float4 coef = make_float4(0.f, 0.f, 0.f, 0.f);
+            const bool live = row < rows;
+            if (!w.q && live) {
+                target = p.target[row] - v0 - col0;     // column of this thread's share
+                if (BWD) {
+                    lse2 = p.lse2[row];
+                    rest = p.rest[row];
+                    coef = p.coef[row];
+                } else {
+                    ref = p.refs[row];
+                }
+            }
+            if (BWD && w.q) scale = *p.weight_scale;
+            // what is about to be overwritten has been read; what is about to be added to has the pieces before
+            if (!w.q && w.piece >= VL_BUFFERS &&
+                !wait_count(p.read + (w.piece - VL_BUFFERS) * p.pitch + w.slot, list.feature_tiles)) { fail = 12; break; }
+            if (!BWD && w.q && !wait_count(p.added + w.mt * list.feature_tiles + w.nt, 2 * VL_EPI_WARPS * w.piece)) { fail = 13; break; }
+            if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
+            tc_fence_after_sync();
+            if (w.q && rank == 0 && warp == 2 && lane == 0) vl_count(p.read + w.piece * p.pitch + w.slot);
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
+            float m2 = VL_NEG, sum = 0.f;
+            const int piece_row = w.piece % VL_BUFFERS * buffer_rows + row0;
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+                uint32_t r[32];
+                tmem_ld_32x32(at + c, r);
+                tmem_ld_wait();
+                if (c == 96) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
+                }
+                if (!w.q) {
+                    const int words = p.vocab - v0 - col0 - c;       // words there are in this chunk
+                    float v[32];
+                    if (!BWD) {
+                        vl_leave_out(r, words, target - c);
+                        m2 = fmaxf(m2, vl_top(r) * VL_LOG2E);
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             v[e] = live ? vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -ref)) : 0.f;
                             part[e & 3] += v[e];
                         }
-                        store_piece(v, c);
-                    }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
-                } else if (MODE == VL_GRAD) {
-                    const int words = p.vocab - plan.v0 - col0 - c;
-                    float v[32];
+                        sum += (part[0] + part[1]) + (part[2] + part[3]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -lse2)) * coef.x;
-                    const bool cut = words < 32 || (unsigned)(target - c) < 32u || !live;
-                    if (__any_sync(0xffffffffu, cut)) {
-                        const float hit = coef.z * (1.f - rest) - coef.y * rest;    // c p_t - b (1 - p_t)
+                        for (int e = 0; e < 32; ++e) v[e] = vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -lse2)) * coef.x;
+                        if (__any_sync(0xffffffffu, words < 32 || (unsigned)(target - c) < 32u || !live)) {
+                            const float hit = coef.z * (1.f - rest) - coef.y * rest;    // c p_t - b (1 - p_t)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            if (e == target - c) v[e] = hit;
-                            if (e >= words || !live) v[e] = 0.f;
+                            for (int e = 0; e < 32; ++e) {
+                                if (e == target - c) v[e] = hit;
+                                if (e >= words || !live) v[e] = 0.f;
+                            }
                         }
                     }
-                    store_piece(v, c);
-                } else if (MODE == VL_HIDDEN) {
+                    if ((c & 32) == 0) box_begin();
+                    put16(v, c);
+                    if ((c & 32) != 0) box_end(&maps.piece_out, 0, piece_row + ((col0 + c) >> 6) * rows_dev, false);
+                } else if (!BWD) {
                     if (col0 + c >= p.hidden) continue;
-                    if (__any_sync(0xffffffffu, scale != 1.f)) {       // a reference has moved: sums so far go along
-                        float* out = p.planes + ((long long)w.slice * rows_dev + row) * p.hidden + col0 + c;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (col0 + c + e < p.hidden) out[e] = fmaf(out[e], scale, __uint_as_float(r[e]));
-                        continue;
-                    }
                     box_begin();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) box_put(i, r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-                    box_end(col0 + c, w.slice * rows_dev + row0, p.index > 0);
+                    box_end(&maps.out, col0 + c, row0, w.piece > 0);
                 } else {
                     if (col0 + (c & 64) >= p.hidden) continue;
                     if ((c & 32) == 0) box_begin();
@@ -580,28 +825,26 @@ vl_gemm_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlPa
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * scale;
                     put16(v, c);
-                    if ((c & 32) != 0) box_end(col0 + (c & 64), plan.v0 + row0, false);
-                }
-            }
-            if (MODE <= VL_SOFT) {
-                p.parts[(long long)(plan.v0 / VL_TILE * 2 + 2 * w.nt + half) * p.rows_pad + row] = make_float2(m2, sum);
-                if (MODE == VL_SOFT && live && !p.again && m2 > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) {
-                    int* f = p.flags + (long long)p.index * p.flags_pitch;      // (several threads write the same)
-                    f[0] = 1;
-                    f[1 + w.mt] = 1;
+                    if ((c & 32) != 0) box_end(&maps.out, col0 + (c & 64), v0 + row0, false);
                 }
             }
             ++n;
+            if (!w.q && !BWD) {
+                p.parts[(long long)(v0 / VL_TILE * 2 + 2 * w.nt + half) * p.rows_pad + row] = make_float2(m2, sum);
+                if (live && m2 > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) {      // (several threads write the same)
+                    p.flags[0] = 1;
+                    p.flags[1 + w.mt] = 1;
+                }
+            }
+            if (lane == 0 && (!w.q || !BWD)) {      // (backward's Q writes what nobody waits for)
+                bulk_wait();
+                vl_count(w.q ? p.added + w.mt * list.feature_tiles + w.nt : p.written + w.piece * p.pitch + w.slot);
+            }
         }
-        if (MODE != VL_STATS && lane == 0) bulk_wait();
+        if (lane == 0) bulk_wait();
     }
 
-    if (fail) {
-        atomicCAS(p.status, 0, 100 + fail);
-        // copies and MMAs in flight get time to land before shared memory and TMEM go away
-        const unsigned long long t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    }
+    if (fail) vl_failed(p.status, fail);
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();
@@ -636,9 +879,8 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
     for (long long i = threadIdx.x; i < row0; i += VL_GATHER_WARPS * 32) n += takes_part(a.targets[i]) ? 1 : 0;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) before[warp] = n;
-    if (a.flags != nullptr)
-        for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_flags; i += (long long)gridDim.x * blockDim.x)
-            a.flags[i] = 0;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_counters; i += (long long)gridDim.x * blockDim.x)
+        a.counters[i] = 0;
     __syncthreads();
     if (warp == 0) {
         int start = 0;
@@ -704,26 +946,25 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
 }
 
 // Joins a row's statistics, 32 rows by 32 shares of the parts per CTA. PROBE: the first words' maxima give the row's
-// reference. Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's references,
-// of which the parts of `piece` word tiles each had one.
+// reference. Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's reference.
 template <bool PROBE>
 __global__ void __launch_bounds__(1024)
-vl_merge_kernel(const VocabLossArgs a, int n_parts, int word_tiles, int soft) {
+vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float2 join[32][33];
     const int rows = *a.count, row = blockIdx.x * 32 + threadIdx.x;
     if (blockIdx.x * 32 >= rows) return;
-    const int piece = soft ? vl_piece_tiles(vl_div_up(rows, VL_TILE), word_tiles, a.capacity, a.slots) : 1;
     float m = VL_NEG, s = 0.f;
     if (row < rows) {
+        const float ref = soft ? a.refs[row] : 0.f;
 #pragma unroll 4
         for (int i = threadIdx.y; i < n_parts; i += 32) {
             float2 x = a.parts[(long long)i * a.rows_pad + row];
-            if (soft) x.x = a.refs[(long long)(i / 2 / piece + 1) * a.rows_pad + row];
-            const float top = fmaxf(m, x.x);
-            s = s * vl_ex2(m - top) + x.y * vl_ex2(x.x - top);
-            m = top;
+            if (soft) x.x = ref;
+            x = vl_join(make_float2(m, s), x);
+            m = x.x;
+            s = x.y;
         }
     }
     join[threadIdx.x][threadIdx.y] = make_float2(m, s);
@@ -732,10 +973,7 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int word_tiles, int soft) {
     float2 x = join[threadIdx.y][threadIdx.x];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, x.x, o), os = __shfl_xor_sync(0xffffffffu, x.y, o);
-        const float top = fmaxf(x.x, om);
-        x.y = x.y * vl_ex2(x.x - top) + os * vl_ex2(om - top);
-        x.x = top;
+        x = vl_join(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
     }
     const int at = blockIdx.x * 32 + threadIdx.y;
     if (threadIdx.x != 0 || at >= rows) return;
@@ -766,27 +1004,28 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int word_tiles, int soft) {
     a.lse[a.source[at]] = logit + loss;
 }
 
-// U: the planes' sum over the row's sum of exponentials.
-__global__ void __launch_bounds__(256)
-vl_mean_kernel(const VocabLossArgs a, int word_tiles) {
+// A CTA per row tile: where a row outgrew its reference, new ones from the maxima; the first CTA lists those tiles.
+__global__ void __launch_bounds__(VL_TILE)
+vl_again_kernel(const VocabLossArgs a, int word_tiles) {
     grid_dep_wait();
     grid_dep_launch();
-    const int rows = *a.count, quads = (int)(a.hidden / 4);
-    if (rows == 0) return;
-    const int row_tiles = vl_div_up(rows, VL_TILE);
-    const int steps = vl_piece_tiles(row_tiles, word_tiles, a.capacity, a.slots) * (VL_TILE / VL_BK);
-    const int slices = vl_slices(row_tiles * vl_div_up((int)a.hidden, VL_TILE), steps, a.slots);
-    const long long plane = (long long)row_tiles * VL_TILE * a.hidden;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * quads; i += (long long)gridDim.x * 256) {
-        const float norm = a.norm[i / quads];
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int z = 0; z < slices; ++z) {
-            const float4 x = *reinterpret_cast<const float4*>(a.planes + z * plane + i * 4);
-            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-        }
-        reinterpret_cast<float4*>(a.mean)[i] = make_float4(v.x * norm, v.y * norm, v.z * norm, v.w * norm);
+    const int rows = *a.count, row_tiles = vl_div_up(rows, VL_TILE);
+    if (a.flags[0] == 0 || (int)blockIdx.x >= row_tiles) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.list[0] = 0;
+        return;
     }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        int n = 0;
+        for (int t = 0; t < row_tiles; ++t)
+            if (a.flags[1 + t] != 0) a.list[1 + n++] = t;
+        a.list[0] = n;
+    }
+    const int row = blockIdx.x * VL_TILE + threadIdx.x;
+    if (a.flags[1 + blockIdx.x] == 0 || row >= rows) return;
+    float top = VL_NEG;
+#pragma unroll 8
+    for (int i = 0; i < 2 * word_tiles; ++i) top = fmaxf(top, a.parts[(long long)i * a.rows_pad + row].x);
+    if (top > a.refs[row] + (a.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) a.refs[row] = ceilf(top) - 6.f;
 }
 
 // ------------------------------------------------------------------------------------- backward
@@ -811,6 +1050,7 @@ vl_coef_kernel(const VocabLossArgs a) {
     __shared__ float part[32];
     float top = 0.f;
     const int rows = *a.count;
+    for (long long i = threadIdx.x; i < a.n_counters; i += 1024) a.counters[i] = 0;
     for (int at = threadIdx.x; at < rows; at += 1024) {
         const long long row = a.source[at];
         top = fmaxf(top, fmaxf(fabsf(vl_upstream(a.d_losses, a.d_losses_stride, row)), fabsf(vl_upstream(a.d_lse, a.d_lse_stride, row))));
@@ -843,8 +1083,8 @@ vl_hidden_kernel(const VocabLossArgs a) {
         uint4 out = make_uint4(0u, 0u, 0u, 0u);
         if (at >= 0) {
             const float b = vl_upstream(a.d_losses, a.d_losses_stride, row), z = vl_upstream(a.d_lse, a.d_lse_stride, row);
-            const float rest = a.rest[at], mean = b + z, hit = z * (1.f - rest) - b * rest;
-            const float4* u = reinterpret_cast<const float4*>(a.mean + (long long)at * a.hidden) + 2 * c;
+            const float rest = a.rest[at], mean = (b + z) * a.norm[at], hit = z * (1.f - rest) - b * rest;
+            const float4* u = reinterpret_cast<const float4*>(a.sums + (long long)at * a.hidden) + 2 * c;
             const float4 x = u[0], y = u[1];
             const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.weight) + (long long)a.target[at] * a.ld_w) + c);
             const float2 w0 = vl_two(w.x, a.bf16), w1 = vl_two(w.y, a.bf16), w2 = vl_two(w.z, a.bf16), w3 = vl_two(w.w, a.bf16);
@@ -864,31 +1104,23 @@ static long long vl_rows_pad(long long rows) { return (rows + VL_TILE - 1) / VL_
 
 static int vl_word_tiles(long long vocab) { return (int)((vocab + VL_TILE - 1) / VL_TILE); }
 
-// Tiles that the 16-bit piece has room for, the most pieces that any number of rows up to `rows` makes of the
-// vocabulary, and the planes of U they need, in units of rows_pad rows.
+// Tiles that a piece has room for, and the most pieces that any number of rows up to `rows` makes of the vocabulary.
 struct VlRoom {
-    int capacity, pieces, planes;
+    int capacity, pieces;
 };
-static VlRoom vl_room(long long rows, long long vocab, long long hidden, int slots) {
-    VlRoom r = {VL_PIECE_UNITS, 1, 1};
+static VlRoom vl_room(long long rows, long long vocab) {
     const long long row_tiles = vl_rows_pad(rows) / VL_TILE;
-    const int word_tiles = vl_word_tiles(vocab), feature_tiles = vl_div_up((int)hidden, VL_TILE);
-    if (r.capacity < 4 * row_tiles) r.capacity = (int)(4 * row_tiles);
-    if (r.capacity > row_tiles * word_tiles) r.capacity = (int)(row_tiles * word_tiles);
-    long long most = row_tiles;
-    for (long long t = 1; t <= row_tiles; ++t) {
-        const int tiles = vl_piece_tiles((int)t, word_tiles, r.capacity, slots), pieces = vl_div_up(word_tiles, tiles);
-        if (pieces > r.pieces) r.pieces = pieces;
-        const long long planes = t * vl_slices((int)t * feature_tiles, tiles * (VL_TILE / VL_BK), slots);
-        if (planes > most) most = planes;
-    }
-    r.planes = (int)((most + row_tiles - 1) / row_tiles);
+    const int word_tiles = vl_word_tiles(vocab);
+    VlRoom r = {VL_PIECE_UNITS, 1};
+    if (r.capacity < VL_PIECE_LEAST * row_tiles) r.capacity = (int)(VL_PIECE_LEAST * row_tiles);
+    // (more row tiles, fewer tiles of words in a piece)
+    r.pieces = vl_div_up(word_tiles, vl_piece_tiles((int)row_tiles, word_tiles, r.capacity));
     return r;
 }
 
 // What the forward keeps for the backward.
 struct VlKept {
-    size_t count, place, source, target, lse, rest, gathered, mean, bytes;
+    size_t count, place, source, target, lse, rest, norm, sums, gathered, bytes;
 };
 static VlKept vl_kept(long long rows, long long hidden, int grads) {
     VlKept k = {};
@@ -901,15 +1133,36 @@ static VlKept vl_kept(long long rows, long long hidden, int grads) {
     k.target = take(pad * 4);
     k.lse = take(pad * 4);
     k.rest = take(pad * 4);
-    if (grads & 1) k.mean = take((size_t)rows * (size_t)hidden * 4);
+    k.norm = take(pad * 4);
+    if (grads & 1) k.sums = take(pad * (size_t)hidden * 4);
     k.gathered = at;                       // last: without a gradient of the weight it is scratch of the forward
     if (grads & 2) take(pad * (size_t)hidden * 2);
     k.bytes = at;
     return k;
 }
 
+// Counters of a sweep, and of the forward's two.
+struct VlCounters {
+    long long ticket, written, read, added, each, flags, list, total;
+    int pitch;
+};
+static VlCounters vl_counters(const VocabLossArgs& a, const VlRoom& room, bool backward) {
+    VlCounters c = {};
+    const long long row_tiles = vl_rows_pad(a.rows) / VL_TILE, feature_tiles = vl_div_up((int)a.hidden, VL_TILE);
+    c.pitch = backward ? VL_PIECE_TILES : (int)row_tiles;
+    c.ticket = 0;
+    c.written = 32;
+    c.read = c.written + (long long)room.pieces * c.pitch;
+    c.added = c.read + (long long)room.pieces * c.pitch;
+    c.each = c.added + (backward ? 0 : row_tiles * feature_tiles);
+    c.flags = (backward ? 1 : 2) * c.each;
+    c.list = c.flags + (backward ? 0 : 1 + row_tiles);
+    c.total = c.list + (backward ? 0 : 1 + row_tiles);
+    return c;
+}
+
 struct VlScratch {
-    size_t parts, target_logit, norm, refs, flags, gathered, coef, weight_scale, piece, planes, bytes;
+    size_t parts, target_logit, refs, counters, gathered, coef, weight_scale, piece, bytes;
     VlRoom room;
 };
 
@@ -918,24 +1171,24 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
     const size_t pad = (size_t)vl_rows_pad(a.rows);
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t r = at; at += vl_align(n); return r; };
-    if ((backward && a.d_weight != nullptr) || (!backward && (a.grads & 1)))
-        s.room = vl_room(a.rows, a.vocab, a.hidden, a.sm_count / 2);
+    s.room = vl_room(a.rows, a.vocab);
+    const size_t piece = (size_t)VL_BUFFERS * (size_t)s.room.capacity * VL_TILE * VL_TILE * 2;
+    const size_t counters = (size_t)vl_counters(a, s.room, backward).total * 4;
     if (!backward) {
         const size_t n_parts = (size_t)vl_word_tiles(a.vocab) * 2, few_parts = (size_t)a.sm_count * 4;
         s.parts = take((n_parts > few_parts ? n_parts : few_parts) * 8 * pad);
         s.target_logit = take(pad * 4);
         if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
         if (a.grads & 1) {
-            s.norm = take(pad * 4);
-            s.refs = take((size_t)(s.room.pieces + 1) * pad * 4);
-            s.flags = take((size_t)s.room.pieces * (1 + pad / VL_TILE) * 4);
-            s.piece = take((size_t)s.room.capacity * VL_TILE * VL_TILE * 2);
-            s.planes = take((size_t)s.room.planes * pad * (size_t)a.hidden * 4);
+            s.refs = take(pad * 4);
+            s.counters = take(counters);
+            s.piece = take(piece);
         }
     } else if (a.d_weight != nullptr) {
         s.coef = take(pad * 16);
         s.weight_scale = take(4);
-        s.piece = take((size_t)s.room.capacity * VL_TILE * VL_TILE * 2);
+        s.counters = take(counters);
+        s.piece = take(piece);
     }
     s.bytes = at;
     return s;
@@ -945,16 +1198,15 @@ size_t vocab_loss_kept_bytes(long long rows, long long hidden, int grads) { retu
 
 size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward) { return vl_scratch(a, backward).bytes; }
 
-template <int MODE>
-static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long units, int sm_count, cudaStream_t stream,
-                             int* ctas = nullptr) {
-    auto kernel = vl_gemm_kernel<MODE>;
-    constexpr int VL_SMEM = VlSmemOf<MODE>::TOTAL;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, VL_SMEM);
+// CTA pairs of a kernel that takes tensor maps and parameters: one per pair of SMs as far as there are units.
+template <typename Maps, typename Params>
+static cudaError_t vl_launch(void (*kernel)(Maps, Params), int threads, int smem, const Maps& maps, const Params& p, long long units,
+                             int sm_count, cudaStream_t stream, int* ctas = nullptr) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(VL_THREADS);
-    cfg.dynamicSmemBytes = VL_SMEM;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -965,13 +1217,7 @@ static cudaError_t vl_launch(const VlMaps& maps, const VlParams& p, long long un
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    // pairs that can be resident at once: a pair sits in one GPC, so the runtime knows (asked once)
-    static const int most = [&] {
-        cfg.gridDim = dim3((unsigned)(sm_count / 2 * 2));
-        int n = 0;
-        return cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0 ? n : 0x7FFFFFFF;
-    }();
-    long long pairs = sm_count / 2 < most ? sm_count / 2 : most;
+    long long pairs = sm_count / 2;
     if (units < pairs) pairs = units;
     if (pairs < 1) pairs = 1;
     cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -984,9 +1230,9 @@ static bool vl_map(CUtensorMap* map, int bf16, const void* base, long long inner
                        (uint64_t)outer, (uint64_t)pitch * 2, VL_BK, (uint32_t)box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// The 16-bit piece: blocks of [rows][64 words], read in boxes of 128 rows (rows as M) or 64 (as steps), written in 32.
+// The 16-bit pieces: blocks of [rows][64 words], read in boxes of 128 rows (rows as M) or 64 (as steps), written in 32.
 static bool vl_piece_map(CUtensorMap* map, const VocabLossArgs& a, int box_outer) {
-    return vl_map(map, a.bf16, a.piece, VL_BK, (long long)a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, box_outer);
+    return vl_map(map, a.bf16, a.piece, VL_BK, (long long)VL_BUFFERS * a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, box_outer);
 }
 
 static void vl_use_kept(VocabLossArgs& a) {
@@ -998,23 +1244,26 @@ static void vl_use_kept(VocabLossArgs& a) {
     a.target = reinterpret_cast<int*>(base + k.target);
     a.lse_rows = reinterpret_cast<float*>(base + k.lse);
     a.rest = reinterpret_cast<float*>(base + k.rest);
-    a.mean = reinterpret_cast<float*>(base + k.mean);
+    a.norm = reinterpret_cast<float*>(base + k.norm);
+    a.sums = reinterpret_cast<float*>(base + k.sums);
     a.gathered = base + k.gathered;
     a.rows_pad = vl_rows_pad(a.rows);
-    a.slots = a.sm_count / 2;
 }
 
-static VlParams vl_params(const VocabLossArgs& a) {
-    VlParams p = {};
+static VlSweepParams vl_sweep_params(const VocabLossArgs& a, const VlCounters& c, int sweep) {
+    VlSweepParams p = {};
     p.count = a.count; p.status = a.status; p.bf16 = a.bf16;
     p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab);
-    p.capacity = a.capacity; p.slots = a.slots;
-    p.target = a.target; p.parts = a.parts; p.rows_pad = a.rows_pad;
-    p.refs = a.refs; p.flags = a.flags; p.flags_pitch = 1 + (int)(a.rows_pad / VL_TILE);
-    p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef;
-    p.piece = a.piece; p.planes = a.planes; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
+    p.capacity = a.capacity; p.rows_pad = a.rows_pad; p.target = a.target; p.piece = a.piece;
+    int* counters = a.counters + sweep * c.each;
+    p.ticket = counters + c.ticket; p.written = counters + c.written; p.read = counters + c.read; p.added = counters + c.added;
+    p.pitch = c.pitch;
+    p.parts = a.parts; p.refs = a.refs; p.flags = a.flags; p.list = a.list; p.again = sweep;
+    p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
     return p;
 }
+
+constexpr int VL_SWEEP_SMEM = VlSmem<128, 6, true>::TOTAL;
 
 cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream, const char** why) {
     *why = "";
@@ -1022,70 +1271,72 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     if (a.rows <= 0) return cudaSuccess;
     vl_use_kept(a);
     const VlScratch s = vl_scratch(a, false);
+    const VlCounters counters = vl_counters(a, s.room, false);
     char* ws = static_cast<char*>(a.workspace);
     a.parts = reinterpret_cast<float2*>(ws + s.parts);
     a.target_logit = reinterpret_cast<float*>(ws + s.target_logit);
     if (!(a.grads & 2)) a.gathered = ws + s.gathered;
     const bool soft = (a.grads & 1) != 0;
     if (soft) {
-        a.norm = reinterpret_cast<float*>(ws + s.norm);
         a.refs = reinterpret_cast<float*>(ws + s.refs);
-        a.flags = reinterpret_cast<int*>(ws + s.flags);
-        a.n_flags = s.room.pieces * (1 + a.rows_pad / VL_TILE);
+        a.counters = reinterpret_cast<int*>(ws + s.counters);
+        a.n_counters = counters.total;
+        a.flags = a.counters + counters.flags;
+        a.list = a.counters + counters.list;
         a.piece = ws + s.piece;
-        a.planes = reinterpret_cast<float*>(ws + s.planes);
         a.capacity = s.room.capacity;
     }
     const int per = a.rows <= 4096 ? 8 : 32;
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
-    VlMaps logits = {}, hidden = {};
     // Up to 64 rows without a gradient of x: the words take the tensor cores' long side. (64 rows of 3584 features against
-    // 151,936 words: 216 us with the rows there, which costs four times the products; the weight alone takes 168.)
+    // 151,936 words: 216 us with the rows there, which costs four times the products, 196 this way; the weight alone
+    // takes 168.)
     const bool few = !soft && a.rows <= 64;
     const int few_rows = a.rows <= 32 ? 32 : 64;
+    VlMaps logits = {};
+    VlSweepMaps maps = {};
     bool ok = few ? vl_map(&logits.a, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) &&
                         vl_map(&logits.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, few_rows / 2)
                   : vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
                         vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
-    if (ok && soft)
-        ok = vl_piece_map(&logits.c, a, 32) && vl_piece_map(&hidden.a, a, 128) &&
-             vl_map(&hidden.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) &&
-             make_map_2d(&hidden.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.planes, (uint64_t)a.hidden,
-                         (uint64_t)s.room.planes * (uint64_t)a.rows_pad, (uint64_t)a.hidden * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (ok && soft) {
+        maps.rows = logits.a;
+        maps.words = logits.b;
+        ok = vl_piece_map(&maps.piece_in, a, 128) && vl_map(&maps.other, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) &&
+             vl_piece_map(&maps.piece_out, a, 32) &&
+             make_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.sums, (uint64_t)a.hidden, (uint64_t)a.rows_pad,
+                         (uint64_t)a.hidden * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
     if (!ok) { *why = "cuTensorMapEncodeTiled"; return cudaErrorInvalidValue; }
-    VlParams base = vl_params(a);
-    base.n_rows = few_rows;
-    int n_parts = 2 * base.word_tiles;
+    VlParams p = {};
+    p.count = a.count; p.status = a.status; p.bf16 = a.bf16;
+    p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab); p.n_rows = few_rows;
+    p.target = a.target; p.parts = a.parts; p.rows_pad = a.rows_pad;
     const long long row_tiles = a.rows_pad / VL_TILE;
     const dim3 merge_grid((unsigned)((a.rows + 31) / 32)), merge_block(32, 32);
-    if (!soft) {
+    int n_parts = 2 * p.word_tiles;
+    if (few) {
         int ctas = 0;
-        e = few ? vl_launch<VL_FEW>(logits, base, base.word_tiles, a.sm_count, stream, &ctas)
-                : vl_launch<VL_STATS>(logits, base, row_tiles * base.word_tiles, a.sm_count, stream);
-        if (few) n_parts = 4 * ctas;
-        if (e != cudaSuccess) { *why = "statistics"; return e; }
+        e = vl_launch(vl_stats_kernel<VL_FEW>, VL_THREADS, VlSmemOf<VL_FEW>::TOTAL, logits, p, p.word_tiles, a.sm_count, stream, &ctas);
+        n_parts = 4 * ctas;
+    } else if (!soft) {
+        e = vl_launch(vl_stats_kernel<VL_STATS>, VL_THREADS, VlSmemOf<VL_STATS>::TOTAL, logits, p, row_tiles * p.word_tiles, a.sm_count, stream);
     } else {
-        VlParams probe = base;
+        VlParams probe = p;
         if (probe.word_tiles > VL_PROBE_TILES) probe.word_tiles = VL_PROBE_TILES;
-        e = vl_launch<VL_STATS>(logits, probe, row_tiles * probe.word_tiles, a.sm_count, stream);
-        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, probe.word_tiles, 0);
+        e = vl_launch(vl_stats_kernel<VL_STATS>, VL_THREADS, VlSmemOf<VL_STATS>::TOTAL, logits, probe, row_tiles * probe.word_tiles, a.sm_count, stream);
+        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, 0);
         if (e != cudaSuccess) { *why = "references"; return e; }
-        const long long units = row_tiles * base.word_tiles < a.capacity ? row_tiles * base.word_tiles : a.capacity;
-        for (int i = 0; i < s.room.pieces; ++i) {
-            VlParams p = base;
-            p.index = i;
-            e = vl_launch<VL_SOFT>(logits, p, units, a.sm_count, stream);
-            p.again = 1;
-            if (e == cudaSuccess) e = vl_launch<VL_SOFT>(logits, p, units, a.sm_count, stream);
-            if (e != cudaSuccess) { *why = "softmax"; return e; }
-            e = vl_launch<VL_HIDDEN>(hidden, p, row_tiles * vl_div_up(p.hidden, VL_TILE) * VL_MAX_SLICES, a.sm_count, stream);
-            if (e != cudaSuccess) { *why = "gradient of the hidden states"; return e; }
+        const long long units = row_tiles * (p.word_tiles + vl_div_up(p.hidden, VL_TILE));
+        for (int sweep = 0; sweep < 2 && e == cudaSuccess; ++sweep) {
+            e = vl_launch(vl_sweep_kernel<false>, VL_SWEEP_THREADS, VL_SWEEP_SMEM, maps, vl_sweep_params(a, counters, sweep), units, a.sm_count, stream);
+            if (sweep == 0 && e == cudaSuccess)
+                e = launch_pdl(vl_again_kernel, dim3((unsigned)row_tiles), dim3(VL_TILE), 0, stream, a, p.word_tiles);
         }
     }
-    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, base.word_tiles, soft ? 1 : 0);
-    if (e == cudaSuccess && soft)
-        e = launch_pdl(vl_mean_kernel, dim3((unsigned)(a.sm_count * 8)), dim3(256), 0, stream, a, base.word_tiles);
+    if (e != cudaSuccess) { *why = "statistics"; return e; }
+    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, soft ? 1 : 0);
     if (e != cudaSuccess) *why = "merge";
     return e;
 }
@@ -1096,6 +1347,7 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     if (a.rows <= 0) return cudaSuccess;
     vl_use_kept(a);
     const VlScratch s = vl_scratch(a, true);
+    const VlCounters counters = vl_counters(a, s.room, true);
     char* ws = static_cast<char*>(a.workspace);
     cudaError_t e = cudaSuccess;
     if (a.d_x != nullptr) {
@@ -1105,27 +1357,23 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     if (a.d_weight == nullptr) return e;
     a.coef = reinterpret_cast<float4*>(ws + s.coef);
     a.weight_scale = reinterpret_cast<float*>(ws + s.weight_scale);
+    a.counters = reinterpret_cast<int*>(ws + s.counters);
+    a.n_counters = counters.total;
     a.piece = ws + s.piece;
     a.capacity = s.room.capacity;
     e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) { *why = "row factors"; return e; }
-    VlMaps logits = {}, weight = {};
-    if (!vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
-        !vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) ||
-        !vl_piece_map(&logits.c, a, 32) || !vl_piece_map(&weight.a, a, 64) ||
-        !vl_map(&weight.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64) ||
-        !vl_map(&weight.c, a.bf16, a.d_weight, a.hidden, a.vocab, a.hidden, 32)) {
+    VlSweepMaps maps = {};
+    if (!vl_map(&maps.rows, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) ||
+        !vl_map(&maps.words, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) ||
+        !vl_piece_map(&maps.piece_in, a, 64) || !vl_map(&maps.other, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 64) ||
+        !vl_piece_map(&maps.piece_out, a, 32) || !vl_map(&maps.out, a.bf16, a.d_weight, a.hidden, a.vocab, a.hidden, 32)) {
         *why = "cuTensorMapEncodeTiled";
         return cudaErrorInvalidValue;
     }
-    VlParams p = vl_params(a);
-    const long long units = a.rows_pad / VL_TILE * p.word_tiles < a.capacity ? a.rows_pad / VL_TILE * p.word_tiles : a.capacity;
-    for (p.index = 0; p.index < s.room.pieces; ++p.index) {
-        e = vl_launch<VL_GRAD>(logits, p, units, a.sm_count, stream);
-        if (e != cudaSuccess) { *why = "gradient of the logits"; return e; }
-        e = vl_launch<VL_WEIGHT>(weight, p, (long long)p.word_tiles * vl_div_up(p.hidden, VL_TILE), a.sm_count, stream);
-        if (e != cudaSuccess) { *why = "gradient of the head"; return e; }
-    }
+    const long long units = (long long)vl_word_tiles(a.vocab) * (a.rows_pad / VL_TILE + vl_div_up((int)a.hidden, VL_TILE));
+    e = vl_launch(vl_sweep_kernel<true>, VL_SWEEP_THREADS, VL_SWEEP_SMEM, maps, vl_sweep_params(a, counters, 0), units, a.sm_count, stream);
+    if (e != cudaSuccess) *why = "gradient of the head";
     return e;
 }
 
