@@ -56,9 +56,21 @@ def act8_quantize(x):
     return Act8(*kept, x.shape, x.dtype)
 
 
+def _refuse_parts(kept):
+    if not (kept.codes.is_cuda and kept.steps.is_cuda):
+        raise ValueError("hackaton_b200: activations in 8 bits need CUDA tensors (there is no CPU path)")
+    raise ValueError(f"hackaton_b200: codes {tuple(kept.codes.shape)} {kept.codes.dtype} and steps {tuple(kept.steps.shape)} "
+                     f"{kept.steps.dtype} are not a tensor of shape {tuple(kept.shape)} as act8_quantize makes it")
+
+
 def act8_dequantize(kept):
     """The values that `kept` holds, in the shape and type it was made from."""
-    return _lib.host().act8_dequantize(kept.codes, kept.steps, kept.shape, _LIKE[kept.dtype])
+    if kept.dtype not in _TYPES:
+        raise TypeError(f"hackaton_b200: activations are kept from fp16, bf16 or fp32, got {kept.dtype}")
+    values = _lib.host().act8_dequantize(kept.codes, kept.steps, kept.shape, _LIKE[kept.dtype])
+    if values is None:
+        _refuse_parts(kept)
+    return values
 
 
 def lora_grad_act8(kept, s):
@@ -71,5 +83,7 @@ def lora_grad_act8(kept, s):
             raise TypeError(f"hackaton_b200: the LoRA gradient computes from fp16, got {kept.dtype} and {s.dtype}")
         if s.device != kept.codes.device:
             raise ValueError(f"hackaton_b200: operands on {kept.codes.device} and {s.device}")
-        raise ValueError(f"hackaton_b200: {tuple(s.shape)} for an input of shape {tuple(kept.shape)}")
+        if s.dim() == 0 or s.shape[-1] != 16 or s.numel() != kept.codes.shape[0] * 16:
+            raise ValueError(f"hackaton_b200: {tuple(s.shape)} for an input of shape {tuple(kept.shape)}")
+        _refuse_parts(kept)
     return grad

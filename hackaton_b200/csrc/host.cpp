@@ -348,7 +348,21 @@ std::optional<std::tuple<Tensor, Tensor>> act8_quantize(const Tensor& x) {
     return std::make_tuple(codes, steps);
 }
 
-Tensor act8_dequantize(const Tensor& codes, const Tensor& steps, const std::vector<int64_t>& shape, const Tensor& like) {
+// Whether codes and steps lie as the kernels read them, for rows of `cols` values.
+bool act8_fits(const Tensor& codes, const Tensor& steps, int64_t cols) {
+    const int64_t blocks = (cols + 31) / 32;
+    return codes.is_cuda() && steps.device() == codes.device() && codes.scalar_type() == at::kChar &&
+           steps.scalar_type() == at::kByte && codes.dim() == 2 && steps.dim() == 2 && codes.is_contiguous() &&
+           steps.is_contiguous() && codes.size(1) == 32 * blocks && steps.size(1) == blocks && steps.size(0) == codes.size(0) &&
+           (reinterpret_cast<uintptr_t>(codes.const_data_ptr()) & 15) == 0;
+}
+
+// None for parts that do not make a tensor of that shape.
+Opt act8_dequantize(const Tensor& codes, const Tensor& steps, const std::vector<int64_t>& shape, const Tensor& like) {
+    if (shape.empty() || !act8_fits(codes, steps, shape.back())) return {};
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+    if (shape.back() > 0 && rows != codes.size(0)) return {};
     const c10::cuda::CUDAGuard guard(codes.device());
     Tensor out = at::empty(shape, codes.options().dtype(like.scalar_type()));
     check(nf4b200_act8_dequantize(codes.const_data_ptr(), steps.const_data_ptr(), out.data_ptr(),
@@ -377,6 +391,11 @@ std::tuple<Tensor, Tensor> act8_swiglu_bwd(const Tensor& d2, const Tensor& gc, c
     return {dg, du};
 }
 
+// Gradients of gradients are refused: the kernels' results would enter them as constants.
+void differentiate_once(const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "hackaton_b200: ", what, " has no second derivative (create_graph)");
+}
+
 struct SiluMulAct8 : torch::autograd::Function<SiluMulAct8> {
     static Tensor forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up) {
         auto [hidden, gc, gs, uc, us] = act8_swiglu_fwd(flat_rows(gate), flat_rows(up));
@@ -384,6 +403,7 @@ struct SiluMulAct8 : torch::autograd::Function<SiluMulAct8> {
         return hidden.view(gate.sizes());
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        differentiate_once("silu_mul with keep8");
         const auto kept = ctx->get_saved_variables();
         auto [dg, du] = act8_swiglu_bwd(flat_rows(grads[0]), kept[0], kept[1], kept[2], kept[3]);
         return {dg.view(grads[0].sizes()), du.view(grads[0].sizes())};
@@ -399,6 +419,7 @@ Opt silu_mul_act8(const Tensor& gate, const Tensor& up) {
 
 // None for an s that does not fit the kept input.
 Opt act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s, int64_t cols) {
+    if (!act8_fits(codes, steps, cols)) return {};
     const int64_t rows = codes.size(0);
     if (s.scalar_type() != at::kHalf || s.device() != codes.device() || s.dim() == 0 || s.size(-1) != RANK || s.numel() != rows * RANK)
         return {};
@@ -458,6 +479,7 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
         return {stream, normed};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        differentiate_once("sandwich_norm");
         const auto kept = ctx->get_saved_variables();
         const Tensor &s = kept[0], &d = kept[1], &post = kept[2], &pre = kept[3], &gate = kept[4], &rstd = kept[5];
         variable_list g(8);
@@ -583,6 +605,7 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
         return {losses.view(targets.sizes()), lse.view(targets.sizes())};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        differentiate_once("vocab_cross_entropy");
         variable_list g(4);
         if (!grads[0].defined() && !grads[1].defined()) return g;
         const auto kept = ctx->get_saved_variables();
