@@ -58,6 +58,12 @@ constexpr int VL_LAG = 2, VL_BUFFERS = VL_LAG + 2;
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
+// The tensor cores cut off what an addition to an accumulator leaves behind its 24 bits, always in one direction, so
+// that a logit's error grows with the length of its chain of additions. A chain of logits is at most VL_CHAIN steps of 64;
+// longer ones are cut, and the parts added in the epilogue's registers with rounding. (3584 features, losses against 64 bits: one
+// chain 1.2e-6 in norm, FIGURE in two; in fp32 throughout 6.8e-7.)
+constexpr int VL_CHAIN = 32;
+constexpr int VL_FEW_CHAINS = 4;           // of at most 64 columns each: there is room for all of a tile's
 constexpr int VL_EPI_WARPS = 8;
 constexpr int VL_SMEM_MAX = 232448, VL_BAR_ROOM = 512;
 // Shared memory of a CTA: the ring (128 rows of A and ROWS of B per step), a box of 32 rows x 128 bytes per epilogue warp
@@ -152,6 +158,21 @@ __device__ __forceinline__ float vl_ex2(float x) {
 
 __device__ __forceinline__ void vl_sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// Steps of a chain where there are so many.
+__host__ __device__ inline int vl_chain(int steps) { return vl_div_up(steps, vl_div_up(steps, VL_CHAIN)); }
+
+// acc += a thread's 128 columns of a chain that is not the last.
+__device__ __forceinline__ void vl_add_chain(float (&acc)[128], uint32_t at) {
+#pragma unroll
+    for (int c = 0; c < 128; c += 16) {
+        uint32_t r[16];
+        tmem_ld_32x16(at + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[c + e] += __uint_as_float(r[e]);
+    }
 }
 
 // The largest of 32 accumulator values (a NaN left out).
@@ -289,6 +310,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK);
+    const int chain = MODE == VL_FEW ? vl_div_up(steps, VL_FEW_CHAINS) : vl_chain(steps);
     const int units = rows == 0 ? 0 : MODE == VL_FEW ? p.word_tiles : row_tiles * p.word_tiles;
     int fail = 0;
 
@@ -314,20 +336,26 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             const uint32_t idesc = vl_idesc(MODE == VL_FEW ? p.n_rows : VL_TILE, false, false, p.bf16);
             const uint32_t base4 = (base & 0x3FFFFu) >> 4;
             uint32_t g = 0, n = 0;
-            for (int u = pair; u < units && !fail; u += pairs, ++n) {
-                const int b = (int)(n & 1u);
-                if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
-                tc_fence_after_sync();
-                for (int it = 0; it < steps; ++it, ++g) {
-                    const int s = (int)(g % STAGES);
-                    if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
-                    tc_fence_after_sync();
-                    const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4);
-                    vl_mma_step(tmem + b * VL_TILE, a4, a4 + (L::A_BYTES >> 4), false, false, idesc, it == 0);
-                    umma_commit_pair(bar_empty(s), (uint16_t)3);
+            for (int u = pair; u < units && !fail; u += pairs) {
+                uint32_t d = 0;
+                for (int at = 0; at < steps && !fail; at += chain) {
+                    if (MODE != VL_FEW || at == 0) {      // a buffer to a chain, or (few rows) to all of a tile's
+                        if (!mbar_wait_cluster(bar_drained(n & 1u), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
+                        tc_fence_after_sync();
+                        d = tmem + (n & 1u) * VL_TILE;
+                    }
+                    const int end = min(at + chain, steps);
+                    for (int it = at; it < end; ++it, ++g) {
+                        const int s = (int)(g % STAGES);
+                        if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
+                        tc_fence_after_sync();
+                        const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4);
+                        vl_mma_step(d, a4, a4 + (L::A_BYTES >> 4), false, false, idesc, it == at);
+                        umma_commit_pair(bar_empty(s), (uint16_t)3);
+                    }
+                    d += 64;
+                    if (!fail && (MODE != VL_FEW || end == steps)) umma_commit_pair(bar_done(n++ & 1u), (uint16_t)3);
                 }
-                if (fail) break;
-                umma_commit_pair(bar_done(b), (uint16_t)3);
             }
         } else if (lane == 0) {
             const uint32_t lead_full0 = mapa_shared(bar_full(0), 0u);
@@ -356,17 +384,21 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             if (!mbar_wait(bar_done(b), (it >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
             const int word0 = u * VL_TILE + (int)rank * 128 + q * 32;
-            uint32_t r[32];
-            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + row0;
-            if (n == 32) {
-                tmem_ld_32x32(at, r);
-            } else {
-                uint32_t h[16];
-                tmem_ld_32x16(at, h);
+            float r[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = j < 16 ? h[j] : 0u;
+            for (int j = 0; j < 32; ++j) r[j] = 0.f;
+            for (int c = 0; c * chain < steps; ++c) {
+                const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + c * 64 + row0;
+#pragma unroll
+                for (int j = 0; j < 32; j += 16) {
+                    if (j >= n) break;
+                    uint32_t h[16];
+                    tmem_ld_32x16(at + j, h);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) r[j + e] += __uint_as_float(h[e]);
+                }
             }
-            tmem_ld_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
@@ -375,7 +407,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
                 if (j >= n) break;
-                float x2 = there ? __uint_as_float(r[j]) * VL_LOG2E : VL_NEG;
+                float x2 = there ? r[j] * VL_LOG2E : VL_NEG;
                 if (hits >> j & 1u) x2 = __shfl_sync(0xffffffffu, target, j) == word0 + lane ? VL_NEG : x2;
                 const float top = fmaxf(m[j], x2);
                 s[j] = fmaf(s[j], vl_ex2(m[j] - top), there && x2 != VL_NEG ? vl_ex2(x2 - top) : 0.f);
@@ -400,6 +432,18 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
         const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
         uint32_t n = 0;
         for (int u = pair; u < units && !fail; u += pairs, ++n) {
+            float acc[128];
+#pragma unroll
+            for (int e = 0; e < 128; ++e) acc[e] = 0.f;
+            for (int it = chain; it < steps; it += chain, ++n) {
+                if (!mbar_wait(bar_done(n & 1u), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
+                tc_fence_after_sync();
+                vl_add_chain(acc, tmem + ((uint32_t)(q * 32) << 16) + (n & 1u) * VL_TILE + half * 128);
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * (n & 1u));
+            }
+            if (fail) break;
             const int row = u % row_tiles * VL_TILE + (int)rank * 128 + q * 32 + lane, nt = u / row_tiles;
             const int col0 = nt * VL_TILE + half * 128, b = (int)(n & 1u);
             const int target = row < rows ? p.target[row] - col0 : -1;      // column of this thread's share
@@ -407,7 +451,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             tc_fence_after_sync();
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
             float m2 = VL_NEG, sum = 0.f;
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < 128; c += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(at + c, r);
@@ -417,6 +461,8 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
                 }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + acc[c + e]);
                 vl_leave_out(r, p.vocab - col0 - c, target - c);
                 const float top2 = vl_top(r) * VL_LOG2E;
                 if (top2 > m2) {
@@ -449,7 +495,7 @@ struct VlUnit {
     int mt;              // row tile (P, forward's Q)
     int slot;            // where its counters are: row tile among those of the sweep (forward), word tile of the piece
     int nt;              // P: word tile of the piece; Q: feature tile
-    int steps;
+    int steps, chain;    // of 64; accumulated in one go
 };
 
 struct VlList {          // the list of units
@@ -507,6 +553,7 @@ __device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const V
     r.mt = r.q && BWD ? 0 : p.again ? p.list[1 + first] : first;
     r.slot = BWD ? (r.q ? first : r.nt) : first;
     r.steps = !r.q ? vl_div_up(p.hidden, VL_BK) : BWD ? vl_div_up(w.rows, VL_BK) : r.tiles * (VL_TILE / VL_BK);
+    r.chain = r.q ? r.steps : vl_chain(r.steps);
     return r;
 }
 
@@ -666,22 +713,21 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             uint32_t g = 0, n = 0;
             for (int t; !fail && (t = next_ticket(false)) >= 0;) {
                 const VlUnit w = vl_unit<BWD>(t, p, list);
-                if (w.steps <= 0) continue;
-                const int b = (int)(n & 1u);
-                if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
-                tc_fence_after_sync();
-                for (int it = 0; it < w.steps; ++it, ++g) {
-                    const int s = (int)(g % STAGES);
-                    if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
+                for (int at = 0; at < w.steps && !fail; at += w.chain, ++n) {
+                    const int b = (int)(n & 1u), end = min(at + w.chain, w.steps);
+                    if (!mbar_wait_cluster(bar_drained(b), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
                     tc_fence_after_sync();
-                    const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4), b4 = a4 + (L::A_BYTES >> 4);
-                    if (w.q) vl_mma_step(tmem + b * VL_TILE, a4, b4, BWD, true, idesc_q, it == 0);
-                    else     vl_mma_step(tmem + b * VL_TILE, a4, b4, false, false, idesc_p, it == 0);
-                    umma_commit_pair(bar_empty(s), (uint16_t)3);
+                    for (int it = at; it < end; ++it, ++g) {
+                        const int s = (int)(g % STAGES);
+                        if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
+                        tc_fence_after_sync();
+                        const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4), b4 = a4 + (L::A_BYTES >> 4);
+                        if (w.q) vl_mma_step(tmem + b * VL_TILE, a4, b4, BWD, true, idesc_q, it == at);
+                        else     vl_mma_step(tmem + b * VL_TILE, a4, b4, false, false, idesc_p, it == at);
+                        umma_commit_pair(bar_empty(s), (uint16_t)3);
+                    }
+                    if (!fail) umma_commit_pair(bar_done(b), (uint16_t)3);
                 }
-                if (fail) break;
-                umma_commit_pair(bar_done(b), (uint16_t)3);
-                ++n;
             }
         } else if (lane == 0) {
             const uint32_t lead_full0 = mapa_shared(bar_full(0), 0u);
@@ -760,6 +806,18 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                         static_cast<unsigned short*>(p.d_weight)[(long long)(v0 + row) * p.hidden + c] = 0;
                 continue;
             }
+            float acc[128];
+#pragma unroll
+            for (int e = 0; e < 128; ++e) acc[e] = 0.f;
+            for (int it = w.chain; it < w.steps; it += w.chain, ++n) {       // (logits alone)
+                if (!mbar_wait(bar_done(n & 1u), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
+                tc_fence_after_sync();
+                vl_add_chain(acc, tmem + ((uint32_t)(q * 32) << 16) + (n & 1u) * VL_TILE + half * 128);
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * (n & 1u));
+            }
+            if (fail) break;
             const int b = (int)(n & 1u);
             // what the values meet, asked for before the tile is complete
             int target = -1;
@@ -787,9 +845,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
             float m2 = VL_NEG, sum = 0.f;
             const int piece_row = w.piece % VL_BUFFERS * buffer_rows + row0;
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-                uint32_t r[32];
+            auto load = [&](int c, uint32_t (&r)[32]) {        // the last chunk's makes room for the unit after the next
                 tmem_ld_32x32(at + c, r);
                 tmem_ld_wait();
                 if (c == 96) {
@@ -797,7 +853,14 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
                 }
-                if (!w.q) {
+            };
+            if (!w.q) {
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t r[32];
+                    load(c, r);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + acc[c + e]);
                     const int words = p.vocab - v0 - col0 - c;       // words there are in this chunk
                     float v[32];
                     if (!BWD) {
@@ -825,20 +888,27 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     if ((c & 32) == 0) box_begin();
                     put16(v, c);
                     if ((c & 32) != 0) box_end(&maps.piece_out, 0, piece_row + ((col0 + c) >> 6) * rows_dev, false);
-                } else if (!BWD) {
-                    if (col0 + c >= p.hidden) continue;
-                    box_begin();
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t r[32];
+                    load(c, r);
+                    if (!BWD) {
+                        if (col0 + c >= p.hidden) continue;
+                        box_begin();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) box_put(i, r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-                    box_end(&maps.out, col0 + c, row0, w.piece > 0);
-                } else {
-                    if (col0 + (c & 64) >= p.hidden) continue;
-                    if ((c & 32) == 0) box_begin();
-                    float v[32];
+                        for (int i = 0; i < 8; ++i) box_put(i, r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                        box_end(&maps.out, col0 + c, row0, w.piece > 0);
+                    } else {
+                        if (col0 + (c & 64) >= p.hidden) continue;
+                        if ((c & 32) == 0) box_begin();
+                        float v[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * scale;
-                    put16(v, c);
-                    if ((c & 32) != 0) box_end(&maps.out, col0 + (c & 64), v0 + row0, false);
+                        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * scale;
+                        put16(v, c);
+                        if ((c & 32) != 0) box_end(&maps.out, col0 + (c & 64), v0 + row0, false);
+                    }
                 }
             }
             ++n;

@@ -365,3 +365,21 @@ def test_without_gradients_and_nan(cuda_lib):
     with torch.no_grad():
         losses, lse = vocab_cross_entropy(h, w, t)
         check({"losses": losses, "lse": lse}, exact(h, w, t))
+
+
+@pytest.mark.parametrize("rows,grad", [(5, False), (70, False), (70, True)])
+def test_long_rows_keep_their_digits(cuda_lib, rows, grad):
+    """16,384 features of one sign: a sum of 1024 steps of 16 products only grows, and each step may cut off a unit of what it has
+    reached, twice over (its products, the addition): in one chain 1024 units of the final value. In chains of 128 steps that is 2 * 65,
+    and one for each of eight chains."""
+    from hackaton_b200 import vocab_cross_entropy
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h = (0.05 * torch.rand(rows, 16384, device="cuda", generator=g)).to(torch.bfloat16)
+    w = (0.2 * torch.rand(700, 16384, device="cuda", generator=g)).to(torch.bfloat16)
+    t = torch.randint(0, 700, (rows,), device="cuda", generator=g)
+    logits = h.double() @ w.double().t()
+    want = torch.logsumexp(logits, 1)
+    top = logits.max(1).values
+    lse = vocab_cross_entropy(h.requires_grad_(grad), w, t)[1].detach()
+    assert ((lse.double() - want).abs() <= (138 * top + 64 + 4 * top) * UNIT).all()
