@@ -61,7 +61,7 @@ constexpr int VL_BK = 64;
 // The tensor cores cut off what an addition to an accumulator leaves behind its 24 bits, always in one direction, so
 // that a logit's error grows with the length of its chain of additions. A chain of logits is at most VL_CHAIN steps of 64;
 // longer ones are cut, and the parts added in the epilogue's registers with rounding. (3584 features, losses against 64 bits: one
-// chain 1.2e-6 in norm, FIGURE in two; in fp32 throughout 6.8e-7.)
+// chain 1.2e-6 in norm, in two 4e-7, in four 2e-7; fp32 products and sums 1.5e-7.)
 constexpr int VL_CHAIN = 32;
 constexpr int VL_FEW_CHAINS = 4;           // of at most 64 columns each: there is room for all of a tile's
 constexpr int VL_EPI_WARPS = 8;
@@ -88,6 +88,7 @@ enum VlMode {
 
 struct VlMaps {
     CUtensorMap a, b;
+    CUtensorMap a_part;      // VL_FEW: W in boxes of 16 words, for a CTA's last, part-filled tile
 };
 
 struct VlParams {
@@ -97,6 +98,7 @@ struct VlParams {
     int vocab, hidden;
     int word_tiles;          // to be looked at
     int n_rows;              // VL_FEW: columns of the accumulator, 32 or 64
+    int cta_words;           // VL_FEW: words of a CTA, one behind the other
     const int* target;       // per gathered row
     float2* parts;           // [parts][rows_pad]: maximum (base 2), sum relative to it
     long long rows_pad;
@@ -227,7 +229,8 @@ __device__ __forceinline__ uint32_t vl_pack(float a, float b, int bf16) {
 }
 
 template <int MODE>
-using VlSmemOf = VlSmem<MODE == VL_FEW ? 32 : 128, MODE == VL_FEW ? 11 : 7, false>;
+using VlSmemOf = VlSmem<MODE == VL_FEW ? 32 : 128, MODE == VL_FEW ? 10 : 7, false>;
+constexpr int VL_FEW_DEEP = 2;             // steps of the ring that come and go together
 
 __device__ __forceinline__ float2 vl_join(float2 x, float2 y) {
     const float top = fmaxf(x.x, y.x);
@@ -264,7 +267,7 @@ template <int MODE>
 __global__ void __launch_bounds__(VL_THREADS, 1)
 vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
     using L = VlSmemOf<MODE>;
-    constexpr int STAGES = L::STAGES;
+    constexpr int DEEP = MODE == VL_FEW ? VL_FEW_DEEP : 1, STAGES = L::STAGES / DEEP, STAGE_BYTES = DEEP * L::STAGE_BYTES;
     extern __shared__ uint8_t vl_smem[];
     const uint32_t base = (smem_u32(vl_smem) + 1023u) & ~1023u;
     uint8_t* gen = vl_smem + (base - smem_u32(vl_smem));
@@ -297,11 +300,16 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&maps.a);
         tma_prefetch_desc(&maps.b);
+        if (MODE == VL_FEW) tma_prefetch_desc(&maps.a_part);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
         tmem_relinquish_pair();
     }
+    // The first words come to L2 while the kernel before gathers the rows.
+    if (MODE == VL_FEW && warp == 0 && lane == 0 && (int)blockIdx.x * p.cta_words < p.vocab)
+        for (int k = 0; k < L::STAGES && k * VL_BK < p.hidden; ++k)
+            tma_prefetch_2d(p.cta_words >= 128 ? &maps.a : &maps.a_part, k * VL_BK, (int)blockIdx.x * p.cta_words);
     grid_dep_wait();
     grid_dep_launch();
     tc_fence_before_sync();
@@ -309,25 +317,37 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK);
+    const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK * DEEP);
     const int chain = MODE == VL_FEW ? vl_div_up(steps, VL_FEW_CHAINS) : vl_chain(steps);
-    const int units = rows == 0 ? 0 : MODE == VL_FEW ? p.word_tiles : row_tiles * p.word_tiles;
+    // Few rows: each CTA's words one tile of 128 behind the other, and the pair's tiles are its units.
+    const int tiles = vl_div_up(p.cta_words, 128), word_begin = (int)blockIdx.x * p.cta_words, word_end = min(word_begin + p.cta_words, p.vocab);
+    const int units = rows == 0 ? 0 : MODE == VL_FEW ? (pair + 1) * tiles : row_tiles * p.word_tiles;
+    const int unit0 = MODE == VL_FEW ? pair * tiles : pair, stride = MODE == VL_FEW ? 1 : pairs;
     int fail = 0;
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t g = 0;
-            for (int u = pair; u < units && !fail; u += pairs) {
-                const int am = (MODE == VL_FEW ? u : u % row_tiles) * VL_TILE + (int)rank * 128;
+            for (int u = unit0; u < units && !fail; u += stride) {
+                const int am = MODE == VL_FEW ? word_begin + (u - unit0) * 128 : u % row_tiles * VL_TILE + (int)rank * 128;
                 const int bn = MODE == VL_FEW ? (int)rank * (p.n_rows / 2) : u / row_tiles * VL_TILE + (int)rank * 128;
+                const int words = p.cta_words - (u - unit0) * 128;       // what is left
+                const bool part = MODE == VL_FEW && words < 128;
+                const int bytes = DEEP * ((part ? words * 128 : L::A_BYTES) + (MODE == VL_FEW ? p.n_rows * 64 : L::B_BYTES));
                 for (int it = 0; it < steps; ++it, ++g) {
                     const int s = (int)(g % STAGES);
                     if (!mbar_wait_cluster(bar_empty(s), ((g / STAGES) & 1u) ^ 1u, abort_flag)) { fail = 1; break; }
                     const uint32_t landed = rank == 0 ? bar_full(s) : bar_landed(s);
-                    const uint32_t sa = base + (uint32_t)s * L::STAGE_BYTES;
-                    mbar_arrive_expect_tx(landed, L::A_BYTES + (MODE == VL_FEW ? p.n_rows * 64 : L::B_BYTES));
-                    tma_load_2d(sa, &maps.a, it * VL_BK, am, landed);
-                    tma_load_2d(sa + L::A_BYTES, &maps.b, it * VL_BK, bn, landed);
+                    const uint32_t sa = base + (uint32_t)s * STAGE_BYTES, sb = sa + DEEP * L::A_BYTES;
+                    mbar_arrive_expect_tx(landed, bytes);
+#pragma unroll
+                    for (int k = 0; k < DEEP; ++k) {       // (behind the features: zeros)
+                        const int x = (it * DEEP + k) * VL_BK;
+                        if (!part) tma_load_2d(sa + k * L::A_BYTES, &maps.a, x, am, landed);
+                        else
+                            for (int i = 0; i < words; i += 16) tma_load_2d(sa + k * L::A_BYTES + i * 128, &maps.a_part, x, am + i, landed);
+                        tma_load_2d(sb + k * L::B_BYTES, &maps.b, x, bn, landed);
+                    }
                 }
             }
         }
@@ -336,7 +356,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             const uint32_t idesc = vl_idesc(MODE == VL_FEW ? p.n_rows : VL_TILE, false, false, p.bf16);
             const uint32_t base4 = (base & 0x3FFFFu) >> 4;
             uint32_t g = 0, n = 0;
-            for (int u = pair; u < units && !fail; u += pairs) {
+            for (int u = unit0; u < units && !fail; u += stride) {
                 uint32_t d = 0;
                 for (int at = 0; at < steps && !fail; at += chain) {
                     if (MODE != VL_FEW || at == 0) {      // a buffer to a chain, or (few rows) to all of a tile's
@@ -349,8 +369,10 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
                         const int s = (int)(g % STAGES);
                         if (!mbar_wait_cluster(bar_full(s), (g / STAGES) & 1u, abort_flag)) { fail = 3; break; }
                         tc_fence_after_sync();
-                        const uint32_t a4 = base4 + (uint32_t)s * (L::STAGE_BYTES >> 4);
-                        vl_mma_step(d, a4, a4 + (L::A_BYTES >> 4), false, false, idesc, it == at);
+                        const uint32_t a4 = base4 + (uint32_t)s * (STAGE_BYTES >> 4), b4 = a4 + DEEP * (L::A_BYTES >> 4);
+#pragma unroll
+                        for (int k = 0; k < DEEP; ++k)
+                            vl_mma_step(d, a4 + k * (L::A_BYTES >> 4), b4 + k * (L::B_BYTES >> 4), false, false, idesc, it == at && k == 0);
                         umma_commit_pair(bar_empty(s), (uint16_t)3);
                     }
                     d += 64;
@@ -360,7 +382,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
         } else if (lane == 0) {
             const uint32_t lead_full0 = mapa_shared(bar_full(0), 0u);
             uint32_t g = 0;
-            for (int u = pair; u < units && !fail; u += pairs) {
+            for (int u = unit0; u < units && !fail; u += stride) {
                 for (int it = 0; it < steps; ++it, ++g) {
                     const int s = (int)(g % STAGES);
                     if (!mbar_wait(bar_landed(s), (g / STAGES) & 1u, abort_flag)) { fail = 8; break; }
@@ -379,11 +401,11 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
 #pragma unroll
         for (int j = 0; j < 32; ++j) { m[j] = VL_NEG; s[j] = 0.f; }
         uint32_t it = 0;
-        for (int u = pair; u < units && !fail; u += pairs, ++it) {
+        for (int u = unit0; u < units && !fail; u += stride, ++it) {
             const int b = (int)(it & 1u);
             if (!mbar_wait(bar_done(b), (it >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
-            const int word0 = u * VL_TILE + (int)rank * 128 + q * 32;
+            const int word0 = word_begin + (u - unit0) * 128 + q * 32;
             float r[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0.f;
@@ -402,7 +424,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
-            const bool there = word0 + lane < p.vocab;
+            const bool there = word0 + lane < word_end;
             const unsigned hits = __ballot_sync(0xffffffffu, (unsigned)(target - word0) < 32u);    // rows whose target is here
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -954,7 +976,8 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ int before[VL_GATHER_WARPS];
-    __shared__ int place[32], total;
+    __shared__ int place[32];
+    __shared__ float dots[VL_GATHER_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row0 = (long long)blockIdx.x * per;
     const auto takes_part = [&](long long t) { return t >= 0 && t < a.vocab; };
@@ -986,14 +1009,13 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
                 a.lse[row] = 0.f;
             }
         }
-        if (lane == 0) {
-            total = start + __popc(mask);
-            if (row0 + per >= a.rows) *a.count = total;      // (the last CTA)
-        }
+        if (lane == 0 && row0 + per >= a.rows) *a.count = start + __popc(mask);      // (the last CTA)
     }
     __syncthreads();
     const int vecs = (int)(a.hidden / 8);
-    for (int i = warp; i < per; i += VL_GATHER_WARPS) {
+    // a row to a warp, or to several where there are few rows
+    const int shares = per < VL_GATHER_WARPS ? VL_GATHER_WARPS / per : 1, share = warp % shares;
+    for (int i = warp / shares; i < per; i += VL_GATHER_WARPS / shares) {
         const int at = place[i];
         if (at < 0) continue;
         const long long row = row0 + i;
@@ -1002,7 +1024,7 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
         uint4* out = reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.gathered) + (long long)at * a.hidden);
         float dot = 0.f;
 #pragma unroll 4
-        for (int c = lane; c < vecs; c += 32) {
+        for (int c = share * 32 + lane; c < vecs; c += shares * 32) {
             const uint4 x = __ldg(h + c), y = __ldg(w + c);
             out[c] = x;
             const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
@@ -1017,32 +1039,45 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (lane == 0) a.target_logit[at] = dot;
+        if (lane == 0) {
+            if (shares > 1) dots[warp] = dot;
+            else            a.target_logit[at] = dot;
+        }
     }
-    // the last CTA fills the last tile's empty rows with zeros: they meet the others' in sums over rows
-    if (row0 + per >= a.rows) {
-        const int end = vl_div_up(total, VL_TILE) * VL_TILE;
-        uint4* out = reinterpret_cast<uint4*>(a.gathered);
-        for (long long i = (long long)total * vecs + threadIdx.x; i < (long long)end * vecs; i += VL_GATHER_WARPS * 32)
-            out[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (shares == 1) return;
+    __syncthreads();
+    if (threadIdx.x < per && place[threadIdx.x] >= 0) {
+        float dot = 0.f;
+        for (int k = 0; k < shares; ++k) dot += dots[threadIdx.x * shares + k];
+        a.target_logit[place[threadIdx.x]] = dot;
     }
 }
 
-// Joins a row's statistics, 32 rows by 32 shares of the parts per CTA. PROBE: the first words' maxima give the row's
+// Joins a row's statistics, 8 rows by 128 shares of the parts per CTA. (32 by 32: 8.5 us for 64 rows of 151,936 words, so 5.0.)
+// Where the head's gradient is to come, the last tile's empty rows become zeros: they meet the others' in sums over rows,
+// and nowhere else does what lies there reach a result. PROBE: the first words' maxima give the row's
 // reference. Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's reference.
+constexpr int VL_MERGE_ROWS = 8, VL_MERGE_SHARES = 1024 / VL_MERGE_ROWS;
+
 template <bool PROBE>
 __global__ void __launch_bounds__(1024)
 vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ float2 join[32][33];
-    const int rows = *a.count, row = blockIdx.x * 32 + threadIdx.x;
-    if (blockIdx.x * 32 >= rows) return;
+    __shared__ float2 join[VL_MERGE_ROWS][VL_MERGE_SHARES + 1];
+    const int rows = *a.count, row = blockIdx.x * VL_MERGE_ROWS + threadIdx.x;
+    if (!PROBE && (a.grads & 2)) {
+        const long long vecs = a.hidden / 8, end = (long long)vl_div_up(rows, VL_TILE) * VL_TILE * vecs;
+        uint4* out = reinterpret_cast<uint4*>(a.gathered);
+        for (long long i = rows * vecs + blockIdx.x * 1024 + threadIdx.y * VL_MERGE_ROWS + threadIdx.x; i < end; i += gridDim.x * 1024)
+            out[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (blockIdx.x * VL_MERGE_ROWS >= rows) return;
     float m = VL_NEG, s = 0.f;
     if (row < rows) {
         const float ref = soft ? a.refs[row] : 0.f;
 #pragma unroll 4
-        for (int i = threadIdx.y; i < n_parts; i += 32) {
+        for (int i = threadIdx.y; i < n_parts; i += VL_MERGE_SHARES) {
             float2 x = a.parts[(long long)i * a.rows_pad + row];
             if (soft) x.x = ref;
             x = vl_join(make_float2(m, s), x);
@@ -1053,13 +1088,17 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     join[threadIdx.x][threadIdx.y] = make_float2(m, s);
     __syncthreads();
     // a warp joins one row's shares
-    float2 x = join[threadIdx.y][threadIdx.x];
+    const int thread = threadIdx.y * VL_MERGE_ROWS + threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    if (warp >= VL_MERGE_ROWS) return;
+    float2 x = join[warp][lane];
+#pragma unroll
+    for (int i = 32; i < VL_MERGE_SHARES; i += 32) x = vl_join(x, join[warp][lane + i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         x = vl_join(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
     }
-    const int at = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x != 0 || at >= rows) return;
+    const int at = blockIdx.x * VL_MERGE_ROWS + warp;
+    if (lane != 0 || at >= rows) return;
     const float logit = a.target_logit[at], logit2 = logit * VL_LOG2E;
     if (PROBE) {
         // (fmaxf leaves out a NaN; within what a float keeps whole numbers of)
@@ -1281,10 +1320,16 @@ size_t vocab_loss_kept_bytes(long long rows, long long hidden, int grads) { retu
 
 size_t vocab_loss_workspace_bytes(const VocabLossArgs& a, bool backward) { return vl_scratch(a, backward).bytes; }
 
-// CTA pairs of a kernel that takes tensor maps and parameters: one per pair of SMs as far as there are units.
+// CTA pairs: one per pair of SMs as far as there are units.
+static long long vl_pairs(long long units, int sm_count) {
+    const long long pairs = units < sm_count / 2 ? units : sm_count / 2;
+    return pairs < 1 ? 1 : pairs;
+}
+
+// A kernel of CTA pairs that takes tensor maps and parameters.
 template <typename Maps, typename Params>
 static cudaError_t vl_launch(void (*kernel)(Maps, Params), int threads, int smem, const Maps& maps, const Params& p, long long units,
-                             int sm_count, cudaStream_t stream, int* ctas = nullptr) {
+                             int sm_count, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -1300,11 +1345,7 @@ static cudaError_t vl_launch(void (*kernel)(Maps, Params), int threads, int smem
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    long long pairs = sm_count / 2;
-    if (units < pairs) pairs = units;
-    if (pairs < 1) pairs = 1;
-    cfg.gridDim = dim3((unsigned)(2 * pairs));
-    if (ctas != nullptr) *ctas = (int)(2 * pairs);
+    cfg.gridDim = dim3((unsigned)(2 * vl_pairs(units, sm_count)));
     return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
 
@@ -1369,17 +1410,19 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         a.piece = ws + s.piece;
         a.capacity = s.room.capacity;
     }
-    const int per = a.rows <= 4096 ? 8 : 32;
+    const int per = a.rows <= 512 ? 2 : a.rows <= 4096 ? 8 : 32;     // rows of a CTA (64 x 3584: a row to a warp 11.5 us, to four 5.7)
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
     // Up to 64 rows without a gradient of x: the words take the tensor cores' long side. (64 rows of 3584 features against
-    // 151,936 words: 216 us with the rows there, which costs four times the products, 196 this way; the weight alone
-    // takes 168.)
+    // 151,936 words: with the rows there, which costs four times the products, 216 us, this way 177; the weight's 1.09 GB
+    // alone take 168. All three kernels 187.) Every CTA has as many words, in tiles of 128 and a rest, not a share of
+    // the tiles: those are 8.03 to a pair here.
     const bool few = !soft && a.rows <= 64;
     const int few_rows = a.rows <= 32 ? 32 : 64;
     VlMaps logits = {};
     VlSweepMaps maps = {};
     bool ok = few ? vl_map(&logits.a, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) &&
+                        vl_map(&logits.a_part, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 16) &&
                         vl_map(&logits.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, few_rows / 2)
                   : vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
                         vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
@@ -1397,12 +1440,13 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab); p.n_rows = few_rows;
     p.target = a.target; p.parts = a.parts; p.rows_pad = a.rows_pad;
     const long long row_tiles = a.rows_pad / VL_TILE;
-    const dim3 merge_grid((unsigned)((a.rows + 31) / 32)), merge_block(32, 32);
+    const dim3 merge_grid((unsigned)((a.rows + VL_MERGE_ROWS - 1) / VL_MERGE_ROWS)), merge_block(VL_MERGE_ROWS, VL_MERGE_SHARES);
     int n_parts = 2 * p.word_tiles;
     if (few) {
-        int ctas = 0;
-        e = vl_launch(vl_stats_kernel<VL_FEW>, VL_THREADS, VlSmemOf<VL_FEW>::TOTAL, logits, p, p.word_tiles, a.sm_count, stream, &ctas);
-        n_parts = 4 * ctas;
+        const long long pairs = vl_pairs(p.word_tiles, a.sm_count);
+        p.cta_words = (int)((a.vocab + 2 * pairs * 16 - 1) / (2 * pairs * 16) * 16);
+        e = vl_launch(vl_stats_kernel<VL_FEW>, VL_THREADS, VlSmemOf<VL_FEW>::TOTAL, logits, p, p.word_tiles, a.sm_count, stream);
+        n_parts = (int)(8 * pairs);
     } else if (!soft) {
         e = vl_launch(vl_stats_kernel<VL_STATS>, VL_THREADS, VlSmemOf<VL_STATS>::TOTAL, logits, p, row_tiles * p.word_tiles, a.sm_count, stream);
     } else {
