@@ -273,9 +273,11 @@ act8_swiglu_any_kernel(const Act8Swiglu a, const A8Rows g, int backward) {
 constexpr int A8G_WARPS = 8;
 constexpr int A8G_COLS = 128;
 constexpr int A8G_DEPTH = 4;
-constexpr int A8G_CODES = 16 * A8G_COLS, A8G_STEP_BYTES = A8G_CODES + 16 * 32 + 64;      // codes, s, step bytes
+constexpr int A8G_PITCH = A8G_COLS + 32;      // of a row of codes: the four rows and two columns of eight lanes lie in as many banks
+constexpr int A8G_CODES = 16 * A8G_PITCH, A8G_STEP_BYTES = A8G_CODES + 16 * 32 + 64;      // codes, s, step bytes
 constexpr int A8G_SMEM = A8G_WARPS * A8G_DEPTH * A8G_STEP_BYTES;
-static_assert(A8G_SMEM >= A8G_WARPS / 2 * 16 * (A8G_COLS + 4) * 4, "the warps' sums meet in the same memory");
+constexpr int A8G_SUM_PITCH = A8G_COLS / 32 * 36;
+static_assert(A8G_SMEM >= A8G_WARPS * 16 * A8G_SUM_PITCH * 4, "the warps' sums meet in the same memory");
 
 __device__ __forceinline__ void a8_mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -307,152 +309,160 @@ act8_lora_grad_kernel(const Act8LoraGrad a) {
     // where this lane's copies come from in the step at row 0, and go to
     const int piece = lane & 7, prow = lane >> 3;
     const bool piece_ok = col0 + piece * 16 < a.pitch;
-    const int8_t* const from_codes = a.codes + prow * a.pitch + (piece_ok ? col0 + piece * 16 : 0);
-    const uint32_t to_codes = ring + prow * A8G_COLS + piece * 16;
-    const char* const from_s = reinterpret_cast<const char*>(a.s) + lane * 16;
-    const uint8_t* const from_steps = a.steps + (lane & 15) * blocks + col0 / A8_BLOCK;    // (a tile begins at a multiple of four blocks)
-    const auto fetch = [&](long long r0, int slot) {
-        const uint32_t off = (uint32_t)slot * A8G_STEP_BYTES;
-        if (r0 + 16 <= row_end && piece_ok) {
-            const int8_t* p = from_codes + r0 * a.pitch;
+    const long long first = row_begin + warp * 16;
+    int todo = (int)(row_end - first);         // rows from the step to fetch to the end
+    const int8_t* from_codes = a.codes + (first + prow) * a.pitch + (piece_ok ? col0 + piece * 16 : 0);
+    const char* from_s = reinterpret_cast<const char*>(a.s) + first * 32 + lane * 16;
+    const uint8_t* from_steps = a.steps + (first + (lane & 15)) * blocks + col0 / A8_BLOCK;    // (a tile begins at a multiple of four blocks)
+    const long long row4 = 4 * a.pitch, ahead_codes = A8G_WARPS * 16 * a.pitch, ahead_steps = A8G_WARPS * 16 * blocks;
+    const uint32_t to_codes = prow * A8G_PITCH + piece * 16;
+    const auto fetch = [&](uint32_t at) {
+        if (todo >= 16 && piece_ok) {
+            const int8_t* p = from_codes;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {      // codes: 8 pieces of 16 bytes a row
-                cp_async16(to_codes + off + i * 4 * A8G_COLS, p);
-                p += 4 * a.pitch;
-            }
-        } else if (r0 < row_end) {
+            for (int i = 0; i < 4; ++i, p += row4) cp_async16(at + to_codes + i * 4 * A8G_PITCH, p);      // 8 pieces of 16 bytes a row
+        } else if (todo > 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool there = piece_ok && r0 + i * 4 + prow < row_end;
-                cp_async16_or_zero(to_codes + off + i * 4 * A8G_COLS, there ? from_codes + (r0 + i * 4) * a.pitch : a.codes, there);
+                const bool there = piece_ok && i * 4 + prow < todo;
+                cp_async16_or_zero(at + to_codes + i * 4 * A8G_PITCH, there ? from_codes + i * row4 : a.codes, there);
             }
         }
-        if (r0 < row_end) {
-            const bool there = r0 + (lane >> 1) < row_end, in = r0 + (lane & 15) < row_end;
-            cp_async16_or_zero(ring + off + A8G_CODES + lane * 16, there ? from_s + r0 * 32 : reinterpret_cast<const char*>(a.s), there);
-            if (lane < 16 && step_words)
-                cp_async4_or_zero(ring + off + A8G_CODES + 512 + lane * 4, in ? from_steps + r0 * blocks : a.steps, in);
+        if (todo > 0) {
+            const bool there = (lane >> 1) < todo;
+            cp_async16_or_zero(at + A8G_CODES + lane * 16, there ? from_s : reinterpret_cast<const char*>(a.s), there);
+            if (lane < 16 && step_words) {
+                const bool in = lane < todo;
+                cp_async4_or_zero(at + A8G_CODES + 512 + lane * 4, in ? from_steps : a.steps, in);
+            }
         }
         cp_async_commit();
+        from_codes += ahead_codes;
+        from_s += A8G_WARPS * 16 * 32;
+        from_steps += ahead_steps;
+        todo -= A8G_WARPS * 16;
     };
-    long long r0 = row_begin + warp * 16;
-    for (int k = 0; k < A8G_DEPTH; ++k) fetch(r0 + (long long)k * (A8G_WARPS * 16), k);
+    for (int k = 0; k < A8G_DEPTH; ++k) fetch(ring + k * A8G_STEP_BYTES);
     // the fragment of s, rank-major: contraction index 2t is row t, 2t + 1 row t + 4, 2t + 8 and 2t + 9 rows t + 8, t + 12
     const int k8 = (lane & 7) + (lane >= 16 ? 8 : 0);      // (matrices 0, 1: indices 0 .. 7; 2, 3: 8 .. 15)
-    const uint32_t at_s = ring + A8G_CODES + (((k8 & 7) >> 1) + (k8 & 1) * 4 + (k8 & 8)) * 32 + ((lane >> 3) & 1) * 16;
-    const uint32_t at_codes = ring + t * A8G_COLS + g * 16, at_steps = ring + A8G_CODES + 512 + t * 4 + (g >> 1);
+    const uint32_t at_s = A8G_CODES + (((k8 & 7) >> 1) + (k8 & 1) * 4 + (k8 & 8)) * 32 + ((lane >> 3) & 1) * 16;
+    const uint32_t at_codes = t * A8G_PITCH + g * 16, at_steps = A8G_CODES + 512 + t * 4 + (g >> 1);
     const __half2 bias = __float2half2_rn(1536.f);
-    int slot = 0;
-    for (; r0 < row_end; r0 += A8G_WARPS * 16, slot = (slot + 1) & (A8G_DEPTH - 1)) {
+    uint32_t at = ring;
+    for (int left = (int)(row_end - first); left > 0; left -= A8G_WARPS * 16) {
         cp_async_wait<A8G_DEPTH - 1>();
         __syncwarp();
-        const uint32_t off = (uint32_t)slot * A8G_STEP_BYTES;
-        uint4 q[4];
-        float step[4];
-        bool tiny = false;
+        uint32_t q[4][4], st[4];
+        bool plain = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w)
-                         : "r"(at_codes + off + i * 4 * A8G_COLS));
-            uint32_t st;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i][0]), "=r"(q[i][1]), "=r"(q[i][2]), "=r"(q[i][3])
+                         : "r"(at + at_codes + i * 4 * A8G_PITCH));
             if (step_words) {
-                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(st) : "r"(at_steps + off + i * 16));
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(st[i]) : "r"(at + at_steps + i * 16));
             } else {
-                const long long b = col0 / A8_BLOCK + (g >> 1), row = r0 + t + 4 * i;
-                st = row < row_end && b < blocks ? a.steps[row * blocks + b] : 0u;
+                const long long b = col0 / A8_BLOCK + (g >> 1), row = row_end - left + t + 4 * i;
+                st[i] = t + 4 * i < left && b < blocks ? a.steps[row * blocks + b] : 0u;
             }
-            step[i] = a8_value_of_step(st);      // (NaN stays)
-            tiny = tiny || step[i] < 5.9604644775390625e-8f;
+            plain = plain && (st[i] == 0u || st[i] - 103u <= 132u - 103u);
         }
         uint32_t f[4];
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at_s + off));
-        // steps below 2^-24: that, and a second factor
-        __half2 large[2], small[2];
-        const bool any_tiny = __any_sync(0xffffffffu, tiny);
-        if (any_tiny) {
+                     : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at + at_s));
+        // A code of each of two rows, sign-extended; 0x6600 plus a number from -128 to 127 is 1536 plus it in fp16, and the
+        // sum's upper byte is 0x66, or 0x65 where the number is negative.
+        const auto two = [&](int w, int e, int p) {
+            uint32_t x;
+            asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(q[2 * p][w]), "r"(q[2 * p + 1][w]), "r"(0xC480 + 0x1111 * e));
+            x = (x & 0x03FF03FFu) ^ 0x66006600u;
+            return *reinterpret_cast<const __half2*>(&x);
+        };
+        __half2 large[2];
+        if (__all_sync(0xffffffffu, plain)) {      // steps of 2^-24 to 2^5 (or of nothing): 1536 steps are a number too
+            __half2 off[2];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                float s2[2];
+                large[p] = __floats2half2_rn(__uint_as_float(st[2 * p] << 23), __uint_as_float(st[2 * p + 1] << 23));
+                off[p] = __hneg2(__hmul2(bias, large[p]));
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t b[2];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const __half2 v = __hfma2(two(w, e, p), large[p], off[p]);
+                        b[p] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                    a8_mma16816(acc[4 * w + e], f, b[0], b[1]);
+                }
+        } else {                                   // a step below 2^-24: that, and a second factor. (NaN stays)
+            __half2 small[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                float s1[2], s2[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float& x = step[2 * p + i];
-                    const bool below = x < 5.9604644775390625e-8f;
-                    s2[i] = below ? x * 16777216.f : 1.f;
-                    x = below ? 5.9604644775390625e-8f : x;
+                    s1[i] = a8_value_of_step(st[2 * p + i]);
+                    const bool below = s1[i] < 5.9604644775390625e-8f;
+                    s2[i] = below ? s1[i] * 16777216.f : 1.f;
+                    s1[i] = below ? 5.9604644775390625e-8f : s1[i];
                 }
+                large[p] = __floats2half2_rn(s1[0], s1[1]);
                 small[p] = __floats2half2_rn(s2[0], s2[1]);
             }
-        }
 #pragma unroll
-        for (int p = 0; p < 2; ++p) large[p] = __floats2half2_rn(step[2 * p], step[2 * p + 1]);
+            for (int w = 0; w < 4; ++w)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint32_t word[4];
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t b[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) word[i] = w == 0 ? q[i].x : w == 1 ? q[i].y : w == 2 ? q[i].z : q[i].w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t b[2];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    // a code of each of two rows, sign-extended; 0x6600 plus a number from -128 to 127 is 1536 plus it in fp16,
-                    // and the sum's upper byte is 0x66, or 0x65 where the number is negative
-                    uint32_t two;
-                    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(two) : "r"(word[2 * p]), "r"(word[2 * p + 1]), "r"(0xC480 + 0x1111 * e));
-                    const uint32_t raw = (two & 0x03FF03FFu) ^ 0x66006600u;
-                    __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raw), bias);
-                    if (any_tiny) v = __hmul2(v, small[p]);
-                    v = __hmul2(v, large[p]);
-                    b[p] = *reinterpret_cast<const uint32_t*>(&v);
+                    for (int p = 0; p < 2; ++p) {
+                        const __half2 v = __hmul2(__hmul2(__hsub2(two(w, e, p), bias), small[p]), large[p]);
+                        b[p] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                    a8_mma16816(acc[4 * w + e], f, b[0], b[1]);
                 }
-                a8_mma16816(acc[4 * w + e], f, b[0], b[1]);
-            }
         }
         __syncwarp();      // (every lane has read the slot)
-        fetch(r0 + (long long)A8G_DEPTH * (A8G_WARPS * 16), slot);
+        fetch(at);
+        at = at == ring + (A8G_DEPTH - 1) * A8G_STEP_BYTES ? ring : at + A8G_STEP_BYTES;
     }
     cp_async_wait<0>();
     __syncthreads();
     // acc[j]: ranks g, g, g + 8, g + 8 of columns 16 * (2t) + j and 16 * (2t + 1) + j (N index n stands for the column
-    // group of the lanes with g = n)
-    float (*sums)[16][A8G_COLS + 4] = reinterpret_cast<float (*)[16][A8G_COLS + 4]>(a8_smem);
-    for (int half = A8G_WARPS / 2; half >= 1; half >>= 1) {
-        if (warp >= half && warp < 2 * half) {
+    // group of the lanes with g = n). Every warp lays its sums down, every thread adds the warps' for some outputs. A rank's
+    // 32-column quarters are 36 values apart: the banks of eight lanes with two ranks and four t differ.
+    const uint32_t sums = smem_u32(a8_smem);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                sums[warp - half][g][32 * t + j] = acc[j][0];
-                sums[warp - half][g][32 * t + 16 + j] = acc[j][1];
-                sums[warp - half][g + 8][32 * t + j] = acc[j][2];
-                sums[warp - half][g + 8][32 * t + 16 + j] = acc[j][3];
-            }
-        }
-        __syncthreads();
-        if (warp < half) {
+    for (int h = 0; h < 4; ++h)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                acc[j][0] += sums[warp][g][32 * t + j];
-                acc[j][1] += sums[warp][g][32 * t + 16 + j];
-                acc[j][2] += sums[warp][g + 8][32 * t + j];
-                acc[j][3] += sums[warp][g + 8][32 * t + 16 + j];
-            }
-        }
-        __syncthreads();
-    }
-    if (warp == 0) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            sums[0][g][32 * t + j] = acc[j][0];
-            sums[0][g][32 * t + 16 + j] = acc[j][1];
-            sums[0][g + 8][32 * t + j] = acc[j][2];
-            sums[0][g + 8][32 * t + 16 + j] = acc[j][3];
-        }
-    }
+        for (int j = 0; j < 16; j += 4)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(sums + 4 * ((warp * 16 + g + (h >> 1) * 8) * A8G_SUM_PITCH + t * 36 + (h & 1) * 16 + j)),
+                           "f"(acc[j][h]), "f"(acc[j + 1][h]), "f"(acc[j + 2][h]), "f"(acc[j + 3][h]) : "memory");
     __syncthreads();
     float* out = a.splits > 1 ? a.planes + (long long)blockIdx.y * 16 * a.cols : a.out;
-    for (int i = threadIdx.x; i < 16 * A8G_COLS; i += A8G_WARPS * 32) {
-        const int r = i / A8G_COLS, c = i % A8G_COLS;
-        if (col0 + c < a.cols) out[(long long)r * a.cols + col0 + c] = sums[0][r][c];
+    for (int i = threadIdx.x; i < 16 * A8G_COLS / 4; i += A8G_WARPS * 32) {
+        const int r = i / (A8G_COLS / 4), c = i % (A8G_COLS / 4) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < A8G_WARPS; ++w) {
+            float x[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                         : "r"(sums + 4 * ((w * 16 + r) * A8G_SUM_PITCH + c / 32 * 36 + c % 32)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += x[e];
+        }
+        float* to = out + (long long)r * a.cols + col0 + c;
+        if (a.cols % 4 == 0 && col0 + c < a.cols && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col0 + c + e < a.cols) to[e] = v[e];
+        }
     }
 }
 
