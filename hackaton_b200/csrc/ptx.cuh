@@ -125,6 +125,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
         : "memory");
 }
 
+// On a wait that ran out: its code in the status word, and time for copies and MMAs in flight to land before shared memory
+// and TMEM go away.
+__device__ __forceinline__ void give_up(int* status, int code) {
+    atomicCAS(status, 0, code);
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
 // 2-D tiled store, and the same box added to fp32 values in memory (once per element: no order to depend on). The
 // thread that issues them commits them to its groups; before the shared memory is written again it waits until they have
 // been read (bulk_wait_read), before it ends until they are done (bulk_wait). x as for loads; x, y not negative.

@@ -262,7 +262,7 @@ sandwich_fwd_kernel(const SandwichArgs a) {
         const uint32_t from = room + slot * slot_bytes;
         const int row = now.row;
         if (VEC == 4 && !mbar_wait(bars[slot], phase, bars.abort_flag)) {
-            if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_ROW_WAIT);
+            if (threadIdx.x == 0) give_up(a.status, STATUS_ROW_WAIT);
             return;
         }
         if (now.unit != unit) {
@@ -385,7 +385,7 @@ sandwich_bwd_kernel(const SandwichArgs a) {
     for (int slot = 0; now.row >= 0;) {
         const uint32_t from = room + slot * slot_bytes;
         if (VEC == 4 && !mbar_wait(bars[slot], phase, bars.abort_flag)) {
-            if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_ROW_WAIT);
+            if (threadIdx.x == 0) give_up(a.status, STATUS_ROW_WAIT);
             return;
         }
         if (new_unit) sw_gated<NV, VEC>(a, now.unit / shares, cols, in, post);

@@ -256,13 +256,6 @@ __device__ __forceinline__ uint32_t vl_idesc(int n, bool a_mn, bool b_mn, int bf
     return make_idesc_f16((uint32_t)n, a_mn ? 1u : 0u, b_mn ? 1u : 0u, VL_TILE) | (bf16 ? (1u << 7) | (1u << 10) : 0u);
 }
 
-// On a failed wait: copies and MMAs in flight get time to land before shared memory and TMEM go away.
-__device__ __forceinline__ void vl_failed(int* status, int fail) {
-    atomicCAS(status, 0, 100 + fail);
-    const unsigned long long t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-}
-
 template <int MODE>
 __global__ void __launch_bounds__(VL_THREADS, 1)
 vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlParams p) {
@@ -500,7 +493,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
         }
     }
 
-    if (fail) vl_failed(p.status, fail);
+    if (fail) give_up(p.status, 100 + fail);
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();
@@ -949,7 +942,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
         if (lane == 0) bulk_wait();
     }
 
-    if (fail) vl_failed(p.status, fail);
+    if (fail) give_up(p.status, 100 + fail);
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();
