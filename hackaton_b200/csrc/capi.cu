@@ -952,7 +952,7 @@ int nf4b200_act8_lora_grad(const void* codes, const void* steps, const void* s, 
 }
 
 static int sandwich_check(const char* what, int64_t rows, int64_t hidden, int64_t gates, int delta_dtype, int normed_dtype) {
-    if (rows < 0 || rows > 0x7FFFFFFF || hidden <= 0 || hidden > nf4::SANDWICH_MAX_HIDDEN)
+    if (rows < 0 || rows > 0x7FFF0000 || hidden <= 0 || hidden > nf4::SANDWICH_MAX_HIDDEN)     // (rows and steps in 32 bits)
         return fail(NF4B200_EINVAL, "%s: bad shape %lld x %lld (hidden up to %d)", what, (long long)rows, (long long)hidden,
                     nf4::SANDWICH_MAX_HIDDEN);
     if (gates < 0 || (gates > 0 && rows % gates != 0))

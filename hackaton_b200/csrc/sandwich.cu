@@ -149,6 +149,8 @@ __device__ __forceinline__ void sw_block_sum(float (&v)[N], float4 (*part)[32], 
 #pragma unroll
             for (int o = 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
         turn ^= 1;
+    } else {
+        __syncwarp();      // (what the lanes read may be written again)
     }
 }
 

@@ -49,11 +49,12 @@ constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
 // A piece: at most VL_PIECE_TILES tiles of words and VL_PIECE_UNITS tiles of 256 x 256 (17 MB), at least
-// VL_PIECE_LEAST tiles of words, whatever the rows. Its product comes VL_LAG pieces behind its logits in the list, so that
+// VL_PIECE_LEAST tiles of words up to VL_PIECE_MOST tiles (a piece is read once per 256 features and written once, so L2 is a
+// help, not a need; four pieces of that size are 1 GB), and one behind that. Its product comes VL_LAG pieces behind its logits in the list, so that
 // what a unit waits for was drawn at least a piece earlier, not a moment ago by a pair that is still at it. With 1229 rows
 // (5 row tiles, 80 units of logits to a piece) U takes 1055 us; with a lag of one and pieces of 24 word tiles 1157, of
 // four drawn tickets to a pair in place of two 1191. Larger pieces gain nothing (256 units: 1038 us, dW 1043 for 1027).
-constexpr int VL_PIECE_UNITS = 128, VL_PIECE_TILES = 16, VL_PIECE_LEAST = 8;
+constexpr int VL_PIECE_UNITS = 128, VL_PIECE_TILES = 16, VL_PIECE_LEAST = 8, VL_PIECE_MOST = 2048;
 constexpr int VL_LAG = 2, VL_BUFFERS = VL_LAG + 2;
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
@@ -1227,7 +1228,9 @@ static VlRoom vl_room(long long rows, long long vocab) {
     const long long row_tiles = vl_rows_pad(rows) / VL_TILE;
     const int word_tiles = vl_word_tiles(vocab);
     VlRoom r = {VL_PIECE_UNITS, 1};
-    if (r.capacity < VL_PIECE_LEAST * row_tiles) r.capacity = (int)(VL_PIECE_LEAST * row_tiles);
+    const long long least = VL_PIECE_LEAST * row_tiles < VL_PIECE_MOST ? VL_PIECE_LEAST * row_tiles : VL_PIECE_MOST;
+    if (r.capacity < least) r.capacity = (int)least;
+    if (r.capacity < row_tiles) r.capacity = (int)row_tiles;
     // (more row tiles, fewer tiles of words in a piece)
     r.pieces = vl_div_up(word_tiles, vl_piece_tiles((int)row_tiles, word_tiles, r.capacity));
     return r;

@@ -103,6 +103,13 @@ def test_several_pieces_of_the_vocabulary(cuda_lib, dtype):
     check(run(h, w, t, b, c), exact(h, w, t, b, c))
 
 
+def test_many_rows(cuda_lib):
+    """More tiles of rows than a piece of the vocabulary has room for two tiles of words."""
+    h, w, t = make(263_000, 600, 64, torch.bfloat16, 21, ignored=0.1)
+    b, c = factors(263_000)
+    check(run(h, w, t, b, c), exact(h, w, t, b, c))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_logits_that_outgrow_what_the_first_words_showed(cuda_lib, dtype):
     """Words far behind the first 2048 beat them, and the target, by up to 2^60, in both pieces, for some rows of some
