@@ -317,6 +317,9 @@ struct VocabLossArgs {
     float* lse_rows;             // in the base-2 domain
     float* rest;                 // 1 - p of the target
     float* norm;                 // one over the sum that `sums` is relative to
+    int* links;                  // [rows_pad]: how many rows' targets are a number modulo rows_pad,
+    int* first;                  // one of them, or -1,
+    int* next;                   // and per row another one, or -1
     float* sums;                 // [rows that take part, hidden]: sum of exp(l_v - reference) w_v over v other than the target
     void* gathered;              // the rows themselves
     float2* parts;

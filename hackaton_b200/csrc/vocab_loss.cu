@@ -13,7 +13,9 @@
 // at the end. The target is left out of U and of the sums, so that 1 - p_t and a loss near zero keep their digits, and its
 // share is added in fp32. Where a row meets a logit too far above its reference for the 16-bit type, its row tile's sweep
 // is done again with references from the maxima; the launch for that looks at a flag and leaves. dW needs the final
-// lse: the logits once more, in 16-bit dl this time, and one product.
+// lse: the logits once more, in 16-bit dl this time, and one product. A word's row of dW is mostly what its own
+// rows' targets add, so that what those dl lose in 16 bits shows: it is kept and added in fp32, for four rows of a word.
+// (1229 rows, 5000 words: dW is 2.1e-4 of itself off in fp16, as much as its own rounding alone; without this 3.0e-4.)
 //
 // The tensor cores bound it, and their clock the power that the chip may take, so what counts is that they never pause
 // and that little moves. CTA pairs (tcgen05.mma.cta_group::2) own a 256 x 256 tile, 128 rows by 256 columns of fp32 in
@@ -64,6 +66,7 @@ constexpr int VL_BK = 64;
 // longer ones are cut, and the parts added in the epilogue's registers with rounding. (3584 features, losses against 64 bits: one
 // chain 1.2e-6 in norm, in two 4e-7, in four 2e-7; fp32 products and sums 1.5e-7.)
 constexpr int VL_CHAIN = 32;
+constexpr int VL_LINKS = 16;               // rows of a word (or that share its place in the table) up to which they are looked up
 constexpr int VL_FEW_CHAINS = 4;           // of at most 64 columns each: there is room for all of a tile's
 constexpr int VL_EPI_WARPS = 8;
 constexpr int VL_SMEM_MAX = 232448, VL_BAR_ROOM = 512;
@@ -139,7 +142,11 @@ struct VlSweepParams {
     // backward
     const float* lse2;
     const float* rest;       // 1 - p of the target
-    const float4* coef;      // ((b + c), b, c) over the common power of two, times VL_P_SCALE
+    const float4* coef;      // ((b + c), b, c) over the common power of two, times VL_P_SCALE, and what the target's dl loses
+    const int* links;
+    const int* first;
+    const int* next;
+    const void* gathered;
     void* d_weight;          // [vocab, hidden]
     const float* weight_scale;
 };
@@ -162,6 +169,9 @@ __device__ __forceinline__ float vl_ex2(float x) {
 __device__ __forceinline__ void vl_sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+
+// dl of the target: c p_t - b (1 - p_t).
+__device__ __forceinline__ float vl_hit(float b, float c, float rest) { return c * (1.f - rest) - b * rest; }
 
 // Steps of a chain where there are so many.
 __host__ __device__ inline int vl_chain(int steps) { return vl_div_up(steps, vl_div_up(steps, VL_CHAIN)); }
@@ -218,6 +228,11 @@ __device__ __forceinline__ bool vl_mbar_wait_acquire(uint32_t bar, uint32_t pari
             return false;
         }
     }
+}
+
+__device__ __forceinline__ float2 vl_two(uint32_t w, int bf16) {
+    if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 __device__ __forceinline__ uint32_t vl_pack(float a, float b, int bf16) {
@@ -850,7 +865,27 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     ref = p.refs[row];
                 }
             }
-            if (BWD && w.q) scale = *p.weight_scale;
+            // backward's Q: the last four rows whose target is this thread's word. (Where there are many, what they lose
+            // averages out.)
+            int hits[4] = {-1, -1, -1, -1};
+            if (BWD && w.q) {
+                scale = *p.weight_scale;
+                const int key = (v0 + row) % (int)p.rows_pad;
+                if (v0 + row < p.vocab && p.links[key] <= VL_LINKS)
+                    for (int r = p.first[key]; r >= 0; r = p.next[r]) {
+                        if (p.target[r] != v0 + row) continue;
+                        int x = r;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (x > hits[k]) {
+                                const int y = hits[k];
+                                hits[k] = x;
+                                x = y;
+                            }
+                    }
+                __syncwarp();
+            }
+            const bool any_hit = BWD && w.q && __any_sync(0xffffffffu, hits[0] >= 0);
             // what is about to be overwritten has been read; what is about to be added to has the pieces before
             if (!w.q && w.piece >= VL_BUFFERS &&
                 !wait_count(p.read + (w.piece - VL_BUFFERS) * p.pitch + w.slot, list.feature_tiles)) { fail = 12; break; }
@@ -893,7 +928,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = vl_ex2(fmaf(__uint_as_float(r[e]), VL_LOG2E, -lse2)) * coef.x;
                         if (__any_sync(0xffffffffu, words < 32 || (unsigned)(target - c) < 32u || !live)) {
-                            const float hit = coef.z * (1.f - rest) - coef.y * rest;    // c p_t - b (1 - p_t)
+                            const float hit = vl_hit(coef.y, coef.z, rest);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 if (e == target - c) v[e] = hit;
@@ -921,7 +956,30 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                         if ((c & 32) == 0) box_begin();
                         float v[32];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * scale;
+                        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+                        if (any_hit) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if (hits[k] < 0) continue;
+                                const float lost = p.coef[hits[k]].w;
+                                const uint4* h = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p.gathered) +
+                                                                               (long long)hits[k] * p.hidden + col0 + c);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if (col0 + c + 8 * i >= p.hidden) break;
+                                    const uint4 x = h[i];
+                                    const uint32_t two[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        const float2 y = vl_two(two[e], p.bf16);
+                                        v[8 * i + 2 * e] = fmaf(lost, y.x, v[8 * i + 2 * e]);
+                                        v[8 * i + 2 * e + 1] = fmaf(lost, y.y, v[8 * i + 2 * e + 1]);
+                                    }
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] *= scale;
                         put16(v, c);
                         if ((c & 32) != 0) box_end(&maps.out, col0 + (c & 64), v0 + row0, false);
                     }
@@ -954,14 +1012,6 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
 }
 
 // ------------------------------------------------------------------------------------- rows that take part
-__device__ __forceinline__ float vl_float(unsigned short x, int bf16) {
-    return bf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
-}
-__device__ __forceinline__ float2 vl_two(uint32_t w, int bf16) {
-    if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-
 constexpr int VL_GATHER_WARPS = 8;
 
 // A CTA takes `per` rows of the caller's. Where they go follows from the targets before them, which it counts itself.
@@ -981,6 +1031,11 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
     if (lane == 0) before[warp] = n;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_counters; i += (long long)gridDim.x * blockDim.x)
         a.counters[i] = 0;
+    if (a.grads & 2)
+        for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.rows_pad; i += (long long)gridDim.x * blockDim.x) {
+            a.links[i] = 0;
+            a.first[i] = -1;
+        }
     __syncthreads();
     if (warp == 0) {
         int start = 0;
@@ -1066,6 +1121,7 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
         for (long long i = rows * vecs + blockIdx.x * 1024 + threadIdx.y * VL_MERGE_ROWS + threadIdx.x; i < end; i += gridDim.x * 1024)
             out[i] = make_uint4(0u, 0u, 0u, 0u);
     }
+    const int thread = threadIdx.y * VL_MERGE_ROWS + threadIdx.x, warp = thread >> 5, lane = thread & 31;
     if (blockIdx.x * VL_MERGE_ROWS >= rows) return;
     float m = VL_NEG, s = 0.f;
     if (row < rows) {
@@ -1082,7 +1138,6 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     join[threadIdx.x][threadIdx.y] = make_float2(m, s);
     __syncthreads();
     // a warp joins one row's shares
-    const int thread = threadIdx.y * VL_MERGE_ROWS + threadIdx.x, warp = thread >> 5, lane = thread & 31;
     if (warp >= VL_MERGE_ROWS) return;
     float2 x = join[warp][lane];
 #pragma unroll
@@ -1116,6 +1171,11 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     a.lse_rows[at] = logit2 + loss * VL_LOG2E;
     a.rest[at] = rest;
     if (soft) a.norm[at] = norm;
+    if (a.grads & 2) {        // (their order is of no account: who reads them sorts)
+        const int key = a.target[at] % (int)a.rows_pad;
+        a.next[at] = atomicExch(a.first + key, at);
+        atomicAdd(a.links + key, 1);
+    }
     a.losses[a.source[at]] = loss;
     a.lse[a.source[at]] = logit + loss;
 }
@@ -1156,7 +1216,8 @@ __device__ __forceinline__ float vl_upstream(const float* g, long long stride, l
     return g == nullptr ? 0.f : g[row * stride];
 }
 
-// One CTA: per row that takes part (b + c, b, c) over the power of two above the largest |b|, |c|, times VL_P_SCALE. (A
+// One CTA: per row that takes part (b + c, b, c) over the power of two above the largest |b|, |c|, times VL_P_SCALE, and what
+// the target's dl of that size loses in 16 bits. (A
 // row far below the largest keeps its digits down to 2^-27 of it, and adds nothing that the others' rounding would not
 // cover below.)
 __global__ void __launch_bounds__(1024)
@@ -1182,7 +1243,9 @@ vl_coef_kernel(const VocabLossArgs a) {
     for (int at = threadIdx.x; at < rows; at += 1024) {
         const long long row = a.source[at];
         const float b = vl_upstream(a.d_losses, a.d_losses_stride, row), c = vl_upstream(a.d_lse, a.d_lse_stride, row);
-        a.coef[at] = make_float4((b + c) * inv, b * inv, c * inv, 0.f);
+        const float rest = a.rest[at], hit = vl_hit(b * inv, c * inv, rest);
+        const float there = a.bf16 ? __bfloat162float(__float2bfloat16_rn(hit)) : __half2float(__float2half_rn(hit));
+        a.coef[at] = make_float4((b + c) * inv, b * inv, c * inv, hit - there);
     }
     if (threadIdx.x == 0) *a.weight_scale = power / VL_P_SCALE;
 }
@@ -1199,7 +1262,7 @@ vl_hidden_kernel(const VocabLossArgs a) {
         uint4 out = make_uint4(0u, 0u, 0u, 0u);
         if (at >= 0) {
             const float b = vl_upstream(a.d_losses, a.d_losses_stride, row), z = vl_upstream(a.d_lse, a.d_lse_stride, row);
-            const float rest = a.rest[at], mean = (b + z) * a.norm[at], hit = z * (1.f - rest) - b * rest;
+            const float rest = a.rest[at], mean = (b + z) * a.norm[at], hit = vl_hit(b, z, rest);
             const float4* u = reinterpret_cast<const float4*>(a.sums + (long long)at * a.hidden) + 2 * c;
             const float4 x = u[0], y = u[1];
             const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.weight) + (long long)a.target[at] * a.ld_w) + c);
@@ -1238,7 +1301,7 @@ static VlRoom vl_room(long long rows, long long vocab) {
 
 // What the forward keeps for the backward.
 struct VlKept {
-    size_t count, place, source, target, lse, rest, norm, sums, gathered, bytes;
+    size_t count, place, source, target, lse, rest, norm, links, first, next, sums, gathered, bytes;
 };
 static VlKept vl_kept(long long rows, long long hidden, int grads) {
     VlKept k = {};
@@ -1252,6 +1315,11 @@ static VlKept vl_kept(long long rows, long long hidden, int grads) {
     k.lse = take(pad * 4);
     k.rest = take(pad * 4);
     k.norm = take(pad * 4);
+    if (grads & 2) {
+        k.links = take(pad * 4);
+        k.first = take(pad * 4);
+        k.next = take(pad * 4);
+    }
     if (grads & 1) k.sums = take(pad * (size_t)hidden * 4);
     k.gathered = at;                       // last: without a gradient of the weight it is scratch of the forward
     if (grads & 2) take(pad * (size_t)hidden * 2);
@@ -1365,6 +1433,9 @@ static void vl_use_kept(VocabLossArgs& a) {
     a.lse_rows = reinterpret_cast<float*>(base + k.lse);
     a.rest = reinterpret_cast<float*>(base + k.rest);
     a.norm = reinterpret_cast<float*>(base + k.norm);
+    a.links = reinterpret_cast<int*>(base + k.links);
+    a.first = reinterpret_cast<int*>(base + k.first);
+    a.next = reinterpret_cast<int*>(base + k.next);
     a.sums = reinterpret_cast<float*>(base + k.sums);
     a.gathered = base + k.gathered;
     a.rows_pad = vl_rows_pad(a.rows);
@@ -1379,7 +1450,7 @@ static VlSweepParams vl_sweep_params(const VocabLossArgs& a, const VlCounters& c
     p.ticket = counters + c.ticket; p.written = counters + c.written; p.read = counters + c.read; p.added = counters + c.added;
     p.pitch = c.pitch;
     p.parts = a.parts; p.refs = a.refs; p.flags = a.flags; p.list = a.list; p.again = sweep;
-    p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
+    p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef; p.links = a.links; p.first = a.first; p.next = a.next; p.gathered = a.gathered; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
     return p;
 }
 

@@ -26,8 +26,8 @@ def make(rows, vocab, hidden, dtype, seed=0, spread=1.5, lift=True, ignored=0.0)
     return h.to(dtype), w.to(dtype), t
 
 
-def exact(h, w, t, b=None, c=None):
-    """losses, lse, and from b = dL/d loss and c = dL/d lse the gradients, each with a bound on what the arithmetic may add."""
+def exact(h, w, t, b=None, c=None, whole=False):
+    """losses, lse, and from b = dL/d loss and c = dL/d lse the gradients, each with a bound on what the arithmetic may add (`whole`: dW without what the target's dl loses in 16 bits)."""
     valid = (t >= 0) & (t < w.shape[0])
     h64, w64 = torch.where(valid[:, None], h.double(), 0.0), w.double()
     hidden, half = h.shape[1], torch.finfo(h.dtype).eps / 2
@@ -53,6 +53,8 @@ def exact(h, w, t, b=None, c=None):
     # (rows whose factor is far below the largest are scaled down before the sum over rows)
     top = torch.maximum(b.abs(), c.abs()).max() if len(t) else 0.0
     low = 2.0 ** -25 * 4 * top if h.dtype == torch.float16 else 0.0
+    if whole:
+        off = off - hot * size * half
     dw_off = off.t() @ h64.abs() + (len(t) + 1) * UNIT * (size.t() @ h64.abs()) + low * (size.t() / top.clamp(min=1e-30)).sum(1, keepdim=True)
     out["d_hidden"] = (dh, dh_off + half * (dh.abs() + dh_off) + sub)
     out["d_weight"] = (dw, dw_off + half * (dw.abs() + dw_off) + sub)
@@ -372,6 +374,17 @@ def test_without_gradients_and_nan(cuda_lib):
     with torch.no_grad():
         losses, lse = vocab_cross_entropy(h, w, t)
         check({"losses": losses, "lse": lse}, exact(h, w, t))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 300), (40, 900), (150, 300)])
+def test_targets_rows_of_the_heads_gradient(cuda_lib, dtype, rows, vocab):
+    """Up to four rows to a word: what their dl lose in 16 bits is not lost. Rows that want little (p of the target near zero)
+    leave the target's as the largest by far, so that it would show."""
+    h, w, _ = make(rows, vocab, 128, dtype, 22, spread=1.0, lift=False)
+    t = (torch.arange(rows, device="cuda") % 60) * 5 + (torch.arange(rows, device="cuda") // 60)
+    b, c = factors(rows)
+    check(run(h, w, t, b, 0 * c), exact(h, w, t, b, 0 * c, whole=True))
 
 
 @pytest.mark.parametrize("rows,grad", [(5, False), (70, False), (70, True)])
