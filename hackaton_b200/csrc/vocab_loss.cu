@@ -1150,9 +1150,9 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     if (lane != 0 || at >= rows) return;
     const float logit = a.target_logit[at], logit2 = logit * VL_LOG2E;
     if (PROBE) {
-        // (fmaxf leaves out a NaN; within what a float keeps whole numbers of)
-        const float ref = fmaxf(fmaxf(x.x - VL_BELOW, logit2 - VL_BELOW_TARGET), -1.0e6f);
-        a.refs[at] = floorf(fminf(ref, 1.0e6f));
+        // (fmaxf leaves out a NaN; where there is nothing finite to go by, any number will do)
+        const float ref = fmaxf(x.x - VL_BELOW, logit2 - VL_BELOW_TARGET);
+        a.refs[at] = fabsf(ref) < 1.0e29f ? floorf(ref) : 0.f;
         return;
     }
     const float d = x.x - logit2;      // log2 of what the others' sum is relative to, over the target's
@@ -1523,9 +1523,11 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, 0);
         if (e != cudaSuccess) { *why = "references"; return e; }
         const long long units = row_tiles * (p.word_tiles + vl_div_up(p.hidden, VL_TILE));
-        for (int sweep = 0; sweep < 2 && e == cudaSuccess; ++sweep) {
+        // (no row outgrows a reference that all words were asked for)
+        const bool sure = p.word_tiles <= VL_PROBE_TILES;
+        for (int sweep = 0; sweep < (sure ? 1 : 2) && e == cudaSuccess; ++sweep) {
             e = vl_launch(vl_sweep_kernel<false>, VL_SWEEP_THREADS, VL_SWEEP_SMEM, maps, vl_sweep_params(a, counters, sweep), units, a.sm_count, stream);
-            if (sweep == 0 && e == cudaSuccess)
+            if (!sure && sweep == 0 && e == cudaSuccess)
                 e = launch_pdl(vl_again_kernel, dim3((unsigned)row_tiles), dim3(VL_TILE), 0, stream, a, p.word_tiles);
         }
     }

@@ -244,6 +244,22 @@ def test_large_logits(cuda_lib):
     assert all(v.isfinite().all() for v in got.values())
 
 
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("vocab", [900, 5000])
+def test_logits_of_millions(cuda_lib, vocab, sign):
+    """References far from zero on either side, over a vocabulary that is asked for them as a whole and one that is not."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    h = sign * (100 + torch.rand(70, 512, device="cuda", generator=g)).half()
+    w = (100 + 0.01 * torch.randint(0, 3, (vocab, 512), device="cuda", generator=g)).half()
+    t = torch.randint(0, vocab, (70,), device="cuda", generator=g)
+    b, c = factors(70)
+    got = run(h, w, t, b, c)
+    want = exact(h, w, t, b, c)
+    for name in ("losses", "lse"):
+        assert ((got[name].double() - want[name][0]).abs() <= want[name][1] * 1.001).all()
+    assert all(v.isfinite().all() for v in got.values())
+
+
 def test_nan_and_infinity_show(cuda_lib):
     h, w, t = make(300, 600, 64, torch.float16, 11)
     b, c = factors(300)
