@@ -204,30 +204,11 @@ __device__ __forceinline__ void vl_leave_out(uint32_t (&r)[32], int words, int t
         if (e >= words || e == target) r[e] = __float_as_uint(VL_NEG);
 }
 
-// Arrival and wait that order memory over the cluster (tickets are written by the pair's other CTA).
-__device__ __forceinline__ void vl_mbar_arrive_release(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ bool vl_mbar_wait_acquire(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    unsigned long long t0 = 0;
-    for (;;) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t"
-            ".reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t"
-            "}\n"
-            : "=r"(done) : "r"(bar), "r"(parity), "r"(TRY_WAIT_HINT_NS) : "memory");
-        if (done) return true;
-        const unsigned long long now = globaltimer_ns();
-        if (t0 == 0) t0 = now;
-        if (*abort_flag) return false;
-        if (now - t0 > WAIT_TIMEOUT_NS) {
-            *abort_flag = 1;
-            return false;
-        }
-    }
+// A word to a CTA of the cluster, its arrival and its bytes counted by a barrier there.
+__device__ __forceinline__ void vl_send(uint32_t cluster_addr, int value, uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], 4;" ::"r"(cluster_bar) : "memory");
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                 ::"r"(cluster_addr), "r"(value), "r"(cluster_bar) : "memory");
 }
 
 __device__ __forceinline__ float2 vl_two(uint32_t w, int bf16) {
@@ -588,14 +569,21 @@ __device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const V
     return r;
 }
 
-// Bounded wait for a counter in memory. What its writers wrote before is visible behind it, to TMA too.
-__device__ __forceinline__ bool vl_wait_count(const int* counter, int least, volatile int* abort_flag) {
+__device__ __forceinline__ int vl_counted(const int* counter) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
+    return v;
+}
+
+// Bounded wait for a counter in memory. What its writers wrote before is visible behind it, to TMA too. `before`: done
+// once, before there is anything to wait for.
+template <typename F>
+__device__ __forceinline__ bool vl_wait_count(const int* counter, int least, volatile int* abort_flag, F before) {
     if (least <= 0) return true;
     unsigned long long t0 = 0;
     for (;;) {
-        int v;
-        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
-        if (v >= least) break;
+        if (vl_counted(counter) >= least) break;
+        if (t0 == 0) before();
         const unsigned long long now = globaltimer_ns();
         if (t0 == 0) t0 = now;
         if (*abort_flag) return false;
@@ -695,11 +683,11 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
     uint32_t drawn = 0;
     auto next_ticket = [&](bool whole_warp) -> int {
         const int k = (int)(drawn % VL_TICKETS);
-        if (!vl_mbar_wait_acquire(bar_drawn(k), (drawn / VL_TICKETS) & 1u, abort_flag)) { fail = 9; return -1; }
+        if (!mbar_wait(bar_drawn(k), (drawn / VL_TICKETS) & 1u, abort_flag)) { fail = 9; return -1; }
         int t;
         asm volatile("ld.shared.s32 %0, [%1];" : "=r"(t) : "r"(tickets + 4u * k) : "memory");
-        if (whole_warp) __syncwarp();
-        if (!whole_warp || lane == 0) vl_mbar_arrive_release(lead_taken0 + 8u * k);
+        if (whole_warp) t = __shfl_sync(0xffffffffu, t, 0);       // (all have read it)
+        if (!whole_warp || lane == 0) mbar_arrive_cluster(lead_taken0 + 8u * k);
         ++drawn;
         return t;
     };
@@ -712,7 +700,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                 const int in_buffer = w.piece % VL_BUFFERS * buffer_rows, v0 = w.piece * list.tiles * VL_TILE;
                 if (w.q) {     // the piece has to be there
                     const int least = 2 * VL_EPI_WARPS * (BWD ? list.active : w.tiles);
-                    if (!vl_wait_count(p.written + w.piece * p.pitch + w.slot, least, abort_flag)) { fail = 10; break; }
+                    if (!vl_wait_count(p.written + w.piece * p.pitch + w.slot, least, abort_flag, [] {})) { fail = 10; break; }
                 }
                 const int am = (w.q && BWD ? w.slot : w.mt) * VL_TILE + (int)rank * 128, bn = w.nt * VL_TILE + (int)rank * 128;
                 for (int it = 0; it < w.steps; ++it, ++g) {
@@ -775,17 +763,14 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
     } else if (warp == VL_EPI_WARPS + 2) {
         // ------------------------------------------------------------------ draws the pair's tickets
         if (lane == 0 && rank == 0) {
-            const uint32_t peer_tickets = mapa_shared(tickets, 1u), peer_drawn0 = mapa_shared(bar_drawn(0), 1u);
-            const uint32_t own_drawn0 = mapa_shared(bar_drawn(0), 0u);
+            const uint32_t tickets0[2] = {mapa_shared(tickets, 0u), mapa_shared(tickets, 1u)};
+            const uint32_t drawn0[2] = {mapa_shared(bar_drawn(0), 0u), mapa_shared(bar_drawn(0), 1u)};
             for (uint32_t n = 0;; ++n) {
                 const int k = (int)(n % VL_TICKETS);
-                if (!vl_mbar_wait_acquire(bar_taken(k), ((n / VL_TICKETS) & 1u) ^ 1u, abort_flag)) { fail = 11; break; }
+                if (!mbar_wait_cluster(bar_taken(k), ((n / VL_TICKETS) & 1u) ^ 1u, abort_flag)) { fail = 11; break; }
                 int t = atomicAdd(p.ticket, 1);
                 if (t >= list.total) t = -1;
-                asm volatile("st.shared.s32 [%0], %1;" ::"r"(tickets + 4u * k), "r"(t) : "memory");
-                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(peer_tickets + 4u * k), "r"(t) : "memory");
-                vl_mbar_arrive_release(own_drawn0 + 8u * k);
-                vl_mbar_arrive_release(peer_drawn0 + 8u * k);
+                for (int c = 0; c < 2; ++c) vl_send(tickets0[c] + 4u * k, t, drawn0[c] + 8u * k);
                 if (t < 0) break;
             }
         }
@@ -818,11 +803,23 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                 box_put((c & 32) / 8 + i, vl_pack(v[8 * i], v[8 * i + 1], p.bf16), vl_pack(v[8 * i + 2], v[8 * i + 3], p.bf16),
                         vl_pack(v[8 * i + 4], v[8 * i + 5], p.bf16), vl_pack(v[8 * i + 6], v[8 * i + 7], p.bf16));
         };
+        // A unit's stores are counted once they are done, which takes a microsecond: not waited for where the next
+        // tile is there already, but before anything that could have to wait for what they lead to.
+        int* owed = nullptr;       // the counter
+        auto settle = [&]() {
+            if (lane == 0 && owed != nullptr) {
+                bulk_wait();
+                vl_count(owed);
+            }
+            owed = nullptr;
+        };
         // Lane 0 waits for a counter, everybody for lane 0.
         auto wait_count = [&](const int* counter, int least) -> bool {
             int ok = 1;
-            if (lane == 0) ok = vl_wait_count(counter, least, abort_flag) ? 1 : 0;
-            return __shfl_sync(0xffffffffu, ok, 0) != 0;
+            if (lane == 0) ok = vl_wait_count(counter, least, abort_flag, settle) ? (owed == nullptr ? 3 : 1) : 0;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (ok & 2) owed = nullptr;
+            return ok != 0;
         };
         uint32_t n = 0;
         for (int t; !fail && (t = next_ticket(true)) >= 0;) {
@@ -837,6 +834,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                         static_cast<unsigned short*>(p.d_weight)[(long long)(v0 + row) * p.hidden + c] = 0;
                 continue;
             }
+            if (owed != nullptr && (w.q || !__all_sync(0xffffffffu, mbar_test(bar_done(n & 1u), (n >> 1) & 1u)))) settle();
             float acc[128];
 #pragma unroll
             for (int e = 0; e < 128; ++e) acc[e] = 0.f;
@@ -939,6 +937,13 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     if ((c & 32) == 0) box_begin();
                     put16(v, c);
                     if ((c & 32) != 0) box_end(&maps.piece_out, 0, piece_row + ((col0 + c) >> 6) * rows_dev, false);
+                    if (c == 32 && owed != nullptr) {
+                        if (lane == 0) {
+                            bulk_wait_but<1>();
+                            vl_count(owed);
+                        }
+                        owed = nullptr;
+                    }
                 }
             } else {
 #pragma unroll 1
@@ -993,11 +998,10 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     p.flags[1 + w.mt] = 1;
                 }
             }
-            if (lane == 0 && (!w.q || !BWD)) {      // (backward's Q writes what nobody waits for)
-                bulk_wait();
-                vl_count(w.q ? p.added + w.mt * list.feature_tiles + w.nt : p.written + w.piece * p.pitch + w.slot);
-            }
+            if (!w.q || !BWD)       // (backward's Q writes what nobody waits for)
+                owed = w.q ? p.added + w.mt * list.feature_tiles + w.nt : p.written + w.piece * p.pitch + w.slot;
         }
+        settle();
         if (lane == 0) bulk_wait();
     }
 
