@@ -329,7 +329,7 @@ struct VocabLossArgs {
     int* flags;
     int* list;
     void* piece;
-    int capacity;
+    long long piece_units;       // tiles of 256 x 256 that there is room for
     float4* coef;
     float* weight_scale;
 };

@@ -26,8 +26,7 @@
 // each unit waiting, with counters in memory, for what it reads or overwrites; all of that has smaller tickets, which
 // running CTAs have drawn, so that nothing depends on how many CTAs are resident. (As a launch per piece and product, a
 // pair idled 11 of 66 us per launch.) The 16-bit piece is laid out in blocks of [rows][64 words], which is how TMA reads
-// it along either side; four pieces are in the works at a time, their size chosen on the device for the rows there are,
-// so that they and their words stay in L2. Measured, 151,936 words x 1536, mean of a hundred in a row (the chip at its
+// it along either side; a few pieces are in the works at a time, their size chosen on the device for the rows there are. Measured, 151,936 words x 1536, mean of a hundred in a row (the chip at its
 // power limit, 1.1 to 1.2 GHz): U and the sums for 2048 rows 1654 us (1156 TFLOP/s), for 1229 rows 1055 us (1087), dW of
 // 1229 rows 1027 us (1117).
 // Nothing is added in an order that depends on timing: U's tiles take the pieces' products one after the other.
@@ -50,14 +49,17 @@ constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 
 constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
-// A piece: at most VL_PIECE_TILES tiles of words and VL_PIECE_UNITS tiles of 256 x 256 (17 MB), at least
-// VL_PIECE_LEAST tiles of words up to VL_PIECE_MOST tiles (a piece is read once per 256 features and written once, so L2 is a
-// help, not a need; four pieces of that size are 1 GB), and one behind that. Its product comes VL_LAG pieces behind its logits in the list, so that
-// what a unit waits for was drawn at least a piece earlier, not a moment ago by a pair that is still at it. With 1229 rows
-// (5 row tiles, 80 units of logits to a piece) U takes 1055 us; with a lag of one and pieces of 24 word tiles 1157, of
-// four drawn tickets to a pair in place of two 1191. Larger pieces gain nothing (256 units: 1038 us, dW 1043 for 1027).
-constexpr int VL_PIECE_UNITS = 128, VL_PIECE_TILES = 16, VL_PIECE_LEAST = 8, VL_PIECE_MOST = 2048;
-constexpr int VL_LAG = 2, VL_BUFFERS = VL_LAG + 2;
+// Pieces (vl_shape). Forward as large as VL_PIECE_UNITS tiles of 256 x 256 allow (67 MB): each adds to all of U, which costs
+// more than a piece that leaves L2. (U of 2048 rows, 151,936 words x 1536, the mean of 500 in a row: 75 pieces 1674 us, 38
+// pieces, three of which fill L2, 1745, 10 pieces 1651, 5 of twice the size 1627.) Few row tiles: a piece for every second
+// product unit of a pair, or pairs go without. The backward's product is written, not added: small pieces that stay in L2
+// (1229 rows: 8 tiles of words 1030 us, 16 1053, 64 1069). With many rows at least VL_PIECE_LEAST tiles of words
+// up to VL_PIECE_MOST tiles (a gigabyte of scratch), one behind that.
+// A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD units lie between: what a unit
+// waits for was drawn well before it, not a moment ago by a pair that is still at it (1229 rows, 80 units of logits to a
+// piece: one piece behind 1201 us, two 1107).
+constexpr int VL_PIECE_UNITS = 512, VL_PIECE_TILES = 64, VL_BWD_TILES = 8, VL_PIECE_LEAST = 8, VL_PIECE_MOST = 2048;
+constexpr int VL_AHEAD = 148, VL_MOST_LAG = 24;
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
@@ -122,7 +124,6 @@ struct VlSweepParams {
     int bf16;
     int vocab, hidden;
     int word_tiles;
-    int capacity;            // tiles that a piece may have
     long long rows_pad;
     const int* target;
     void* piece;             // [buffer][block of 64 words][rows of the tiles][64]
@@ -153,11 +154,31 @@ struct VlSweepParams {
 
 __host__ __device__ inline int vl_div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Tiles of words in a piece for so many row tiles.
-__host__ __device__ inline int vl_piece_tiles(int row_tiles, int word_tiles, int capacity) {
-    int t = capacity / (row_tiles > 0 ? row_tiles : 1);
-    if (t > VL_PIECE_TILES) t = VL_PIECE_TILES;
-    return t < word_tiles ? t : word_tiles;
+struct VlShape {
+    int tiles, pieces, lag, buffers;      // tiles of words in a piece; pieces that have a buffer at a time
+};
+__host__ __device__ inline VlShape vl_shape(int row_tiles, int word_tiles, int feature_tiles, bool backward) {
+    VlShape s;
+    const int a = row_tiles > 0 ? row_tiles : 1;
+    int least = VL_PIECE_MOST / a;
+    if (least > VL_PIECE_LEAST) least = VL_PIECE_LEAST;
+    if (least < 1) least = 1;
+    long long t = VL_BWD_TILES;
+    if (!backward) {
+        t = (long long)word_tiles * a * feature_tiles / VL_AHEAD;
+        if (t > VL_PIECE_TILES) t = VL_PIECE_TILES;
+    }
+    if (t > VL_PIECE_UNITS / a) t = VL_PIECE_UNITS / a;
+    if (t < least) t = least;
+    if (t > word_tiles) t = word_tiles;
+    s.tiles = (int)t;
+    s.pieces = vl_div_up(word_tiles, s.tiles);
+    const long long units = (long long)a * s.tiles + (long long)(backward ? s.tiles : a) * feature_tiles;
+    s.lag = units >= VL_AHEAD ? 1 : vl_div_up(VL_AHEAD, (int)units);
+    if (s.lag > VL_MOST_LAG) s.lag = VL_MOST_LAG;
+    if (s.lag > s.pieces) s.lag = s.pieces;
+    s.buffers = s.lag + 2 < s.pieces ? s.lag + 2 : s.pieces;
+    return s;
 }
 
 __device__ __forceinline__ float vl_ex2(float x) {
@@ -511,7 +532,7 @@ struct VlUnit {
 };
 
 struct VlList {          // the list of units
-    int rows, row_tiles, active, feature_tiles, tiles, pieces, last_tiles, p, q, p_last, q_last, total;
+    int rows, row_tiles, active, feature_tiles, tiles, pieces, lag, buffers, last_tiles, p, q, p_last, q_last, total;
 };
 
 template <bool BWD>
@@ -521,8 +542,11 @@ __device__ __forceinline__ VlList vl_list(const VlSweepParams& p) {
     w.row_tiles = vl_div_up(w.rows, VL_TILE);
     w.active = p.again ? p.list[0] : w.row_tiles;
     w.feature_tiles = vl_div_up(p.hidden, VL_TILE);
-    w.tiles = vl_piece_tiles(w.row_tiles, p.word_tiles, p.capacity);
-    w.pieces = vl_div_up(p.word_tiles, w.tiles);
+    const VlShape s = vl_shape(w.row_tiles, p.word_tiles, w.feature_tiles, BWD);
+    w.tiles = s.tiles;
+    w.pieces = s.pieces;
+    w.lag = s.lag;
+    w.buffers = s.buffers;
     w.last_tiles = p.word_tiles - (w.pieces - 1) * w.tiles;
     w.p = w.active * w.tiles;
     w.p_last = w.active * w.last_tiles;
@@ -535,8 +559,8 @@ __device__ __forceinline__ VlList vl_list(const VlSweepParams& p) {
 template <bool BWD>
 __device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const VlList& w) {
     VlUnit r;
-    const int p_units = max(w.p, 1), lead = min(VL_LAG, w.pieces);      // pieces of which only the logits come first
-    const int head = w.pieces > VL_LAG ? VL_LAG * w.p : (w.pieces - 1) * w.p + w.p_last;
+    const int p_units = max(w.p, 1), lead = w.lag;           // pieces of which only the logits come first
+    const int head = w.pieces > w.lag ? w.lag * w.p : (w.pieces - 1) * w.p + w.p_last;
     r.q = k >= head;
     if (!r.q) {
         r.piece = min(k / p_units, lead - 1);
@@ -550,7 +574,7 @@ __device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const V
             k -= first * (w.p + w.q);
             const int ps = first == blocks - 1 ? w.p_last : w.p;
             r.q = k >= ps;
-            r.piece = first + VL_LAG;
+            r.piece = first + w.lag;
             if (r.q) k -= ps;
         }
         if (r.q) {
@@ -674,7 +698,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     const VlList list = vl_list<BWD>(p);
     const int rows = list.rows, rows_dev = list.row_tiles * VL_TILE;
-    const int buffer_rows = p.capacity * VL_TILE * (VL_TILE / 64);     // of 64 words, in one buffer
+    const int buffer_rows = list.tiles * (VL_TILE / 64) * rows_dev;     // of 64 words, in one buffer
     int fail = 0;
 
     // The next unit's ticket, or -1 behind the last; every reader takes them in turn: one lane for itself, or a warp, of
@@ -697,7 +721,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             uint32_t g = 0;
             for (int t; !fail && (t = next_ticket(false)) >= 0;) {
                 const VlUnit w = vl_unit<BWD>(t, p, list);
-                const int in_buffer = w.piece % VL_BUFFERS * buffer_rows, v0 = w.piece * list.tiles * VL_TILE;
+                const int in_buffer = w.piece % list.buffers * buffer_rows, v0 = w.piece * list.tiles * VL_TILE;
                 if (w.q) {     // the piece has to be there
                     const int least = 2 * VL_EPI_WARPS * (BWD ? list.active : w.tiles);
                     if (!vl_wait_count(p.written + w.piece * p.pitch + w.slot, least, abort_flag, [] {})) { fail = 10; break; }
@@ -885,15 +909,15 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             }
             const bool any_hit = BWD && w.q && __any_sync(0xffffffffu, hits[0] >= 0);
             // what is about to be overwritten has been read; what is about to be added to has the pieces before
-            if (!w.q && w.piece >= VL_BUFFERS &&
-                !wait_count(p.read + (w.piece - VL_BUFFERS) * p.pitch + w.slot, list.feature_tiles)) { fail = 12; break; }
+            if (!w.q && w.piece >= list.buffers &&
+                !wait_count(p.read + (w.piece - list.buffers) * p.pitch + w.slot, list.feature_tiles)) { fail = 12; break; }
             if (!BWD && w.q && !wait_count(p.added + w.mt * list.feature_tiles + w.nt, 2 * VL_EPI_WARPS * w.piece)) { fail = 13; break; }
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
             if (w.q && rank == 0 && warp == 2 && lane == 0) vl_count(p.read + w.piece * p.pitch + w.slot);
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
             float m2 = VL_NEG, sum = 0.f;
-            const int piece_row = w.piece % VL_BUFFERS * buffer_rows + row0;
+            const int piece_row = w.piece % list.buffers * buffer_rows + row0;
             auto load = [&](int c, uint32_t (&r)[32]) {        // the last chunk's makes room for the unit after the next
                 tmem_ld_32x32(at + c, r);
                 tmem_ld_wait();
@@ -1287,19 +1311,20 @@ static long long vl_rows_pad(long long rows) { return (rows + VL_TILE - 1) / VL_
 
 static int vl_word_tiles(long long vocab) { return (int)((vocab + VL_TILE - 1) / VL_TILE); }
 
-// Tiles that a piece has room for, and the most pieces that any number of rows up to `rows` makes of the vocabulary.
+// Tiles of 256 x 256 that the pieces' buffers need, and the most pieces, for any number of rows up to `rows`.
 struct VlRoom {
-    int capacity, pieces;
+    long long units;
+    int pieces;
 };
-static VlRoom vl_room(long long rows, long long vocab) {
-    const long long row_tiles = vl_rows_pad(rows) / VL_TILE;
-    const int word_tiles = vl_word_tiles(vocab);
-    VlRoom r = {VL_PIECE_UNITS, 1};
-    const long long least = VL_PIECE_LEAST * row_tiles < VL_PIECE_MOST ? VL_PIECE_LEAST * row_tiles : VL_PIECE_MOST;
-    if (r.capacity < least) r.capacity = (int)least;
-    if (r.capacity < row_tiles) r.capacity = (int)row_tiles;
-    // (more row tiles, fewer tiles of words in a piece)
-    r.pieces = vl_div_up(word_tiles, vl_piece_tiles((int)row_tiles, word_tiles, r.capacity));
+static VlRoom vl_room(long long rows, long long vocab, long long hidden, bool backward) {
+    const int row_tiles = (int)(vl_rows_pad(rows) / VL_TILE), word_tiles = vl_word_tiles(vocab);
+    VlRoom r = {0, 1};
+    for (int a = 1; a <= row_tiles; ++a) {
+        const VlShape s = vl_shape(a, word_tiles, vl_div_up((int)hidden, VL_TILE), backward);
+        const long long units = (long long)s.buffers * s.tiles * a;
+        if (units > r.units) r.units = units;
+        if (s.pieces > r.pieces) r.pieces = s.pieces;
+    }
     return r;
 }
 
@@ -1339,7 +1364,7 @@ struct VlCounters {
 static VlCounters vl_counters(const VocabLossArgs& a, const VlRoom& room, bool backward) {
     VlCounters c = {};
     const long long row_tiles = vl_rows_pad(a.rows) / VL_TILE, feature_tiles = vl_div_up((int)a.hidden, VL_TILE);
-    c.pitch = backward ? VL_PIECE_TILES : (int)row_tiles;
+    c.pitch = backward ? VL_BWD_TILES : (int)row_tiles;
     c.ticket = 0;
     c.written = 32;
     c.read = c.written + (long long)room.pieces * c.pitch;
@@ -1361,8 +1386,8 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
     const size_t pad = (size_t)vl_rows_pad(a.rows);
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t r = at; at += vl_align(n); return r; };
-    s.room = vl_room(a.rows, a.vocab);
-    const size_t piece = (size_t)VL_BUFFERS * (size_t)s.room.capacity * VL_TILE * VL_TILE * 2;
+    s.room = vl_room(a.rows, a.vocab, a.hidden, backward);
+    const size_t piece = (size_t)s.room.units * VL_TILE * VL_TILE * 2;
     const size_t counters = (size_t)vl_counters(a, s.room, backward).total * 4;
     if (!backward) {
         const size_t n_parts = (size_t)vl_word_tiles(a.vocab) * 2, few_parts = (size_t)a.sm_count * 4;
@@ -1424,7 +1449,7 @@ static bool vl_map(CUtensorMap* map, int bf16, const void* base, long long inner
 
 // The 16-bit pieces: blocks of [rows][64 words], read in boxes of 128 rows (rows as M) or 64 (as steps), written in 32.
 static bool vl_piece_map(CUtensorMap* map, const VocabLossArgs& a, int box_outer) {
-    return vl_map(map, a.bf16, a.piece, VL_BK, (long long)VL_BUFFERS * a.capacity * VL_TILE * (VL_TILE / VL_BK), VL_BK, box_outer);
+    return vl_map(map, a.bf16, a.piece, VL_BK, a.piece_units * VL_TILE * (VL_TILE / VL_BK), VL_BK, box_outer);
 }
 
 static void vl_use_kept(VocabLossArgs& a) {
@@ -1449,7 +1474,7 @@ static VlSweepParams vl_sweep_params(const VocabLossArgs& a, const VlCounters& c
     VlSweepParams p = {};
     p.count = a.count; p.status = a.status; p.bf16 = a.bf16;
     p.vocab = (int)a.vocab; p.hidden = (int)a.hidden; p.word_tiles = vl_word_tiles(a.vocab);
-    p.capacity = a.capacity; p.rows_pad = a.rows_pad; p.target = a.target; p.piece = a.piece;
+    p.rows_pad = a.rows_pad; p.target = a.target; p.piece = a.piece;
     int* counters = a.counters + sweep * c.each;
     p.ticket = counters + c.ticket; p.written = counters + c.written; p.read = counters + c.read; p.added = counters + c.added;
     p.pitch = c.pitch;
@@ -1479,7 +1504,7 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         a.flags = a.counters + counters.flags;
         a.list = a.counters + counters.list;
         a.piece = ws + s.piece;
-        a.capacity = s.room.capacity;
+        a.piece_units = s.room.units;
     }
     const int per = a.rows <= 512 ? 2 : a.rows <= 4096 ? 8 : 32;     // rows of a CTA (64 x 3584: a row to a warp 11.5 us, to four 5.7)
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
@@ -1560,7 +1585,7 @@ cudaError_t launch_vocab_loss_bwd(const VocabLossArgs& a_in, cudaStream_t stream
     a.counters = reinterpret_cast<int*>(ws + s.counters);
     a.n_counters = counters.total;
     a.piece = ws + s.piece;
-    a.capacity = s.room.capacity;
+    a.piece_units = s.room.units;
     e = launch_pdl(vl_coef_kernel, dim3(1), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) { *why = "row factors"; return e; }
     VlSweepMaps maps = {};
