@@ -51,15 +51,17 @@ constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
 // Pieces (vl_shape). Forward as large as VL_PIECE_UNITS tiles of 256 x 256 allow (67 MB): each adds to all of U, which costs
 // more than a piece that leaves L2. (U of 2048 rows, 151,936 words x 1536, the mean of 500 in a row: 75 pieces 1674 us, 38
-// pieces, three of which fill L2, 1745, 10 pieces 1651, 5 of twice the size 1627.) Few row tiles: a piece for every second
-// product unit of a pair, or pairs go without. The backward's product is written, not added: small pieces that stay in L2
+// pieces, three of which fill L2, 1745, 10 pieces 1651, 5 of twice the size 1627.) Few row tiles: pieces so small that
+// there are VL_PRODUCTS units of the product, two for each of 74 pairs (256 rows: 24 tiles of words 320 us, 8 671, 64 366). The backward's product is written, not added: small pieces that stay in L2
 // (1229 rows: 8 tiles of words 1030 us, 16 1053, 64 1069). With many rows at least VL_PIECE_LEAST tiles of words
 // up to VL_PIECE_MOST tiles (a gigabyte of scratch), one behind that.
 // A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD units lie between: what a unit
 // waits for was drawn well before it, not a moment ago by a pair that is still at it (1229 rows, 80 units of logits to a
-// piece: one piece behind 1201 us, two 1107).
+// piece: one piece behind 1201 us, two 1107; dW of 256 rows, 56 units to a piece: three behind 347, six 300; of 1229, 88
+// units: two 1030, three 1038).
 constexpr int VL_PIECE_UNITS = 512, VL_PIECE_TILES = 64, VL_BWD_TILES = 8, VL_PIECE_LEAST = 8, VL_PIECE_MOST = 2048;
-constexpr int VL_AHEAD = 148, VL_MOST_LAG = 24;
+constexpr int VL_AHEAD = 222, VL_MOST_LAG = 24;      // (three units for each of 74 pairs)
+constexpr int VL_PRODUCTS = 148;
 
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
@@ -165,7 +167,7 @@ __host__ __device__ inline VlShape vl_shape(int row_tiles, int word_tiles, int f
     if (least < 1) least = 1;
     long long t = VL_BWD_TILES;
     if (!backward) {
-        t = (long long)word_tiles * a * feature_tiles / VL_AHEAD;
+        t = (long long)word_tiles * a * feature_tiles / VL_PRODUCTS;
         if (t > VL_PIECE_TILES) t = VL_PIECE_TILES;
     }
     if (t > VL_PIECE_UNITS / a) t = VL_PIECE_UNITS / a;
