@@ -23,12 +23,13 @@
 // Operands come by TMA in 64-deep steps through a ring of six. A sweep is one kernel (vl_sweep_kernel): first logits, then
 // the product with the 16-bit piece, as units of one list that the pairs draw tickets from,
 //     P(0) P(1)  P(2) Q(0)  P(3) Q(1)  ...  Q(last)     P(i): logits tiles of piece i, Q(i): tiles of the product with it
-// each unit waiting, with counters in memory, for what it reads or overwrites; all of that has smaller tickets, which
-// running CTAs have drawn, so that nothing depends on how many CTAs are resident. (As a launch per piece and product, a
-// pair idled 11 of 66 us per launch.) The 16-bit piece is laid out in blocks of [rows][64 words], which is how TMA reads
-// it along either side; a few pieces are in the works at a time, their size chosen on the device for the rows there are. Measured, 151,936 words x 1536, mean of a hundred in a row (the chip at its
-// power limit, 1.1 to 1.2 GHz): U and the sums for 2048 rows 1654 us (1156 TFLOP/s), for 1229 rows 1055 us (1087), dW of
-// 1229 rows 1027 us (1117).
+// (here two pieces behind), each unit waiting, with counters in memory, for what it reads or overwrites; all of that has
+// smaller tickets, which running CTAs have drawn, so that nothing depends on how many CTAs are resident. (As a launch per
+// piece and product, a pair idled 11 of 66 us per launch. Tickets handed on with fences of cluster scope cost the thread
+// that issues the products 2300 of 21,400 cycles a unit; as asynchronous stores that a barrier counts, 200.) The 16-bit
+// piece is laid out in blocks of [rows][64 words], which is how TMA reads it along either side. Measured, 151,936 words x
+// 1536, mean of 500 in a row (the chip at its power limit, 1.1 to 1.2 GHz): U and the sums for 2048 rows 1651 us
+// (1158 TFLOP/s), for 1229 rows 1088 us (1054), dW of 1229 rows 1038 us (1105); a library's product of 8192^3 then 1340.
 // Nothing is added in an order that depends on timing: U's tiles take the pieces' products one after the other.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -52,9 +53,10 @@ constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference 
 // Pieces (vl_shape). Forward as large as VL_PIECE_UNITS tiles of 256 x 256 allow (67 MB): each adds to all of U, which costs
 // more than a piece that leaves L2. (U of 2048 rows, 151,936 words x 1536, the mean of 500 in a row: 75 pieces 1674 us, 38
 // pieces, three of which fill L2, 1745, 10 pieces 1651, 5 of twice the size 1627.) Few row tiles: pieces so small that
-// there are VL_PRODUCTS units of the product, two for each of 74 pairs (256 rows: 24 tiles of words 320 us, 8 671, 64 366). The backward's product is written, not added: small pieces that stay in L2
-// (1229 rows: 8 tiles of words 1030 us, 16 1053, 64 1069). With many rows at least VL_PIECE_LEAST tiles of words
-// up to VL_PIECE_MOST tiles (a gigabyte of scratch), one behind that.
+// there are VL_PRODUCTS units of the product, two for each of 74 pairs (256 rows: 24 tiles of words 320 us, 8 671, 64
+// 366). The backward's product is written, not added: small pieces that stay in L2 (1229 rows: 8 tiles of words 1030 us, 16
+// 1053, 64 1069). With many rows at least VL_PIECE_LEAST tiles of words up to VL_PIECE_MOST tiles (a gigabyte of scratch),
+// one behind that.
 // A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD units lie between: what a unit
 // waits for was drawn well before it, not a moment ago by a pair that is still at it (1229 rows, 80 units of logits to a
 // piece: one piece behind 1201 us, two 1107; dW of 256 rows, 56 units to a piece: three behind 347, six 300; of 1229, 88
@@ -96,7 +98,6 @@ enum VlMode {
 
 struct VlMaps {
     CUtensorMap a, b;
-    CUtensorMap a_part;      // VL_FEW: W in boxes of 16 words, for a CTA's last, part-filled tile
 };
 
 struct VlParams {
@@ -106,7 +107,8 @@ struct VlParams {
     int vocab, hidden;
     int word_tiles;          // to be looked at
     int n_rows;              // VL_FEW: columns of the accumulator, 32 or 64
-    int cta_words;           // VL_FEW: words of a CTA, one behind the other
+    int cta_tiles;           // VL_FEW: tiles of a CTA, one behind the other,
+    int tile_words;          // and the words of each, at most 128
     const int* target;       // per gathered row
     float2* parts;           // [parts][rows_pad]: maximum (base 2), sum relative to it
     long long rows_pad;
@@ -313,16 +315,15 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&maps.a);
         tma_prefetch_desc(&maps.b);
-        if (MODE == VL_FEW) tma_prefetch_desc(&maps.a_part);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
         tmem_relinquish_pair();
     }
     // The first words come to L2 while the kernel before gathers the rows.
-    if (MODE == VL_FEW && warp == 0 && lane == 0 && (int)blockIdx.x * p.cta_words < p.vocab)
-        for (int k = 0; k < L::STAGES && k * VL_BK < p.hidden; ++k)
-            tma_prefetch_2d(p.cta_words >= 128 ? &maps.a : &maps.a_part, k * VL_BK, (int)blockIdx.x * p.cta_words);
+    const int word_begin = MODE == VL_FEW ? (int)blockIdx.x * p.cta_tiles * p.tile_words : 0;
+    if (MODE == VL_FEW && warp == 0 && lane == 0 && word_begin < p.vocab)
+        for (int k = 0; k < L::STAGES && k * VL_BK < p.hidden; ++k) tma_prefetch_2d(&maps.a, k * VL_BK, word_begin);
     grid_dep_wait();
     grid_dep_launch();
     tc_fence_before_sync();
@@ -332,21 +333,18 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     const uint32_t tmem = *tmem_slot;
     const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK * DEEP);
     const int chain = MODE == VL_FEW ? vl_div_up(steps, VL_FEW_CHAINS) : vl_chain(steps);
-    // Few rows: each CTA's words one tile of 128 behind the other, and the pair's tiles are its units.
-    const int tiles = vl_div_up(p.cta_words, 128), word_begin = (int)blockIdx.x * p.cta_words, word_end = min(word_begin + p.cta_words, p.vocab);
-    const int units = rows == 0 ? 0 : MODE == VL_FEW ? (pair + 1) * tiles : row_tiles * p.word_tiles;
-    const int unit0 = MODE == VL_FEW ? pair * tiles : pair, stride = MODE == VL_FEW ? 1 : pairs;
+    // Few rows: a pair's units are its tiles.
+    const int units = rows == 0 ? 0 : MODE == VL_FEW ? (pair + 1) * p.cta_tiles : row_tiles * p.word_tiles;
+    const int unit0 = MODE == VL_FEW ? pair * p.cta_tiles : pair, stride = MODE == VL_FEW ? 1 : pairs;
     int fail = 0;
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t g = 0;
             for (int u = unit0; u < units && !fail; u += stride) {
-                const int am = MODE == VL_FEW ? word_begin + (u - unit0) * 128 : u % row_tiles * VL_TILE + (int)rank * 128;
+                const int am = MODE == VL_FEW ? word_begin + (u - unit0) * p.tile_words : u % row_tiles * VL_TILE + (int)rank * 128;
                 const int bn = MODE == VL_FEW ? (int)rank * (p.n_rows / 2) : u / row_tiles * VL_TILE + (int)rank * 128;
-                const int words = p.cta_words - (u - unit0) * 128;       // what is left
-                const bool part = MODE == VL_FEW && words < 128;
-                const int bytes = DEEP * ((part ? words * 128 : L::A_BYTES) + (MODE == VL_FEW ? p.n_rows * 64 : L::B_BYTES));
+                const int bytes = DEEP * (MODE == VL_FEW ? p.tile_words * 128 + p.n_rows * 64 : L::A_BYTES + L::B_BYTES);
                 for (int it = 0; it < steps; ++it, ++g) {
                     const int s = (int)(g % STAGES);
                     if (!mbar_wait_cluster(bar_empty(s), ((g / STAGES) & 1u) ^ 1u, abort_flag)) { fail = 1; break; }
@@ -356,9 +354,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
 #pragma unroll
                     for (int k = 0; k < DEEP; ++k) {       // (behind the features: zeros)
                         const int x = (it * DEEP + k) * VL_BK;
-                        if (!part) tma_load_2d(sa + k * L::A_BYTES, &maps.a, x, am, landed);
-                        else
-                            for (int i = 0; i < words; i += 16) tma_load_2d(sa + k * L::A_BYTES + i * 128, &maps.a_part, x, am + i, landed);
+                        tma_load_2d(sa + k * L::A_BYTES, &maps.a, x, am, landed);
                         tma_load_2d(sb + k * L::B_BYTES, &maps.b, x, bn, landed);
                     }
                 }
@@ -405,7 +401,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
         }
     } else if constexpr (MODE == VL_FEW) {
         // ------------------------------------------------------------------ epilogue: a word's values of half the rows
-        // A thread keeps maximum and sum of the words that come by its lane, for each of its 16 or 32 rows, over all tiles;
+        // (Lanes behind a tile's words hold what the ring held before.) A thread keeps maximum and sum of the words that come by its lane, for each of its 16 or 32 rows, over all tiles;
         // the lanes of a warp meet at the end.
         const int q = warp & 3, half = (warp - 2) >> 2, n = p.n_rows / 2, row0 = half * n;
         const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
@@ -418,7 +414,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             const int b = (int)(it & 1u);
             if (!mbar_wait(bar_done(b), (it >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
-            const int word0 = word_begin + (u - unit0) * 128 + q * 32;
+            const int word0 = word_begin + (u - unit0) * p.tile_words + q * 32;
             float r[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0.f;
@@ -437,7 +433,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
-            const bool there = word0 + lane < word_end;
+            const bool there = word0 + lane < p.vocab && q * 32 + lane < p.tile_words;
             const unsigned hits = __ballot_sync(0xffffffffu, (unsigned)(target - word0) < 32u);    // rows whose target is here
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -1512,15 +1508,16 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
     // Up to 64 rows without a gradient of x: the words take the tensor cores' long side. (64 rows of 3584 features against
-    // 151,936 words: with the rows there, which costs four times the products, 216 us, this way 177; the weight's 1.09 GB
-    // alone take 168. All three kernels 187.) Every CTA has as many words, in tiles of 128 and a rest, not a share of
-    // the tiles: those are 8.03 to a pair here.
+    // 151,936 words: with the rows there, which costs four times the products, 216 us; this way all three kernels take 176, the
+    // weight's 1.09 GB alone 168.) Every CTA has as many words, in tiles of one size (9 of 115 here): as shares of tiles of
+    // 128, of which there are 8.03 to a CTA, 197 us, as eight of them and a rest in boxes of 16 words 187.
     const bool few = !soft && a.rows <= 64;
     const int few_rows = a.rows <= 32 ? 32 : 64;
     VlMaps logits = {};
     VlSweepMaps maps = {};
-    bool ok = few ? vl_map(&logits.a, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128) &&
-                        vl_map(&logits.a_part, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 16) &&
+    const long long few_ctas = 2 * vl_pairs(vl_word_tiles(a.vocab), a.sm_count);
+    const int cta_tiles = vl_div_up((int)a.vocab, (int)few_ctas * 128), tile_words = vl_div_up((int)a.vocab, (int)few_ctas * cta_tiles);
+    bool ok = few ? vl_map(&logits.a, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, tile_words) &&
                         vl_map(&logits.b, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, few_rows / 2)
                   : vl_map(&logits.a, a.bf16, a.gathered, a.hidden, a.rows_pad, a.hidden, 128) &&
                         vl_map(&logits.b, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 128);
@@ -1541,10 +1538,10 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     const dim3 merge_grid((unsigned)((a.rows + VL_MERGE_ROWS - 1) / VL_MERGE_ROWS)), merge_block(VL_MERGE_ROWS, VL_MERGE_SHARES);
     int n_parts = 2 * p.word_tiles;
     if (few) {
-        const long long pairs = vl_pairs(p.word_tiles, a.sm_count);
-        p.cta_words = (int)((a.vocab + 2 * pairs * 16 - 1) / (2 * pairs * 16) * 16);
+        p.cta_tiles = cta_tiles;
+        p.tile_words = tile_words;
         e = vl_launch(vl_stats_kernel<VL_FEW>, VL_THREADS, VlSmemOf<VL_FEW>::TOTAL, logits, p, p.word_tiles, a.sm_count, stream);
-        n_parts = (int)(8 * pairs);
+        n_parts = (int)(4 * few_ctas);
     } else if (!soft) {
         e = vl_launch(vl_stats_kernel<VL_STATS>, VL_THREADS, VlSmemOf<VL_STATS>::TOTAL, logits, p, row_tiles * p.word_tiles, a.sm_count, stream);
     } else {
