@@ -70,8 +70,10 @@ constexpr int VL_BK = 64;
 // The tensor cores cut off what an addition to an accumulator leaves behind its 24 bits, always in one direction, so
 // that a logit's error grows with the length of its chain of additions. A chain of logits is at most VL_CHAIN steps of 64;
 // longer ones are cut, and the parts added in the epilogue's registers with rounding. (3584 features, losses against 64 bits: one
-// chain 1.2e-6 in norm, in two 4e-7, in four 2e-7; fp32 products and sums 1.5e-7.)
-constexpr int VL_CHAIN = 32;
+// chain 1.2e-6 in norm, chains of 32 steps 4e-7, of 8 1.2e-7; fp32 products and sums 1.5e-7.) Up to VL_CHAIN_ROWS row tiles,
+// among few rows, a single confident one's small loss shows (2 rows of 2920 features, chains of 32 3.0e-6, of 8 below 1e-6), and the
+// cuts cost nothing: at most VL_CHAIN_FEW steps. (2048 rows x 1536, U: 1725 us in one chain, 1760 in two, 1797 in three.)
+constexpr int VL_CHAIN = 32, VL_CHAIN_FEW = 8, VL_CHAIN_ROWS = 2;
 constexpr int VL_LINKS = 16;               // rows of a word (or that share its place in the table) up to which they are looked up
 constexpr int VL_FEW_CHAINS = 4;           // of at most 64 columns each: there is room for all of a tile's
 constexpr int VL_EPI_WARPS = 8;
@@ -199,7 +201,9 @@ __device__ __forceinline__ void vl_sts128(uint32_t addr, uint32_t x, uint32_t y,
 __device__ __forceinline__ float vl_hit(float b, float c, float rest) { return c * (1.f - rest) - b * rest; }
 
 // Steps of a chain where there are so many.
-__host__ __device__ inline int vl_chain(int steps) { return vl_div_up(steps, vl_div_up(steps, VL_CHAIN)); }
+__device__ __forceinline__ int vl_chain(int steps, int row_tiles) {
+    return vl_div_up(steps, vl_div_up(steps, row_tiles <= VL_CHAIN_ROWS ? VL_CHAIN_FEW : VL_CHAIN));
+}
 
 // acc += a thread's 128 columns of a chain that is not the last.
 __device__ __forceinline__ void vl_add_chain(float (&acc)[128], uint32_t at) {
@@ -332,7 +336,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK * DEEP);
-    const int chain = MODE == VL_FEW ? vl_div_up(steps, VL_FEW_CHAINS) : vl_chain(steps);
+    const int chain = MODE == VL_FEW ? vl_div_up(steps, VL_FEW_CHAINS) : vl_chain(steps, row_tiles);
     // Few rows: a pair's units are its tiles.
     const int units = rows == 0 ? 0 : MODE == VL_FEW ? (pair + 1) * p.cta_tiles : row_tiles * p.word_tiles;
     const int unit0 = MODE == VL_FEW ? pair * p.cta_tiles : pair, stride = MODE == VL_FEW ? 1 : pairs;
@@ -587,7 +591,7 @@ __device__ __forceinline__ VlUnit vl_unit(int k, const VlSweepParams& p, const V
     r.mt = r.q && BWD ? 0 : p.again ? p.list[1 + first] : first;
     r.slot = BWD ? (r.q ? first : r.nt) : first;
     r.steps = !r.q ? vl_div_up(p.hidden, VL_BK) : BWD ? vl_div_up(w.rows, VL_BK) : r.tiles * (VL_TILE / VL_BK);
-    r.chain = r.q ? r.steps : vl_chain(r.steps);
+    r.chain = r.q ? r.steps : vl_chain(r.steps, w.row_tiles);
     return r;
 }
 
