@@ -320,7 +320,7 @@ struct VocabLossArgs {
     int* links;                  // [rows_pad]: how many rows' targets are a number modulo rows_pad,
     int* first;                  // one of them, or -1,
     int* next;                   // and per row another one, or -1
-    float* sums;                 // [rows that take part, hidden]: sum of exp(l_v - reference) w_v over v other than the target
+    float* sums;                 // planes of [row tiles * 256, hidden]: sum of exp(l_v - reference) w_v over v other than the target
     void* gathered;              // the rows themselves
     float2* parts;
     float* refs;

@@ -49,23 +49,24 @@ constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 
 // target's logit less VL_BELOW_TARGET; fp16 takes what lies up to 2^15 above it, bf16 2^100.
 constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
+constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
 // Pieces (vl_shape). Forward as large as VL_PIECE_UNITS tiles of 256 x 256 allow (67 MB): each adds to all of U, which costs
 // more than a piece that leaves L2. (U of 2048 rows, 151,936 words x 1536, the mean of 500 in a row: 75 pieces 1674 us, 38
 // pieces, three of which fill L2, 1745, 10 pieces 1651, 5 of twice the size 1627.) Few row tiles: pieces so small that
-// there are VL_PRODUCTS units of the product, two for each of 74 pairs (256 rows: 24 tiles of words 320 us, 8 671, 64
-// 366). The backward's product is written, not added: small pieces that stay in L2 (1229 rows: 8 tiles of words 1030 us, 16
+// there are VL_PRODUCTS units of the product, two for each of 74 pairs (256 rows in one plane: 24 tiles of words 320 us, 8
+// 671, 64 366). The backward's product is written, not added: small pieces that stay in L2 (1229 rows: 8 tiles of words 1030 us, 16
 // 1053, 64 1069). With many rows at least VL_PIECE_LEAST tiles of words up to VL_PIECE_MOST tiles (a gigabyte of scratch),
 // one behind that.
-// A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD units lie between: what a unit
+// A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD_ units lie between: what a unit
 // waits for was drawn well before it, not a moment ago by a pair that is still at it (1229 rows, 80 units of logits to a
 // piece: one piece behind 1201 us, two 1107; dW of 256 rows, 56 units to a piece: three behind 347, six 300; of 1229, 88
-// units: two 1030, three 1038).
+// units: two 1030, three 1038; U of 256 rows, 30 units: six 304, eight 287, twelve 276).
 constexpr int VL_PIECE_UNITS = 512, VL_PIECE_TILES = 64, VL_BWD_TILES = 8, VL_PIECE_LEAST = 8, VL_PIECE_MOST = 2048;
-constexpr int VL_AHEAD = 222, VL_MOST_LAG = 24;      // (three units for each of 74 pairs)
+constexpr int VL_AHEAD_FWD = 370, VL_AHEAD_BWD = 222, VL_MOST_LAG = 24;      // (five and three units for each of 74 pairs)
 constexpr int VL_PRODUCTS = 148;
+constexpr int VL_PLANE_ROWS = 1024;
 
-constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_BK = 64;
 // The tensor cores cut off what an addition to an accumulator leaves behind its 24 bits, always in one direction, so
 // that a logit's error grows with the length of its chain of additions. A chain of logits is at most VL_CHAIN steps of 64;
@@ -160,6 +161,13 @@ struct VlSweepParams {
 
 __host__ __device__ inline int vl_div_up(int a, int b) { return (a + b - 1) / b; }
 
+// Rows that U's planes have together. Pieces add to the planes in turn, as many as there is room for: where there are few
+// row tiles, one addition behind the other, 8 us each, would be most of the time (256 rows: 341 us, with four planes 287).
+__host__ __device__ inline long long vl_plane_rows(long long rows_pad) { return rows_pad > VL_PLANE_ROWS ? rows_pad : VL_PLANE_ROWS; }
+__host__ __device__ inline int vl_planes(long long rows_pad, int row_tiles) {
+    return row_tiles > 0 ? (int)(vl_plane_rows(rows_pad) / VL_TILE / row_tiles) : 1;
+}
+
 struct VlShape {
     int tiles, pieces, lag, buffers;      // tiles of words in a piece; pieces that have a buffer at a time
 };
@@ -180,7 +188,8 @@ __host__ __device__ inline VlShape vl_shape(int row_tiles, int word_tiles, int f
     s.tiles = (int)t;
     s.pieces = vl_div_up(word_tiles, s.tiles);
     const long long units = (long long)a * s.tiles + (long long)(backward ? s.tiles : a) * feature_tiles;
-    s.lag = units >= VL_AHEAD ? 1 : vl_div_up(VL_AHEAD, (int)units);
+    const int ahead = backward ? VL_AHEAD_BWD : VL_AHEAD_FWD;
+    s.lag = units >= ahead ? 1 : vl_div_up(ahead, (int)units);
     if (s.lag > VL_MOST_LAG) s.lag = VL_MOST_LAG;
     if (s.lag > s.pieces) s.lag = s.pieces;
     s.buffers = s.lag + 2 < s.pieces ? s.lag + 2 : s.pieces;
@@ -534,7 +543,7 @@ struct VlUnit {
 };
 
 struct VlList {          // the list of units
-    int rows, row_tiles, active, feature_tiles, tiles, pieces, lag, buffers, last_tiles, p, q, p_last, q_last, total;
+    int rows, row_tiles, active, feature_tiles, tiles, pieces, lag, buffers, planes, last_tiles, p, q, p_last, q_last, total;
 };
 
 template <bool BWD>
@@ -549,6 +558,7 @@ __device__ __forceinline__ VlList vl_list(const VlSweepParams& p) {
     w.pieces = s.pieces;
     w.lag = s.lag;
     w.buffers = s.buffers;
+    w.planes = vl_planes(p.rows_pad, w.row_tiles);
     w.last_tiles = p.word_tiles - (w.pieces - 1) * w.tiles;
     w.p = w.active * w.tiles;
     w.p_last = w.active * w.last_tiles;
@@ -913,7 +923,9 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             // what is about to be overwritten has been read; what is about to be added to has the pieces before
             if (!w.q && w.piece >= list.buffers &&
                 !wait_count(p.read + (w.piece - list.buffers) * p.pitch + w.slot, list.feature_tiles)) { fail = 12; break; }
-            if (!BWD && w.q && !wait_count(p.added + w.mt * list.feature_tiles + w.nt, 2 * VL_EPI_WARPS * w.piece)) { fail = 13; break; }
+            const int plane = w.piece % list.planes;
+            int* const added = p.added + (plane * list.row_tiles + w.mt) * list.feature_tiles + w.nt;
+            if (!BWD && w.q && !wait_count(added, 2 * VL_EPI_WARPS * (w.piece / list.planes))) { fail = 13; break; }
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
             if (w.q && rank == 0 && warp == 2 && lane == 0) vl_count(p.read + w.piece * p.pitch + w.slot);
@@ -981,7 +993,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                         box_begin();
 #pragma unroll
                         for (int i = 0; i < 8; ++i) box_put(i, r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-                        box_end(&maps.out, col0 + c, row0, w.piece > 0);
+                        box_end(&maps.out, col0 + c, plane * rows_dev + row0, w.piece >= list.planes);
                     } else {
                         if (col0 + (c & 64) >= p.hidden) continue;
                         if ((c & 32) == 0) box_begin();
@@ -1025,7 +1037,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                 }
             }
             if (!w.q || !BWD)       // (backward's Q writes what nobody waits for)
-                owed = w.q ? p.added + w.mt * list.feature_tiles + w.nt : p.written + w.piece * p.pitch + w.slot;
+                owed = w.q ? added : p.written + w.piece * p.pitch + w.slot;
         }
         settle();
         if (lane == 0) bulk_wait();
@@ -1285,7 +1297,10 @@ __global__ void __launch_bounds__(256)
 vl_hidden_kernel(const VocabLossArgs a) {
     grid_dep_wait();
     grid_dep_launch();
-    const int vecs = (int)(a.hidden / 8);
+    const int vecs = (int)(a.hidden / 8), row_tiles = vl_div_up(*a.count, VL_TILE);
+    const int planes = min(vl_planes(a.rows_pad, row_tiles),
+                           vl_shape(row_tiles, vl_div_up((int)a.vocab, VL_TILE), vl_div_up((int)a.hidden, VL_TILE), false).pieces);
+    const long long plane = (long long)row_tiles * VL_TILE * a.hidden / 4;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.rows * vecs; i += (long long)gridDim.x * 256) {
         const long long row = i / vecs;
         const int c = (int)(i - row * vecs), at = a.place[row];
@@ -1294,7 +1309,12 @@ vl_hidden_kernel(const VocabLossArgs a) {
             const float b = vl_upstream(a.d_losses, a.d_losses_stride, row), z = vl_upstream(a.d_lse, a.d_lse_stride, row);
             const float rest = a.rest[at], mean = (b + z) * a.norm[at], hit = vl_hit(b, z, rest);
             const float4* u = reinterpret_cast<const float4*>(a.sums + (long long)at * a.hidden) + 2 * c;
-            const float4 x = u[0], y = u[1];
+            float4 x = u[0], y = u[1];
+            for (int k = 1; k < planes; ++k) {
+                const float4 v = u[k * plane], w = u[k * plane + 1];
+                x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+                y = make_float4(y.x + w.x, y.y + w.y, y.z + w.z, y.w + w.w);
+            }
             const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.weight) + (long long)a.target[at] * a.ld_w) + c);
             const float2 w0 = vl_two(w.x, a.bf16), w1 = vl_two(w.y, a.bf16), w2 = vl_two(w.z, a.bf16), w3 = vl_two(w.w, a.bf16);
             out = make_uint4(vl_pack(fmaf(mean, x.x, hit * w0.x), fmaf(mean, x.y, hit * w0.y), a.bf16),
@@ -1351,7 +1371,7 @@ static VlKept vl_kept(long long rows, long long hidden, int grads) {
         k.first = take(pad * 4);
         k.next = take(pad * 4);
     }
-    if (grads & 1) k.sums = take(pad * (size_t)hidden * 4);
+    if (grads & 1) k.sums = take((size_t)vl_plane_rows((long long)pad) * (size_t)hidden * 4);
     k.gathered = at;                       // last: without a gradient of the weight it is scratch of the forward
     if (grads & 2) take(pad * (size_t)hidden * 2);
     k.bytes = at;
@@ -1371,7 +1391,7 @@ static VlCounters vl_counters(const VocabLossArgs& a, const VlRoom& room, bool b
     c.written = 32;
     c.read = c.written + (long long)room.pieces * c.pitch;
     c.added = c.read + (long long)room.pieces * c.pitch;
-    c.each = c.added + (backward ? 0 : row_tiles * feature_tiles);
+    c.each = c.added + (backward ? 0 : vl_plane_rows(vl_rows_pad(a.rows)) / VL_TILE * feature_tiles);
     c.flags = (backward ? 1 : 2) * c.each;
     c.list = c.flags + (backward ? 0 : 1 + row_tiles);
     c.total = c.list + (backward ? 0 : 1 + row_tiles);
@@ -1530,7 +1550,7 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         maps.words = logits.b;
         ok = vl_piece_map(&maps.piece_in, a, 128) && vl_map(&maps.other, a.bf16, a.weight, a.hidden, a.vocab, a.ld_w, 64) &&
              vl_piece_map(&maps.piece_out, a, 32) &&
-             make_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.sums, (uint64_t)a.hidden, (uint64_t)a.rows_pad,
+             make_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, a.sums, (uint64_t)a.hidden, (uint64_t)vl_plane_rows(a.rows_pad),
                          (uint64_t)a.hidden * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     }
     if (!ok) { *why = "cuTensorMapEncodeTiled"; return cudaErrorInvalidValue; }
