@@ -58,12 +58,12 @@ constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference 
 // 671, 64 366). The backward's product is written, not added: small pieces that stay in L2 (1229 rows: 8 tiles of words 1030 us, 16
 // 1053, 64 1069). With many rows at least VL_PIECE_LEAST tiles of words up to VL_PIECE_MOST tiles (a gigabyte of scratch),
 // one behind that.
-// A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD_ units lie between: what a unit
-// waits for was drawn well before it, not a moment ago by a pair that is still at it (1229 rows, 80 units of logits to a
-// piece: one piece behind 1201 us, two 1107; dW of 256 rows, 56 units to a piece: three behind 347, six 300; of 1229, 88
-// units: two 1030, three 1038; U of 256 rows, 30 units: six 304, eight 287, twelve 276).
+// A piece's product comes `lag` pieces behind its logits in the list, so many that VL_AHEAD_ units of logits (and as much work
+// on products) lie between: what a unit waits for was drawn well before it, not a moment ago by a pair that is still at it.
+// (U of 1229 rows, 80 units to a piece: one piece behind 1201 us, two 1107; of 256 rows, 24 units: six 304, eight 287,
+// twelve 276. dW of 16 rows x 3584, 8 units: two 880, four 717, eight 692; of 1229 rows, 40 units: two 1030, three 1038.)
 constexpr int VL_PIECE_UNITS = 512, VL_PIECE_TILES = 64, VL_BWD_TILES = 8, VL_PIECE_LEAST = 8, VL_PIECE_MOST = 2048;
-constexpr int VL_AHEAD_FWD = 370, VL_AHEAD_BWD = 222, VL_MOST_LAG = 24;      // (five and three units for each of 74 pairs)
+constexpr int VL_AHEAD_FWD = 278, VL_AHEAD_BWD = 111, VL_MOST_LAG = 24;
 constexpr int VL_PRODUCTS = 148;
 constexpr int VL_PLANE_ROWS = 1024;
 
@@ -187,7 +187,7 @@ __host__ __device__ inline VlShape vl_shape(int row_tiles, int word_tiles, int f
     if (t > word_tiles) t = word_tiles;
     s.tiles = (int)t;
     s.pieces = vl_div_up(word_tiles, s.tiles);
-    const long long units = (long long)a * s.tiles + (long long)(backward ? s.tiles : a) * feature_tiles;
+    const long long units = (long long)a * s.tiles;
     const int ahead = backward ? VL_AHEAD_BWD : VL_AHEAD_FWD;
     s.lag = units >= ahead ? 1 : vl_div_up(ahead, (int)units);
     if (s.lag > VL_MOST_LAG) s.lag = VL_MOST_LAG;
@@ -904,9 +904,9 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             int hits[4] = {-1, -1, -1, -1};
             if (BWD && w.q) {
                 scale = *p.weight_scale;
-                const int key = (v0 + row) % (int)p.rows_pad;
-                if (v0 + row < p.vocab && p.links[key] <= VL_LINKS)
-                    for (int r = p.first[key]; r >= 0; r = p.next[r]) {
+                const int key = (v0 + row) % (int)p.rows_pad, links = p.links[key], first = p.first[key];
+                if (v0 + row < p.vocab && links <= VL_LINKS)
+                    for (int r = first; r >= 0; r = p.next[r]) {
                         if (p.target[r] != v0 + row) continue;
                         int x = r;
 #pragma unroll
