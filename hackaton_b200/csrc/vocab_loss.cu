@@ -648,7 +648,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
     using L = VlSmem<128, 6, true>;
     constexpr int STAGES = L::STAGES;
     constexpr int BARS = 3 * STAGES + 4 + 2 * VL_TICKETS;
-    constexpr uint32_t ALL = 2 * (VL_EPI_WARPS + 2);      // who reads a ticket: both CTAs' TMA, MMA (peer: its word) and epilogue
+    constexpr uint32_t ALL = 2 * (VL_EPI_WARPS + 2) + 1;  // who reads a ticket: both CTAs' TMA, MMA (peer: its word) and epilogue, the counter
     extern __shared__ uint8_t vl_smem[];
     const uint32_t base = (smem_u32(vl_smem) + 1023u) & ~1023u;
     uint8_t* gen = vl_smem + (base - smem_u32(vl_smem));
@@ -680,7 +680,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(bar_done(b), 1);
-            mbar_init(bar_drained(b), 2 * VL_EPI_WARPS);
+            mbar_init(bar_drained(b), 2 * VL_EPI_WARPS + 1);
         }
         for (int k = 0; k < VL_TICKETS; ++k) {
             mbar_init(bar_drawn(k), 1);
@@ -809,6 +809,19 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                 for (int c = 0; c < 2; ++c) vl_send(tickets0[c] + 4u * k, t, drawn0[c] + 8u * k);
                 if (t < 0) break;
             }
+        } else if (lane == 0) {
+            // ---------------------------------------------------------- the peer: counts the units that have read a piece
+            // (A fence and a count take 2700 cycles: in an epilogue warp a third of its time for a tile of few rows' dW.)
+            const uint32_t lead_drained = mapa_shared(bar_drained(0), 0u);
+            uint32_t n = 0;
+            for (int t; !fail && (t = next_ticket(false)) >= 0;) {
+                const VlUnit w = vl_unit<BWD>(t, p, list);
+                for (int it = 0; it < w.steps; it += w.chain, ++n) {
+                    if (!mbar_wait(bar_done(n & 1u), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
+                    mbar_arrive_cluster(lead_drained + 8u * (n & 1u));
+                }
+                if (!fail && w.q && w.steps > 0) vl_count(p.read + w.piece * p.pitch + w.slot);
+            }
         }
     } else {
         // ------------------------------------------------------------------ epilogue: a row's half tile per thread
@@ -928,7 +941,6 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             if (!BWD && w.q && !wait_count(added, 2 * VL_EPI_WARPS * (w.piece / list.planes))) { fail = 13; break; }
             if (!mbar_wait(bar_done(b), (n >> 1) & 1u, abort_flag)) { fail = 5; break; }
             tc_fence_after_sync();
-            if (w.q && rank == 0 && warp == 2 && lane == 0) vl_count(p.read + w.piece * p.pitch + w.slot);
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + half * 128;
             float m2 = VL_NEG, sum = 0.f;
             const int piece_row = w.piece % list.buffers * buffer_rows + row0;
