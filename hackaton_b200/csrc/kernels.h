@@ -423,7 +423,7 @@ cudaError_t launch_lora_grad_batch(const LoraGradBatch& b, cudaStream_t stream);
 int set_error(int code, const char* fmt, ...);
 
 // Device-side status word: 0, or the first code a kernel recorded since it was last read:
-//   100 + role   a bounded wait of the fused GEMM ran out (role = which wait)
+//   100 + role   a bounded wait of the fused GEMM or of the vocabulary loss ran out (role = which wait)
 //   190          the norms around a block: the bounded wait for a row ran out
 //   200          cross-entropy: a target index beyond the vocabulary (row treated as ignored)
 //   300          scale table: a block scale outside fp16's normal range (inf, subnormal or zero)

@@ -87,8 +87,8 @@ int nf4b200_prepare_scales(const nf4b200_weight* w, void* scales16, void* stream
 /*
  * Reads and clears the device-side status word of the current device (synchronises the device).
  * 0 = no kernel reported anything since the last call. Otherwise the call returns NF4B200_EDEVICE
- * and *status_out holds the first code recorded: 100..199 a bounded wait of the fused GEMM ran
- * out; 200 cross-entropy met a target index beyond the vocabulary (that row was treated as
+ * and *status_out holds the first code recorded: 100..199 a bounded wait of the fused GEMM, of
+ * the vocabulary loss or (190) of the norms around a block ran out; 200 cross-entropy met a target index beyond the vocabulary (that row was treated as
  * ignored, nothing was read out of bounds); 300 nf4b200_prepare_scales met a block scale outside
  * fp16's normal range (the fused GEMM multiplies table and scale in fp16 and cannot represent
  * that block; the standalone decode can); 400 the self-test below.
