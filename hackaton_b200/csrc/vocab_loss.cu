@@ -11,8 +11,9 @@
 // operations (R rows, V words, K features) instead of three: a piece's exponentials are taken relative to a reference
 // per row that is fixed before the sweep (from the first words and the target's own logit), and the sum's 1 / s comes
 // at the end. The target is left out of U and of the sums, so that 1 - p_t and a loss near zero keep their digits, and its
-// share is added in fp32. Where a row meets a logit too far above its reference for the 16-bit type, its row tile's sweep
-// is done again with references from the maxima; the launch for that looks at a flag and leaves. dW needs the final
+// share is added in fp32. Where a row meets a logit too far above its reference for the 16-bit type, or (fp16) none that
+// is not too far below it, its row tile's sweep is done again with references from the maxima; the launch for that finds
+// nothing to do nearly always. dW needs the final
 // lse: the logits once more, in 16-bit dl this time, and one product. A word's row of dW is mostly what its own
 // rows' targets add, so that what those dl lose in 16 bits shows: it is kept and added in fp32, for four rows of a word.
 // (1229 rows, 5000 words: dW is 2.1e-4 of itself off in fp16, as much as its own rounding alone; without this 3.0e-4.)
@@ -46,9 +47,14 @@ constexpr float VL_LN2 = 0.6931471805599453f;
 constexpr float VL_NEG = -1.0e30f;         // a finite "minus infinity"
 constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 2^13, down to 2^-24 / 2^13
 // A row's reference for its exponentials (base 2): the larger of the first words' maximum less VL_BELOW and the
-// target's logit less VL_BELOW_TARGET; fp16 takes what lies up to 2^15 above it, bf16 2^100.
-constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET = 10.f;
+// target's logit less VL_BELOW_TARGET_; fp16 takes what lies up to 2^15 above it, bf16 2^100. In fp16 the largest of the other words
+// may not lie further than VL_LOW below it either: a word's exponential is off by 2^-25 there, 2^-22 of the largest, and those
+// down to 2^-11 of that one are normal numbers. (With 10 for fp16 too and no such limit, a target 19 above the next word
+// left dH 1.8e-3 of itself off, one 23 above 7e-2. bf16's range has room for both.) Where the first words are all there are, they
+// alone give the reference.
+constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET_F16 = 24.f, VL_BELOW_TARGET_BF16 = 10.f, VL_LOW = 3.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
+constexpr float VL_NO_LIMIT = 3.0e38f;
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
 // Pieces (vl_shape). Forward as large as VL_PIECE_UNITS tiles of 256 x 256 allow (67 MB): each adds to all of U, which costs
@@ -144,7 +150,8 @@ struct VlSweepParams {
     // forward
     float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum relative to the reference
     const float* refs;       // [rows_pad]
-    int* flags;              // [1 + row tiles]: whether any row, and which tiles' rows, outgrew their references
+    int* flags;              // [row tiles]: whether a row outgrew its reference
+    float* low;              // [rows_pad]: what a row has to reach for its reference to hold, VL_NO_LIMIT once it has; or null
     const int* list;         // a sweep done again: number of row tiles, their indexes
     int again;
     // backward
@@ -899,7 +906,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             const int b = (int)(n & 1u);
             // what the values meet, asked for before the tile is complete
             int target = -1;
-            float lse2 = 0.f, rest = 0.f, ref = 0.f, scale = 1.f;
+            float lse2 = 0.f, rest = 0.f, ref = 0.f, low = VL_NO_LIMIT, scale = 1.f;
             float4 coef = make_float4(0.f, 0.f, 0.f, 0.f);
             const bool live = row < rows;
             if (!w.q && live) {
@@ -910,6 +917,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     coef = p.coef[row];
                 } else {
                     ref = p.refs[row];
+                    if (p.low != nullptr) low = p.low[row];
                 }
             }
             // backward's Q: the last four rows whose target is this thread's word. (Where there are many, what they lose
@@ -1043,10 +1051,9 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             ++n;
             if (!w.q && !BWD) {
                 p.parts[(long long)(v0 / VL_TILE * 2 + 2 * w.nt + half) * p.rows_pad + row] = make_float2(m2, sum);
-                if (live && m2 > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) {      // (several threads write the same)
-                    p.flags[0] = 1;
-                    p.flags[1 + w.mt] = 1;
-                }
+                // (several threads write the same)
+                if (live && m2 > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) p.flags[w.mt] = 1;
+                if (low < VL_NO_LIMIT && m2 >= low) p.low[row] = VL_NO_LIMIT;
             }
             if (!w.q || !BWD)       // (backward's Q writes what nobody waits for)
                 owed = w.q ? added : p.written + w.piece * p.pitch + w.slot;
@@ -1159,12 +1166,12 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
 // Joins a row's statistics, 8 rows by 128 shares of the parts per CTA. (32 by 32: 8.5 us for 64 rows of 151,936 words, so 5.0.)
 // Where the head's gradient is to come, the last tile's empty rows become zeros: they meet the others' in sums over rows,
 // and nowhere else does what lies there reach a result. PROBE: the first words' maxima give the row's
-// reference. Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's reference.
+// reference (`sure`: they are all words). Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's reference.
 constexpr int VL_MERGE_ROWS = 8, VL_MERGE_SHARES = 1024 / VL_MERGE_ROWS;
 
 template <bool PROBE>
 __global__ void __launch_bounds__(1024)
-vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
+vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft, int sure) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float2 join[VL_MERGE_ROWS][VL_MERGE_SHARES + 1];
@@ -1205,8 +1212,12 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     const float logit = a.target_logit[at], logit2 = logit * VL_LOG2E;
     if (PROBE) {
         // (fmaxf leaves out a NaN; where there is nothing finite to go by, any number will do)
-        const float ref = fmaxf(x.x - VL_BELOW, logit2 - VL_BELOW_TARGET);
-        a.refs[at] = fabsf(ref) < 1.0e29f ? floorf(ref) : 0.f;
+        const bool others = x.x > 0.5f * VL_NEG;
+        float ref = x.x - VL_BELOW;
+        if (!sure || !others) ref = fmaxf(ref, logit2 - (a.bf16 ? VL_BELOW_TARGET_BF16 : VL_BELOW_TARGET_F16));
+        ref = fabsf(ref) < 1.0e29f ? floorf(ref) : 0.f;
+        a.refs[at] = ref;
+        if (a.low != nullptr) a.low[at] = others && x.x < ref - VL_LOW ? ref - VL_LOW : VL_NO_LIMIT;
         return;
     }
     const float d = x.x - logit2;      // log2 of what the others' sum is relative to, over the target's
@@ -1234,28 +1245,21 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     a.lse[a.source[at]] = logit + loss;
 }
 
-// A CTA per row tile: where a row outgrew its reference, new ones from the maxima; the first CTA lists those tiles.
+// A CTA per row tile: where a row's reference does not hold, the tile goes onto the list (in any order) with new ones from
+// the maxima.
 __global__ void __launch_bounds__(VL_TILE)
 vl_again_kernel(const VocabLossArgs a, int word_tiles) {
     grid_dep_wait();
     grid_dep_launch();
-    const int rows = *a.count, row_tiles = vl_div_up(rows, VL_TILE);
-    if (a.flags[0] == 0 || (int)blockIdx.x >= row_tiles) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.list[0] = 0;
-        return;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        int n = 0;
-        for (int t = 0; t < row_tiles; ++t)
-            if (a.flags[1 + t] != 0) a.list[1 + n++] = t;
-        a.list[0] = n;
-    }
-    const int row = blockIdx.x * VL_TILE + threadIdx.x;
-    if (a.flags[1 + blockIdx.x] == 0 || row >= rows) return;
+    const int rows = *a.count, row = blockIdx.x * VL_TILE + threadIdx.x;
+    const bool low = a.low != nullptr && row < rows && a.low[row] < VL_NO_LIMIT;
+    if (!__syncthreads_or(low || a.flags[blockIdx.x] != 0)) return;
+    if (threadIdx.x == 0) a.list[1 + atomicAdd(a.list, 1)] = blockIdx.x;
+    if (row >= rows) return;
     float top = VL_NEG;
 #pragma unroll 8
     for (int i = 0; i < 2 * word_tiles; ++i) top = fmaxf(top, a.parts[(long long)i * a.rows_pad + row].x);
-    if (top > a.refs[row] + (a.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) a.refs[row] = ceilf(top) - 6.f;
+    if (low || top > a.refs[row] + (a.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) a.refs[row] = ceilf(top) - 6.f;
 }
 
 // ------------------------------------------------------------------------------------- backward
@@ -1405,13 +1409,13 @@ static VlCounters vl_counters(const VocabLossArgs& a, const VlRoom& room, bool b
     c.added = c.read + (long long)room.pieces * c.pitch;
     c.each = c.added + (backward ? 0 : vl_plane_rows(vl_rows_pad(a.rows)) / VL_TILE * feature_tiles);
     c.flags = (backward ? 1 : 2) * c.each;
-    c.list = c.flags + (backward ? 0 : 1 + row_tiles);
+    c.list = c.flags + (backward ? 0 : row_tiles);
     c.total = c.list + (backward ? 0 : 1 + row_tiles);
     return c;
 }
 
 struct VlScratch {
-    size_t parts, target_logit, refs, counters, gathered, coef, weight_scale, piece, bytes;
+    size_t parts, target_logit, refs, low, counters, gathered, coef, weight_scale, piece, bytes;
     VlRoom room;
 };
 
@@ -1430,6 +1434,7 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
         if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
         if (a.grads & 1) {
             s.refs = take(pad * 4);
+            s.low = take(pad * 4);
             s.counters = take(counters);
             s.piece = take(piece);
         }
@@ -1512,7 +1517,7 @@ static VlSweepParams vl_sweep_params(const VocabLossArgs& a, const VlCounters& c
     int* counters = a.counters + sweep * c.each;
     p.ticket = counters + c.ticket; p.written = counters + c.written; p.read = counters + c.read; p.added = counters + c.added;
     p.pitch = c.pitch;
-    p.parts = a.parts; p.refs = a.refs; p.flags = a.flags; p.list = a.list; p.again = sweep;
+    p.parts = a.parts; p.refs = a.refs; p.flags = a.flags; p.low = sweep == 0 ? a.low : nullptr; p.list = a.list; p.again = sweep;
     p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef; p.links = a.links; p.first = a.first; p.next = a.next; p.gathered = a.gathered; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
     return p;
 }
@@ -1530,9 +1535,10 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     a.parts = reinterpret_cast<float2*>(ws + s.parts);
     a.target_logit = reinterpret_cast<float*>(ws + s.target_logit);
     if (!(a.grads & 2)) a.gathered = ws + s.gathered;
-    const bool soft = (a.grads & 1) != 0;
+    const bool soft = (a.grads & 1) != 0, sure = vl_word_tiles(a.vocab) <= VL_PROBE_TILES;
     if (soft) {
         a.refs = reinterpret_cast<float*>(ws + s.refs);
+        if (!sure && !a.bf16) a.low = reinterpret_cast<float*>(ws + s.low);
         a.counters = reinterpret_cast<int*>(ws + s.counters);
         a.n_counters = counters.total;
         a.flags = a.counters + counters.flags;
@@ -1584,19 +1590,17 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         VlParams probe = p;
         if (probe.word_tiles > VL_PROBE_TILES) probe.word_tiles = VL_PROBE_TILES;
         e = vl_launch(vl_stats_kernel<VL_STATS>, VL_THREADS, VlSmemOf<VL_STATS>::TOTAL, logits, probe, row_tiles * probe.word_tiles, a.sm_count, stream);
-        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, 0);
+        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, 0, sure ? 1 : 0);
         if (e != cudaSuccess) { *why = "references"; return e; }
         const long long units = row_tiles * (p.word_tiles + vl_div_up(p.hidden, VL_TILE));
-        // (no row outgrows a reference that all words were asked for)
-        const bool sure = p.word_tiles <= VL_PROBE_TILES;
-        for (int sweep = 0; sweep < (sure ? 1 : 2) && e == cudaSuccess; ++sweep) {
+        for (int sweep = 0; sweep < (sure ? 1 : 2) && e == cudaSuccess; ++sweep) {      // (references from all words hold)
             e = vl_launch(vl_sweep_kernel<false>, VL_SWEEP_THREADS, VL_SWEEP_SMEM, maps, vl_sweep_params(a, counters, sweep), units, a.sm_count, stream);
             if (!sure && sweep == 0 && e == cudaSuccess)
                 e = launch_pdl(vl_again_kernel, dim3((unsigned)row_tiles), dim3(VL_TILE), 0, stream, a, p.word_tiles);
         }
     }
     if (e != cudaSuccess) { *why = "statistics"; return e; }
-    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, soft ? 1 : 0);
+    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, soft ? 1 : 0, 0);
     if (e != cudaSuccess) *why = "merge";
     return e;
 }
