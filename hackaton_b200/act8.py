@@ -45,7 +45,8 @@ class Act8:
 
 
 def act8_quantize(x):
-    """`x` (fp16, bf16 or fp32, CUDA, at least one dimension) in 8 bits; blocks run along the last dimension."""
+    """`x` (fp16, bf16 or fp32, CUDA, at least one dimension) in 8 bits; blocks run along the last dimension. No gradient
+    leads back from the parts to `x` (it is what a backward pass keeps); a tangent of forward mode is refused."""
     kept = _lib.host().act8_quantize(x)
     if kept is None:
         if x.dtype not in _TYPES:
@@ -76,7 +77,7 @@ def act8_dequantize(kept):
 def lora_grad_act8(kept, s):
     """sᵀ . x as fp32 [16, cols] for an fp16 input x kept in 8 bits and fp16 s [..., 16] with a row for each of
     its rows: the gradient of a LoRA pair's first factor (`lora.lora_grad` with rank-major output), in a fixed
-    order of additions."""
+    order of additions. As a part of backward passes it has no gradient of its own."""
     grad = _lib.host().act8_lora_grad(kept.codes, kept.steps, s, kept.shape[-1]) if kept.dtype is torch.float16 else None
     if grad is None:
         if kept.dtype != torch.float16 or s.dtype != torch.float16:

@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -321,6 +322,13 @@ Tensor rmsnorm_bwd(const Tensor& x2, const Tensor& weight, const Tensor& rstd, c
     return dx;
 }
 
+// Forward-mode differentiation is refused: nothing here would carry a tangent along.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> operands) {
+    for (const Tensor* t : operands)
+        TORCH_CHECK_NOT_IMPLEMENTED(t == nullptr || !t->_fw_grad(0).defined(), "hackaton_b200: ", what,
+                                    " has no forward-mode derivative (an operand carries a tangent)");
+}
+
 int type_code(at::ScalarType t) { return t == at::kHalf ? NF4B200_F16 : t == at::kBFloat16 ? NF4B200_BF16 : NF4B200_F32; }
 
 // (codes, steps) of a contiguous [rows, cols] tensor; see hackaton_b200.act8.
@@ -340,6 +348,7 @@ Tensor flat_rows(const Tensor& t) {
 std::optional<std::tuple<Tensor, Tensor>> act8_quantize(const Tensor& x) {
     const auto type = x.scalar_type();
     if (!x.is_cuda() || x.dim() == 0 || (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat)) return {};
+    no_tangent("act8_quantize", {&x});
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor x2 = flat_rows(x.requires_grad() ? x.detach() : x);
     auto [codes, steps] = act8_room(x2, x2.size(0), x2.size(1));
@@ -414,6 +423,7 @@ Opt silu_mul_act8(const Tensor& gate, const Tensor& up) {
     if (!gate.is_cuda() || gate.device() != up.device() || gate.scalar_type() != at::kHalf || up.scalar_type() != at::kHalf ||
         gate.sizes() != up.sizes())
         return {};
+    no_tangent("silu_mul with keep8", {&gate, &up});
     return SiluMulAct8::apply(gate, up);
 }
 
@@ -423,6 +433,7 @@ Opt act8_lora_grad(const Tensor& codes, const Tensor& steps, const Tensor& s, in
     const int64_t rows = codes.size(0);
     if (s.scalar_type() != at::kHalf || s.device() != codes.device() || s.dim() == 0 || s.size(-1) != RANK || s.numel() != rows * RANK)
         return {};
+    no_tangent("lora_grad_act8", {&s});
     const c10::cuda::CUDAGuard guard(codes.device());
     Tensor s2 = flat_rows(s.requires_grad() ? s.detach() : s);
     if ((reinterpret_cast<uintptr_t>(s2.const_data_ptr()) & 15) != 0) s2 = s2.clone();
@@ -531,6 +542,7 @@ std::optional<std::tuple<Tensor, Tensor>> sandwich_norm(const Tensor& residual, 
     if (gate.has_value() && (!weight(*gate) || gate->dim() == 0 || gate->dim() > 2 || gate->size(-1) != hidden ||
                              (rows > 0 && (gate->numel() == 0 || rows % (gate->numel() / hidden) != 0))))
         return {};
+    no_tangent("sandwich_norm", {&residual, &delta, &post, &pre, gate.has_value() ? &*gate : nullptr});
     if (at::GradMode::is_enabled() && (residual.requires_grad() || delta.requires_grad() || post.requires_grad() ||
                                        pre.requires_grad() || (gate.has_value() && gate->requires_grad()))) {
         const variable_list out = SandwichNorm::apply(residual, delta, post, pre, gate, scale, eps, f32_out);
@@ -626,6 +638,7 @@ std::optional<std::tuple<Tensor, Tensor>> vocab_loss(const Tensor& hidden, const
         weight.dim() != 2 || hidden.dim() != targets.dim() + 1 || weight.size(0) == 0 || weight.size(1) == 0 ||
         weight.size(1) % 8 != 0 || hidden.size(-1) != weight.size(1) || hidden.sizes().slice(0, targets.dim()) != targets.sizes())
         return {};
+    no_tangent("vocab_cross_entropy", {&hidden, &weight});
     int64_t grads = 0;
     if (at::GradMode::is_enabled()) grads = (hidden.requires_grad() ? 1 : 0) | (weight.requires_grad() ? 2 : 0);
     if (grads != 0) {

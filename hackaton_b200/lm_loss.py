@@ -190,7 +190,7 @@ def vocab_cross_entropy(hidden, weight, targets):
     `linear_cross_entropy` (fp16, frozen head, one loss with its gradient made in the forward) this one takes bf16, gives
     the head's gradient and writes no logits. For the gradient of hidden the forward keeps fp32 [rows, features] (at least
     1024 rows of it), for the head's the rows that take part. Scratch while it runs with gradients: 16-bit pieces of the
-    softmax, 0.2 GB at 2048 to 16,384 rows, 0.8 GB up to half a million. No second derivatives."""
+    softmax, 0.2 GB at 2048 to 16,384 rows, 0.8 GB up to half a million. No second derivatives, no forward mode."""
     out = _lib.host().vocab_loss(hidden, weight, targets)
     if out is None:
         _refuse_vocab(hidden, weight, targets)
