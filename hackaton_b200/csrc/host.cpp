@@ -379,10 +379,11 @@ Opt act8_dequantize(const Tensor& codes, const Tensor& steps, const std::vector<
     return out;
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> act8_swiglu_fwd(const Tensor& gate2, const Tensor& up2) {
+// (Outputs of an autograd function get their shapes when they are made: a view of one could not be changed in place.)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> act8_swiglu_fwd(const Tensor& gate2, const Tensor& up2, at::IntArrayRef shape) {
     const c10::cuda::CUDAGuard guard(gate2.device());
     const int64_t rows = gate2.size(0), cols = gate2.size(1);
-    Tensor hidden = at::empty_like(gate2);
+    Tensor hidden = at::empty(shape, gate2.options().memory_format(c10::nullopt));
     auto [gc, gs] = act8_room(gate2, rows, cols);
     auto [uc, us] = act8_room(up2, rows, cols);
     check(nf4b200_act8_swiglu_fwd(gate2.const_data_ptr(), up2.const_data_ptr(), hidden.data_ptr(), gc.data_ptr(),
@@ -407,9 +408,9 @@ void differentiate_once(const char* what) {
 
 struct SiluMulAct8 : torch::autograd::Function<SiluMulAct8> {
     static Tensor forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up) {
-        auto [hidden, gc, gs, uc, us] = act8_swiglu_fwd(flat_rows(gate), flat_rows(up));
+        auto [hidden, gc, gs, uc, us] = act8_swiglu_fwd(flat_rows(gate), flat_rows(up), gate.sizes());
         ctx->save_for_backward({gc, gs, uc, us});
-        return hidden.view(gate.sizes());
+        return hidden;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         differentiate_once("silu_mul with keep8");
@@ -565,14 +566,14 @@ int64_t sized(int64_t bytes) {
     return bytes;
 }
 
-// (losses, logsumexps, what the gradient needs)
+// (losses, logsumexps, both in the targets' shape, what the gradient needs)
 std::tuple<Tensor, Tensor, Tensor> vocab_loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t grads) {
     const c10::cuda::CUDAGuard guard(x.device());
     const int64_t hidden = weight.size(1), vocab = weight.size(0);
     const Tensor x2 = rows_view(x, hidden), w = head_view(weight), t = targets.reshape({-1}).contiguous();
     const int64_t rows = x2.size(0);
     const auto options = x.options().dtype(at::kFloat).memory_format(c10::nullopt);
-    Tensor losses = at::empty({rows}, options), lse = at::empty({rows}, options);
+    Tensor losses = at::empty(targets.sizes(), options), lse = at::empty(targets.sizes(), options);
     Tensor kept = at::empty({sized(nf4b200_vocab_loss_kept_bytes(rows, hidden, (int)grads))}, options.dtype(at::kByte));
     const int64_t need = sized(nf4b200_vocab_loss_workspace_bytes(rows, vocab, hidden, (int)grads, 0));
     const Scratch ws(need, x2);
@@ -614,7 +615,7 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
         ctx->saved_data["grads"] = grads;
         ctx->saved_data["rows"] = targets.numel();
         ctx->saved_data["shape"] = hidden.sizes().vec();
-        return {losses.view(targets.sizes()), lse.view(targets.sizes())};
+        return {losses, lse};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         differentiate_once("vocab_cross_entropy");
@@ -646,7 +647,7 @@ std::optional<std::tuple<Tensor, Tensor>> vocab_loss(const Tensor& hidden, const
         return std::make_tuple(out[0], out[1]);
     }
     auto [losses, lse, kept] = vocab_loss_fwd(hidden, weight, targets, 0);
-    return std::make_tuple(losses.view(targets.sizes()), lse.view(targets.sizes()));
+    return std::make_tuple(losses, lse);
 }
 
 struct Rotation {   // everything about one rotation that is not a tensor

@@ -31,3 +31,29 @@ def test_forward_mode_is_refused(cuda_lib):
                 call(dual)
             with torch.no_grad(), pytest.raises(RuntimeError):
                 call(dual)
+
+
+def test_outputs_can_be_changed_in_place(cuda_lib):
+    from hackaton_b200 import sandwich_norm, silu_mul, vocab_cross_entropy
+
+    g, u = (activations(6, 64, torch.float16, k).clamp(-4, 4).requires_grad_() for k in (1, 2))
+    for shape in ((6, 64), (2, 3, 64)):
+        want = torch.autograd.grad((silu_mul(g.view(shape), u.view(shape), keep8=True) * 2).sum(), [g, u])
+        got = silu_mul(g.view(shape), u.view(shape), keep8=True)
+        got.mul_(2)
+        assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(got.sum(), [g, u])))
+        w = torch.ones(5, 64, device="cuda", dtype=torch.float16)
+        t = torch.arange(6, device="cuda").view(shape[:-1]) % 5
+        mask = (t > 1).float()
+        losses, lse = vocab_cross_entropy(g.view(*shape), w, t)
+        want = torch.autograd.grad((losses * mask).sum() + (lse * 3).sum(), [g])[0]
+        losses, lse = vocab_cross_entropy(g.view(*shape), w, t)
+        losses.mul_(mask)
+        lse *= 3
+        assert torch.equal(want, torch.autograd.grad(losses.sum() + lse.sum(), [g])[0])
+    ones = torch.ones(64, device="cuda")
+    stream, normed = sandwich_norm(g.detach().float(), u, ones, ones, 1e-6)
+    want = torch.autograd.grad((normed * 2).sum(), [u])[0]
+    stream, normed = sandwich_norm(g.detach().float(), u, ones, ones, 1e-6)
+    normed.mul_(2)
+    assert torch.equal(want, torch.autograd.grad(normed.sum(), [u])[0])
