@@ -195,7 +195,7 @@ class NF4LinearGroupAct8(NF4LinearGroup):
 
 def nf4_linear_group(x, projections: Sequence[Projection], keep8=False):
     """Outputs of all `projections` applied to the same x, computed by one grouped launch. With `keep8`, x is
-    kept once, in 8 bits, for the gradients of the LoRA pairs' first factors (act8.py)."""
+    kept once, in 8 bits, for the gradients of the LoRA pairs' first factors (act8.py), where gradients are on."""
     params = []
     for pr in projections:
         if (pr.lora_a is None) != (pr.lora_b is None):
@@ -203,4 +203,4 @@ def nf4_linear_group(x, projections: Sequence[Projection], keep8=False):
         if pr.lora_a is not None and pr.lora_a.shape[0] != RANK:
             raise ValueError(f"LoRA rank must be {RANK}")
         params += [pr.bias, pr.lora_a, pr.lora_b]
-    return (NF4LinearGroupAct8 if keep8 else NF4LinearGroup).apply(x, list(projections), *params)
+    return (NF4LinearGroupAct8 if keep8 and torch.is_grad_enabled() else NF4LinearGroup).apply(x, list(projections), *params)

@@ -195,7 +195,8 @@ class NF4LoRALinear(torch.autograd.Function):
 
 def nf4_lora_linear(x, packed, bias, state, lora_a, lora_b, scaling, x_lora=None, keep8=False):
     """y = x . Wᵀ + bias + scaling * (x_lora . Aᵀ) . Bᵀ; x_lora defaults to x. With `keep8`, x_lora is kept in 8
-    bits for the gradient of A (act8.py)."""
+    bits for the gradient of A (act8.py), where gradients are on."""
     if x_lora is None:
         x_lora = x
-    return NF4LoRALinear.apply(x, x_lora, packed.reshape(-1), bias, state, lora_a, lora_b, scaling, bool(keep8))
+    return NF4LoRALinear.apply(x, x_lora, packed.reshape(-1), bias, state, lora_a, lora_b, scaling,
+                               bool(keep8) and torch.is_grad_enabled())

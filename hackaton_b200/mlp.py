@@ -199,7 +199,7 @@ def nf4_swiglu_mlp(x, gate_proj: Projection, up_proj: Projection, down_proj: Pro
     linear. With `keep8`, gate, up and the inputs of LoRA projections are kept in 8 bits for the backward (act8.py)."""
     projs = (gate_proj, up_proj, down_proj)
     if all(p.bias is None and p.lora_a is None and p.lora_b is None for p in projs):
-        return NF4SwiGLUMLP.apply(x, *[(p.packed, p.state) for p in projs], bool(keep8))
+        return NF4SwiGLUMLP.apply(x, *[(p.packed, p.state) for p in projs], bool(keep8) and torch.is_grad_enabled())
     from .lora import nf4_lora_linear
     from .nf4 import nf4_linear
     hidden = nf4_gate_up_swiglu(x, gate_proj, up_proj, keep8)

@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
-from test_act8_gpu import activations
+from test_act8_gpu import activations, lora_parts
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,24 @@ def test_outputs_can_be_changed_in_place(cuda_lib):
     stream, normed = sandwich_norm(g.detach().float(), u, ones, ones, 1e-6)
     normed.mul_(2)
     assert torch.equal(want, torch.autograd.grad(normed.sum(), [u])[0])
+
+
+def test_nothing_is_kept_without_gradients(cuda_lib, monkeypatch):
+    """An evaluation pass with trainable factors does not quantise what no backward will read."""
+    from hackaton_b200 import Projection, act8, group, lora, mlp, nf4_linear_group, nf4_lora_linear, nf4_swiglu_mlp
+
+    packed, state, a, b = lora_parts(128, 256, 9)
+    x = activations(40, 256, torch.float16, 7).clamp(-8, 8)
+    gate, up, down = (Projection(*lora_parts(n, k, 30 + i)[:2]) for i, (n, k) in enumerate(((512, 256), (512, 256), (256, 512))))
+    pair = Projection(packed, state, None, a, b, 2.0)
+    calls = [lambda v: nf4_lora_linear(v, packed, None, state, a, b, 2.0, keep8=True), lambda v: nf4_linear_group(v, [pair], keep8=True)[0],
+             lambda v: nf4_swiglu_mlp(v, gate, up, down, keep8=True)]
+    want = [call(x.clone().requires_grad_()) for call in calls]
+    quantised = []
+    for module in (lora, group, mlp):
+        monkeypatch.setattr(module, "act8_quantize", lambda t: quantised.append(t.shape) or act8.act8_quantize(t))
+    for w, call in zip(want, calls):
+        with torch.no_grad():
+            assert torch.equal(w, call(x.clone().requires_grad_()))
+        assert not quantised
+    assert calls[0](x.clone().requires_grad_()).requires_grad and quantised
