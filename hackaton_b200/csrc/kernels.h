@@ -313,6 +313,7 @@ struct VocabLossArgs {
     int* place;                  // [rows]: where among them, or -1
     int* source;                 // per such row: whose it is
     int* target;
+    int* before;                 // many rows: per block of them how many come before it, or null
     float* target_logit;
     float* lse_rows;             // in the base-2 domain
     float* rest;                 // 1 - p of the target

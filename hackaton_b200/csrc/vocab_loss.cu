@@ -1075,7 +1075,67 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
 // ------------------------------------------------------------------------------------- rows that take part
 constexpr int VL_GATHER_WARPS = 8;
 
-// A CTA takes `per` rows of the caller's. Where they go follows from the targets before them, which it counts itself.
+// Rows that take part among VL_COUNT_ROWS each, and how many come before each such block: where there are so many rows that a
+// CTA of the gather would count too long. (8 words x 8 features, every CTA counting all targets before its own, and this way: 16,384 rows
+// 41 and 44 us, 32,768 65 and 66, 131,072 254 and 183, 2,097,152 25.0 and 2.8 ms.)
+constexpr int VL_COUNT_ROWS = 1024, VL_COUNT_FROM = 32768;
+
+__device__ __forceinline__ bool vl_takes_part(const VocabLossArgs& a, long long t) { return t >= 0 && t < a.vocab; }
+
+__global__ void __launch_bounds__(256)
+vl_count_kernel(const VocabLossArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ int part[8];
+    const long long row0 = (long long)blockIdx.x * VL_COUNT_ROWS;
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < VL_COUNT_ROWS; k += 256) {
+        const long long row = row0 + k + threadIdx.x;
+        n += row < a.rows && vl_takes_part(a, a.targets[row]) ? 1 : 0;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    n = 0;
+    for (int i = 0; i < 8; ++i) n += part[i];
+    a.before[blockIdx.x] = n;
+}
+
+// Counts to sums of those before, by one CTA.
+__global__ void __launch_bounds__(1024)
+vl_before_kernel(const VocabLossArgs a, int blocks) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ int part[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int start = 0;
+    for (int i0 = 0; i0 < blocks; i0 += 1024) {
+        const int i = i0 + threadIdx.x, n = i < blocks ? a.before[i] : 0;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        if (lane == 31) part[warp] = sum;
+        __syncthreads();
+        int all = part[lane];        // every warp adds up the warps
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, all, o);
+            if (lane >= o) all += x;
+        }
+        const int warps_before = __shfl_sync(0xffffffffu, all, (warp + 31) & 31);
+        if (i < blocks) a.before[i] = start + (warp > 0 ? warps_before : 0) + sum - n;
+        start += __shfl_sync(0xffffffffu, all, 31);
+        __syncthreads();
+    }
+}
+
+// A CTA takes `per` rows of the caller's. Where they go follows from the targets before them, which it counts itself, from the
+// beginning of its block where there are sums for blocks.
 __global__ void __launch_bounds__(VL_GATHER_WARPS * 32)
 vl_gather_kernel(const VocabLossArgs a, int per) {
     grid_dep_wait();
@@ -1085,9 +1145,9 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
     __shared__ float dots[VL_GATHER_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row0 = (long long)blockIdx.x * per;
-    const auto takes_part = [&](long long t) { return t >= 0 && t < a.vocab; };
+    const long long block = a.before != nullptr ? row0 / VL_COUNT_ROWS : 0;
     int n = 0;
-    for (long long i = threadIdx.x; i < row0; i += VL_GATHER_WARPS * 32) n += takes_part(a.targets[i]) ? 1 : 0;
+    for (long long i = block * VL_COUNT_ROWS + threadIdx.x; i < row0; i += VL_GATHER_WARPS * 32) n += vl_takes_part(a, a.targets[i]) ? 1 : 0;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) before[warp] = n;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_counters; i += (long long)gridDim.x * blockDim.x)
@@ -1099,12 +1159,12 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
         }
     __syncthreads();
     if (warp == 0) {
-        int start = 0;
+        int start = a.before != nullptr ? a.before[block] : 0;
         for (int i = 0; i < VL_GATHER_WARPS; ++i) start += before[i];
         const long long row = row0 + lane;
         const bool in = lane < per && row < a.rows;
         const long long t = in ? a.targets[row] : -1;
-        const bool part = in && takes_part(t);
+        const bool part = in && vl_takes_part(a, t);
         if (in && t >= a.vocab) atomicCAS(a.status, 0, STATUS_CE_TARGET_RANGE);   // treated as ignored, and recorded
         const unsigned mask = __ballot_sync(0xffffffffu, part);
         const int at = start + __popc(mask & ((1u << lane) - 1u));
@@ -1415,7 +1475,7 @@ static VlCounters vl_counters(const VocabLossArgs& a, const VlRoom& room, bool b
 }
 
 struct VlScratch {
-    size_t parts, target_logit, refs, low, counters, gathered, coef, weight_scale, piece, bytes;
+    size_t parts, target_logit, before, refs, low, counters, gathered, coef, weight_scale, piece, bytes;
     VlRoom room;
 };
 
@@ -1431,6 +1491,7 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
         const size_t n_parts = (size_t)vl_word_tiles(a.vocab) * 2, few_parts = (size_t)a.sm_count * 4;
         s.parts = take((n_parts > few_parts ? n_parts : few_parts) * 8 * pad);
         s.target_logit = take(pad * 4);
+        s.before = take(a.rows > VL_COUNT_FROM ? pad / VL_COUNT_ROWS * 4 + 4 : 0);
         if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
         if (a.grads & 1) {
             s.refs = take(pad * 4);
@@ -1546,8 +1607,16 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         a.piece = ws + s.piece;
         a.piece_units = s.room.units;
     }
+    cudaError_t e = cudaSuccess;
+    if (a.rows > VL_COUNT_FROM) {
+        a.before = reinterpret_cast<int*>(ws + s.before);
+        const int blocks = (int)((a.rows + VL_COUNT_ROWS - 1) / VL_COUNT_ROWS);
+        e = launch_pdl(vl_count_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+        if (e == cudaSuccess) e = launch_pdl(vl_before_kernel, dim3(1), dim3(1024), 0, stream, a, blocks);
+        if (e != cudaSuccess) { *why = "counts"; return e; }
+    }
     const int per = a.rows <= 512 ? 2 : a.rows <= 4096 ? 8 : 32;     // rows of a CTA (64 x 3584: a row to a warp 11.5 us, to four 5.7)
-    cudaError_t e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
+    e = launch_pdl(vl_gather_kernel, dim3((unsigned)((a.rows + per - 1) / per)), dim3(VL_GATHER_WARPS * 32), 0, stream, a, per);
     if (e != cudaSuccess) { *why = "gather"; return e; }
     // Up to 64 rows without a gradient of x: the words take the tensor cores' long side. (64 rows of 3584 features against
     // 151,936 words: with the rows there, which costs four times the products, 216 us; this way all three kernels take 176, the
