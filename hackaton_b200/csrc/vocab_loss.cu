@@ -79,10 +79,11 @@ constexpr int VL_BK = 64;
 // longer ones are cut, and the parts added in the epilogue's registers with rounding. (3584 features, losses against 64 bits: one
 // chain 1.2e-6 in norm, chains of 32 steps 4e-7, of 8 1.2e-7; fp32 products and sums 1.5e-7.) Up to VL_CHAIN_ROWS row tiles,
 // among few rows, a single confident one's small loss shows (2 rows of 2920 features, chains of 32 3.0e-6, of 8 below 1e-6), and the
-// cuts cost nothing: at most VL_CHAIN_FEW steps. (2048 rows x 1536, U: 1725 us in one chain, 1760 in two, 1797 in three.)
+// cuts cost nothing: at most VL_CHAIN_FEW steps, and so where the words take the long side (64 x 3584 against 151,936 words 180.0 us
+// in four chains of 14 steps, 180.5 in seven of 8). (2048 rows x 1536, U: 1725 us in one chain, 1760 in two, 1797 in three.)
 constexpr int VL_CHAIN = 32, VL_CHAIN_FEW = 8, VL_CHAIN_ROWS = 2;
 constexpr int VL_LINKS = 16;               // rows of a word (or that share its place in the table) up to which they are looked up
-constexpr int VL_FEW_CHAINS = 4;           // of at most 64 columns each: there is room for all of a tile's
+constexpr int VL_FEW_CHAINS = 4;           // that share a buffer, 64 columns each
 constexpr int VL_EPI_WARPS = 8;
 constexpr int VL_SMEM_MAX = 232448, VL_BAR_ROOM = 512;
 // Shared memory of a CTA: the ring (128 rows of A and ROWS of B per step), a box of 32 rows x 128 bytes per epilogue warp
@@ -352,7 +353,7 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     const int rows = *p.count, row_tiles = vl_div_up(rows, VL_TILE), steps = vl_div_up(p.hidden, VL_BK * DEEP);
-    const int chain = MODE == VL_FEW ? vl_div_up(steps, VL_FEW_CHAINS) : vl_chain(steps, row_tiles);
+    const int chain = MODE == VL_FEW ? vl_div_up(steps, vl_div_up(steps, VL_CHAIN_FEW / DEEP)) : vl_chain(steps, row_tiles);
     // Few rows: a pair's units are its tiles.
     const int units = rows == 0 ? 0 : MODE == VL_FEW ? (pair + 1) * p.cta_tiles : row_tiles * p.word_tiles;
     const int unit0 = MODE == VL_FEW ? pair * p.cta_tiles : pair, stride = MODE == VL_FEW ? 1 : pairs;
@@ -387,8 +388,8 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
             uint32_t g = 0, n = 0;
             for (int u = unit0; u < units && !fail; u += stride) {
                 uint32_t d = 0;
-                for (int at = 0; at < steps && !fail; at += chain) {
-                    if (MODE != VL_FEW || at == 0) {      // a buffer to a chain, or (few rows) to all of a tile's
+                for (int at = 0, k = 0; at < steps && !fail; at += chain, ++k) {
+                    if (MODE != VL_FEW || k % VL_FEW_CHAINS == 0) {      // a buffer to a chain, or (few rows) to some of a tile's
                         if (!mbar_wait_cluster(bar_drained(n & 1u), ((n >> 1) & 1u) ^ 1u, abort_flag)) { fail = 6; break; }
                         tc_fence_after_sync();
                         d = tmem + (n & 1u) * VL_TILE;
@@ -405,7 +406,8 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
                         umma_commit_pair(bar_empty(s), (uint16_t)3);
                     }
                     d += 64;
-                    if (!fail && (MODE != VL_FEW || end == steps)) umma_commit_pair(bar_done(n++ & 1u), (uint16_t)3);
+                    if (!fail && (MODE != VL_FEW || end == steps || k % VL_FEW_CHAINS == VL_FEW_CHAINS - 1))
+                        umma_commit_pair(bar_done(n++ & 1u), (uint16_t)3);
                 }
             }
         } else if (lane == 0) {
@@ -429,30 +431,33 @@ vl_stats_kernel(const __grid_constant__ VlMaps maps, const __grid_constant__ VlP
         float m[32], s[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) { m[j] = VL_NEG; s[j] = 0.f; }
-        uint32_t it = 0;
-        for (int u = unit0; u < units && !fail; u += stride, ++it) {
-            const int b = (int)(it & 1u);
-            if (!mbar_wait(bar_done(b), (it >> 1) & 1u, abort_flag)) { fail = 5; break; }
-            tc_fence_after_sync();
+        uint32_t buffer = 0;
+        for (int u = unit0; u < units && !fail; u += stride) {
             const int word0 = word_begin + (u - unit0) * p.tile_words + q * 32;
             float r[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0.f;
-            for (int c = 0; c * chain < steps; ++c) {
-                const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + c * 64 + row0;
+            for (int it = 0; it < steps; it += VL_FEW_CHAINS * chain, ++buffer) {
+                const int b = (int)(buffer & 1u);
+                if (!mbar_wait(bar_done(b), (buffer >> 1) & 1u, abort_flag)) { fail = 5; break; }
+                tc_fence_after_sync();
+                for (int c = 0; c < VL_FEW_CHAINS && it + c * chain < steps; ++c) {
+                    const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * VL_TILE + c * 64 + row0;
 #pragma unroll
-                for (int j = 0; j < 32; j += 16) {
-                    if (j >= n) break;
-                    uint32_t h[16];
-                    tmem_ld_32x16(at + j, h);
-                    tmem_ld_wait();
+                    for (int j = 0; j < 32; j += 16) {
+                        if (j >= n) break;
+                        uint32_t h[16];
+                        tmem_ld_32x16(at + j, h);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) r[j + e] += __uint_as_float(h[e]);
+                        for (int e = 0; e < 16; ++e) r[j + e] += __uint_as_float(h[e]);
+                    }
                 }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(lead_drained + 8u * b);
+            if (fail) break;
             const bool there = word0 + lane < p.vocab && q * 32 + lane < p.tile_words;
             const unsigned hits = __ballot_sync(0xffffffffu, (unsigned)(target - word0) < 32u);    // rows whose target is here
 #pragma unroll

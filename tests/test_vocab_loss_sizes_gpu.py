@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_vocab_loss_gpu import check, exact, make
+from test_vocab_loss_gpu import UNIT, check, exact, make
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,22 @@ def test_time_grows_with_the_rows(cuda_lib):
 
     time(1 << 19)
     assert time(1 << 21) <= 8 * time(1 << 19)
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("hidden", [2920, 16384, 65536])
+def test_chains_of_long_rows_without_gradients(cuda_lib, rows, hidden):
+    """Features of one sign: a sum in the tensor cores only grows, and each of its steps of 16 products may cut off a unit of what it has
+    reached twice (its products, the addition). Chains of at most eight steps of 64 features, 32 of 16, are off by 64 units of themselves, and as
+    much of the whole when they are added up, with half a unit of rounding for each."""
+    from hackaton_b200 import vocab_cross_entropy
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h = (0.05 * torch.rand(rows, hidden, device="cuda", generator=g)).to(torch.bfloat16)
+    w = (0.2 * torch.rand(700, hidden, device="cuda", generator=g)).to(torch.bfloat16)
+    t = torch.randint(0, 700, (rows,), device="cuda", generator=g)
+    logits = h.double() @ w.double().t()
+    want, top = torch.logsumexp(logits, 1), logits.max(1).values
+    lse = vocab_cross_entropy(h, w, t)[1]
+    chains = -(-hidden // 512)
+    assert ((lse.double() - want).abs() <= ((64 + chains / 2 + 4) * top + 64) * UNIT).all()
