@@ -971,6 +971,7 @@ int nf4b200_sandwich_norm_fwd(const void* residual, const void* delta, int delta
     if (rc != NF4B200_OK) return rc;
     if (rows > 0 && (!residual || !delta || !post || !pre || !stream_out || !normed || (gates > 0) != (gate != nullptr)))
         return fail(NF4B200_EINVAL, "sandwich_norm_fwd: NULL argument");
+    if (!aligned16(rstd)) return fail(NF4B200_EINVAL, "sandwich_norm_fwd: rstd is not 16-byte aligned");
     nf4::SandwichArgs a = {};
     a.residual = static_cast<const float*>(residual); a.delta = delta;
     a.post = static_cast<const float*>(post); a.pre = static_cast<const float*>(pre); a.gate = static_cast<const float*>(gate);
@@ -1002,6 +1003,7 @@ int nf4b200_sandwich_norm_bwd(const void* stream_in, const void* delta, int delt
     if (rows > 0 && (!stream_in || !delta || !post || !pre || !rstd || !d_normed || (gates > 0) != (gate != nullptr) ||
                      (gates == 0 && d_gate)))
         return fail(NF4B200_EINVAL, "sandwich_norm_bwd: NULL argument, or a gradient of no gate");
+    if (!aligned16(rstd)) return fail(NF4B200_EINVAL, "sandwich_norm_bwd: rstd is not 16-byte aligned");
     const int64_t need = rows == 0 ? 0 : 4 * nf4::sandwich_workspace_floats(rows, (int)hidden, gates, d->sms);
     if (need > 0 && (!workspace || workspace_bytes < (size_t)need || !aligned16(workspace)))
         return fail(NF4B200_EINVAL, "sandwich_norm_bwd: needs %lld bytes of scratch", (long long)need);

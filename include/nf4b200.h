@@ -276,7 +276,8 @@ int nf4b200_act8_lora_grad(const void* codes, const void* steps, const void* s, 
  *   normed = stream * rsqrt(mean(stream^2) + eps) * pre
  * residual, stream fp32 and delta of delta_dtype [rows, hidden]; post, pre fp32 [hidden]; gate fp32 [gates, hidden]
  * or NULL with gates = 0: gate row g serves rows g * rows / gates onwards (gates divides rows). normed is of
- * normed_dtype: delta's, or NF4B200_F32. hidden up to 16384. rstd [rows, 4] fp32 is what the backward needs, or NULL.
+ * normed_dtype: delta's, or NF4B200_F32. hidden up to 16384. rstd [rows, 4] fp32, 16-byte aligned, is what the backward
+ * needs, or NULL.
  * Backward: d_stream (fp32, or NULL) is the gradient that reaches the stream directly, d_normed of normed_dtype;
  * d_residual fp32, d_delta, d_post, d_pre and d_gate ([gates, hidden]) may each be NULL. Scratch as
  * _workspace_bytes says, 16-byte aligned; the weights' sums are made in a fixed order. The reference has the pre-norm
