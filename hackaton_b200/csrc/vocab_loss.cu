@@ -45,7 +45,7 @@ namespace nf4 {
 constexpr float VL_LOG2E = 1.4426950408889634f;
 constexpr float VL_LN2 = 0.6931471805599453f;
 constexpr float VL_NEG = -1.0e30f;         // a finite "minus infinity"
-constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: below 4 * 2^13, down to 2^-24 / 2^13
+constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: at most 2 * 2^13, down to 2^-24 / 2^13
 // A row's reference for its exponentials (base 2): the larger of the first words' maximum less VL_BELOW and the
 // target's logit less VL_BELOW_TARGET_; fp16 takes what lies up to 2^15 above it, bf16 2^100. In fp16 the largest of the other words
 // may not lie further than VL_LOW below it either: a word's exponential is off by 2^-25 there, 2^-22 of the largest, and those
@@ -1339,10 +1339,12 @@ __device__ __forceinline__ float vl_upstream(const float* g, long long stride, l
     return g == nullptr ? 0.f : g[row * stride];
 }
 
-// One CTA: per row that takes part (b + c, b, c) over the power of two above the largest |b|, |c|, times VL_P_SCALE, and what
-// the target's dl of that size loses in 16 bits. (A
-// row far below the largest keeps its digits down to 2^-27 of it, and adds nothing that the others' rounding would not
-// cover below.)
+// One CTA: per row that takes part (b + c, b, c) over a common power of two, times VL_P_SCALE, and what the target's dl of that
+// size loses in 16 bits. The power is the one above the largest |b| (1 - p_t) and |c|: no dl is more than twice that, and the
+// largest are near it however certain the rows are. (Above the largest |b|, rows 22 nats above their other words alone left dW's rows
+// of those a percent off in fp16.) A row far below the largest keeps its digits down to 2^-27 of it, and adds nothing that the others'
+// rounding would not cover below. VL_B_MOST keeps b over the power finite.
+constexpr float VL_B_MOST = 5.421010862427522e-20f;      // 2^-64
 __global__ void __launch_bounds__(1024)
 vl_coef_kernel(const VocabLossArgs a) {
     grid_dep_wait();
@@ -1353,7 +1355,8 @@ vl_coef_kernel(const VocabLossArgs a) {
     for (long long i = threadIdx.x; i < a.n_counters; i += 1024) a.counters[i] = 0;
     for (int at = threadIdx.x; at < rows; at += 1024) {
         const long long row = a.source[at];
-        top = fmaxf(top, fmaxf(fabsf(vl_upstream(a.d_losses, a.d_losses_stride, row)), fabsf(vl_upstream(a.d_lse, a.d_lse_stride, row))));
+        const float b = fabsf(vl_upstream(a.d_losses, a.d_losses_stride, row)), c = fabsf(vl_upstream(a.d_lse, a.d_lse_stride, row));
+        top = fmaxf(top, fmaxf(b * fmaxf(a.rest[at], VL_B_MOST), c));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

@@ -103,3 +103,32 @@ def test_nan_and_infinity_beside_confident_rows(cuda_lib, dtype):
         assert got[name][4].isnan().all()
     assert not got["losses"][280].isfinite() and not got["d_hidden"][280].isfinite().all()
     cuda_lib.device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gaps", [[2], [18], [22], [26], [30], [34], [18, 30], [2, 30], [60]])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_head_gradients_of_confident_rows(cuda_lib, dtype, gaps, rows):
+    """Where every row is nearly certain, what there is keeps its digits: a row's dl are rounded to half a step each, or in fp16 to 2^-25 / 2^13
+    of twice the largest 1 - p of a target (times its factor); for the target's word what that loses is added in fp32."""
+    h, w, t = confident((gaps * rows)[:max(rows, len(gaps))], 1500, dtype)
+    b = torch.full((len(t),), 2.0 ** 20, device="cuda")
+    got = run(h, w, t, b, 0 * b)["d_weight"]
+    h64, w64 = h.double(), w.double()
+    half = torch.finfo(dtype).eps / 2
+    logits = h64 @ w64.t()
+    eta = h.shape[1] * UNIT * (h64.abs() @ w64.abs().t()).max(1).values + (64 + 4 * logits.abs().max(1).values) * UNIT
+    p = torch.softmax(logits, 1)
+    hot = torch.zeros_like(p).scatter_(1, t[:, None], 1.0)
+    others = p * (1 - hot)
+    rest = others.sum(1, keepdim=True)
+    dl = b[:, None].double() * (others - hot * rest)
+    floor = 2.0 ** -25 / 8192 * 2 * (b.double() * rest[:, 0]).max() if dtype == torch.float16 else 0.0
+    off = dl.abs() * (half * (1 - hot) + 3 * eta[:, None] + 64 * UNIT) + floor * (1 - hot)
+    dw = dl.t() @ h64
+    bound = off.t() @ h64.abs() + (len(t) + 1) * UNIT * (dl.abs().t() @ h64.abs())
+    sub = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    bound = bound + half * (dw.abs() + bound) + sub
+    beyond = (dw.abs() + bound >= torch.finfo(dtype).max) & (got.double() == dw.sign() * float("inf"))      # (2^20 times a gap of 2)
+    far = torch.where(beyond, 0.0, (got.double() - dw).abs() / bound)
+    assert (far <= 1.001).all(), float(far.max())
