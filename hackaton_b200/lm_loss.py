@@ -189,8 +189,11 @@ def vocab_cross_entropy(hidden, weight, targets):
     differences of sequences' log probabilities, and a penalty on lse are plain torch on top of them. Next to
     `linear_cross_entropy` (fp16, frozen head, one loss with its gradient made in the forward) this one takes bf16, gives
     the head's gradient and writes no logits. For the gradient of hidden the forward keeps fp32 [rows, features] (at least
-    1024 rows of it), for the head's the rows that take part. Scratch while it runs with gradients: 16-bit pieces of the
-    softmax, 0.2 GB at 2048 to 16,384 rows, 0.8 GB up to half a million. No second derivatives, no forward mode."""
+    1024 rows of it), for the head's a copy of hidden. Scratch of the forward while it runs: 16 bytes per row and 256 words for the rows'
+    maxima and sums (9.5 KB a row at 151,936 words), a copy of hidden unless that is kept, and with hidden's gradient 16-bit
+    pieces of the softmax of at most 0.2 GB up to 16,384 rows and 0.8 GB up to half a million. Together, at 151,936 words x
+    1536 with a frozen head: 0.05 GB for 256 rows, 0.23 for 2048, 0.41 for 16,384, 1.6 for 65,536, 7.4 for 524,288. The backward of the head: 0.03
+    GB for 2048 rows, 0.8 from 65,536. No second derivatives, no forward mode."""
     out = _lib.host().vocab_loss(hidden, weight, targets)
     if out is None:
         _refuse_vocab(hidden, weight, targets)

@@ -63,3 +63,16 @@ def test_chains_of_long_rows_without_gradients(cuda_lib, rows, hidden):
     lse = vocab_cross_entropy(h, w, t)[1]
     chains = -(-hidden // 512)
     assert ((lse.double() - want).abs() <= ((64 + chains / 2 + 4) * top + 64) * UNIT).all()
+
+
+@pytest.mark.parametrize("rows,grads,backward,gigabytes", [(256, 1, 0, 0.05), (2048, 1, 0, 0.23), (16384, 1, 0, 0.41), (65536, 1, 0, 1.6),
+                                                           (524288, 1, 0, 7.4), (2048, 3, 1, 0.03), (65536, 3, 1, 0.8), (524288, 3, 1, 0.8)])
+def test_scratch_is_as_documented(cuda_lib, rows, grads, backward, gigabytes):
+    """The figures that vocab_cross_entropy's docstring gives, to the digits that it gives."""
+    need = cuda_lib.lib().nf4b200_vocab_loss_workspace_bytes(rows, 151936, 1536, grads, backward)
+    assert abs(need / 1e9 - gigabytes) <= (0.05 if gigabytes >= 0.5 else 0.005)
+    if not backward:      # and what they are made of
+        rest = need - rows / 256 * 594 * 2 * 256 * 8 - (rows * 1536 * 2 if grads == 1 else 0)
+        # (0.8 GB as given, below 0.85: pieces of 805 MB at 524,288 rows, 12 bytes a row, and two sweeps' counters, two for each of 594 pieces
+        # and 2048 row tiles, 4 bytes each, 19.5 MB)
+        assert 0 <= rest <= {256: 0.05e9, 2048: 0.21e9, 16384: 0.21e9}.get(rows, 0.85e9)
