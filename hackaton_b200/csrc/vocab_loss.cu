@@ -16,7 +16,9 @@
 // nothing to do nearly always. dW needs the final
 // lse: the logits once more, in 16-bit dl this time, and one product. A word's row of dW is mostly what its own
 // rows' targets add, so that what those dl lose in 16 bits shows: it is kept and added in fp32, for four rows of a word.
-// (1229 rows, 5000 words: dW is 2.1e-4 of itself off in fp16, as much as its own rounding alone; without this 3.0e-4.)
+// (1229 rows, 5000 words: dW is 2.1e-4 of itself off in fp16, as much as its own rounding alone; without this 3.0e-4.) What the
+// probabilities of other words lose is not given back: where one of those holds most of its rows, dH and dW are 1.08 to 1.19 times as far
+// off as products and sums in fp32 with the same rounding at the end (at most 1.5 times over 40,000 small random cases).
 //
 // The tensor cores bound it, and their clock the power that the chip may take, so what counts is that they never pause
 // and that little moves. CTA pairs (tcgen05.mma.cta_group::2) own a 256 x 256 tile, 128 rows by 256 columns of fp32 in
