@@ -68,9 +68,12 @@ def sandwich_norm(residual, delta, post_weight, pre_weight, eps, gate=None, resi
     """(stream, normed) as above. residual: fp32 [..., hidden]; delta: the block's output, fp16, bf16 or fp32 of the same
     shape; post_weight, pre_weight: fp32 [hidden]; gate: None, or fp32 [hidden], or leading dimensions of the stream's
     followed by ones ([batch, 1, hidden] over [batch, tokens, hidden]), or [gates, hidden] over [rows, hidden] with row g
-    for the g-th share of consecutive rows; residual_scale: a number; out_dtype of `normed`: delta's type (the default)
+    for the g-th share of consecutive rows; residual_scale: a number (a tensor that requires a gradient is
+    refused); out_dtype of `normed`: delta's type (the default)
     or fp32. Gradients flow to all five tensors, once
     and in reverse mode."""
+    if isinstance(residual_scale, torch.Tensor) and residual_scale.requires_grad:
+        raise TypeError("hackaton_b200: sandwich_norm: residual_scale is a number, no gradient flows to it; scale the residual before the call")
     given = gate
     if gate is not None and residual.dim() != 2 and gate.dim() > 1 and gate.shape[-1] == residual.shape[-1]:
         gate = _gate_rows(gate, residual.shape) if residual.numel() else gate.reshape(-1, gate.shape[-1])
