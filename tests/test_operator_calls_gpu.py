@@ -78,3 +78,28 @@ def test_nothing_is_kept_without_gradients(cuda_lib, monkeypatch):
             assert torch.equal(w, call(x.clone().requires_grad_()))
         assert not quantised
     assert calls[0](x.clone().requires_grad_()).requires_grad and quantised
+
+
+def test_checkpoints_and_saved_tensors_elsewhere(cuda_lib):
+    """Run again for the backward, or with what is saved moved to the host meanwhile: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+
+    from hackaton_b200 import sandwich_norm, silu_mul, vocab_cross_entropy
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(40, 64, device="cuda", generator=g).half().requires_grad_()
+    ones = torch.ones(64, device="cuda").requires_grad_()
+    head = torch.randn(300, 64, device="cuda", generator=g).half().requires_grad_()
+    t = torch.randint(0, 300, (40,), device="cuda", generator=g)
+
+    def loss(x, ones, head):
+        stream, y = sandwich_norm(x.float(), silu_mul(x, x, keep8=True), ones, ones, 1e-6)
+        return vocab_cross_entropy(y, head, t)[0].sum() + stream.mean()
+
+    leaves = [x, ones, head]
+    want = torch.autograd.grad(loss(*leaves), leaves)
+    again = torch.autograd.grad(checkpoint(loss, *leaves, use_reentrant=False), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        moved = loss(*leaves)
+    moved = torch.autograd.grad(moved, leaves)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, again, moved))

@@ -76,3 +76,19 @@ def test_scratch_is_as_documented(cuda_lib, rows, grads, backward, gigabytes):
         # (0.8 GB as given, below 0.85: pieces of 805 MB at 524,288 rows, 12 bytes a row, and two sweeps' counters, two for each of 594 pieces
         # and 2048 row tiles, 4 bytes each, 19.5 MB)
         assert 0 <= rest <= {256: 0.05e9, 2048: 0.21e9, 16384: 0.21e9}.get(rows, 0.85e9)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,hidden", [(1, 300, 64), (16, 5000, 320), (33, 1003, 1536), (64, 40007, 64)])
+def test_few_rows_with_the_head_alone_trained(cuda_lib, dtype, rows, vocab, hidden):
+    """Losses by the path of few rows without hidden's gradient, the head's gradient behind it."""
+    from hackaton_b200 import vocab_cross_entropy
+    from test_vocab_loss_gpu import factors
+
+    h, w, t = make(rows, vocab, hidden, dtype, rows, ignored=0.2 if rows > 4 else 0.0)
+    b, c = factors(rows)
+    w.requires_grad_()
+    losses, lse = vocab_cross_entropy(h, w, t)
+    (d,) = torch.autograd.grad([losses, lse], [w], [b, c])
+    want = exact(h, w.detach(), t, b, c)
+    check({"losses": losses.detach(), "lse": lse.detach(), "d_weight": d}, {k: want[k] for k in ("losses", "lse", "d_weight")})
