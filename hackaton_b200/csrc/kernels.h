@@ -325,7 +325,6 @@ struct VocabLossArgs {
     void* gathered;              // the rows themselves
     float2* parts;
     float* refs;
-    float* low;                  // fp16, where the first words are not all: bounds that rows have to reach (VlSweepParams)
     int* counters;               // of the sweeps, and `flags` and `list` behind them
     long long n_counters;
     int* flags;

@@ -9,11 +9,10 @@
 //   dH = (b + c) U + (c p_t - b (1 - p_t)) w_t,   U = sum_{v != t} p_v w_v
 // so the forward forms U in the same sweep over the vocabulary as the statistics, two matrix products of 2 R V K
 // operations (R rows, V words, K features) instead of three: a piece's exponentials are taken relative to a reference
-// per row that is fixed before the sweep (from the first words and the target's own logit), and the sum's 1 / s comes
-// at the end. The target is left out of U and of the sums, so that 1 - p_t and a loss near zero keep their digits, and its
-// share is added in fp32. Where a row meets a logit too far above its reference for the 16-bit type, or (fp16) none that
-// is not too far below it, its row tile's sweep is done again with references from the maxima; the launch for that finds
-// nothing to do nearly always. dW needs the final
+// per row that is fixed before the sweep (from the first words, in bf16 also the target's own logit), and the sum's 1 / s
+// comes at the end. The target is left out of U and of the sums, so that 1 - p_t and a loss near zero keep their digits, and its
+// share is added in fp32. Where a row meets a logit too far above its reference for the 16-bit type, its row tile's sweep
+// is done again with references from the maxima; the launch for that looks at a flag and leaves. dW needs the final
 // lse: the logits once more, in 16-bit dl this time, and one product. A word's row of dW is mostly what its own
 // rows' targets add, so that what those dl lose in 16 bits shows: it is kept and added in fp32, for four rows of a word.
 // (1229 rows, 5000 words: dW is 2.1e-4 of itself off in fp16, as much as its own rounding alone; without this 3.0e-4.) What the
@@ -48,15 +47,13 @@ constexpr float VL_LOG2E = 1.4426950408889634f;
 constexpr float VL_LN2 = 0.6931471805599453f;
 constexpr float VL_NEG = -1.0e30f;         // a finite "minus infinity"
 constexpr float VL_P_SCALE = 8192.f;       // of the 16-bit gradient: at most 2 * 2^13, down to 2^-24 / 2^13
-// A row's reference for its exponentials (base 2): the larger of the first words' maximum less VL_BELOW and the
-// target's logit less VL_BELOW_TARGET_; fp16 takes what lies up to 2^15 above it, bf16 2^100. In fp16 the largest of the other words
-// may not lie further than VL_LOW below it either: a word's exponential is off by 2^-25 there, 2^-22 of the largest, and those
-// down to 2^-11 of that one are normal numbers. (With 10 for fp16 too and no such limit, a target 19 above the next word
-// left dH 1.8e-3 of itself off, one 23 above 7e-2. bf16's range has room for both.) Where the first words are all there are, they
-// alone give the reference.
-constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET_F16 = 24.f, VL_BELOW_TARGET_BF16 = 10.f, VL_LOW = 3.f;
+// A row's reference for its exponentials (base 2): the first words' maximum less VL_BELOW; fp16 takes what lies up to 2^15 above it,
+// bf16 2^100. The target has no part in it, as it has none in the sums: fp16 then holds each word to 2^-28 of the largest or better,
+// however certain the row is. (With 2^10 below the target as the least, a target 19 nats above the next word left dH 1.8e-3 of itself off,
+// one 23 above 7e-2. 151,936 words, one of them 4 to 20 nats above all others, those spread by 1 to 3: the largest at 2^3 costs dH 4e-5 at
+// most, at 1 4e-4, at 2^-3 2e-3.) bf16's range has room for 2^10 below the target too, which spares second sweeps.
+constexpr float VL_BELOW = 3.f, VL_BELOW_TARGET_BF16 = 10.f;
 constexpr float VL_ROOM_F16 = 15.f, VL_ROOM_BF16 = 100.f;
-constexpr float VL_NO_LIMIT = 3.0e38f;
 constexpr int VL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int VL_PROBE_TILES = 8;          // tiles of words that the reference is taken from
 // Pieces (vl_shape). Forward as large as VL_PIECE_UNITS tiles of 256 x 256 allow (67 MB): each adds to all of U, which costs
@@ -154,7 +151,6 @@ struct VlSweepParams {
     float2* parts;           // [2 * word tiles][rows_pad]: maximum (base 2), sum relative to the reference
     const float* refs;       // [rows_pad]
     int* flags;              // [row tiles]: whether a row outgrew its reference
-    float* low;              // [rows_pad]: what a row has to reach for its reference to hold, VL_NO_LIMIT once it has; or null
     const int* list;         // a sweep done again: number of row tiles, their indexes
     int again;
     // backward
@@ -913,7 +909,7 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
             const int b = (int)(n & 1u);
             // what the values meet, asked for before the tile is complete
             int target = -1;
-            float lse2 = 0.f, rest = 0.f, ref = 0.f, low = VL_NO_LIMIT, scale = 1.f;
+            float lse2 = 0.f, rest = 0.f, ref = 0.f, scale = 1.f;
             float4 coef = make_float4(0.f, 0.f, 0.f, 0.f);
             const bool live = row < rows;
             if (!w.q && live) {
@@ -924,7 +920,6 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                     coef = p.coef[row];
                 } else {
                     ref = p.refs[row];
-                    if (p.low != nullptr) low = p.low[row];
                 }
             }
             // backward's Q: the last four rows whose target is this thread's word. (Where there are many, what they lose
@@ -1060,7 +1055,6 @@ vl_sweep_kernel(const __grid_constant__ VlSweepMaps maps, const __grid_constant_
                 p.parts[(long long)(v0 / VL_TILE * 2 + 2 * w.nt + half) * p.rows_pad + row] = make_float2(m2, sum);
                 // (several threads write the same)
                 if (live && m2 > ref + (p.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) p.flags[w.mt] = 1;
-                if (low < VL_NO_LIMIT && m2 >= low) p.low[row] = VL_NO_LIMIT;
             }
             if (!w.q || !BWD)       // (backward's Q writes what nobody waits for)
                 owed = w.q ? added : p.written + w.piece * p.pitch + w.slot;
@@ -1233,12 +1227,12 @@ vl_gather_kernel(const VocabLossArgs a, int per) {
 // Joins a row's statistics, 8 rows by 128 shares of the parts per CTA. (32 by 32: 8.5 us for 64 rows of 151,936 words, so 5.0.)
 // Where the head's gradient is to come, the last tile's empty rows become zeros: they meet the others' in sums over rows,
 // and nowhere else does what lies there reach a result. PROBE: the first words' maxima give the row's
-// reference (`sure`: they are all words). Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's reference.
+// reference. Otherwise the whole vocabulary's give loss and lse; `soft`: the sums are relative to the row's reference.
 constexpr int VL_MERGE_ROWS = 8, VL_MERGE_SHARES = 1024 / VL_MERGE_ROWS;
 
 template <bool PROBE>
 __global__ void __launch_bounds__(1024)
-vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft, int sure) {
+vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ float2 join[VL_MERGE_ROWS][VL_MERGE_SHARES + 1];
@@ -1279,12 +1273,9 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft, int sure) {
     const float logit = a.target_logit[at], logit2 = logit * VL_LOG2E;
     if (PROBE) {
         // (fmaxf leaves out a NaN; where there is nothing finite to go by, any number will do)
-        const bool others = x.x > 0.5f * VL_NEG;
         float ref = x.x - VL_BELOW;
-        if (!sure || !others) ref = fmaxf(ref, logit2 - (a.bf16 ? VL_BELOW_TARGET_BF16 : VL_BELOW_TARGET_F16));
-        ref = fabsf(ref) < 1.0e29f ? floorf(ref) : 0.f;
-        a.refs[at] = ref;
-        if (a.low != nullptr) a.low[at] = others && x.x < ref - VL_LOW ? ref - VL_LOW : VL_NO_LIMIT;
+        if (a.bf16 || x.x <= 0.5f * VL_NEG) ref = fmaxf(ref, logit2 - VL_BELOW_TARGET_BF16);
+        a.refs[at] = fabsf(ref) < 1.0e29f ? floorf(ref) : 0.f;
         return;
     }
     const float d = x.x - logit2;      // log2 of what the others' sum is relative to, over the target's
@@ -1312,21 +1303,20 @@ vl_merge_kernel(const VocabLossArgs a, int n_parts, int soft, int sure) {
     a.lse[a.source[at]] = logit + loss;
 }
 
-// A CTA per row tile: where a row's reference does not hold, the tile goes onto the list (in any order) with new ones from
+// A CTA per row tile: where a row outgrew its reference, the tile goes onto the list (in any order), with new references from
 // the maxima.
 __global__ void __launch_bounds__(VL_TILE)
 vl_again_kernel(const VocabLossArgs a, int word_tiles) {
     grid_dep_wait();
     grid_dep_launch();
-    const int rows = *a.count, row = blockIdx.x * VL_TILE + threadIdx.x;
-    const bool low = a.low != nullptr && row < rows && a.low[row] < VL_NO_LIMIT;
-    if (!__syncthreads_or(low || a.flags[blockIdx.x] != 0)) return;
+    if (a.flags[blockIdx.x] == 0) return;
     if (threadIdx.x == 0) a.list[1 + atomicAdd(a.list, 1)] = blockIdx.x;
+    const int rows = *a.count, row = blockIdx.x * VL_TILE + threadIdx.x;
     if (row >= rows) return;
     float top = VL_NEG;
 #pragma unroll 8
     for (int i = 0; i < 2 * word_tiles; ++i) top = fmaxf(top, a.parts[(long long)i * a.rows_pad + row].x);
-    if (low || top > a.refs[row] + (a.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) a.refs[row] = ceilf(top) - 6.f;
+    if (top > a.refs[row] + (a.bf16 ? VL_ROOM_BF16 : VL_ROOM_F16)) a.refs[row] = ceilf(top) - 6.f;
 }
 
 // ------------------------------------------------------------------------------------- backward
@@ -1485,7 +1475,7 @@ static VlCounters vl_counters(const VocabLossArgs& a, const VlRoom& room, bool b
 }
 
 struct VlScratch {
-    size_t parts, target_logit, before, refs, low, counters, gathered, coef, weight_scale, piece, bytes;
+    size_t parts, target_logit, before, refs, counters, gathered, coef, weight_scale, piece, bytes;
     VlRoom room;
 };
 
@@ -1505,7 +1495,6 @@ static VlScratch vl_scratch(const VocabLossArgs& a, bool backward) {
         if (!(a.grads & 2)) s.gathered = take(pad * (size_t)a.hidden * 2);
         if (a.grads & 1) {
             s.refs = take(pad * 4);
-            s.low = take(pad * 4);
             s.counters = take(counters);
             s.piece = take(piece);
         }
@@ -1588,7 +1577,7 @@ static VlSweepParams vl_sweep_params(const VocabLossArgs& a, const VlCounters& c
     int* counters = a.counters + sweep * c.each;
     p.ticket = counters + c.ticket; p.written = counters + c.written; p.read = counters + c.read; p.added = counters + c.added;
     p.pitch = c.pitch;
-    p.parts = a.parts; p.refs = a.refs; p.flags = a.flags; p.low = sweep == 0 ? a.low : nullptr; p.list = a.list; p.again = sweep;
+    p.parts = a.parts; p.refs = a.refs; p.flags = a.flags; p.list = a.list; p.again = sweep;
     p.lse2 = a.lse_rows; p.rest = a.rest; p.coef = a.coef; p.links = a.links; p.first = a.first; p.next = a.next; p.gathered = a.gathered; p.d_weight = a.d_weight; p.weight_scale = a.weight_scale;
     return p;
 }
@@ -1606,10 +1595,9 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
     a.parts = reinterpret_cast<float2*>(ws + s.parts);
     a.target_logit = reinterpret_cast<float*>(ws + s.target_logit);
     if (!(a.grads & 2)) a.gathered = ws + s.gathered;
-    const bool soft = (a.grads & 1) != 0, sure = vl_word_tiles(a.vocab) <= VL_PROBE_TILES;
+    const bool soft = (a.grads & 1) != 0;
     if (soft) {
         a.refs = reinterpret_cast<float*>(ws + s.refs);
-        if (!sure && !a.bf16) a.low = reinterpret_cast<float*>(ws + s.low);
         a.counters = reinterpret_cast<int*>(ws + s.counters);
         a.n_counters = counters.total;
         a.flags = a.counters + counters.flags;
@@ -1669,17 +1657,19 @@ cudaError_t launch_vocab_loss_fwd(const VocabLossArgs& a_in, cudaStream_t stream
         VlParams probe = p;
         if (probe.word_tiles > VL_PROBE_TILES) probe.word_tiles = VL_PROBE_TILES;
         e = vl_launch(vl_stats_kernel<VL_STATS>, VL_THREADS, VlSmemOf<VL_STATS>::TOTAL, logits, probe, row_tiles * probe.word_tiles, a.sm_count, stream);
-        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, 0, sure ? 1 : 0);
+        if (e == cudaSuccess) e = launch_pdl(vl_merge_kernel<true>, merge_grid, merge_block, 0, stream, a, 2 * probe.word_tiles, 0);
         if (e != cudaSuccess) { *why = "references"; return e; }
         const long long units = row_tiles * (p.word_tiles + vl_div_up(p.hidden, VL_TILE));
-        for (int sweep = 0; sweep < (sure ? 1 : 2) && e == cudaSuccess; ++sweep) {      // (references from all words hold)
+        // (no row outgrows a reference that all words were asked for)
+        const bool sure = p.word_tiles <= VL_PROBE_TILES;
+        for (int sweep = 0; sweep < (sure ? 1 : 2) && e == cudaSuccess; ++sweep) {
             e = vl_launch(vl_sweep_kernel<false>, VL_SWEEP_THREADS, VL_SWEEP_SMEM, maps, vl_sweep_params(a, counters, sweep), units, a.sm_count, stream);
             if (!sure && sweep == 0 && e == cudaSuccess)
                 e = launch_pdl(vl_again_kernel, dim3((unsigned)row_tiles), dim3(VL_TILE), 0, stream, a, p.word_tiles);
         }
     }
     if (e != cudaSuccess) { *why = "statistics"; return e; }
-    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, soft ? 1 : 0, 0);
+    e = launch_pdl(vl_merge_kernel<false>, merge_grid, merge_block, 0, stream, a, n_parts, soft ? 1 : 0);
     if (e != cudaSuccess) *why = "merge";
     return e;
 }

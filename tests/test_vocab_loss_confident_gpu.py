@@ -2,8 +2,8 @@
 far below it, and of the rows beside them.
 
 Bound. The exponentials of the words other than the target are rounded to 16 bits: half a step of each, or half of
-the smallest number of the type, which in fp16 is 2^-25 where the largest of them lies no further than 2^3 below a row's
-reference: 2^-22 of the largest. The rest is fp32 arithmetic as in test_vocab_loss_gpu.py (eta: a logit's error), and the output's own
+the smallest number of the type, which in fp16 is 2^-25 where the largest of them lies at least 2^3 above a row's
+reference: 2^-28 of the largest. The rest is fp32 arithmetic as in test_vocab_loss_gpu.py (eta: a logit's error), and the output's own
 rounding."""
 
 import pytest
@@ -46,7 +46,7 @@ def bound_of(h, w, t, b):
     p = torch.softmax(logits, 1)
     hot = torch.zeros_like(p).scatter_(1, t[:, None], 1.0)
     others = p * (1 - hot)
-    low = 2.0 ** -22 if h.dtype == torch.float16 else 0.0
+    low = 2.0 ** -28 if h.dtype == torch.float16 else 0.0
     off = others * (half + 3 * eta[:, None] + 8 * UNIT) + low * others.max(1, keepdim=True).values * (1 - hot)
     size = others + hot * others.sum(1, keepdim=True)
     off = off + hot * others.sum(1, keepdim=True) * (3 * eta[:, None] + 64 * UNIT)
@@ -103,6 +103,26 @@ def test_nan_and_infinity_beside_confident_rows(cuda_lib, dtype):
         assert got[name][4].isnan().all()
     assert not got["losses"][280].isfinite() and not got["d_hidden"][280].isfinite().all()
     cuda_lib.device_status()
+
+
+@pytest.mark.parametrize("gap", [14, 17, 18, 18.8, 20, 24, 30])
+def test_many_words_far_below_one(cuda_lib, gap):
+    """Beside a certain target one word, and 40,000 that are e^-12 of it each, a third of it together, in a direction of their own: they
+    reach the gradient. (In norm: roundings that are 2^-12 of each term, and 40,000 times 2^-28 of the largest.)"""
+    h, w, t = confident([gap] * 8, 40007, torch.float16)
+    w[:, 2:] = 0
+    w[t] = 0
+    w[t, 1] = -0.5
+    w[t, 2 + torch.arange(8, device="cuda")] = 1.0
+    w[1900] = 0
+    w[1900, 20] = 1.0
+    h[:, 1], h[:, 20] = 0.055, 12.0      # (16.45 of fp16's smallest numbers where the one word is at 2^-2.7)
+    h[torch.arange(8, device="cuda"), 2 + torch.arange(8, device="cuda")] = gap + 12.0
+    b = torch.full((8,), 65536.0, device="cuda")
+    got = run(h, w, t, b, 0 * b)["d_hidden"]
+    dh, _ = bound_of(h, w, t, b)
+    sub = 2.0 ** -25 * h.shape[1] ** 0.5
+    assert ((got.double() - dh).norm(dim=1) <= dh.norm(dim=1) * (2.0 ** -11 + 2.0 ** -12.7) + sub).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
