@@ -152,3 +152,16 @@ def test_head_gradients_of_confident_rows(cuda_lib, dtype, gaps, rows):
     beyond = (dw.abs() + bound >= torch.finfo(dtype).max) & (got.double() == dw.sign() * float("inf"))      # (2^20 times a gap of 2)
     far = torch.where(beyond, 0.0, (got.double() - dw).abs() / bound)
     assert (far <= 1.001).all(), float(far.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tiles_done_again_repeat_themselves(cuda_lib, dtype):
+    """Rows of several tiles meet a word behind the first 2048 that is far above those: whichever order the tiles are done again in."""
+    h, w, t = confident([40, 3, 250, 9] * 300, 5000, dtype, late=True)
+    b = torch.ones(1200, device="cuda")
+    first = run(h, w, t, b, 0 * b)
+    dh, bound = bound_of(h, w, t, b)
+    assert ((first["d_hidden"].double() - dh).abs() <= bound * 1.001).all()
+    for _ in range(8):
+        again = run(h, w, t, b, 0 * b)
+        assert all(torch.equal(first[k], again[k]) for k in first)
